@@ -150,7 +150,9 @@ def prepare(case, seed):
             s["q"] = (torch.randn(B, Hkv * c["G"], D, device="cuda", generator=g) * 1.5).bfloat16()
         return s
     x = torch.randn(c["N"], c["V"], device="cuda", generator=g) * 2.5
-    peak = torch.randint(c["V"], (c["N"], 12), device="cuda", generator=g)
+    # twelve different places a row (writing one twice would leave its value to chance)
+    peak = (torch.randint(c["V"], (c["N"], 1), device="cuda", generator=g)
+            + torch.arange(12, device="cuda") * (c["V"] // 12)) % c["V"]
     x.scatter_(1, peak, torch.rand(c["N"], 12, device="cuda", generator=g) * 14 + 3)
     if c["masked"]:  # vocabulary columns that no token has
         x[:, torch.randperm(c["V"], device="cuda", generator=g)[:c["masked"]]] = -math.inf
