@@ -117,11 +117,12 @@ static int* bounds_word(const at::Device& d) {
   auto it = words.find(d.index());
   if (it == words.end()) {
     const c10::cuda::CUDAGuard g(d);
-    // allocated outside any stream capture: the first RoPE call on a device must come before capture
+    // allocated outside any stream capture: the first call that needs it on a device must come before capture
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     C10_CUDA_CHECK(cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(d.index()).stream(), &cap));
     TORCH_CHECK(cap == cudaStreamCaptureStatusNone,
-                "the first RoPE call on a device allocates its index-error word: make it before stream capture");
+                "the first RoPE, 4-bit cache or token log-prob call on a device allocates its index-error word: "
+                "make it before stream capture");
     int* w = nullptr;
     C10_CUDA_CHECK(cudaMalloc(&w, sizeof(int)));
     C10_CUDA_CHECK(cudaMemset(w, 0, sizeof(int)));
@@ -747,6 +748,225 @@ void paged_write(const at::Tensor& k_new, const at::Tensor& v_new, at::Tensor& k
            "paged_write");
 }
 
+// ---------------------------------------------------------------- paged KV cache in 4 bits
+// Where a call brings no status word, index errors go to the device's shared one.
+static int* status_or_bounds(const c10::optional<at::Tensor>& status, const at::Tensor& ref) {
+  if (!status.has_value()) return bounds_word(ref.device());
+  check_dev(status, ref, "status");
+  TORCH_CHECK(status->scalar_type() == at::kInt && status->numel() >= 1, "status: int32");
+  return status->data_ptr<int>();
+}
+
+static int64_t q4_block_bytes(int64_t D) { return 16 * (D / 2 + 4 * (D / std::min<int64_t>(D, 64))); }
+
+static void check_q4_pools(const at::Tensor& k_pool, const at::Tensor& v_pool, int64_t D) {
+  TORCH_CHECK(D == 32 || D == 64 || D == 128, "the 4-bit cache has heads of 32, 64 or 128, got ", std::to_string(D));
+  check_cuda(k_pool, "k_pool");
+  check_dev(v_pool, k_pool, "v_pool");
+  for (const at::Tensor* p : {&k_pool, &v_pool})
+    TORCH_CHECK(p->scalar_type() == at::kByte && p->dim() == 3 && p->is_contiguous() &&
+                          p->size(2) == q4_block_bytes(D) && reinterpret_cast<uintptr_t>(p->data_ptr()) % 16 == 0,
+                      "pool: contiguous 16-byte aligned uint8 [blocks, Hkv, ", std::to_string(q4_block_bytes(D)),
+                      "] for heads of ", std::to_string(D));
+  TORCH_CHECK(v_pool.sizes() == k_pool.sizes(), "k_pool and v_pool differ in shape");
+  TORCH_CHECK(k_pool.size(0) < (1LL << 31) && k_pool.size(1) >= 1 && k_pool.size(1) < 65536, "pool size");
+}
+
+static void check_ints(const at::Tensor& t, const at::Tensor& ref, at::IntArrayRef shape, const char* name) {
+  check_dev(t, ref, name);
+  if (t.scalar_type() == at::kInt && t.is_contiguous() && t.sizes() == shape) return;
+  std::string want;  // numbers go into messages as text: the stream that TORCH_CHECK builds them with cannot format
+  for (const int64_t n : shape) want += (want.empty() ? "" : ", ") + std::to_string(n);  // them in this library
+  TORCH_CHECK(false, name, ": contiguous int32 of shape [", want, "] expected");
+}
+
+// A [rows, heads, D] bf16 operand that kernels read with 16-byte loads: as it is, or a contiguous copy.
+static at::Tensor rows16(const at::Tensor& t) {
+  const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void q4_write(const at::Tensor& k_new, const at::Tensor& v_new, at::Tensor& k_pool, at::Tensor& v_pool,
+              const at::Tensor& slot_block, const at::Tensor& slot_off, const c10::optional<at::Tensor>& status) {
+  check_bf16(k_new, "k_new");
+  check_bf16(v_new, "v_new");
+  TORCH_CHECK(k_new.dim() == 3 && v_new.sizes() == k_new.sizes(), "k_new, v_new: [N, Hkv, D]");
+  check_q4_pools(k_pool, v_pool, k_new.size(2));
+  check_dev(k_new, k_pool, "k_new");
+  check_dev(v_new, k_pool, "v_new");
+  TORCH_CHECK(k_new.size(1) == k_pool.size(1), "k_new and the pool differ in KV heads");
+  const int64_t N = k_new.size(0);
+  check_ints(slot_block, k_pool, {N}, "slot_block");
+  check_ints(slot_off, k_pool, {N}, "slot_off");
+  const c10::cuda::CUDAGuard g(k_pool.device());
+  const at::Tensor k = rows16(k_new), v = rows16(v_new);
+  CHECK_OK(rlb_q4_write(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                        k_pool.data_ptr(), v_pool.data_ptr(), slot_block.data_ptr<int>(), slot_off.data_ptr<int>(), N,
+                        (int)k_pool.size(1), (int)k_new.size(2), (int)k_pool.size(0), status_or_bounds(status, k_pool),
+                        cur_stream()),
+           "q4_write");
+}
+
+std::vector<at::Tensor> q4_read(const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& slot_block,
+                                const at::Tensor& slot_off, int64_t D, const c10::optional<at::Tensor>& status) {
+  check_q4_pools(k_pool, v_pool, D);
+  const int64_t N = slot_block.numel(), Hkv = k_pool.size(1);
+  check_ints(slot_block, k_pool, {N}, "slot_block");
+  check_ints(slot_off, k_pool, {N}, "slot_off");
+  const c10::cuda::CUDAGuard g(k_pool.device());
+  auto opts = k_pool.options().dtype(at::kBFloat16);
+  auto k = at::empty({N, Hkv, D}, opts), v = at::empty({N, Hkv, D}, opts);
+  CHECK_OK(rlb_q4_read(k_pool.data_ptr(), v_pool.data_ptr(), slot_block.data_ptr<int>(), slot_off.data_ptr<int>(),
+                       nullptr, nullptr, 0, 0, N, (int)Hkv, (int)D, (int)k_pool.size(0), k.data_ptr(), v.data_ptr(),
+                       status_or_bounds(status, k_pool), cur_stream()),
+           "q4_read");
+  return {k, v};
+}
+
+std::vector<at::Tensor> q4_gather(const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& tables,
+                                  const at::Tensor& lens, int64_t D, int64_t max_len,
+                                  const c10::optional<at::Tensor>& status) {
+  check_q4_pools(k_pool, v_pool, D);
+  TORCH_CHECK(tables.dim() == 2, "block_tables: [B, max_blocks]");
+  TORCH_CHECK(max_len >= 0 && max_len < (1LL << 31), "max_len: at least 0");
+  const int64_t B = tables.size(0), Hkv = k_pool.size(1);
+  check_ints(tables, k_pool, tables.sizes(), "block_tables");
+  check_ints(lens, k_pool, {B}, "ctx_lens");
+  const c10::cuda::CUDAGuard g(k_pool.device());
+  auto opts = k_pool.options().dtype(at::kBFloat16);
+  auto k = at::empty({B, max_len, Hkv, D}, opts), v = at::empty({B, max_len, Hkv, D}, opts);
+  CHECK_OK(rlb_q4_read(k_pool.data_ptr(), v_pool.data_ptr(), nullptr, nullptr, tables.data_ptr<int>(),
+                       lens.data_ptr<int>(), (int)tables.size(1), (int)max_len, B * max_len, (int)Hkv, (int)D,
+                       (int)k_pool.size(0), k.data_ptr(), v.data_ptr(), status_or_bounds(status, k_pool),
+                       cur_stream()),
+           "q4_gather");
+  return {k, v};
+}
+
+static void check_weights(const at::Tensor& weights, const at::Tensor& rows, const at::Tensor& k_pool, int64_t B) {
+  check_dev(weights, k_pool, "weights");
+  TORCH_CHECK(weights.scalar_type() == at::kFloat && weights.dim() == 3 && weights.is_contiguous() &&
+                        weights.size(1) == k_pool.size(1) && weights.size(2) < (1LL << 31),
+                    "weights: contiguous fp32 [rows, Hkv, tokens]");
+  check_ints(rows, k_pool, {B}, "weight_rows");
+}
+
+at::Tensor q4_decode(const at::Tensor& q, const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& tables,
+                     const at::Tensor& lens, double scale, double softcap, int64_t window,
+                     const c10::optional<at::Tensor>& weights, const c10::optional<at::Tensor>& weight_rows,
+                     const c10::optional<at::Tensor>& status) {
+  check_bf16(q, "q");
+  TORCH_CHECK(q.dim() == 3, "q: [B, Hq, D]");
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2);
+  check_q4_pools(k_pool, v_pool, D);
+  check_dev(q, k_pool, "q");
+  const int64_t Hkv = k_pool.size(1);
+  TORCH_CHECK(Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16, "q: a multiple of the KV heads, at most 16 per KV head");
+  TORCH_CHECK(B < 65536, "at most 65535 sequences in a call");
+  TORCH_CHECK(tables.dim() == 2 && tables.size(1) < (1LL << 27), "block_tables: [B, max_blocks]");
+  check_ints(tables, k_pool, {B, tables.size(1)}, "block_tables");
+  check_ints(lens, k_pool, {B}, "ctx_lens");
+  TORCH_CHECK(weights.has_value() == weight_rows.has_value(), "weights and weight_rows come together");
+  if (weights.has_value()) check_weights(*weights, *weight_rows, k_pool, B);
+  const c10::cuda::CUDAGuard g(k_pool.device());
+  const at::Tensor qc = q.is_contiguous() && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0
+                            ? q : q.clone(at::MemoryFormat::Contiguous);
+  auto out = at::empty({B, Hq, D}, q.options());
+  at::Tensor ml;  // softmax maximum and sum of each query head
+  if (weights.has_value()) ml = at::empty({B, Hq, 2}, q.options().dtype(at::kFloat));
+  CHECK_OK(rlb_q4_decode(qc.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), tables.data_ptr<int>(),
+                         lens.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hkv, (int)(Hq / Hkv), (int)D,
+                         (int)tables.size(1), (int)k_pool.size(0), (float)scale, (float)softcap, (int)window,
+                         ml.defined() ? ml.data_ptr<float>() : nullptr,
+                         weights.has_value() ? weights->data_ptr<float>() : nullptr,
+                         weights.has_value() ? weight_rows->data_ptr<int>() : nullptr,
+                         weights.has_value() ? weights->size(0) : 0, weights.has_value() ? (int)weights->size(2) : 0,
+                         status_or_bounds(status, k_pool), cur_stream()),
+           "q4_decode");
+  return out;
+}
+
+std::vector<at::Tensor> q4_evict(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& tables,
+                                 const at::Tensor& lens, const at::Tensor& new_tables, at::Tensor& weights,
+                                 const at::Tensor& weight_rows, int64_t keep, int64_t D, int64_t recent, int64_t sink,
+                                 const c10::optional<at::Tensor>& status) {
+  check_q4_pools(k_pool, v_pool, D);
+  TORCH_CHECK(tables.dim() == 2 && tables.size(1) < (1LL << 27) && new_tables.dim() == 2,
+                    "block tables: [B, blocks]");
+  const int64_t B = tables.size(0);
+  TORCH_CHECK(B < 65536, "at most 65535 sequences in a call");
+  check_ints(tables, k_pool, {B, tables.size(1)}, "block_tables");
+  check_ints(lens, k_pool, {B}, "ctx_lens");
+  check_ints(new_tables, k_pool, {B, new_tables.size(1)}, "new_tables");
+  check_weights(weights, weight_rows, k_pool, B);
+  TORCH_CHECK(keep >= 1 && recent >= 0 && sink >= 0 && recent + sink <= keep,
+                    "keep at least one token, and no fewer than sink + recent");
+  TORCH_CHECK(new_tables.size(1) < (1LL << 27) && new_tables.size(1) * 16 >= keep,
+                    "new_tables: blocks for `keep` tokens");
+  const c10::cuda::CUDAGuard g(k_pool.device());
+  const int64_t Hkv = k_pool.size(1);
+  auto kept = at::empty({B, Hkv, keep}, lens.options()), new_lens = at::empty({B}, lens.options());
+  CHECK_OK(rlb_q4_evict(k_pool.data_ptr(), v_pool.data_ptr(), tables.data_ptr<int>(), lens.data_ptr<int>(),
+                        new_tables.data_ptr<int>(), weights.data_ptr<float>(), weight_rows.data_ptr<int>(),
+                        kept.data_ptr<int>(), new_lens.data_ptr<int>(), (int)B, (int)Hkv, (int)D, (int)tables.size(1),
+                        (int)new_tables.size(1), (int)k_pool.size(0), weights.size(0), (int)weights.size(2), (int)keep,
+                        (int)recent, (int)sink, status_or_bounds(status, k_pool), cur_stream()),
+           "q4_evict");
+  return {kept, new_lens};
+}
+
+// ---------------------------------------------------------------- token log-probs from logits
+static int logit_type(const at::Tensor& x) {
+  return x.scalar_type() == at::kFloat ? 0 : x.scalar_type() == at::kBFloat16 ? 1 : x.scalar_type() == at::kHalf ? 2 : -1;
+}
+
+// logits [N, V] (unit inner stride), targets [N] int64 -> {maximum, log of the sum, lp, ent [N], top_lp [N, k] fp32,
+// top_ids [N, k] int64}
+std::vector<at::Tensor> token_logprob(const at::Tensor& logits, const at::Tensor& targets, int64_t k,
+                                      const c10::optional<at::Tensor>& status) {
+  check_cuda(logits, "logits");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) < (1LL << 31) && logits.stride(1) == 1 &&
+                        logits.size(0) < (1LL << 31), "logits: [N, V] with unit inner stride");
+  TORCH_CHECK(logit_type(logits) >= 0, "logits: fp32, bf16 or fp16");
+  check_dev(targets, logits, "targets");
+  TORCH_CHECK(targets.scalar_type() == at::kLong && targets.is_contiguous() && targets.dim() == 1 &&
+                        targets.size(0) == logits.size(0), "targets: contiguous int64 [N]");
+  TORCH_CHECK(k >= 0 && k <= 64 && k <= logits.size(1), "top: 0 to 64, and no more than the vocabulary");
+  const c10::cuda::CUDAGuard g(logits.device());
+  const int64_t N = logits.size(0);
+  auto fopt = logits.options().dtype(at::kFloat);
+  auto stats = at::empty({4, N}, fopt);
+  auto top_lp = at::empty({N, k}, fopt), top_ids = at::empty({N, k}, logits.options().dtype(at::kLong));
+  float* st = stats.data_ptr<float>();
+  CHECK_OK(rlb_token_logprob(logits.data_ptr(), logit_type(logits), logits.stride(0), N, (int)logits.size(1),
+                             lptr(targets), (int)k, st, st + N, st + 2 * N, st + 3 * N, top_lp.data_ptr<float>(), lptr(top_ids),
+                             status_or_bounds(status, logits), cur_stream()),
+           "token_logprob");
+  return {stats[0], stats[1], stats[2], stats[3], top_lp, top_ids};
+}
+
+at::Tensor token_logprob_bwd(const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& m,
+                             const at::Tensor& ls, const at::Tensor& ent, const at::Tensor& top_ids, const c10::optional<at::Tensor>& g_lp,
+                             const c10::optional<at::Tensor>& g_ent, const c10::optional<at::Tensor>& g_top) {
+  check_cuda(logits, "logits");
+  const int64_t N = logits.size(0), k = top_ids.size(1);
+  auto check_f = [&](const c10::optional<at::Tensor>& t, int64_t n, const char* name) {
+    if (!t.has_value()) return (const float*)nullptr;
+    check_dev(*t, logits, name);
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == n, name, ": contiguous fp32");
+    return (const float*)t->data_ptr<float>();
+  };
+  const c10::cuda::CUDAGuard g(logits.device());
+  auto dx = at::empty({N, logits.size(1)}, logits.options());
+  CHECK_OK(rlb_token_logprob_bwd(logits.data_ptr(), logit_type(logits), logits.stride(0), N, (int)logits.size(1),
+                                 lptr(targets), check_f(m, N, "m"), check_f(ls, N, "ls"), check_f(ent, N, "ent"), lptr(top_ids), (int)k,
+                                 check_f(g_lp, N, "g_lp"), check_f(g_ent, N, "g_ent"), check_f(g_top, N * k, "g_top"),
+                                 dx.data_ptr(), cur_stream()),
+           "token_logprob_bwd");
+  return dx;
+}
+
 // ---------------------------------------------------------------- sampler
 std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& temperature, int64_t seed) {
   TORCH_CHECK(logits.dim() == 2 && logits.stride(-1) == 1, "logits must be [rows, V] with unit inner stride");
@@ -1001,6 +1221,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fmha_bwd", &fmha_bwd);
   m.def("paged_decode", &paged_decode);
   m.def("paged_write", &paged_write);
+  m.def("q4_write", &q4_write);
+  m.def("q4_read", &q4_read);
+  m.def("q4_gather", &q4_gather);
+  m.def("q4_decode", &q4_decode);
+  m.def("q4_evict", &q4_evict);
+  m.def("token_logprob", &token_logprob);
+  m.def("token_logprob_bwd", &token_logprob_bwd);
   m.def("sample", &sample);
   m.def("rl_loss", &rl_loss);
   m.def("moe_route", &moe_route);

@@ -120,6 +120,33 @@ cudaError_t rlb_paged_write(const void* k_new, const void* v_new, void* k_pool, 
                             const int* slot_off, int B, int Hkv, int D, int num_blocks, int* status, int sms,
                             cudaStream_t s);
 
+// Paged KV cache in 4 bits (paged_q4.cu describes the pools' layout).  Strides are in elements, D is 32, 64 or 128.
+cudaError_t rlb_q4_write(const void* k_new, const void* v_new, long long k_sn, long long k_sh, long long v_sn,
+                         long long v_sh, void* k_pool, void* v_pool, const int* slot_block, const int* slot_off,
+                         long long N, int Hkv, int D, int num_blocks, int* status, cudaStream_t s);
+// Rows by slot, or with `tables` by sequence and position (N = sequences x max_len, zeros behind each length).
+cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_block, const int* slot_off,
+                        const int* tables, const int* lens, int max_blocks, int max_len, long long N, int Hkv, int D,
+                        int num_blocks, void* k_out, void* v_out, int* status, cudaStream_t s);
+cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool, const int* tables, const int* lens,
+                          void* out, int B, int Hkv, int G, int D, int max_blocks, int num_blocks, float scale,
+                          float softcap, int window, float* ml, float* weights, const int* weight_rows,
+                          long long w_rows, int w_len, int* status, cudaStream_t s);
+cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const int* lens, const int* new_tables,
+                         float* weights, const int* weight_rows, int* kept, int* new_lens, int B, int Hkv, int D,
+                         int max_blocks, int new_blocks, int num_blocks, long long w_rows, int w_len, int keep,
+                         int recent, int sink, int* status, cudaStream_t s);
+
+// Token log-probs, entropy and the k largest entries of each row of logits (dtype 0 fp32, 1 bf16, 2 fp16).
+cudaError_t rlb_token_logprob(const void* logits, int dtype, long long ld, long long rows, int V, const long long* tgt,
+                              int k, float* m, float* ls, float* lp, float* ent, float* top_lp, long long* top_ids, int* status,
+                              cudaStream_t s);
+cudaError_t rlb_token_logprob_bwd(const void* logits, int dtype, long long ld, long long rows, int V,
+                                  const long long* tgt, const float* m, const float* ls, const float* ent,
+                                  const long long* top_ids,
+                                  int k, const float* g_lp, const float* g_ent, const float* g_top, void* dx,
+                                  cudaStream_t s);
+
 // Fused temperature sampler (Gumbel-max) with the sampled token's log-probability.
 cudaError_t rlb_sample(const void* logits, int is_bf16, long long ld, int rows, int V, const float* temperature,
                        unsigned long long seed, long long* tokens, float* logprobs, cudaStream_t s);

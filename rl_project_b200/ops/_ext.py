@@ -24,7 +24,7 @@ except BaseException as exc:  # noqa: BLE001
 
 
 # kernels launched by each binding (launch accounting for benchmarks)
-_LAUNCHES = {"rmsnorm_bwd": 2, "grad_norm": 2, "adam_chunk_size": 0, "adam_tensor_desc_bytes": 0, "bounds_status": 0}
+_LAUNCHES = {"rmsnorm_bwd": 2, "q4_evict": 2, "grad_norm": 2, "adam_chunk_size": 0, "adam_tensor_desc_bytes": 0, "bounds_status": 0}
 
 
 class _Counted:
@@ -113,5 +113,6 @@ def raise_bounds_error(code: int) -> None:
 
 def check_bounds(device: torch.device, clear: bool = True) -> None:
     """Raise ``KernelError`` if a kernel on ``device`` reported an out-of-range index into the shared
-    index-error word (RoPE positions outside the cos / sin table).  Synchronises with the device."""
+    index-error word (RoPE positions outside the cos / sin table, slots and blocks of the 4-bit KV cache, targets
+    of ``token_logprobs``).  Synchronises with the device."""
     raise_bounds_error(bounds_code(device, clear))

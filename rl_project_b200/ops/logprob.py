@@ -13,12 +13,15 @@ are processed in chunks and recomputed in backward.
 
 Replaces ``F.cross_entropy`` at ``src/forgeline/models/transformer/model.py:154``
 and ``token_logprobs_from_logits`` at ``src/forgeline/models/policy.py:47-50``.
+
+``token_logprobs(logits, targets, top)`` (csrc/token_logprob.cu) takes logits that exist already (a serving step's, a
+Hugging Face model's) and returns the targets' log-probs, the entropy and the ``top`` alternatives, differentiably.
 """
 
 from __future__ import annotations
 
 import os
-from typing import List, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -147,3 +150,77 @@ def logprobs_from_logits(logits: torch.Tensor, targets: torch.Tensor) -> torch.T
     t = targets.reshape(-1).to(torch.long)
     lp = -F.cross_entropy(flat.float(), t, reduction="none", ignore_index=-1)
     return lp.view(targets.shape)
+
+
+# ---------------------------------------------------------------- log-probs, entropy and alternatives from logits
+TOP_MOST = 64
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor  # [...] fp32: log p(target), 0 where the target is -1
+    entropy: torch.Tensor  # [...] fp32
+    top_logprobs: torch.Tensor  # [..., top] fp32, falling
+    top_ids: torch.Tensor  # [..., top] int64, the lowest id first among equal logits
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, targets, top, status):
+        m, ls, lp, ent, top_lp, top_ids = native().token_logprob(x, targets, top, status)
+        ctx.save_for_backward(x, targets, m, ls, ent, top_ids)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return lp, ent, top_lp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _):
+        grads = [g.float().contiguous() if g is not None else None for g in (g_lp, g_ent, g_top)]
+        return native().token_logprob_bwd(*ctx.saved_tensors, *grads), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
+                   status: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """``logits [..., V]`` (fp32, bf16 or fp16) and ``targets [...]`` (-1: none) -> :class:`TokenLogprobs`.
+
+    One pass over the logits; gradients flow to them from the log-probs, the entropy and the alternatives' log-probs.
+    Entries of -inf are tokens that cannot occur; a row of nothing else has log-probs -inf, entropy 0 and no
+    gradient, a row with NaN or +inf gives NaN.  ``top`` is at most 64.  A target outside the vocabulary has log-prob
+    0 and is reported in ``status`` or the device's index-error word (on CPU: ``IndexError``).
+    """
+    V = logits.shape[-1]
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"logits: fp32, bf16 or fp16, got {logits.dtype}")
+    if targets.shape != logits.shape[:-1]:
+        raise ValueError(f"targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
+    if not 0 <= top <= min(TOP_MOST, V):
+        raise ValueError(f"top must be 0 to {TOP_MOST} and no more than the vocabulary ({V}), got {top}")
+    x = logits.reshape(-1, V)
+    t = targets.reshape(-1).to(torch.long).contiguous()
+    shape = targets.shape
+    if x.is_cuda:
+        x = x if x.stride(1) == 1 else x.contiguous()
+        if x.requires_grad and torch.is_grad_enabled():
+            lp, ent, top_lp, ids = _TokenLogprobs.apply(x, t, int(top), status)
+        else:
+            _, _, lp, ent, top_lp, ids = native().token_logprob(x.detach(), t, int(top), status)
+    else:
+        if t.numel() and t.max() >= V:
+            raise IndexError("a target lies outside the vocabulary")
+        lp, ent, top_lp, ids = _token_logprobs_reference(x, t, int(top))
+    if logits.dim() == 2:
+        return TokenLogprobs(lp, ent, top_lp, ids)
+    return TokenLogprobs(lp.view(shape), ent.view(shape), top_lp.view(*shape, top), ids.view(*shape, top))
+
+
+def _token_logprobs_reference(x: torch.Tensor, t: torch.Tensor, top: int):
+    x = x.float()
+    dead = (x == float("-inf")).all(-1, keepdim=True)
+    logp = torch.where(dead, torch.zeros_like(x), x).log_softmax(-1)
+    lp = logp.gather(-1, t.clamp(min=0)[:, None])[:, 0]
+    p = logp.exp()
+    ent = -torch.where(p == 0, torch.zeros_like(p), p * logp.masked_fill(p == 0, 0.0)).sum(-1)
+    ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top]
+    inf, zero = torch.full_like(lp, float("-inf")), torch.zeros_like(lp)
+    lp = torch.where(t >= 0, torch.where(dead[:, 0], inf, lp), zero)
+    return lp, torch.where(dead[:, 0], zero, ent), logp.gather(-1, ids).masked_fill(dead, float("-inf")), ids
