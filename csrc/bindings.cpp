@@ -769,7 +769,7 @@ static void check_q4_pools(const at::Tensor& k_pool, const at::Tensor& v_pool, i
                       "pool: contiguous 16-byte aligned uint8 [blocks, Hkv, ", std::to_string(q4_block_bytes(D)),
                       "] for heads of ", std::to_string(D));
   TORCH_CHECK(v_pool.sizes() == k_pool.sizes(), "k_pool and v_pool differ in shape");
-  TORCH_CHECK(k_pool.size(0) < (1LL << 31) && k_pool.size(1) >= 1 && k_pool.size(1) < 65536, "pool size");
+  TORCH_CHECK(k_pool.size(0) >= 1 && k_pool.size(0) < (1LL << 31) && k_pool.size(1) >= 1 && k_pool.size(1) < 65536, "pool size");
 }
 
 static void check_ints(const at::Tensor& t, const at::Tensor& ref, at::IntArrayRef shape, const char* name) {
@@ -873,16 +873,26 @@ at::Tensor q4_decode(const at::Tensor& q, const at::Tensor& k_pool, const at::Te
   const at::Tensor qc = q.is_contiguous() && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0
                             ? q : q.clone(at::MemoryFormat::Contiguous);
   auto out = at::empty({B, Hq, D}, q.options());
-  at::Tensor ml;  // softmax maximum and sum of each query head
-  if (weights.has_value()) ml = at::empty({B, Hq, 2}, q.options().dtype(at::kFloat));
+  const int max_blocks = (int)tables.size(1);
+  const int64_t splits = rlb_q4_decode_splits((int)B, (int)Hkv, max_blocks, sm_count());
+  const bool weighted = weights.has_value();
+  at::Tensor scratch;  // partial outputs and statistics of the splits, scores for the weights
+  const int64_t n_part = splits > 1 || weighted ? B * Hq * splits : 0;
+  const int64_t n_scores = weighted ? B * Hkv * max_blocks * 16 * ((Hq / Hkv + 1) / 2 * 2) : 0;
+  float *part = nullptr, *ml = nullptr, *scores = nullptr;
+  if (n_part) {
+    scratch = at::empty({n_scores + n_part * (D + 2)}, q.options().dtype(at::kFloat));
+    part = scratch.data_ptr<float>() + n_scores;  // the scores first: they are written in pairs
+    ml = part + n_part * D;
+    if (weighted) scores = scratch.data_ptr<float>();
+  }
   CHECK_OK(rlb_q4_decode(qc.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), tables.data_ptr<int>(),
-                         lens.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hkv, (int)(Hq / Hkv), (int)D,
-                         (int)tables.size(1), (int)k_pool.size(0), (float)scale, (float)softcap, (int)window,
-                         ml.defined() ? ml.data_ptr<float>() : nullptr,
-                         weights.has_value() ? weights->data_ptr<float>() : nullptr,
-                         weights.has_value() ? weight_rows->data_ptr<int>() : nullptr,
-                         weights.has_value() ? weights->size(0) : 0, weights.has_value() ? (int)weights->size(2) : 0,
-                         status_or_bounds(status, k_pool), cur_stream()),
+                         lens.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hkv, (int)(Hq / Hkv), (int)D, max_blocks,
+                         (int)k_pool.size(0), (float)scale, (float)softcap, (int)window, (int)splits, part, ml, scores,
+                         weighted ? weights->data_ptr<float>() : nullptr,
+                         weighted ? weight_rows->data_ptr<int>() : nullptr, weighted ? weights->size(0) : 0,
+                         weighted ? (int)weights->size(2) : 0, sm_count(), status_or_bounds(status, k_pool),
+                         cur_stream()),
            "q4_decode");
   return out;
 }

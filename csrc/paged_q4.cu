@@ -8,6 +8,7 @@
 // over the group: the inputs are bf16, so the minimum is exact, and the codes are chosen against the rounded scale.
 // Group-major codes keep the 16 tokens x 64 dimensions that a matrix instruction works on contiguous (512 bytes).
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace rlb {
 
@@ -128,6 +129,27 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 }
 
 // ---------------------------------------------------------------- decode attention
+// One CTA takes a stretch of one (sequence, KV head); each of its warps takes every fourth block of the stretch and
+// works alone: its lane 0 brings blocks (codes, scales and minima of K and V, one contiguous piece each) into the
+// warp's own ring of shared memory with bulk copies, and the warp computes on matrix instructions
+// (mma.sync m16n8k16, bf16 x bf16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
+// query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
+// them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
+// memory) would need the unpacked values written back to shared memory first.
+//
+// S^T = K Q^T.  K's codes enter as the exact bf16 numbers code - 8 (bits 0x4300 | code are 128 + code), so with the
+// token's scale s and minimum m:  k . q = s ((code - 8) . q) + (m + 8 s) sum(q), per group of dimensions.  The order
+// of the dimensions inside the product is free as long as Q's registers use the same: a lane reads 16 consecutive
+// dimensions of a token as two words and takes nibbles j and j + 4 of a word as one operand register.
+// O^T = V^T P^T.  The token's scale goes into the weight, p s, and its minimum into a separate sum of p (m + 8 s).
+// p s is split into two bf16 numbers (the second the first's rounding error), two instructions instead of
+// one, which keeps it to 2^-16: bf16 alone would add an error as large as the output's own rounding.
+// The tokens' order is free too: row g of S^T is token (g & 1) * 4 + g / 2 (of each half of the block), which after
+// the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's gives lane t of a quad the tokens t,
+// t + 4, t + 8, t + 12, and the four V words that it reads for them lie in different banks.
+//
+// Softmax statistics are fp32 in base 2.  The running maximum is only raised (and the sums rescaled) when a score
+// exceeds it by 8, so weights stay below 2^8 relative to it.
 struct Q4Cache {
   const uint8_t *k_pool, *v_pool;
   const int *tables, *lens;
@@ -135,117 +157,418 @@ struct Q4Cache {
   float scale, softcap;
 };
 
-// A lane's D / 32 dimensions of a stored row; false where the token's block is not in the pool.
-template <int D>
-RLB_DEVICE bool q4_row(const Q4Cache& c, const uint8_t* pool, int b, int h, int t, float* f) {
+constexpr int kDecodeWarps = 4;
+constexpr int kDecodeStages = 4;
+constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
+
+RLB_DEVICE void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+RLB_DEVICE uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+RLB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+               : "memory");
+}
+
+// Nibbles j of both halves of a word as two bf16 numbers code - 8.
+RLB_DEVICE uint32_t codes_bf16(uint32_t w, int j) {
+  const uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+  const uint32_t c136 = 0x43084308u;
+  __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&c136));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+RLB_DEVICE uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// The tokens that split `sp` of `n` takes of [t0, len): whole blocks, equal shares of the sequence's own length.
+RLB_DEVICE void q4_range(int t0, int len, int sp, int n, int& b0, int& b1) {
+  const int first = t0 / kTok, total = len > t0 ? (len - 1) / kTok - first + 1 : 0;
+  const int per = (total + n - 1) / n;
+  b0 = first + min(total, sp * per);
+  b1 = first + min(total, (sp + 1) * per);
+}
+
+RLB_DEVICE int q4_len(const Q4Cache& c, int b, int* status) {
+  const int len = c.lens[b], most = c.max_blocks * kTok;
+  if (len > most) report(status, kBadIndex);
+  return min(max(len, 0), most);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// NT: tiles of 8 query heads.  `part` [B][Hq][splits][D] and `ml` [B][Hq][splits][2] receive unnormalised outputs and
+// statistics; with one split and no `scores` the output is written instead.  `scores` [B][Hkv][tokens][Gs] receives
+// the base-2 scores for q4_finish_kernel.
+template <int D, int NT>
+__global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_kernel(
+    const __nv_bfloat16* __restrict__ q, Q4Cache c, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
+    float* __restrict__ ml, float* __restrict__ scores, int Gs, int* status) {
   using L = Q4<D>;
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, grp = lane * E / L::kGroup, in_grp = lane * E % L::kGroup;
-  const int blk = c.tables[(long long)b * c.max_blocks + t / kTok], off = t % kTok;
-  if (blk < 0 || blk >= c.num_blocks) return false;
-  const uint8_t* src = pool + ((long long)blk * c.Hkv + h) * L::kBytes;
-  const uint32_t meta = *reinterpret_cast<const uint32_t*>(src + L::kCodes + (grp * kTok + off) * 4);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int byte = src[(grp * kTok + off) * L::kRow + (in_grp + e) / 2];
-    f[e] = fmaf((float)(((in_grp + e) & 1) ? byte >> 4 : byte & 15), bf16_lo_f(meta), bf16_hi_f(meta));
-  }
-  return true;
-}
-
-template <int D>
-RLB_DEVICE float q4_score(const Q4Cache& c, int b, int h, int t, const float* qf) {
-  float f[D / 32], s = 0.f;
-  if (!q4_row<D>(c, c.k_pool, b, h, t, f)) return -INFINITY;
-#pragma unroll
-  for (int e = 0; e < D / 32; ++e) s += qf[e] * f[e];
-  s = warp_sum(s) * c.scale;
-  return c.softcap > 0.f ? tanhf(s / c.softcap) * c.softcap : s;
-}
-
-// One CTA per (query head, sequence); each warp takes every fourth token, a lane D / 32 dimensions of it.  `ml`
-// (optional, [B][Hq][2]) receives the softmax's maximum and sum.
-template <int D>
-__global__ void __launch_bounds__(128) q4_decode_kernel(const __nv_bfloat16* __restrict__ q, Q4Cache c,
-                                                        __nv_bfloat16* __restrict__ out, float* __restrict__ ml,
-                                                        int* status) {
-  constexpr int E = D / 32;
-  const int hq = blockIdx.x, b = blockIdx.y, h = hq / c.G;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = (long long)b * c.Hkv * c.G + hq;
-  int len = c.lens[b];
-  if (len > c.max_blocks * kTok) {
-    report(status, kBadIndex);
-    len = c.max_blocks * kTok;
-  }
+  constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16, HT = NT * 8;
+  constexpr int kStage = 2 * L::kBytes;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kDecodeWarps][kDecodeStages];
+  const int h = blockIdx.x, b = blockIdx.y, sp = blockIdx.z, splits = gridDim.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = c.G;
+  const int len = q4_len(c, b, status);
   const int t0 = c.window > 0 && len > c.window ? len - c.window : 0;
-  float qf[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) qf[e] = __bfloat162float(q[row * D + lane * E + e]);
-  float m = -INFINITY, l = 0.f, acc[E] = {};
-  for (int t = t0 + warp; t < len; t += 4) {
-    const float s = q4_score<D>(c, b, h, t, qf);
-    float f[E];
-    if (!q4_row<D>(c, c.v_pool, b, h, t, f)) {
-      report(status, kBadIndex);
-      continue;
-    }
-    const float mn = fmaxf(m, s), cr = expf(m - mn), p = expf(s - mn);
-    l = l * cr + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * cr + p * f[e];
-    m = mn;
-  }
-  __shared__ float sm[4], sl[4], sa[4][D];
+  int jb0, jb1;
+  q4_range(t0, len, sp, splits, jb0, jb1);
+  const int mine = jb1 - jb0 > warp ? (jb1 - jb0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's blocks
+  uint8_t* ring = smem + warp * kDecodeStages * kStage;
+  const int* table = c.tables + (long long)b * c.max_blocks + jb0 + warp;
+
   if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+    for (int s = 0; s < kDecodeStages; ++s) sm100::mbar_init(&bars[warp][s], 1);
+    sm100::fence_barrier_init();
+    sm100::fence_async_shared();
   }
+  __syncwarp();
+
+  int ids = 0;
+  uint32_t good = 0;  // bit i % 32: block i is in the pool
+  auto issue = [&](int i) {
+    if (i >= mine) return;
+    if ((i & 31) == 0) ids = i + lane < mine ? table[(long long)(i + lane) * kDecodeWarps] : 0;
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    const bool ok = id >= 0 && id < c.num_blocks;
+    good = (good & ~(1u << (i & 31))) | ((uint32_t)ok << (i & 31));
+    if (lane == 0) {
+      if (!ok) report(status, kBadIndex);
+      const long long at = ((long long)(ok ? id : 0) * c.Hkv + h) * L::kBytes;  // a bad block is masked below
+      uint8_t* dst = ring + (i % kDecodeStages) * kStage;
+      uint64_t* bar = &bars[warp][i % kDecodeStages];
+      sm100::mbar_arrive_expect_tx(bar, kStage);
+      bulk_load(dst, c.k_pool + at, L::kBytes, bar);
+      bulk_load(dst + L::kBytes, c.v_pool + at, L::kBytes, bar);
+    }
+  };
 #pragma unroll
-  for (int e = 0; e < E; ++e) sa[warp][lane * E + e] = acc[e];
+  for (int i = 0; i < kDecodeStages; ++i) issue(i);
+
+  // Q's registers for S^T (column n = head g of each tile) and the heads' sums per group
+  uint32_t qb[NT][NG][WPL][4];
+  float qs[NT][NG][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < NG; ++r) {
+      const int head = n * 8 + g;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPL; ++w) {
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (head < G)
+          unpack8(ldg8(q + (((long long)b * c.Hkv + h) * G + head) * D + r * L::kGroup + (t * WPL + w) * 8), f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qb[n][r][w][j] = pack_bf16(f[j], f[j + 4]);
+          sum += f[j] + f[j + 4];
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // the quad's lanes hold head g's sum
+      qs[n][r][0] = __shfl_sync(0xffffffffu, sum, t * 8);      // heads 2t and 2t + 1
+      qs[n][r][1] = __shfl_sync(0xffffffffu, sum, t * 8 + 4);
+    }
+
+  float m[NT][2], mref[NT][2], l[NT][2], z[NT][NG][2], o[NT][NG][MT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[n][e] = -INFINITY;
+      mref[n][e] = l[n][e] = 0.f;
+#pragma unroll
+      for (int r = 0; r < NG; ++r) {
+        z[n][r][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[n][r][i][e] = o[n][r][i][e + 2] = 0.f;
+      }
+    }
+
+  const int tok = (g & 1) * 4 + (g >> 1);  // this lane's tokens in S^T: tok and tok + 8
+  bool alive = true;
+  for (int i = 0; i < mine; ++i) {
+    const int stage = i % kDecodeStages;
+    if (!sm100::mbar_wait_bounded(&bars[warp][stage], (i / kDecodeStages) & 1, kWaitLimit)) {
+      if (lane == 0) report(status, kTimeout);
+      alive = false;
+    }
+    if (!__all_sync(0xffffffffu, alive)) {  // wait, bounded, for the copies still under way, then stop
+      for (int k = i + 1; k < min(mine, i + kDecodeStages); ++k)
+        sm100::mbar_wait_bounded(&bars[warp][k % kDecodeStages], (k / kDecodeStages) & 1, kWaitLimit);
+      break;
+    }
+    const uint8_t* ks = ring + stage * kStage;
+    const uint8_t* vs = ks + L::kBytes;
+    const int base = (jb0 + warp + i * kDecodeWarps) * kTok;
+    const bool ok = (good >> (i & 31)) & 1;
+    const bool seen0 = ok && base + tok >= t0 && base + tok < len;
+    const bool seen1 = ok && base + tok + 8 >= t0 && base + tok + 8 < len;
+
+    // scores
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int r = 0; r < NG; ++r) {
+      float acc[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+      uint32_t u0[WPL], u1[WPL];
+      const uint8_t* row = ks + (r * kTok + tok) * L::kRow + t * WPL * 4;
+      if constexpr (WPL == 2) {
+        *reinterpret_cast<uint2*>(u0) = *reinterpret_cast<const uint2*>(row);
+        *reinterpret_cast<uint2*>(u1) = *reinterpret_cast<const uint2*>(row + 8 * L::kRow);
+      } else {
+        u0[0] = *reinterpret_cast<const uint32_t*>(row);
+        u1[0] = *reinterpret_cast<const uint32_t*>(row + 8 * L::kRow);
+      }
+#pragma unroll
+      for (int w = 0; w < WPL; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const uint32_t a[4] = {codes_bf16(u0[w], j), codes_bf16(u1[w], j), codes_bf16(u0[w], j + 1),
+                                 codes_bf16(u1[w], j + 1)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_bf16(acc[n], a, qb[n][r][w][j], qb[n][r][w][j + 1]);
+        }
+      const uint32_t me0 = *reinterpret_cast<const uint32_t*>(ks + L::kCodes + (r * kTok + tok) * 4);
+      const uint32_t me1 = *reinterpret_cast<const uint32_t*>(ks + L::kCodes + (r * kTok + tok + 8) * 4);
+      const float s0 = bf16_lo_f(me0), s1 = bf16_lo_f(me1);
+      const float z0 = fmaf(8.f, s0, bf16_hi_f(me0)), z1 = fmaf(8.f, s1, bf16_hi_f(me1));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[n][e] += fmaf(s0, acc[n][e], z0 * qs[n][r][e]);
+          s[n][e + 2] += fmaf(s1, acc[n][e + 2], z1 * qs[n][r][e]);
+        }
+    }
+    bool raise = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = s[n][e] * c.scale;
+        if (c.softcap > 0.f) x = tanhf(x / c.softcap) * c.softcap;
+        s[n][e] = (e < 2 ? seen0 : seen1) ? x * kLog2e : -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) raise |= fmaxf(s[n][e], s[n][e + 2]) > m[n][e] + 8.f;
+      if (scores != nullptr) {
+        const int head = n * 8 + 2 * t;
+        float* row = scores + (((long long)b * c.Hkv + h) * c.max_blocks * kTok + base + tok) * Gs + head;
+        if (head < Gs) {
+          *reinterpret_cast<float2*>(row) = make_float2(s[n][0], s[n][1]);
+          *reinterpret_cast<float2*>(row + 8 * Gs) = make_float2(s[n][2], s[n][3]);
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+          for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
+          x = fmaxf(x, m[n][e]);
+          const float f = m[n][e] == -INFINITY ? 0.f : sm100::ex2_approx(m[n][e] - x);
+          m[n][e] = x;
+          mref[n][e] = x == -INFINITY ? 0.f : x;
+          l[n][e] *= f;
+#pragma unroll
+          for (int r = 0; r < NG; ++r) {
+            z[n][r][e] *= f;
+#pragma unroll
+            for (int k = 0; k < MT; ++k) {
+              o[n][r][k][e] *= f;
+              o[n][r][k][e + 2] *= f;
+            }
+          }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[n][e] = sm100::ex2_approx(s[n][e] - mref[n][e]);
+        s[n][e + 2] = sm100::ex2_approx(s[n][e + 2] - mref[n][e]);
+        l[n][e] += s[n][e] + s[n][e + 2];
+      }
+
+    // outputs
+#pragma unroll
+    for (int r = 0; r < NG; ++r) {
+      const uint32_t me0 = *reinterpret_cast<const uint32_t*>(vs + L::kCodes + (r * kTok + tok) * 4);
+      const uint32_t me1 = *reinterpret_cast<const uint32_t*>(vs + L::kCodes + (r * kTok + tok + 8) * 4);
+      // unseen slots may hold anything, NaN scales too
+      const float s0 = seen0 ? bf16_lo_f(me0) : 0.f, s1 = seen1 ? bf16_lo_f(me1) : 0.f;
+      const float z0 = seen0 ? fmaf(8.f, s0, bf16_hi_f(me0)) : 0.f, z1 = seen1 ? fmaf(8.f, s1, bf16_hi_f(me1)) : 0.f;
+      uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float p[4] = {s[n][0] * s0, s[n][1] * s0, s[n][2] * s1, s[n][3] * s1};
+        z[n][r][0] += fmaf(s[n][0], z0, s[n][2] * z1);
+        z[n][r][1] += fmaf(s[n][1], z0, s[n][3] * z1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t hi = pack_bf16(p[2 * k], p[2 * k + 1]);
+          const uint32_t lo = pack_bf16(p[2 * k] - bf16_lo_f(hi), p[2 * k + 1] - bf16_hi_f(hi));
+          bh[n][k] = transpose8x8(hi);
+          bl[n][k] = transpose8x8(lo);
+        }
+      }
+      // dimensions of the group's codes for this lane: 8 g .. 8 g + 7 (4 g .. 4 g + 3), tokens t, t + 4, t + 8, t + 12
+      uint32_t pair[2][WPL];  // [tokens (t, t + 4) or (t + 8, t + 12)][dimensions 0-3 or 4-7], token in each half
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint8_t* row = vs + (r * kTok + t + 8 * k) * L::kRow + g * WPL * 2;
+        if constexpr (WPL == 2) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(row), y = *reinterpret_cast<const uint32_t*>(row + 4 * L::kRow);
+          pair[k][0] = __byte_perm(x, y, 0x5410);
+          pair[k][1] = __byte_perm(x, y, 0x7632);
+        } else {
+          pair[k][0] = *reinterpret_cast<const uint16_t*>(row) |
+                       ((uint32_t)*reinterpret_cast<const uint16_t*>(row + 4 * L::kRow) << 16);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {  // rows g and g + 8 of tile k are dimensions 2k and 2k + 1 of the lane's
+        const int w = k >> 1, j = 2 * (k & 1);
+        const uint32_t a[4] = {codes_bf16(pair[0][w], j), codes_bf16(pair[0][w], j + 1), codes_bf16(pair[1][w], j),
+                               codes_bf16(pair[1][w], j + 1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16(o[n][r][k], a, bh[n][0], bh[n][1]);
+          mma_bf16(o[n][r][k], a, bl[n][0], bl[n][1]);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage
+    issue(i + kDecodeStages);
+  }
+
+  // the warps' sums, through shared memory (the ring is free once every warp is here)
   __syncthreads();
-  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float Lsum = 0.f, cr[4];
+  float* sm_o = reinterpret_cast<float*>(smem);                    // [warps][HT][D]
+  float* sm_ml = sm_o + kDecodeWarps * HT * D;                     // [warps][HT][2]
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    cr[w] = sm[w] == -INFINITY ? 0.f : expf(sm[w] - M);
-    Lsum += sl[w] * cr[w];
-  }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float a = 0.f;
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) a += sa[w][d] * cr[w];
-    out[row * D + d] = __float2bfloat16(Lsum != 0.f ? a / Lsum : 0.f);
-  }
-  if (ml != nullptr && threadIdx.x == 0) {
-    ml[row * 2] = M;
-    ml[row * 2 + 1] = Lsum;
+    for (int e = 0; e < 2; ++e) {
+      float x = l[n][e];
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
+      const int head = n * 8 + 2 * t + e;
+      if (g == 0) {
+        sm_ml[(warp * HT + head) * 2] = m[n][e];
+        sm_ml[(warp * HT + head) * 2 + 1] = x;
+      }
+#pragma unroll
+      for (int r = 0; r < NG; ++r) {
+        float y = z[n][r][e];
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
+        float* dst = sm_o + (warp * HT + head) * D + r * L::kGroup + g * MT * 2;
+#pragma unroll
+        for (int k = 0; k < MT; ++k) {
+          dst[2 * k] = o[n][r][k][e] + y;
+          dst[2 * k + 1] = o[n][r][k][e + 2] + y;
+        }
+      }
+    }
+  __syncthreads();
+  const bool whole = splits == 1 && scores == nullptr;
+  for (int x = threadIdx.x; x < G * D; x += kDecodeWarps * 32) {
+    const int head = x / D, d = x % D;
+    float M = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) M = fmaxf(M, sm_ml[(w * HT + head) * 2]);
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      const float mw = sm_ml[(w * HT + head) * 2];
+      const float f = mw == -INFINITY ? 0.f : sm100::ex2_approx(mw - M);
+      sum += sm_ml[(w * HT + head) * 2 + 1] * f;
+      acc += sm_o[(w * HT + head) * D + d] * f;
+    }
+    const long long row = ((long long)b * c.Hkv + h) * G + head;
+    if (whole) {
+      out[row * D + d] = __float2bfloat16(sum != 0.f ? acc / sum : 0.f);
+    } else {
+      part[(row * splits + sp) * D + d] = acc;
+      if (d == 0) {
+        ml[(row * splits + sp) * 2] = M;
+        ml[(row * splits + sp) * 2 + 1] = sum;
+      }
+    }
   }
 }
 
-// Adds each token's attention weight, summed over its KV head's query heads, to its accumulator.
+// Joins the splits of one (sequence, KV head): CTA 0 of its `gridDim.z` writes the outputs, and with `weights` each
+// adds a stretch of the tokens' attention weights, summed over the heads, to their accumulators.
 template <int D>
-__global__ void __launch_bounds__(128) q4_weights_kernel(const __nv_bfloat16* __restrict__ q, Q4Cache c,
-                                                         const float* __restrict__ ml, float* __restrict__ weights,
-                                                         const int* __restrict__ weight_rows, long long w_rows,
-                                                         int w_len, int* status) {
-  constexpr int E = D / 32;
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = weight_rows[b], len = min(c.lens[b], c.max_blocks * kTok);
-  if (len <= 0 || r < 0) return;
-  if (r >= w_rows || len > w_len) report(status, kBadIndex);
+__global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
+                                                        const float* __restrict__ ml, int splits,
+                                                        __nv_bfloat16* __restrict__ out,
+                                                        const float* __restrict__ scores, int Gs,
+                                                        float* __restrict__ weights,
+                                                        const int* __restrict__ weight_rows, long long w_rows,
+                                                        int w_len, int* status) {
+  __shared__ float sm_m[16], sm_r[16];  // each head's maximum and 1 / sum
+  const int h = blockIdx.x, b = blockIdx.y, G = c.G;
+  const long long row0 = ((long long)b * c.Hkv + h) * G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int head = warp; head < G; head += 8) {
+    const float* p = ml + (row0 + head) * splits * 2;
+    float M = -INFINITY, sum = 0.f;
+    for (int s = lane; s < splits; s += 32) M = fmaxf(M, p[2 * s]);
+    M = warp_max(M);
+    for (int s = lane; s < splits; s += 32) sum += p[2 * s] == -INFINITY ? p[2 * s + 1] : p[2 * s + 1] * sm100::ex2_approx(p[2 * s] - M);
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      sm_m[head] = M;
+      sm_r[head] = sum != 0.f ? 1.f / sum : 0.f;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.z == 0)
+    for (int x = threadIdx.x; x < G * D; x += 256) {
+      const int head = x / D, d = x % D;
+      const float* p = ml + (row0 + head) * splits * 2;
+      const float* a = part + (row0 + head) * splits * D + d;
+      float acc = 0.f;
+      for (int s = 0; s < splits; ++s)
+        acc += p[2 * s] == -INFINITY ? a[(long long)s * D] : a[(long long)s * D] * sm100::ex2_approx(p[2 * s] - sm_m[head]);
+      out[(row0 + head) * D + d] = __float2bfloat16(acc * sm_r[head]);
+    }
+  if (weights == nullptr) return;
+  const int r = weight_rows[b], len = min(max(c.lens[b], 0), c.max_blocks * kTok);
+  if (len == 0 || r < 0) return;
+  if (threadIdx.x == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
   if (r >= w_rows) return;
   const int t0 = c.window > 0 && len > c.window ? len - c.window : 0;
-  for (int t = t0 + warp; t < min(len, w_len); t += 4) {
+  float* w = weights + ((long long)r * c.Hkv + h) * w_len;
+  const float* sc = scores + ((long long)b * c.Hkv + h) * c.max_blocks * kTok * Gs;
+  for (int t = t0 + blockIdx.z * 256 + threadIdx.x; t < min(len, w_len); t += gridDim.z * 256) {
     float p = 0.f;
-    for (int g = 0; g < c.G; ++g) {
-      const long long row = ((long long)b * c.Hkv + h) * c.G + g;
-      float qf[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) qf[e] = __bfloat162float(q[row * D + lane * E + e]);
-      p += expf(q4_score<D>(c, b, h, t, qf) - ml[row * 2]) / ml[row * 2 + 1];
-    }
-    if (lane == 0 && p > 0.f) atomicAdd(weights + ((long long)r * c.Hkv + h) * w_len + t, p);
+    for (int head = 0; head < G; ++head) p += sm100::ex2_approx(sc[(long long)t * Gs + head] - sm_m[head]) * sm_r[head];
+    if (p > 0.f) atomicAdd(w + t, p);
   }
 }
 
@@ -423,18 +746,46 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
   return cudaGetLastError();
 }
 
+template <int D, int NT>
+static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, int B, int splits, float* part, float* ml,
+                                    float* scores, int Gs, int* status, cudaStream_t s) {
+  constexpr int ring = kDecodeWarps * kDecodeStages * 2 * Q4<D>::kBytes;
+  constexpr int join = kDecodeWarps * NT * 8 * (D + 2) * 4;
+  constexpr int smem = ring > join ? ring : join;
+  static_assert(smem <= 47 * 1024, "above 48 KB a kernel has to ask for its shared memory");
+  q4_decode_kernel<D, NT><<<dim3(c.Hkv, B, splits), kDecodeWarps * 32, smem, s>>>(
+      (const __nv_bfloat16*)q, c, (__nv_bfloat16*)out, part, ml, scores, Gs, status);
+  return cudaGetLastError();
+}
+
+int rlb_q4_decode_splits(int B, int Hkv, int max_blocks, int sms) {
+  // Enough CTAs for several waves (ragged lengths leave a tail), but a block or two for each warp at least.
+  const long long rows = (long long)B * Hkv;
+  const long long want = (8LL * sms + rows - 1) / rows, most = (max_blocks + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
+  const long long n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
+}
+
 cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool, const int* tables, const int* lens,
                           void* out, int B, int Hkv, int G, int D, int max_blocks, int num_blocks, float scale,
-                          float softcap, int window, float* ml, float* weights, const int* weight_rows,
-                          long long w_rows, int w_len, int* status, cudaStream_t s) {
+                          float softcap, int window, int splits, float* part, float* ml, float* scores, float* weights,
+                          const int* weight_rows, long long w_rows, int w_len, int sms, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
   const Q4Cache c{(const uint8_t*)k_pool, (const uint8_t*)v_pool, tables, lens, Hkv, G, max_blocks, num_blocks,
                   window, scale, softcap};
-  RLB_Q4_D((q4_decode_kernel<DD><<<dim3(Hkv * G, B), 128, 0, s>>>((const __nv_bfloat16*)q, c, (__nv_bfloat16*)out, ml,
-                                                                  status)));
-  if (weights != nullptr)
-    RLB_Q4_D((q4_weights_kernel<DD><<<dim3(Hkv, B), 128, 0, s>>>((const __nv_bfloat16*)q, c, ml, weights, weight_rows,
-                                                                 w_rows, w_len, status)));
+  const int Gs = (G + 1) & ~1;
+  cudaError_t e = cudaSuccess;
+  RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, splits, part, ml, scores, Gs, status, s))
+                      : (q4_decode_launch<DD, 2>(q, c, out, B, splits, part, ml, scores, Gs, status, s)));
+  if (e != cudaSuccess || (splits == 1 && weights == nullptr)) return e;
+  int chunks = 1;  // CTAs per (sequence, KV head) that add weights: four waves of the GPU, 256 tokens each at least
+  if (weights != nullptr) {
+    const long long rows = (long long)B * Hkv, want = (16LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 255) / 256;
+    chunks = (int)(want < most ? want : most);
+    if (chunks < 1) chunks = 1;
+  }
+  RLB_Q4_D((q4_finish_kernel<DD><<<dim3(Hkv, B, chunks), 256, 0, s>>>(c, part, ml, splits, (__nv_bfloat16*)out, scores,
+                                                                       Gs, weights, weight_rows, w_rows, w_len, status)));
   return cudaGetLastError();
 }
 
