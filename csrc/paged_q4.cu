@@ -7,6 +7,8 @@
 //   minimum = min x,  scale = bf16((max x - min x) / 15),  code = clamp(rint((x - minimum) / scale), 0, 15)
 // over the group: the inputs are bf16, so the minimum is exact, and the codes are chosen against the rounded scale.
 // Group-major codes keep the 16 tokens x 64 dimensions that a matrix instruction works on contiguous (512 bytes).
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 }
 
 // ---------------------------------------------------------------- decode attention
-// One CTA takes a stretch of one (sequence, KV head); each of its warps takes every fourth block of the stretch and
+// One CTA takes a stretch of one (sequence, KV head); each of its warps takes every fourth pair of blocks of the stretch and
 // works alone: its lane 0 brings blocks (codes, scales and minima of K and V, one contiguous piece each) into the
 // warp's own ring of shared memory with bulk copies, and the warp computes on matrix instructions
 // (mma.sync m16n8k16, bf16 x bf16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
@@ -137,19 +139,23 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
 // memory) would need the unpacked values written back to shared memory first.
 //
-// S^T = K Q^T.  K's codes enter as the exact bf16 numbers code - 8 (bits 0x4300 | code are 128 + code), so with the
-// token's scale s and minimum m:  k . q = s ((code - 8) . q) + (m + 8 s) sum(q), per group of dimensions.  The order
-// of the dimensions inside the product is free as long as Q's registers use the same: a lane reads 16 consecutive
-// dimensions of a token as two words and takes nibbles j and j + 4 of a word as one operand register.
-// O^T = V^T P^T.  The token's scale goes into the weight, p s, and its minimum into a separate sum of p (m + 8 s).
-// p s is split into two bf16 numbers (the second the first's rounding error), two instructions instead of
-// one, which keeps it to 2^-16: bf16 alone would add an error as large as the output's own rounding.
+// Codes become fp16 numbers code - 8 exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are
+// 1024 + 16 code, so half of the nibbles need no shift, and one packed fma takes the offset (and the 16) away.
+// S^T = K Q^T.  With a token's scale s and minimum m:  k . q = s ((code - 8) . q) + (m + 8 s) sum(q), per group of
+// dimensions.  Q is fp16 after division by a power of two per head (its largest element then lies in [2^13, 2^14)):
+// bf16's 8 bits fit, and what falls below 2^-24 is 2^-38 of the largest.  The order of the dimensions inside the
+// product is free as long as Q's registers use the same: a lane reads 16 consecutive dimensions of a token as two
+// words and takes nibbles j and j + 4 of a word as one operand register.
+// O^T = V^T P^T.  The token's scale goes into the weight and its minimum into a separate fp32 sum of p (m + 8 s).
+// The weights p s are rounded to fp16 (2^-11 of each, an eighth of what the output's own rounding to bf16 may
+// add); to stay in range they are divided by a power of two at least an eighth of the largest scale so far, so p s <= 2^12.
 // The tokens' order is free too: row g of S^T is token (g & 1) * 4 + g / 2 (of each half of the block), which after
 // the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's gives lane t of a quad the tokens t,
 // t + 4, t + 8, t + 12, and the four V words that it reads for them lie in different banks.
 //
 // Softmax statistics are fp32 in base 2.  The running maximum is only raised (and the sums rescaled) when a score
-// exceeds it by 8, so weights stay below 2^8 relative to it.
+// exceeds it by 8, so weights stay below 2^8 relative to it.  A warp takes two blocks per turn, which shares the
+// waits, votes and bookkeeping among 32 tokens.
 struct Q4Cache {
   const uint8_t *k_pool, *v_pool;
   const int *tables, *lens;
@@ -158,11 +164,11 @@ struct Q4Cache {
 };
 
 constexpr int kDecodeWarps = 4;
-constexpr int kDecodeStages = 4;
+constexpr int kPair = 2;                 // blocks a turn
 constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
 
-RLB_DEVICE void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+RLB_DEVICE void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -179,18 +185,27 @@ RLB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
                : "memory");
 }
 
-// Nibbles j of both halves of a word as two bf16 numbers code - 8.
-RLB_DEVICE uint32_t codes_bf16(uint32_t w, int j) {
-  const uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
-  const uint32_t c136 = 0x43084308u;
-  __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&c136));
-  return *reinterpret_cast<uint32_t*>(&r);
+// Nibbles j and j + 4 of a word (j = 0, 1, 2, 3) as two fp16 numbers code - 8.
+RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t x = w >> 8;
+  const __half2 off0 = __half2half2(__ushort_as_half(0xe408)), off1 = __half2half2(__ushort_as_half(0xd480));  // -1032, -72
+  const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+  const uint32_t v[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x64006400u,
+                         (x & 0x000f000fu) | 0x64006400u, (x & 0x00f000f0u) | 0x64006400u};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&v[j]);
+    const __half2 y = j & 1 ? __hfma2(h, sixteenth, off1) : __hadd2(h, off0);
+    r[j] = *reinterpret_cast<const uint32_t*>(&y);
+  }
 }
 
-RLB_DEVICE uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&r);
+RLB_DEVICE uint32_t pack_f16(float lo, float hi) {
+  const __half2 r = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
+
+RLB_DEVICE float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // The tokens that split `sp` of `n` takes of [t0, len): whole blocks, equal shares of the sequence's own length.
 RLB_DEVICE void q4_range(int t0, int len, int sp, int n, int& b0, int& b1) {
@@ -208,183 +223,185 @@ RLB_DEVICE int q4_len(const Q4Cache& c, int b, int* status) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// NT: tiles of 8 query heads.  `part` [B][Hq][splits][D] and `ml` [B][Hq][splits][2] receive unnormalised outputs and
-// statistics; with one split and no `scores` the output is written instead.  `scores` [B][Hkv][tokens][Gs] receives
-// the base-2 scores for q4_finish_kernel.
+// One turn's work of a warp: the pair of blocks at `ks` (each K then V).  MASKED: some of the tokens are not seen.
 template <int D, int NT>
-__global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_kernel(
-    const __nv_bfloat16* __restrict__ q, Q4Cache c, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
-    float* __restrict__ ml, float* __restrict__ scores, int Gs, int* status) {
+struct Q4Warp {
   using L = Q4<D>;
-  constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16, HT = NT * 8;
-  constexpr int kStage = 2 * L::kBytes;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kDecodeWarps][kDecodeStages];
-  const int h = blockIdx.x, b = blockIdx.y, sp = blockIdx.z, splits = gridDim.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = c.G;
-  const int len = q4_len(c, b, status);
-  const int t0 = c.window > 0 && len > c.window ? len - c.window : 0;
-  int jb0, jb1;
-  q4_range(t0, len, sp, splits, jb0, jb1);
-  const int mine = jb1 - jb0 > warp ? (jb1 - jb0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's blocks
-  uint8_t* ring = smem + warp * kDecodeStages * kStage;
-  const int* table = c.tables + (long long)b * c.max_blocks + jb0 + warp;
+  static constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16;
+  uint32_t qb[NT][NG][WPL][4];                   // Q^T's registers (column n = head g of each tile)
+  float qs[NT][NG][2], qf[NT][2];                // heads 2t, 2t + 1: sums of q, and the factor of their scores
+  float m[NT][2], mref[NT][2], l[NT][2];         // running maximum, what exponents are taken against, sum
+  float z[NT][NG][2], o[NT][NG][MT][4], vn;      // sums of p (m + 8 s), of p s (code - 8) times vn = 2^(130 - ve)
+  int ve;                                        // exponent field of the largest scale of V so far
 
-  if (lane == 0) {
-    for (int s = 0; s < kDecodeStages; ++s) sm100::mbar_init(&bars[warp][s], 1);
-    sm100::fence_barrier_init();
-    sm100::fence_async_shared();
-  }
-  __syncwarp();
-
-  int ids = 0;
-  uint32_t good = 0;  // bit i % 32: block i is in the pool
-  auto issue = [&](int i) {
-    if (i >= mine) return;
-    if ((i & 31) == 0) ids = i + lane < mine ? table[(long long)(i + lane) * kDecodeWarps] : 0;
-    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
-    const bool ok = id >= 0 && id < c.num_blocks;
-    good = (good & ~(1u << (i & 31))) | ((uint32_t)ok << (i & 31));
-    if (lane == 0) {
-      if (!ok) report(status, kBadIndex);
-      const long long at = ((long long)(ok ? id : 0) * c.Hkv + h) * L::kBytes;  // a bad block is masked below
-      uint8_t* dst = ring + (i % kDecodeStages) * kStage;
-      uint64_t* bar = &bars[warp][i % kDecodeStages];
-      sm100::mbar_arrive_expect_tx(bar, kStage);
-      bulk_load(dst, c.k_pool + at, L::kBytes, bar);
-      bulk_load(dst + L::kBytes, c.v_pool + at, L::kBytes, bar);
-    }
-  };
+  RLB_DEVICE void load_q(const __nv_bfloat16* q, int G, float scale) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int i = 0; i < kDecodeStages; ++i) issue(i);
-
-  // Q's registers for S^T (column n = head g of each tile) and the heads' sums per group
-  uint32_t qb[NT][NG][WPL][4];
-  float qs[NT][NG][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int r = 0; r < NG; ++r) {
+    for (int n = 0; n < NT; ++n) {
       const int head = n * 8 + g;
-      float sum = 0.f;
+      float f[NG][WPL][8], big = 0.f;
 #pragma unroll
-      for (int w = 0; w < WPL; ++w) {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (head < G)
-          unpack8(ldg8(q + (((long long)b * c.Hkv + h) * G + head) * D + r * L::kGroup + (t * WPL + w) * 8), f);
+      for (int r = 0; r < NG; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          qb[n][r][w][j] = pack_bf16(f[j], f[j + 4]);
-          sum += f[j] + f[j + 4];
+        for (int w = 0; w < WPL; ++w) {
+          if (head < G) unpack8(ldg8(q + head * D + r * L::kGroup + (t * WPL + w) * 8), f[r][w]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (head >= G) f[r][w][j] = 0.f;
+            big = fmaxf(big, fabsf(f[r][w][j]));
+          }
         }
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // the quad's lanes hold head g's sum
-      qs[n][r][0] = __shfl_sync(0xffffffffu, sum, t * 8);      // heads 2t and 2t + 1
-      qs[n][r][1] = __shfl_sync(0xffffffffu, sum, t * 8 + 4);
-    }
-
-  float m[NT][2], mref[NT][2], l[NT][2], z[NT][NG][2], o[NT][NG][MT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      m[n][e] = -INFINITY;
-      mref[n][e] = l[n][e] = 0.f;
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // q 2^e has its largest element in [2^13, 2^14)
+      const int e = min(max(140 - (int)(__float_as_uint(big) >> 23), -126), 126);
+      const float up = pow2(e);
+      float factor = scale * pow2(-e);
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
-        z[n][r][e] = 0.f;
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) o[n][r][i][e] = o[n][r][i][e + 2] = 0.f;
+        for (int w = 0; w < WPL; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = f[r][w][j] * up, y = f[r][w][j + 4] * up;
+            qb[n][r][w][j] = pack_f16(x, y);
+            sum += x + y;
+          }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        qs[n][r][0] = __shfl_sync(0xffffffffu, sum, t * 8);
+        qs[n][r][1] = __shfl_sync(0xffffffffu, sum, t * 8 + 4);
       }
+      qf[n][0] = __shfl_sync(0xffffffffu, factor, t * 8);
+      qf[n][1] = __shfl_sync(0xffffffffu, factor, t * 8 + 4);
     }
-
-  const int tok = (g & 1) * 4 + (g >> 1);  // this lane's tokens in S^T: tok and tok + 8
-  bool alive = true;
-  for (int i = 0; i < mine; ++i) {
-    const int stage = i % kDecodeStages;
-    if (!sm100::mbar_wait_bounded(&bars[warp][stage], (i / kDecodeStages) & 1, kWaitLimit)) {
-      if (lane == 0) report(status, kTimeout);
-      alive = false;
-    }
-    if (!__all_sync(0xffffffffu, alive)) {  // wait, bounded, for the copies still under way, then stop
-      for (int k = i + 1; k < min(mine, i + kDecodeStages); ++k)
-        sm100::mbar_wait_bounded(&bars[warp][k % kDecodeStages], (k / kDecodeStages) & 1, kWaitLimit);
-      break;
-    }
-    const uint8_t* ks = ring + stage * kStage;
-    const uint8_t* vs = ks + L::kBytes;
-    const int base = (jb0 + warp + i * kDecodeWarps) * kTok;
-    const bool ok = (good >> (i & 31)) & 1;
-    const bool seen0 = ok && base + tok >= t0 && base + tok < len;
-    const bool seen1 = ok && base + tok + 8 >= t0 && base + tok + 8 < len;
-
-    // scores
-    float s[NT][4];
+    vn = pow2(126);
+    ve = 4;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int r = 0; r < NG; ++r) {
-      float acc[NT][4];
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        mref[n][e] = l[n][e] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-      uint32_t u0[WPL], u1[WPL];
-      const uint8_t* row = ks + (r * kTok + tok) * L::kRow + t * WPL * 4;
-      if constexpr (WPL == 2) {
-        *reinterpret_cast<uint2*>(u0) = *reinterpret_cast<const uint2*>(row);
-        *reinterpret_cast<uint2*>(u1) = *reinterpret_cast<const uint2*>(row + 8 * L::kRow);
-      } else {
-        u0[0] = *reinterpret_cast<const uint32_t*>(row);
-        u1[0] = *reinterpret_cast<const uint32_t*>(row + 8 * L::kRow);
-      }
+        for (int r = 0; r < NG; ++r) {
+          z[n][r][e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < WPL; ++w)
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          const uint32_t a[4] = {codes_bf16(u0[w], j), codes_bf16(u1[w], j), codes_bf16(u0[w], j + 1),
-                                 codes_bf16(u1[w], j + 1)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_bf16(acc[n], a, qb[n][r][w][j], qb[n][r][w][j + 1]);
+          for (int i = 0; i < MT; ++i) o[n][r][i][e] = o[n][r][i][e + 2] = 0.f;
         }
-      const uint32_t me0 = *reinterpret_cast<const uint32_t*>(ks + L::kCodes + (r * kTok + tok) * 4);
-      const uint32_t me1 = *reinterpret_cast<const uint32_t*>(ks + L::kCodes + (r * kTok + tok + 8) * 4);
-      const float s0 = bf16_lo_f(me0), s1 = bf16_lo_f(me1);
-      const float z0 = fmaf(8.f, s0, bf16_hi_f(me0)), z1 = fmaf(8.f, s1, bf16_hi_f(me1));
+      }
+  }
+
+  // seen: bit 2k + i: this lane's token i of block k.  `scores`: this lane's token 0 of block 0, or null.
+  template <bool MASKED>
+  RLB_DEVICE void turn(const uint8_t* ks, unsigned seen, float softcap, float* scores, int Gs) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int tok = (g & 1) * 4 + (g >> 1);  // this lane's tokens of a block in S^T: tok and tok + 8
+    float s[NT][kPair][4];
+#pragma unroll
+    for (int k = 0; k < kPair; ++k)
+#pragma unroll
+      for (int r = 0; r < NG; ++r) {
+        const uint8_t* blk = ks + k * 2 * L::kBytes;
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        uint32_t u0[WPL], u1[WPL];
+        const uint8_t* row = blk + (r * kTok + tok) * L::kRow + t * WPL * 4;
+        if constexpr (WPL == 2) {
+          *reinterpret_cast<uint2*>(u0) = *reinterpret_cast<const uint2*>(row);
+          *reinterpret_cast<uint2*>(u1) = *reinterpret_cast<const uint2*>(row + 8 * L::kRow);
+        } else {
+          u0[0] = *reinterpret_cast<const uint32_t*>(row);
+          u1[0] = *reinterpret_cast<const uint32_t*>(row + 8 * L::kRow);
+        }
+#pragma unroll
+        for (int w = 0; w < WPL; ++w) {
+          uint32_t c0[4], c1[4];
+          codes_f16(u0[w], c0);
+          codes_f16(u1[w], c1);
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const uint32_t a[4] = {c0[j], c1[j], c0[j + 1], c1[j + 1]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(acc[n], a, qb[n][r][w][j], qb[n][r][w][j + 1]);
+          }
+        }
+        const uint32_t me0 = *reinterpret_cast<const uint32_t*>(blk + L::kCodes + (r * kTok + tok) * 4);
+        const uint32_t me1 = *reinterpret_cast<const uint32_t*>(blk + L::kCodes + (r * kTok + tok + 8) * 4);
+        const float s0 = bf16_lo_f(me0), s1 = bf16_lo_f(me1);
+        const float z0 = fmaf(8.f, s0, bf16_hi_f(me0)), z1 = fmaf(8.f, s1, bf16_hi_f(me1));
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = fmaf(s0, acc[n][e], z0 * qs[n][r][e]), y = fmaf(s1, acc[n][e + 2], z1 * qs[n][r][e]);
+            s[n][k][e] = r == 0 ? x : s[n][k][e] + x;
+            s[n][k][e + 2] = r == 0 ? y : s[n][k][e + 2] + y;
+          }
+      }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < kPair; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][k][e] *= qf[n][e & 1];
+    if (softcap > 0.f) {  // (the factor then lacks log2 e)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[n][e] += fmaf(s0, acc[n][e], z0 * qs[n][r][e]);
-          s[n][e + 2] += fmaf(s1, acc[n][e + 2], z1 * qs[n][r][e]);
-        }
+        for (int k = 0; k < kPair; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][k][e] = tanhf(s[n][k][e] / softcap) * (softcap * kLog2e);
     }
     bool raise = false;
+    uint32_t vm[kPair][NG][2], vmax = 0;  // V's (scale, minimum) of this lane's tokens
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = s[n][e] * c.scale;
-        if (c.softcap > 0.f) x = tanhf(x / c.softcap) * c.softcap;
-        s[n][e] = (e < 2 ? seen0 : seen1) ? x * kLog2e : -INFINITY;
-      }
+      for (int k = 0; k < kPair; ++k)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) raise |= fmaxf(s[n][e], s[n][e + 2]) > m[n][e] + 8.f;
-      if (scores != nullptr) {
-        const int head = n * 8 + 2 * t;
-        float* row = scores + (((long long)b * c.Hkv + h) * c.max_blocks * kTok + base + tok) * Gs + head;
-        if (head < Gs) {
-          *reinterpret_cast<float2*>(row) = make_float2(s[n][0], s[n][1]);
-          *reinterpret_cast<float2*>(row + 8 * Gs) = make_float2(s[n][2], s[n][3]);
-        }
+        for (int e = 0; e < 4; ++e)
+          if (MASKED && !((seen >> (2 * k + (e >> 1))) & 1)) s[n][k][e] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        raise |= fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2])) > m[n][e] + 8.f;
+      if (scores != nullptr && n * 8 + 2 * t < Gs) {
+#pragma unroll
+        for (int k = 0; k < kPair; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (!MASKED || ((seen >> (4 + 2 * k + i)) & 1))
+              *reinterpret_cast<float2*>(scores + (k * kTok + 8 * i) * Gs + n * 8 + 2 * t) =
+                  make_float2(s[n][k][2 * i], s[n][k][2 * i + 1]);
       }
     }
+#pragma unroll
+    for (int k = 0; k < kPair; ++k)
+#pragma unroll
+      for (int r = 0; r < NG; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          vm[k][r][i] = *reinterpret_cast<const uint32_t*>(ks + (2 * k + 1) * L::kBytes + L::kCodes + (r * kTok + tok + 8 * i) * 4);
+          if (MASKED && !((seen >> (2 * k + i)) & 1)) vm[k][r][i] = 0;  // unseen slots may hold anything, NaN too
+          vmax = __vmaxu2(vmax, vm[k][r][i]);
+        }
+    const int e_here = (vmax >> 7) & 0xff;  // the exponent field of the largest scale (scales are not negative)
+    raise |= e_here > ve;
     if (__any_sync(0xffffffffu, raise)) {
+      int e_all = e_here;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) e_all = max(e_all, __shfl_xor_sync(0xffffffffu, e_all, k));
+      e_all = min(max(e_all, ve), 252);
+      const float fv = pow2(max(ve - e_all, -126));
+      ve = e_all;
+      vn = pow2(130 - ve);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(s[n][e], s[n][e + 2]);
+          float x = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
           x = fmaxf(x, m[n][e]);
@@ -397,8 +414,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_
             z[n][r][e] *= f;
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
-              o[n][r][k][e] *= f;
-              o[n][r][k][e + 2] *= f;
+              o[n][r][k][e] *= f * fv;
+              o[n][r][k][e + 2] *= f * fv;
             }
           }
         }
@@ -406,90 +423,176 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[n][e] = sm100::ex2_approx(s[n][e] - mref[n][e]);
-        s[n][e + 2] = sm100::ex2_approx(s[n][e + 2] - mref[n][e]);
-        l[n][e] += s[n][e] + s[n][e + 2];
-      }
-
-    // outputs
+      for (int k = 0; k < kPair; ++k)
 #pragma unroll
-    for (int r = 0; r < NG; ++r) {
-      const uint32_t me0 = *reinterpret_cast<const uint32_t*>(vs + L::kCodes + (r * kTok + tok) * 4);
-      const uint32_t me1 = *reinterpret_cast<const uint32_t*>(vs + L::kCodes + (r * kTok + tok + 8) * 4);
-      // unseen slots may hold anything, NaN scales too
-      const float s0 = seen0 ? bf16_lo_f(me0) : 0.f, s1 = seen1 ? bf16_lo_f(me1) : 0.f;
-      const float z0 = seen0 ? fmaf(8.f, s0, bf16_hi_f(me0)) : 0.f, z1 = seen1 ? fmaf(8.f, s1, bf16_hi_f(me1)) : 0.f;
-      uint32_t bh[NT][2], bl[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float p[4] = {s[n][0] * s0, s[n][1] * s0, s[n][2] * s1, s[n][3] * s1};
-        z[n][r][0] += fmaf(s[n][0], z0, s[n][2] * z1);
-        z[n][r][1] += fmaf(s[n][1], z0, s[n][3] * z1);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t hi = pack_bf16(p[2 * k], p[2 * k + 1]);
-          const uint32_t lo = pack_bf16(p[2 * k] - bf16_lo_f(hi), p[2 * k + 1] - bf16_hi_f(hi));
-          bh[n][k] = transpose8x8(hi);
-          bl[n][k] = transpose8x8(lo);
+        for (int e = 0; e < 4; ++e) {
+          s[n][k][e] = sm100::ex2_approx(s[n][k][e] - mref[n][e & 1]);
+          l[n][e & 1] += s[n][k][e];
         }
-      }
-      // dimensions of the group's codes for this lane: 8 g .. 8 g + 7 (4 g .. 4 g + 3), tokens t, t + 4, t + 8, t + 12
-      uint32_t pair[2][WPL];  // [tokens (t, t + 4) or (t + 8, t + 12)][dimensions 0-3 or 4-7], token in each half
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint8_t* row = vs + (r * kTok + t + 8 * k) * L::kRow + g * WPL * 2;
-        if constexpr (WPL == 2) {
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(row), y = *reinterpret_cast<const uint32_t*>(row + 4 * L::kRow);
-          pair[k][0] = __byte_perm(x, y, 0x5410);
-          pair[k][1] = __byte_perm(x, y, 0x7632);
-        } else {
-          pair[k][0] = *reinterpret_cast<const uint16_t*>(row) |
-                       ((uint32_t)*reinterpret_cast<const uint16_t*>(row + 4 * L::kRow) << 16);
-        }
-      }
+    for (int k = 0; k < kPair; ++k)
 #pragma unroll
-      for (int k = 0; k < MT; ++k) {  // rows g and g + 8 of tile k are dimensions 2k and 2k + 1 of the lane's
-        const int w = k >> 1, j = 2 * (k & 1);
-        const uint32_t a[4] = {codes_bf16(pair[0][w], j), codes_bf16(pair[0][w], j + 1), codes_bf16(pair[1][w], j),
-                               codes_bf16(pair[1][w], j + 1)};
+      for (int r = 0; r < NG; ++r) {
+        const uint8_t* blk = ks + (2 * k + 1) * L::kBytes;
+        const float s0 = bf16_lo_f(vm[k][r][0]), s1 = bf16_lo_f(vm[k][r][1]);
+        const float z0 = fmaf(8.f, s0, bf16_hi_f(vm[k][r][0])), z1 = fmaf(8.f, s1, bf16_hi_f(vm[k][r][1]));
+        const float w0 = s0 * vn, w1 = s1 * vn;
+        uint32_t b[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_bf16(o[n][r][k], a, bh[n][0], bh[n][1]);
-          mma_bf16(o[n][r][k], a, bl[n][0], bl[n][1]);
+          b[n][0] = transpose8x8(pack_f16(s[n][k][0] * w0, s[n][k][1] * w0));
+          b[n][1] = transpose8x8(pack_f16(s[n][k][2] * w1, s[n][k][3] * w1));
+          z[n][r][0] = fmaf(s[n][k][0], z0, fmaf(s[n][k][2], z1, z[n][r][0]));
+          z[n][r][1] = fmaf(s[n][k][1], z0, fmaf(s[n][k][3], z1, z[n][r][1]));
+        }
+        // the group's codes for this lane: dimensions 8 g .. 8 g + 7 (4 g .. 4 g + 3), tokens t, t + 4, t + 8, t + 12
+        uint32_t c[2][WPL][4];  // [tokens (t, t + 4) or (t + 8, t + 12)][dimensions 0-3 or 4-7], a token in each half
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint8_t* row = blk + (r * kTok + t + 8 * i) * L::kRow + g * WPL * 2;
+          if constexpr (WPL == 2) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(row);
+            const uint32_t y = *reinterpret_cast<const uint32_t*>(row + 4 * L::kRow);
+            codes_f16(__byte_perm(x, y, 0x5410), c[i][0]);
+            codes_f16(__byte_perm(x, y, 0x7632), c[i][1]);
+          } else {
+            codes_f16(*reinterpret_cast<const uint16_t*>(row) |
+                          ((uint32_t)*reinterpret_cast<const uint16_t*>(row + 4 * L::kRow) << 16),
+                      c[i][0]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {  // rows g and g + 8 of tile i are dimensions 2i and 2i + 1 of the lane's
+          const int w = i >> 1, j = 2 * (i & 1);
+          const uint32_t a[4] = {c[0][w][j], c[0][w][j + 1], c[1][w][j], c[1][w][j + 1]};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(o[n][r][i], a, b[n][0], b[n][1]);
         }
       }
+  }
+};
+
+// NT: tiles of 8 query heads.  `part` [B][Hq][splits][D] and `ml` [B][Hq][splits][2] receive unnormalised outputs and
+// statistics; with one split and no `scores` the output is written instead.  `scores` [B][Hkv][tokens][Gs] receives
+// the base-2 scores for q4_finish_kernel.
+template <int D>
+constexpr int q4_stages() { return D == 128 ? 2 : 4; }  // pairs of blocks in a warp's ring
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_kernel(
+    const __nv_bfloat16* __restrict__ q, Q4Cache c, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
+    float* __restrict__ ml, float* __restrict__ scores, int Gs, int* status) {
+  using L = Q4<D>;
+  using W = Q4Warp<D, NT>;
+  constexpr int HT = NT * 8, S = q4_stages<D>();
+  constexpr int kStage = kPair * 2 * L::kBytes;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kDecodeWarps][S];
+  const int h = blockIdx.x, b = blockIdx.y, sp = blockIdx.z, splits = gridDim.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = c.G;
+  const int len = q4_len(c, b, status);
+  const int t0 = c.window > 0 && len > c.window ? len - c.window : 0;
+  int jb0, jb1;
+  q4_range(t0, len, sp, splits, jb0, jb1);
+  const int pairs = (jb1 - jb0 + kPair - 1) / kPair;
+  const int mine = pairs > warp ? (pairs - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's turns
+  uint8_t* ring = smem + warp * S * kStage;
+  const int* table = c.tables + (long long)b * c.max_blocks;
+
+  if (lane == 0) {
+    for (int s = 0; s < S; ++s) sm100::mbar_init(&bars[warp][s], 1);
+    sm100::fence_barrier_init();
+    sm100::fence_async_shared();
+  }
+  __syncwarp();
+
+  int id = 0;         // lanes 2i and 2i + 1: the blocks of turn i of the current sixteen
+  uint32_t good = 0;  // bits 2 (i % 16), + 1: blocks of turn i that are there
+  auto issue = [&](int i) {
+    if (i >= mine) return;
+    if ((i & 15) == 0) {
+      const int at = jb0 + ((i + (lane >> 1)) * kDecodeWarps + warp) * kPair + (lane & 1);
+      id = at < jb1 ? table[at] : -1;
+      const bool ok = id >= 0 && id < c.num_blocks;
+      if (!ok && at < jb1) report(status, kBadIndex);
+      if (!ok) id = -1;
+    }
+    const int shift = 2 * (i & 15);
+    const unsigned ok = __ballot_sync(0xffffffffu, id >= 0) >> shift & 3u;
+    good = (good & ~(3u << shift)) | (ok << shift);
+    const int blk = __shfl_sync(0xffffffffu, id, shift + (lane & 1));
+    uint64_t* bar = &bars[warp][i % S];
+    if (lane == 0) sm100::mbar_arrive_expect_tx(bar, __popc(ok) * 2 * L::kBytes);
+    __syncwarp();
+    if (lane < 4 && blk >= 0) {  // lane: block lane & 1, K (lanes 0, 1) or V (2, 3)
+      const uint8_t* src = (lane < 2 ? c.k_pool : c.v_pool) + ((long long)blk * c.Hkv + h) * L::kBytes;
+      bulk_load(ring + (i % S) * kStage + ((lane & 1) * 2 + (lane >> 1)) * L::kBytes, src, L::kBytes, bar);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < S; ++i) issue(i);
+
+  W w;
+  w.load_q(q + ((long long)b * c.Hkv + h) * G * D, G, c.softcap > 0.f ? c.scale : c.scale * kLog2e);
+  const int tok = (g & 1) * 4 + (g >> 1);
+  float* srow = scores != nullptr ? scores + (((long long)b * c.Hkv + h) * c.max_blocks * kTok + tok) * Gs : nullptr;
+
+  for (int i = 0; i < mine; ++i) {
+    const bool here = sm100::mbar_wait_bounded(&bars[warp][i % S], (i / S) & 1, kWaitLimit);
+    if (!__all_sync(0xffffffffu, here)) {  // wait, bounded, for the copies still under way, then stop
+      if (lane == 0) report(status, kTimeout);
+      for (int k = i + 1; k < min(mine, i + S); ++k)
+        sm100::mbar_wait_bounded(&bars[warp][k % S], (k / S) & 1, kWaitLimit);
+      break;
+    }
+    const uint8_t* ks = ring + (i % S) * kStage;
+    const int jb = jb0 + (i * kDecodeWarps + warp) * kPair, base = jb * kTok;
+    const unsigned ok = good >> (2 * (i & 15)) & 3u;
+    float* sc = srow != nullptr ? srow + (long long)base * Gs : nullptr;
+    if (ok == 3u && base >= t0 && base + kPair * kTok <= len) {
+      w.template turn<false>(ks, 0u, c.softcap, sc, Gs);
+    } else {
+      unsigned seen = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int x = base + (k >> 1) * kTok + tok + 8 * (k & 1);
+        seen |= (unsigned)((ok >> (k >> 1) & 1) && x >= t0 && x < len) << k;
+        seen |= (unsigned)(x < len && jb + (k >> 1) < jb1) << (4 + k);  // a place in `scores` that is this CTA's
+      }
+      w.template turn<true>(ks, seen, c.softcap, sc, Gs);
     }
     __syncwarp();  // every lane has read the stage
-    issue(i + kDecodeStages);
+    issue(i + S);
   }
 
   // the warps' sums, through shared memory (the ring is free once every warp is here)
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(smem);                    // [warps][HT][D]
   float* sm_ml = sm_o + kDecodeWarps * HT * D;                     // [warps][HT][2]
+  const float back = pow2(w.ve - 130);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float x = l[n][e];
+      float x = w.l[n][e];
 #pragma unroll
       for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
       const int head = n * 8 + 2 * t + e;
       if (g == 0) {
-        sm_ml[(warp * HT + head) * 2] = m[n][e];
+        sm_ml[(warp * HT + head) * 2] = w.m[n][e];
         sm_ml[(warp * HT + head) * 2 + 1] = x;
       }
 #pragma unroll
-      for (int r = 0; r < NG; ++r) {
-        float y = z[n][r][e];
+      for (int r = 0; r < W::NG; ++r) {
+        float y = w.z[n][r][e];
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
-        float* dst = sm_o + (warp * HT + head) * D + r * L::kGroup + g * MT * 2;
+        float* dst = sm_o + (warp * HT + head) * D + r * L::kGroup + g * W::MT * 2;
 #pragma unroll
-        for (int k = 0; k < MT; ++k) {
-          dst[2 * k] = o[n][r][k][e] + y;
-          dst[2 * k + 1] = o[n][r][k][e + 2] + y;
+        for (int k = 0; k < W::MT; ++k) {
+          dst[2 * k] = fmaf(w.o[n][r][k][e], back, y);
+          dst[2 * k + 1] = fmaf(w.o[n][r][k][e + 2], back, y);
         }
       }
     }
@@ -503,7 +606,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_
 #pragma unroll
     for (int w = 0; w < kDecodeWarps; ++w) {
       const float mw = sm_ml[(w * HT + head) * 2];
-      const float f = mw == -INFINITY ? 0.f : sm100::ex2_approx(mw - M);
+      const float f = mw == -INFINITY ? 1.f : sm100::ex2_approx(mw - M);  // (an empty warp's sums are 0, or NaN)
       sum += sm_ml[(w * HT + head) * 2 + 1] * f;
       acc += sm_o[(w * HT + head) * D + d] * f;
     }
@@ -749,7 +852,7 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
 template <int D, int NT>
 static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, int B, int splits, float* part, float* ml,
                                     float* scores, int Gs, int* status, cudaStream_t s) {
-  constexpr int ring = kDecodeWarps * kDecodeStages * 2 * Q4<D>::kBytes;
+  constexpr int ring = kDecodeWarps * q4_stages<D>() * kPair * 2 * Q4<D>::kBytes;
   constexpr int join = kDecodeWarps * NT * 8 * (D + 2) * 4;
   constexpr int smem = ring > join ? ring : join;
   static_assert(smem <= 47 * 1024, "above 48 KB a kernel has to ask for its shared memory");
@@ -759,9 +862,9 @@ static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, 
 }
 
 int rlb_q4_decode_splits(int B, int Hkv, int max_blocks, int sms) {
-  // Enough CTAs for several waves (ragged lengths leave a tail), but a block or two for each warp at least.
+  // Enough CTAs for several waves (ragged lengths leave a tail), but a pair of blocks for each warp.
   const long long rows = (long long)B * Hkv;
-  const long long want = (8LL * sms + rows - 1) / rows, most = (max_blocks + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
+  const long long want = (8LL * sms + rows - 1) / rows, most = (max_blocks + kPair * kDecodeWarps - 1) / (kPair * kDecodeWarps);
   const long long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n);
 }

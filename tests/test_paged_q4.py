@@ -75,7 +75,8 @@ def cache(lens, Hkv, D, dev, extra=0, spare=3):
 
 
 def attention(q, k, v, scale, softcap, window):
-    """fp64 output [Hq, D], weights [Hkv, n] summed over each group, and sum p |v|, of one sequence."""
+    """fp64 output [Hq, D], weights [Hkv, n] summed over each group, and what errors are measured by (check_decode),
+    of one sequence."""
     n, Hkv, D = k.shape
     if n == 0:
         z = torch.zeros(q.shape, dtype=F64)
@@ -86,16 +87,20 @@ def attention(q, k, v, scale, softcap, window):
     if window and n > window:
         s[..., :n - window] = -math.inf
     p = torch.softmax(s, -1)
-    o, a = (torch.einsum("hgt,thd->hgd", p, x).reshape(q.shape) for x in (v, v.abs()))
+    groups = v.unflatten(-1, (-1, min(D, 64)))
+    eight = (groups.amax(-1, keepdim=True) - groups.amin(-1, keepdim=True)).expand_as(groups).flatten(-2) * 8 / 15
+    o, a = (torch.einsum("hgt,thd->hgd", p, x).reshape(q.shape) for x in (v, v.abs() + 8 * eight))
     return o, p.sum(1), a
 
 
 # Decode's error: rounding the output to bf16 is 2^-8 of the value.  Before it, a weight's relative error is that of its
-# exponent (|s| below 2^5 here, held in fp32 with a few roundings: 2^5 * 2^-23 * 4 = 2^-16) plus 2^-16 for a
-# weight split into two bf16 parts, and the sums are fp32: together below 2^-14 of sum p |v|.
+# exponent (|s| below 2^5 here, held in fp32 with a few roundings: 2^5 * 2^-23 * 4 = 2^-16), and the sums are fp32:
+# together below 2^-14 of sum p |v|.  The kernel also rounds each p * scale to fp16, 2^-11 of it, which multiplies a
+# centred code (code - 8, at most 8): 2^-11 sum p 8 scale, with scale a 15th of the spread of the token's group (both
+# ends of which are stored values).  attention() returns sum p |v| + 2^3 sum p 8 scale.
 def check_decode(out, o, a):
     err = (out.cpu().to(F64) - o).abs()
-    assert (err <= 2 ** -8 * o.abs() + 2 ** -14 * a + 1e-30).all(), (err - 2 ** -8 * o.abs()).max()
+    assert (err <= 2 ** -8 * o.abs() + 2 ** -14 * a + 1e-30).all(), (err - 2 ** -8 * o.abs() - 2 ** -14 * a).max()
 
 
 # ---------------------------------------------------------------- storing and reading
