@@ -131,30 +131,36 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 }
 
 // ---------------------------------------------------------------- decode attention
-// One CTA takes a stretch of one (sequence, KV head); each of its warps takes every fourth pair of blocks of the stretch and
-// works alone: its lane 0 brings blocks (codes, scales and minima of K and V, one contiguous piece each) into the
+// The work is the pairs of blocks (32 tokens) of all (sequence, KV head) rows in a line, cut into equal stretches, one
+// for each CTA that fits on the GPU: lengths are ragged and known on the device only, and a grid of whole rows or
+// fixed parts leaves SMs idle at the end (a fifth of the time at 32 sequences of 2048 to 8192 tokens).  A CTA walks
+// the rows of its stretch; each of its warps takes every fourth pair of a row and
+// works alone: its lanes 0 to 3 bring blocks (codes, scales and minima of K and V, one contiguous piece each) into the
 // warp's own ring of shared memory with bulk copies, and the warp computes on matrix instructions
 // (mma.sync m16n8k16, bf16 x bf16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
 // query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
 // them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
 // memory) would need the unpacked values written back to shared memory first.
 //
-// Codes become fp16 numbers code - 8 exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are
-// 1024 + 16 code, so half of the nibbles need no shift, and one packed fma takes the offset (and the 16) away.
-// S^T = K Q^T.  With a token's scale s and minimum m:  k . q = s ((code - 8) . q) + (m + 8 s) sum(q), per group of
-// dimensions.  Q is fp16 after division by a power of two per head (its largest element then lies in [2^13, 2^14)):
-// bf16's 8 bits fit, and what falls below 2^-24 is 2^-38 of the largest.  The order of the dimensions inside the
+// Codes become fp16 numbers exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are 1024 + 16 code, so
+// half of the nibbles need no shift, and a packed add or fma makes code - 8 of them.
+// S^T = K Q^T.  With a token's scale s and minimum m:  k . q = s (code . q) + m sum(q), per group of dimensions.  Q
+// is fp16 after division by a power of two per head (its largest element then lies in [2^13, 2^14)): bf16's 8 bits
+// fit, and what falls below 2^-24 is 2^-38 of the largest.  K's odd nibbles stay 1024 + 16 code: their q are divided by 16,
+// and the sums start at 8 sum(q even) - 64 sum(q odd) instead of zero, which leaves code . q.  The order of the
+// dimensions inside the
 // product is free as long as Q's registers use the same: a lane reads 16 consecutive dimensions of a token as two
 // words and takes nibbles j and j + 4 of a word as one operand register.
 // O^T = V^T P^T.  The token's scale goes into the weight and its minimum into a separate fp32 sum of p (m + 8 s).
 // The weights p s are rounded to fp16 (2^-11 of each, an eighth of what the output's own rounding to bf16 may
-// add); to stay in range they are divided by a power of two at least an eighth of the largest scale so far, so p s <= 2^12.
+// add); to stay in range, p is kept times a power of two that takes the largest scale so far below 2^4: p s <= 2^12.
 // The tokens' order is free too: row g of S^T is token (g & 1) * 4 + g / 2 (of each half of the block), which after
 // the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's gives lane t of a quad the tokens t,
 // t + 4, t + 8, t + 12, and the four V words that it reads for them lie in different banks.
 //
 // Softmax statistics are fp32 in base 2.  The running maximum is only raised (and the sums rescaled) when a score
-// exceeds it by 8, so weights stay below 2^8 relative to it.  A warp takes two blocks per turn, which shares the
+// exceeds it by 8, so weights stay below 2^8 relative to it.  It is a whole number (rounded up), so that it and the
+// factors between the maxima of warps and CTAs are exact.  A warp takes two blocks per turn, which shares the
 // waits, votes and bookkeeping among 32 tokens.
 struct Q4Cache {
   const uint8_t *k_pool, *v_pool;
@@ -167,10 +173,11 @@ constexpr int kDecodeWarps = 4;
 constexpr int kPair = 2;                 // blocks a turn
 constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
 
-RLB_DEVICE void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+RLB_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2,
+                        float c3) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 RLB_DEVICE uint32_t transpose8x8(uint32_t x) {
@@ -185,18 +192,36 @@ RLB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
                : "memory");
 }
 
-// Nibbles j and j + 4 of a word (j = 0, 1, 2, 3) as two fp16 numbers code - 8.
-RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4]) {
+// Two nibbles of a word in one instruction: (w & mask) | 0x64006400.  (Written out because the compiler takes two
+// where both constants are immediates; `magic` comes from a register.)
+template <uint32_t MASK>
+RLB_DEVICE uint32_t nibbles(uint32_t w, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));
+  return r;
+}
+
+RLB_DEVICE uint32_t half2_add(uint32_t x, uint32_t both) {
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&both));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// Nibbles j and j + 4 of a word as two fp16 numbers: code - 8 for j = 0 and 2, for j = 1 and 3 code - 8 too (CENTRED)
+// or 1024 + 16 code.
+template <bool CENTRED>
+RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
   const uint32_t x = w >> 8;
-  const __half2 off0 = __half2half2(__ushort_as_half(0xe408)), off1 = __half2half2(__ushort_as_half(0xd480));  // -1032, -72
-  const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
-  const uint32_t v[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x64006400u,
-                         (x & 0x000f000fu) | 0x64006400u, (x & 0x00f000f0u) | 0x64006400u};
+  r[0] = half2_add(nibbles<0x000f000fu>(w, magic), 0xe408e408u);  // -1032
+  r[1] = nibbles<0x00f000f0u>(w, magic);
+  r[2] = half2_add(nibbles<0x000f000fu>(x, magic), 0xe408e408u);
+  r[3] = nibbles<0x00f000f0u>(x, magic);
+  if (CENTRED) {
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00)), off = __half2half2(__ushort_as_half(0xd480));  // -72
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&v[j]);
-    const __half2 y = j & 1 ? __hfma2(h, sixteenth, off1) : __hadd2(h, off0);
-    r[j] = *reinterpret_cast<const uint32_t*>(&y);
+    for (int j = 1; j < 4; j += 2) {
+      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&r[j]), sixteenth, off);
+      r[j] = *reinterpret_cast<const uint32_t*>(&y);
+    }
   }
 }
 
@@ -207,18 +232,76 @@ RLB_DEVICE uint32_t pack_f16(float lo, float hi) {
 
 RLB_DEVICE float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-// The tokens that split `sp` of `n` takes of [t0, len): whole blocks, equal shares of the sequence's own length.
-RLB_DEVICE void q4_range(int t0, int len, int sp, int n, int& b0, int& b1) {
-  const int first = t0 / kTok, total = len > t0 ? (len - 1) / kTok - first + 1 : 0;
-  const int per = (total + n - 1) / n;
-  b0 = first + min(total, sp * per);
-  b1 = first + min(total, (sp + 1) * per);
-}
-
 RLB_DEVICE int q4_len(const Q4Cache& c, int b, int* status) {
   const int len = c.lens[b], most = c.max_blocks * kTok;
   if (len > most) report(status, kBadIndex);
   return min(max(len, 0), most);
+}
+
+// First token that a sequence of `len` tokens attends to, and its pairs of blocks from there on.
+RLB_DEVICE int q4_first(const Q4Cache& c, int len) { return c.window > 0 && len > c.window ? len - c.window : 0; }
+RLB_DEVICE int q4_pairs(const Q4Cache& c, int len) {
+  if (len == 0) return 0;
+  const int blocks = (len - 1) / kTok - q4_first(c, len) / kTok + 1;
+  return (blocks + kPair - 1) / kPair;
+}
+
+// The pairs of all rows lie in a line: row (b, h) holds [base(b) + h n(b), + n(b)), and CTA k of C the stretch
+// [cut(k), cut(k + 1)).  A part (k, row) gets scratch slot k + row: along the line each next part raises one of the two.
+RLB_DEVICE long long q4_cut(long long k, long long total, int C) { return k * total / C; }
+RLB_DEVICE long long q4_owner(long long x, long long total, int C) { return ((x + 1) * C - 1) / total; }
+
+// Sums of the pairs before sequence `b` and in all, and the sequence that holds pair `x` (in units of Hkv: place
+// x / Hkv per head).  Every thread of the block calls it; scratch: 2 x 32 + 2 numbers.
+struct Q4Line {
+  long long total;  // pairs of all sequences, one KV head
+  long long base;   // pairs before sequence `seq`, one KV head
+  int seq;
+};
+// find >= 0: the sequence that holds pair `find` of the line (all heads); else the sequence `seq` is given.
+RLB_DEVICE Q4Line q4_line(const Q4Cache& c, int B, long long k, int C, int seq, int* status) {
+  __shared__ long long warp_sum_[8], warp_base_[8];
+  __shared__ Q4Line found;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (B + blockDim.x - 1) / blockDim.x;
+  const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += q4_pairs(c, q4_len(c, b, status));
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) warp_sum_[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) before += warp_sum_[w];
+    total += warp_sum_[w];
+  }
+  if (threadIdx.x == 0) found = Q4Line{total, total, B};
+  __syncthreads();
+  if (seq >= 0) {
+    if (b0 <= seq && seq < b1) {
+      for (int b = b0; b < seq; ++b) before += q4_pairs(c, q4_len(c, b, nullptr));
+      found = Q4Line{total, before, seq};
+    }
+  } else {
+    const long long x = q4_cut(k, total * c.Hkv, C);
+    if (before * c.Hkv <= x && x < (before + mine) * c.Hkv) {
+      for (int b = b0; b < b1; ++b) {
+        const int n = q4_pairs(c, q4_len(c, b, nullptr));
+        if (x < (before + n) * c.Hkv) {
+          found = Q4Line{total, before, b};
+          break;
+        }
+        before += n;
+      }
+    }
+  }
+  __syncthreads();
+  return found;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -229,10 +312,13 @@ struct Q4Warp {
   using L = Q4<D>;
   static constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16;
   uint32_t qb[NT][NG][WPL][4];                   // Q^T's registers (column n = head g of each tile)
-  float qs[NT][NG][2], qf[NT][2];                // heads 2t, 2t + 1: sums of q, and the factor of their scores
-  float m[NT][2], mref[NT][2], l[NT][2];         // running maximum, what exponents are taken against, sum
-  float z[NT][NG][2], o[NT][NG][MT][4], vn;      // sums of p (m + 8 s), of p s (code - 8) times vn = 2^(130 - ve)
-  int ve;                                        // exponent field of the largest scale of V so far
+  float qs[NT][NG][2], qc[NT][NG][2], qf[NT][2]; // heads 2t, 2t + 1: sums of q, where S starts, the scores' factor
+  float m[NT][2], mref[NT][2], l[NT][2];         // what a score may reach (8 above the maximum when that was last
+                                                 // raised), what exponents are taken against, sum of p
+  float z[NT][NG][2], o[NT][NG][MT][4];          // sums of p (m + 8 s) and of p s (code - 8)
+  int ve;                                        // exponent field of the largest scale of V so far: p is kept times
+                                                 // 2^(130 - ve), and so are the sums
+  uint32_t magic;                                // 0x64006400
 
   RLB_DEVICE void load_q(const __nv_bfloat16* q, int G, float scale) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -259,25 +345,32 @@ struct Q4Warp {
       float factor = scale * pow2(-e);
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
-        float sum = 0.f;
+        float sum = 0.f, odd = 0.f;
 #pragma unroll
         for (int w = 0; w < WPL; ++w)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float x = f[r][w][j] * up, y = f[r][w][j + 4] * up;
-            qb[n][r][w][j] = pack_f16(x, y);
+            const float x = f[r][w][j] * up, y = f[r][w][j + 4] * up, part = j & 1 ? 0.0625f : 1.f;
+            qb[n][r][w][j] = pack_f16(x * part, y * part);
             sum += x + y;
+            if (j & 1) odd += x + y;
           }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qs[n][r][0] = __shfl_sync(0xffffffffu, sum, t * 8);
-        qs[n][r][1] = __shfl_sync(0xffffffffu, sum, t * 8 + 4);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          odd += __shfl_xor_sync(0xffffffffu, odd, o);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          qs[n][r][e] = __shfl_sync(0xffffffffu, sum, t * 8 + 4 * e);
+          qc[n][r][e] = 8.f * qs[n][r][e] - 72.f * __shfl_sync(0xffffffffu, odd, t * 8 + 4 * e);
+        }
       }
       qf[n][0] = __shfl_sync(0xffffffffu, factor, t * 8);
       qf[n][1] = __shfl_sync(0xffffffffu, factor, t * 8 + 4);
     }
-    vn = pow2(126);
-    ve = 4;
+    ve = 70;  // (p is then at most 2^8 2^60)
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));  // kept in a register
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -305,8 +398,6 @@ struct Q4Warp {
       for (int r = 0; r < NG; ++r) {
         const uint8_t* blk = ks + k * 2 * L::kBytes;
         float acc[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         uint32_t u0[WPL], u1[WPL];
         const uint8_t* row = blk + (r * kTok + tok) * L::kRow + t * WPL * 4;
         if constexpr (WPL == 2) {
@@ -319,26 +410,30 @@ struct Q4Warp {
 #pragma unroll
         for (int w = 0; w < WPL; ++w) {
           uint32_t c0[4], c1[4];
-          codes_f16(u0[w], c0);
-          codes_f16(u1[w], c1);
+          codes_f16<false>(u0[w], c0, magic);
+          codes_f16<false>(u1[w], c1, magic);
 #pragma unroll
           for (int j = 0; j < 4; j += 2) {
             const uint32_t a[4] = {c0[j], c1[j], c0[j + 1], c1[j + 1]};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(acc[n], a, qb[n][r][w][j], qb[n][r][w][j + 1]);
+            for (int n = 0; n < NT; ++n) {
+              const bool first = w == 0 && j == 0;
+              mma_f16(acc[n], a, qb[n][r][w][j], qb[n][r][w][j + 1], first ? qc[n][r][0] : acc[n][0],
+                      first ? qc[n][r][1] : acc[n][1], first ? qc[n][r][0] : acc[n][2], first ? qc[n][r][1] : acc[n][3]);
+            }
           }
         }
         const uint32_t me0 = *reinterpret_cast<const uint32_t*>(blk + L::kCodes + (r * kTok + tok) * 4);
         const uint32_t me1 = *reinterpret_cast<const uint32_t*>(blk + L::kCodes + (r * kTok + tok + 8) * 4);
-        const float s0 = bf16_lo_f(me0), s1 = bf16_lo_f(me1);
-        const float z0 = fmaf(8.f, s0, bf16_hi_f(me0)), z1 = fmaf(8.f, s1, bf16_hi_f(me1));
+        const float s0 = bf16_lo_f(me0), s1 = bf16_lo_f(me1), z0 = bf16_hi_f(me0), z1 = bf16_hi_f(me1);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float x = fmaf(s0, acc[n][e], z0 * qs[n][r][e]), y = fmaf(s1, acc[n][e + 2], z1 * qs[n][r][e]);
-            s[n][k][e] = r == 0 ? x : s[n][k][e] + x;
-            s[n][k][e + 2] = r == 0 ? y : s[n][k][e + 2] + y;
+            const float x = r == 0 ? z0 * qs[n][r][e] : fmaf(z0, qs[n][r][e], s[n][k][e]);
+            const float y = r == 0 ? z1 * qs[n][r][e] : fmaf(z1, qs[n][r][e], s[n][k][e + 2]);
+            s[n][k][e] = fmaf(s0, acc[n][e], x);
+            s[n][k][e + 2] = fmaf(s1, acc[n][e + 2], y);
           }
       }
 #pragma unroll
@@ -366,7 +461,7 @@ struct Q4Warp {
           if (MASKED && !((seen >> (2 * k + (e >> 1))) & 1)) s[n][k][e] = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        raise |= fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2])) > m[n][e] + 8.f;
+        raise |= fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2])) > m[n][e];
       if (scores != nullptr && n * 8 + 2 * t < Gs) {
 #pragma unroll
         for (int k = 0; k < kPair; ++k)
@@ -396,7 +491,6 @@ struct Q4Warp {
       e_all = min(max(e_all, ve), 252);
       const float fv = pow2(max(ve - e_all, -126));
       ve = e_all;
-      vn = pow2(130 - ve);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -404,18 +498,19 @@ struct Q4Warp {
           float x = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
-          x = fmaxf(x, m[n][e]);
-          const float f = m[n][e] == -INFINITY ? 0.f : sm100::ex2_approx(m[n][e] - x);
-          m[n][e] = x;
-          mref[n][e] = x == -INFINITY ? 0.f : x;
+          const float was = m[n][e] - 8.f;
+          x = fmaxf(ceilf(x), was);
+          const float f = (was == -INFINITY ? 0.f : sm100::ex2_approx(was - x)) * fv;
+          m[n][e] = x + 8.f;
+          mref[n][e] = (x == -INFINITY ? 0.f : x) - (float)(130 - ve);
           l[n][e] *= f;
 #pragma unroll
           for (int r = 0; r < NG; ++r) {
             z[n][r][e] *= f;
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
-              o[n][r][k][e] *= f * fv;
-              o[n][r][k][e + 2] *= f * fv;
+              o[n][r][k][e] *= f;
+              o[n][r][k][e + 2] *= f;
             }
           }
         }
@@ -436,12 +531,11 @@ struct Q4Warp {
         const uint8_t* blk = ks + (2 * k + 1) * L::kBytes;
         const float s0 = bf16_lo_f(vm[k][r][0]), s1 = bf16_lo_f(vm[k][r][1]);
         const float z0 = fmaf(8.f, s0, bf16_hi_f(vm[k][r][0])), z1 = fmaf(8.f, s1, bf16_hi_f(vm[k][r][1]));
-        const float w0 = s0 * vn, w1 = s1 * vn;
         uint32_t b[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          b[n][0] = transpose8x8(pack_f16(s[n][k][0] * w0, s[n][k][1] * w0));
-          b[n][1] = transpose8x8(pack_f16(s[n][k][2] * w1, s[n][k][3] * w1));
+          b[n][0] = transpose8x8(pack_f16(s[n][k][0] * s0, s[n][k][1] * s0));
+          b[n][1] = transpose8x8(pack_f16(s[n][k][2] * s1, s[n][k][3] * s1));
           z[n][r][0] = fmaf(s[n][k][0], z0, fmaf(s[n][k][2], z1, z[n][r][0]));
           z[n][r][1] = fmaf(s[n][k][1], z0, fmaf(s[n][k][3], z1, z[n][r][1]));
         }
@@ -453,12 +547,12 @@ struct Q4Warp {
           if constexpr (WPL == 2) {
             const uint32_t x = *reinterpret_cast<const uint32_t*>(row);
             const uint32_t y = *reinterpret_cast<const uint32_t*>(row + 4 * L::kRow);
-            codes_f16(__byte_perm(x, y, 0x5410), c[i][0]);
-            codes_f16(__byte_perm(x, y, 0x7632), c[i][1]);
+            codes_f16<true>(__byte_perm(x, y, 0x5410), c[i][0], magic);
+            codes_f16<true>(__byte_perm(x, y, 0x7632), c[i][1], magic);
           } else {
-            codes_f16(*reinterpret_cast<const uint16_t*>(row) |
+            codes_f16<true>(*reinterpret_cast<const uint16_t*>(row) |
                           ((uint32_t)*reinterpret_cast<const uint16_t*>(row + 4 * L::kRow) << 16),
-                      c[i][0]);
+                            c[i][0], magic);
           }
         }
 #pragma unroll
@@ -466,21 +560,22 @@ struct Q4Warp {
           const int w = i >> 1, j = 2 * (i & 1);
           const uint32_t a[4] = {c[0][w][j], c[0][w][j + 1], c[1][w][j], c[1][w][j + 1]};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(o[n][r][i], a, b[n][0], b[n][1]);
+          for (int n = 0; n < NT; ++n)
+            mma_f16(o[n][r][i], a, b[n][0], b[n][1], o[n][r][i][0], o[n][r][i][1], o[n][r][i][2], o[n][r][i][3]);
         }
       }
   }
 };
 
-// NT: tiles of 8 query heads.  `part` [B][Hq][splits][D] and `ml` [B][Hq][splits][2] receive unnormalised outputs and
-// statistics; with one split and no `scores` the output is written instead.  `scores` [B][Hkv][tokens][Gs] receives
-// the base-2 scores for q4_finish_kernel.
 template <int D>
 constexpr int q4_stages() { return D == 128 ? 2 : 4; }  // pairs of blocks in a warp's ring
 
+// NT: tiles of 8 query heads.  Rows that lie in one CTA's stretch are finished here, the others' parts go to `part`
+// [slots][G][D] (unnormalised outputs) and `ml` [slots][G][2] (statistics).  `scores` [B][Hkv][tokens][Gs] receives the
+// base-2 scores for q4_finish_kernel, which then needs every row's statistics.
 template <int D, int NT>
-__global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_kernel(
-    const __nv_bfloat16* __restrict__ q, Q4Cache c, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
+__global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_kernel(
+    const __nv_bfloat16* __restrict__ q, Q4Cache c, int B, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
     float* __restrict__ ml, float* __restrict__ scores, int Gs, int* status) {
   using L = Q4<D>;
   using W = Q4Warp<D, NT>;
@@ -488,146 +583,162 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 4 : 2) q4_decode_
   constexpr int kStage = kPair * 2 * L::kBytes;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kDecodeWarps][S];
-  const int h = blockIdx.x, b = blockIdx.y, sp = blockIdx.z, splits = gridDim.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = c.G;
-  const int len = q4_len(c, b, status);
-  const int t0 = c.window > 0 && len > c.window ? len - c.window : 0;
-  int jb0, jb1;
-  q4_range(t0, len, sp, splits, jb0, jb1);
-  const int pairs = (jb1 - jb0 + kPair - 1) / kPair;
-  const int mine = pairs > warp ? (pairs - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's turns
   uint8_t* ring = smem + warp * S * kStage;
-  const int* table = c.tables + (long long)b * c.max_blocks;
-
   if (lane == 0) {
     for (int s = 0; s < S; ++s) sm100::mbar_init(&bars[warp][s], 1);
     sm100::fence_barrier_init();
     sm100::fence_async_shared();
   }
-  __syncwarp();
+  const Q4Line line = q4_line(c, B, blockIdx.x, gridDim.x, -1, blockIdx.x == 0 ? status : nullptr);
+  const long long total = line.total * c.Hkv;
+  long long x = q4_cut(blockIdx.x, total, gridDim.x);
+  const long long x_end = q4_cut(blockIdx.x + 1, total, gridDim.x);
+  long long base = line.base * c.Hkv;
+  int used = 0;  // turns of this warp so far: the ring goes on from row to row
+  bool alive = true;
 
-  int id = 0;         // lanes 2i and 2i + 1: the blocks of turn i of the current sixteen
-  uint32_t good = 0;  // bits 2 (i % 16), + 1: blocks of turn i that are there
-  auto issue = [&](int i) {
-    if (i >= mine) return;
-    if ((i & 15) == 0) {
-      const int at = jb0 + ((i + (lane >> 1)) * kDecodeWarps + warp) * kPair + (lane & 1);
-      id = at < jb1 ? table[at] : -1;
-      const bool ok = id >= 0 && id < c.num_blocks;
-      if (!ok && at < jb1) report(status, kBadIndex);
-      if (!ok) id = -1;
+  for (int b = line.seq; x < x_end;) {
+    const int len = q4_len(c, b, nullptr), n = q4_pairs(c, len);
+    if (x >= base + (long long)n * c.Hkv) {  // sequences without tokens hold nothing
+      base += (long long)n * c.Hkv;
+      ++b;
+      continue;
     }
-    const int shift = 2 * (i & 15);
-    const unsigned ok = __ballot_sync(0xffffffffu, id >= 0) >> shift & 3u;
-    good = (good & ~(3u << shift)) | (ok << shift);
-    const int blk = __shfl_sync(0xffffffffu, id, shift + (lane & 1));
-    uint64_t* bar = &bars[warp][i % S];
-    if (lane == 0) sm100::mbar_arrive_expect_tx(bar, __popc(ok) * 2 * L::kBytes);
-    __syncwarp();
-    if (lane < 4 && blk >= 0) {  // lane: block lane & 1, K (lanes 0, 1) or V (2, 3)
-      const uint8_t* src = (lane < 2 ? c.k_pool : c.v_pool) + ((long long)blk * c.Hkv + h) * L::kBytes;
-      bulk_load(ring + (i % S) * kStage + ((lane & 1) * 2 + (lane >> 1)) * L::kBytes, src, L::kBytes, bar);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < S; ++i) issue(i);
+    const int h = (int)((x - base) / n), p0 = (int)((x - base) % n);
+    const int p1 = (int)min((long long)n, p0 + (x_end - x));
+    x += p1 - p0;
+    const int t0 = q4_first(c, len), jb0 = t0 / kTok + p0 * kPair;
+    const int jb1 = min((len - 1) / kTok + 1, t0 / kTok + p1 * kPair);  // this part's blocks
+    const int mine = p1 - p0 > warp ? (p1 - p0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's turns
+    const int* table = c.tables + (long long)b * c.max_blocks;
 
-  W w;
-  w.load_q(q + ((long long)b * c.Hkv + h) * G * D, G, c.softcap > 0.f ? c.scale : c.scale * kLog2e);
-  const int tok = (g & 1) * 4 + (g >> 1);
-  float* srow = scores != nullptr ? scores + (((long long)b * c.Hkv + h) * c.max_blocks * kTok + tok) * Gs : nullptr;
-
-  for (int i = 0; i < mine; ++i) {
-    const bool here = sm100::mbar_wait_bounded(&bars[warp][i % S], (i / S) & 1, kWaitLimit);
-    if (!__all_sync(0xffffffffu, here)) {  // wait, bounded, for the copies still under way, then stop
-      if (lane == 0) report(status, kTimeout);
-      for (int k = i + 1; k < min(mine, i + S); ++k)
-        sm100::mbar_wait_bounded(&bars[warp][k % S], (k / S) & 1, kWaitLimit);
-      break;
-    }
-    const uint8_t* ks = ring + (i % S) * kStage;
-    const int jb = jb0 + (i * kDecodeWarps + warp) * kPair, base = jb * kTok;
-    const unsigned ok = good >> (2 * (i & 15)) & 3u;
-    float* sc = srow != nullptr ? srow + (long long)base * Gs : nullptr;
-    if (ok == 3u && base >= t0 && base + kPair * kTok <= len) {
-      w.template turn<false>(ks, 0u, c.softcap, sc, Gs);
-    } else {
-      unsigned seen = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int x = base + (k >> 1) * kTok + tok + 8 * (k & 1);
-        seen |= (unsigned)((ok >> (k >> 1) & 1) && x >= t0 && x < len) << k;
-        seen |= (unsigned)(x < len && jb + (k >> 1) < jb1) << (4 + k);  // a place in `scores` that is this CTA's
+    int id = 0;         // lanes 2i and 2i + 1: the blocks of turn i of the current sixteen
+    uint32_t good = 0;  // bits 2 (i % 16), + 1: blocks of turn i that are there
+    auto issue = [&](int i) {
+      if (i >= mine) return;
+      if ((i & 15) == 0) {
+        const int at = jb0 + ((i + (lane >> 1)) * kDecodeWarps + warp) * kPair + (lane & 1);
+        id = at < jb1 ? table[at] : -1;
+        const bool ok = id >= 0 && id < c.num_blocks;
+        if (!ok && at < jb1) report(status, kBadIndex);
+        if (!ok) id = -1;
       }
-      w.template turn<true>(ks, seen, c.softcap, sc, Gs);
-    }
-    __syncwarp();  // every lane has read the stage
-    issue(i + S);
-  }
-
-  // the warps' sums, through shared memory (the ring is free once every warp is here)
-  __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(smem);                    // [warps][HT][D]
-  float* sm_ml = sm_o + kDecodeWarps * HT * D;                     // [warps][HT][2]
-  const float back = pow2(w.ve - 130);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float x = w.l[n][e];
-#pragma unroll
-      for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-      const int head = n * 8 + 2 * t + e;
-      if (g == 0) {
-        sm_ml[(warp * HT + head) * 2] = w.m[n][e];
-        sm_ml[(warp * HT + head) * 2 + 1] = x;
+      const int shift = 2 * (i & 15), stage = (used + i) % S;
+      const unsigned ok = __ballot_sync(0xffffffffu, id >= 0) >> shift & 3u;
+      good = (good & ~(3u << shift)) | (ok << shift);
+      const int blk = __shfl_sync(0xffffffffu, id, shift + (lane & 1));
+      uint64_t* bar = &bars[warp][stage];
+      if (lane == 0) sm100::mbar_arrive_expect_tx(bar, __popc(ok) * 2 * L::kBytes);
+      __syncwarp();
+      if (lane < 4 && blk >= 0) {  // lane: block lane & 1, K (lanes 0, 1) or V (2, 3)
+        const uint8_t* src = (lane < 2 ? c.k_pool : c.v_pool) + ((long long)blk * c.Hkv + h) * L::kBytes;
+        bulk_load(ring + stage * kStage + ((lane & 1) * 2 + (lane >> 1)) * L::kBytes, src, L::kBytes, bar);
       }
+    };
 #pragma unroll
-      for (int r = 0; r < W::NG; ++r) {
-        float y = w.z[n][r][e];
+    for (int i = 0; i < S; ++i) issue(i);
+
+    W w;
+    w.load_q(q + ((long long)b * c.Hkv + h) * G * D, G, c.softcap > 0.f ? c.scale : c.scale * kLog2e);
+    const int tok = (g & 1) * 4 + (g >> 1);
+    float* srow = scores != nullptr ? scores + (((long long)b * c.Hkv + h) * c.max_blocks * kTok + tok) * Gs : nullptr;
+
+    for (int i = 0; i < mine; ++i) {
+      const int turn = used + i, stage = turn % S;
+      const bool here = sm100::mbar_wait_bounded(&bars[warp][stage], (turn / S) & 1, kWaitLimit);
+      if (!__all_sync(0xffffffffu, here)) {  // wait, bounded, for the copies still under way, then stop
+        if (lane == 0) report(status, kTimeout);
+        for (int k = i + 1; k < min(mine, i + S); ++k)
+          sm100::mbar_wait_bounded(&bars[warp][(used + k) % S], ((used + k) / S) & 1, kWaitLimit);
+        alive = false;
+        break;
+      }
+      const uint8_t* ks = ring + stage * kStage;
+      const int jb = jb0 + (i * kDecodeWarps + warp) * kPair, at = jb * kTok;
+      const unsigned ok = good >> (2 * (i & 15)) & 3u;
+      float* sc = srow != nullptr ? srow + (long long)at * Gs : nullptr;
+      if (ok == 3u && at >= t0 && at + kPair * kTok <= len) {
+        w.template turn<false>(ks, 0u, c.softcap, sc, Gs);
+      } else {
+        unsigned seen = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int y = at + (k >> 1) * kTok + tok + 8 * (k & 1);
+          seen |= (unsigned)((ok >> (k >> 1) & 1) && y >= t0 && y < len) << k;
+          seen |= (unsigned)(y < len && jb + (k >> 1) < jb1) << (4 + k);  // a place in `scores` that is this CTA's
+        }
+        w.template turn<true>(ks, seen, c.softcap, sc, Gs);
+      }
+      __syncwarp();  // every lane has read the stage
+      issue(i + S);
+    }
+    used += mine;
+
+    // the warps' sums, through shared memory (the ring is free once every warp is here)
+    if (!__syncthreads_and(alive)) return;
+    float* sm_o = reinterpret_cast<float*>(smem);                    // [warps][HT][D]
+    float* sm_ml = sm_o + kDecodeWarps * HT * D;                     // [warps][HT][2]
+    const float back = pow2(w.ve - 130);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float y = w.l[n][e] * back;
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
-        float* dst = sm_o + (warp * HT + head) * D + r * L::kGroup + g * W::MT * 2;
+        const int head = n * 8 + 2 * t + e;
+        if (g == 0) {
+          sm_ml[(warp * HT + head) * 2] = w.m[n][e] - 8.f;
+          sm_ml[(warp * HT + head) * 2 + 1] = y;
+        }
 #pragma unroll
-        for (int k = 0; k < W::MT; ++k) {
-          dst[2 * k] = fmaf(w.o[n][r][k][e], back, y);
-          dst[2 * k + 1] = fmaf(w.o[n][r][k][e + 2], back, y);
+        for (int r = 0; r < W::NG; ++r) {
+          float y = w.z[n][r][e] * back;
+#pragma unroll
+          for (int k = 4; k < 32; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
+          float* dst = sm_o + (warp * HT + head) * D + r * L::kGroup + g * W::MT * 2;
+#pragma unroll
+          for (int k = 0; k < W::MT; ++k) {
+            dst[2 * k] = fmaf(w.o[n][r][k][e], back, y);
+            dst[2 * k + 1] = fmaf(w.o[n][r][k][e + 2], back, y);
+          }
         }
       }
-    }
-  __syncthreads();
-  const bool whole = splits == 1 && scores == nullptr;
-  for (int x = threadIdx.x; x < G * D; x += kDecodeWarps * 32) {
-    const int head = x / D, d = x % D;
-    float M = -INFINITY, sum = 0.f, acc = 0.f;
+    __syncthreads();
+    const long long row = (long long)b * c.Hkv + h, slot = blockIdx.x + row;
+    const bool whole = p0 == 0 && p1 == n;
+    for (int y = threadIdx.x; y < G * D; y += kDecodeWarps * 32) {
+      const int head = y / D, d = y % D;
+      float M = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) M = fmaxf(M, sm_ml[(w * HT + head) * 2]);
+      for (int w = 0; w < kDecodeWarps; ++w) M = fmaxf(M, sm_ml[(w * HT + head) * 2]);
 #pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) {
-      const float mw = sm_ml[(w * HT + head) * 2];
-      const float f = mw == -INFINITY ? 1.f : sm100::ex2_approx(mw - M);  // (an empty warp's sums are 0, or NaN)
-      sum += sm_ml[(w * HT + head) * 2 + 1] * f;
-      acc += sm_o[(w * HT + head) * D + d] * f;
-    }
-    const long long row = ((long long)b * c.Hkv + h) * G + head;
-    if (whole) {
-      out[row * D + d] = __float2bfloat16(sum != 0.f ? acc / sum : 0.f);
-    } else {
-      part[(row * splits + sp) * D + d] = acc;
-      if (d == 0) {
-        ml[(row * splits + sp) * 2] = M;
-        ml[(row * splits + sp) * 2 + 1] = sum;
+      for (int w = 0; w < kDecodeWarps; ++w) {
+        const float mw = sm_ml[(w * HT + head) * 2];
+        const float f = mw == -INFINITY ? 1.f : sm100::ex2_approx(mw - M);  // (an empty warp's sums are 0, or NaN)
+        sum += sm_ml[(w * HT + head) * 2 + 1] * f;
+        acc += sm_o[(w * HT + head) * D + d] * f;
+      }
+      if (whole) out[(row * G + head) * D + d] = __float2bfloat16(sum != 0.f ? acc / sum : 0.f);
+      else part[(slot * G + head) * D + d] = acc;
+      if (d == 0 && (!whole || scores != nullptr)) {
+        ml[(slot * G + head) * 2] = M;
+        ml[(slot * G + head) * 2 + 1] = sum;
       }
     }
+    sm100::fence_async_shared();  // the next row's copies come after these reads and writes
+    __syncthreads();
   }
 }
 
-// Joins the splits of one (sequence, KV head): CTA 0 of its `gridDim.z` writes the outputs, and with `weights` each
-// adds a stretch of the tokens' attention weights, summed over the heads, to their accumulators.
+// Joins the parts of the rows that several CTAs of q4_decode_kernel (C in all) shared and clears those of empty
+// sequences: CTA 0 of a row's `gridDim.z` writes the outputs, and with `weights` each adds a stretch of the tokens'
+// attention weights, summed over the heads, to their accumulators.
 template <int D>
-__global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
-                                                        const float* __restrict__ ml, int splits,
+__global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, int B, int C, const float* __restrict__ part,
+                                                        const float* __restrict__ ml,
                                                         __nv_bfloat16* __restrict__ out,
                                                         const float* __restrict__ scores, int Gs,
                                                         float* __restrict__ weights,
@@ -635,14 +746,28 @@ __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* 
                                                         int w_len, int* status) {
   __shared__ float sm_m[16], sm_r[16];  // each head's maximum and 1 / sum
   const int h = blockIdx.x, b = blockIdx.y, G = c.G;
-  const long long row0 = ((long long)b * c.Hkv + h) * G;
+  const Q4Line line = q4_line(c, B, 0, C, b, nullptr);
+  const long long row = (long long)b * c.Hkv + h, total = line.total * c.Hkv;
+  const int len = q4_len(c, b, nullptr), n = q4_pairs(c, len);
+  if (n == 0) {
+    for (int x = threadIdx.x; x < G * D; x += 256) out[row * G * D + x] = __float2bfloat16(0.f);
+    return;
+  }
+  const long long start = line.base * c.Hkv + (long long)h * n;
+  const long long first = q4_owner(start, total, C), last = q4_owner(start + n - 1, total, C);
+  if (first == last && weights == nullptr) return;
+  const long long slot = first + row;
+  const int parts = (int)(last - first) + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int head = warp; head < G; head += 8) {
-    const float* p = ml + (row0 + head) * splits * 2;
+    const float* p = ml + (slot * G + head) * 2;
     float M = -INFINITY, sum = 0.f;
-    for (int s = lane; s < splits; s += 32) M = fmaxf(M, p[2 * s]);
+    for (int s = lane; s < parts; s += 32) M = fmaxf(M, p[2LL * s * G]);
     M = warp_max(M);
-    for (int s = lane; s < splits; s += 32) sum += p[2 * s] == -INFINITY ? p[2 * s + 1] : p[2 * s + 1] * sm100::ex2_approx(p[2 * s] - M);
+    for (int s = lane; s < parts; s += 32) {
+      const float ms = p[2LL * s * G], ls = p[2LL * s * G + 1];
+      sum += ms == -INFINITY ? ls : ls * sm100::ex2_approx(ms - M);
+    }
     sum = warp_sum(sum);
     if (lane == 0) {
       sm_m[head] = M;
@@ -650,24 +775,27 @@ __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* 
     }
   }
   __syncthreads();
-  if (blockIdx.z == 0)
+  if (blockIdx.z == 0 && parts > 1)
     for (int x = threadIdx.x; x < G * D; x += 256) {
-      const int head = x / D, d = x % D;
-      const float* p = ml + (row0 + head) * splits * 2;
-      const float* a = part + (row0 + head) * splits * D + d;
+      const int head = x / D;
+      const float* p = ml + (slot * G + head) * 2;
+      const float* a = part + slot * G * D + x;
       float acc = 0.f;
-      for (int s = 0; s < splits; ++s)
-        acc += p[2 * s] == -INFINITY ? a[(long long)s * D] : a[(long long)s * D] * sm100::ex2_approx(p[2 * s] - sm_m[head]);
-      out[(row0 + head) * D + d] = __float2bfloat16(acc * sm_r[head]);
+#pragma unroll 4
+      for (int s = 0; s < parts; ++s) {
+        const float ms = p[2LL * s * G];
+        acc += ms == -INFINITY ? a[(long long)s * G * D] : a[(long long)s * G * D] * sm100::ex2_approx(ms - sm_m[head]);
+      }
+      out[row * G * D + x] = __float2bfloat16(acc * sm_r[head]);
     }
   if (weights == nullptr) return;
-  const int r = weight_rows[b], len = min(max(c.lens[b], 0), c.max_blocks * kTok);
-  if (len == 0 || r < 0) return;
+  const int r = weight_rows[b];
+  if (r < 0) return;
   if (threadIdx.x == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
   if (r >= w_rows) return;
-  const int t0 = c.window > 0 && len > c.window ? len - c.window : 0;
+  const int t0 = q4_first(c, len);
   float* w = weights + ((long long)r * c.Hkv + h) * w_len;
-  const float* sc = scores + ((long long)b * c.Hkv + h) * c.max_blocks * kTok * Gs;
+  const float* sc = scores + row * c.max_blocks * kTok * Gs;
   for (int t = t0 + blockIdx.z * 256 + threadIdx.x; t < min(len, w_len); t += gridDim.z * 256) {
     float p = 0.f;
     for (int head = 0; head < G; ++head) p += sm100::ex2_approx(sc[(long long)t * Gs + head] - sm_m[head]) * sm_r[head];
@@ -850,44 +978,44 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
 }
 
 template <int D, int NT>
-static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, int B, int splits, float* part, float* ml,
+static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, int B, int C, float* part, float* ml,
                                     float* scores, int Gs, int* status, cudaStream_t s) {
   constexpr int ring = kDecodeWarps * q4_stages<D>() * kPair * 2 * Q4<D>::kBytes;
   constexpr int join = kDecodeWarps * NT * 8 * (D + 2) * 4;
   constexpr int smem = ring > join ? ring : join;
   static_assert(smem <= 47 * 1024, "above 48 KB a kernel has to ask for its shared memory");
-  q4_decode_kernel<D, NT><<<dim3(c.Hkv, B, splits), kDecodeWarps * 32, smem, s>>>(
-      (const __nv_bfloat16*)q, c, (__nv_bfloat16*)out, part, ml, scores, Gs, status);
+  q4_decode_kernel<D, NT><<<C, kDecodeWarps * 32, smem, s>>>((const __nv_bfloat16*)q, c, B, (__nv_bfloat16*)out, part,
+                                                              ml, scores, Gs, status);
   return cudaGetLastError();
 }
 
-int rlb_q4_decode_splits(int B, int Hkv, int max_blocks, int sms) {
-  // Enough CTAs for several waves (ragged lengths leave a tail), but a pair of blocks for each warp.
-  const long long rows = (long long)B * Hkv;
-  const long long want = (8LL * sms + rows - 1) / rows, most = (max_blocks + kPair * kDecodeWarps - 1) / (kPair * kDecodeWarps);
-  const long long n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n);
+int rlb_q4_decode_ctas(int B, int Hkv, int G, int max_blocks, int sms) {
+  // As many CTAs as fit at a time, but a pair of blocks for each warp if the tables are full.
+  const long long fit = (long long)sms * (G <= 8 ? 3 : 2);
+  const long long pairs = (long long)B * Hkv * ((max_blocks + kPair - 1) / kPair);
+  const long long want = (pairs + kDecodeWarps - 1) / kDecodeWarps;
+  return (int)(want < 1 ? 1 : want < fit ? want : fit);
 }
 
 cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool, const int* tables, const int* lens,
                           void* out, int B, int Hkv, int G, int D, int max_blocks, int num_blocks, float scale,
-                          float softcap, int window, int splits, float* part, float* ml, float* scores, float* weights,
+                          float softcap, int window, int ctas, float* part, float* ml, float* scores, float* weights,
                           const int* weight_rows, long long w_rows, int w_len, int sms, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
   const Q4Cache c{(const uint8_t*)k_pool, (const uint8_t*)v_pool, tables, lens, Hkv, G, max_blocks, num_blocks,
                   window, scale, softcap};
   const int Gs = (G + 1) & ~1;
   cudaError_t e = cudaSuccess;
-  RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, splits, part, ml, scores, Gs, status, s))
-                      : (q4_decode_launch<DD, 2>(q, c, out, B, splits, part, ml, scores, Gs, status, s)));
-  if (e != cudaSuccess || (splits == 1 && weights == nullptr)) return e;
-  int chunks = 1;  // CTAs per (sequence, KV head) that add weights: four waves of the GPU, 256 tokens each at least
+  RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, ctas, part, ml, scores, Gs, status, s))
+                      : (q4_decode_launch<DD, 2>(q, c, out, B, ctas, part, ml, scores, Gs, status, s)));
+  if (e != cudaSuccess) return e;
+  int chunks = 1;  // CTAs per row that add weights: four waves of the GPU, 256 tokens each at least
   if (weights != nullptr) {
     const long long rows = (long long)B * Hkv, want = (16LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 255) / 256;
     chunks = (int)(want < most ? want : most);
     if (chunks < 1) chunks = 1;
   }
-  RLB_Q4_D((q4_finish_kernel<DD><<<dim3(Hkv, B, chunks), 256, 0, s>>>(c, part, ml, splits, (__nv_bfloat16*)out, scores,
+  RLB_Q4_D((q4_finish_kernel<DD><<<dim3(Hkv, B, chunks), 256, 0, s>>>(c, B, ctas, part, ml, (__nv_bfloat16*)out, scores,
                                                                        Gs, weights, weight_rows, w_rows, w_len, status)));
   return cudaGetLastError();
 }
