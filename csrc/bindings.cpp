@@ -874,18 +874,14 @@ at::Tensor q4_decode(const at::Tensor& q, const at::Tensor& k_pool, const at::Te
                             ? q : q.clone(at::MemoryFormat::Contiguous);
   auto out = at::empty({B, Hq, D}, q.options());
   const int max_blocks = (int)tables.size(1);
-  const int64_t ctas = rlb_q4_decode_ctas((int)B, (int)Hkv, (int)(Hq / Hkv), max_blocks, sm_count());
+  const int G = (int)(Hq / Hkv), ctas = rlb_q4_decode_ctas((int)B, (int)Hkv, G, (int)D, max_blocks, sm_count());
   const bool weighted = weights.has_value();
-  // scratch: scores for the weights (first: they are written in pairs), the parts' outputs and statistics
-  const int64_t n_scores = weighted ? B * Hkv * max_blocks * 16 * ((Hq / Hkv + 1) / 2 * 2) : 0;
-  const int64_t n_part = (ctas + B * Hkv) * (Hq / Hkv);
-  const at::Tensor scratch = at::empty({n_scores + n_part * (D + 2)}, q.options().dtype(at::kFloat));
-  float* part = scratch.data_ptr<float>() + n_scores;
-  float* ml = part + n_part * D;
-  float* scores = weighted ? scratch.data_ptr<float>() : nullptr;
+  const at::Tensor scratch = at::empty({rlb_q4_decode_scratch((int)B, (int)Hkv, G, (int)D, max_blocks, ctas, weighted)},
+                                       q.options().dtype(at::kFloat));
   CHECK_OK(rlb_q4_decode(qc.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), tables.data_ptr<int>(),
-                         lens.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hkv, (int)(Hq / Hkv), (int)D, max_blocks,
-                         (int)k_pool.size(0), (float)scale, (float)softcap, (int)window, (int)ctas, part, ml, scores,
+                         lens.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hkv, G, (int)D, max_blocks,
+                         (int)k_pool.size(0), (float)scale, (float)softcap, (int)window, ctas,
+                         scratch.data_ptr<float>(), weighted,
                          weighted ? weights->data_ptr<float>() : nullptr,
                          weighted ? weight_rows->data_ptr<int>() : nullptr, weighted ? weights->size(0) : 0,
                          weighted ? (int)weights->size(2) : 0, sm_count(), status_or_bounds(status, k_pool),

@@ -128,12 +128,12 @@ cudaError_t rlb_q4_write(const void* k_new, const void* v_new, long long k_sn, l
 cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_block, const int* slot_off,
                         const int* tables, const int* lens, int max_blocks, int max_len, long long N, int Hkv, int D,
                         int num_blocks, void* k_out, void* v_out, int* status, cudaStream_t s);
-// ctas: rlb_q4_decode_ctas().  Scratch (fp32): part [ctas + B Hkv][G][D], ml [ctas + B Hkv][G][2], and with weights
-// scores [B][Hkv][max_blocks * 16][G rounded up to even].
-int rlb_q4_decode_ctas(int B, int Hkv, int G, int max_blocks, int sms);
+// ctas: rlb_q4_decode_ctas(); scratch: rlb_q4_decode_scratch() floats, 8-byte aligned.
+int rlb_q4_decode_ctas(int B, int Hkv, int G, int D, int max_blocks, int sms);
+long long rlb_q4_decode_scratch(int B, int Hkv, int G, int D, int max_blocks, int ctas, bool weighted);
 cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool, const int* tables, const int* lens,
                           void* out, int B, int Hkv, int G, int D, int max_blocks, int num_blocks, float scale,
-                          float softcap, int window, int ctas, float* part, float* ml, float* scores, float* weights,
+                          float softcap, int window, int ctas, float* scratch, bool weighted, float* weights,
                           const int* weight_rows, long long w_rows, int w_len, int sms, int* status, cudaStream_t s);
 cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const int* lens, const int* new_tables,
                          float* weights, const int* weight_rows, int* kept, int* new_lens, int B, int Hkv, int D,

@@ -131,11 +131,11 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 }
 
 // ---------------------------------------------------------------- decode attention
-// The work is the pairs of blocks (32 tokens) of all (sequence, KV head) rows in a line, cut into equal stretches, one
+// The work is the turns (2 or 4 blocks of 16 tokens) of all (sequence, KV head) rows in a line, cut into equal stretches, one
 // for each CTA that fits on the GPU: lengths are ragged and known on the device only, and a grid of whole rows or
 // fixed parts leaves SMs idle at the end (a fifth of the time at 32 sequences of 2048 to 8192 tokens).  A CTA walks
-// the rows of its stretch; each of its warps takes every fourth pair of a row and
-// works alone: its lanes 0 to 3 bring blocks (codes, scales and minima of K and V, one contiguous piece each) into the
+// the rows of its stretch; each of its warps takes every fourth turn of a row and
+// works alone: its first lanes bring blocks (codes, scales and minima of K and V, one contiguous piece each) into the
 // warp's own ring of shared memory with bulk copies, and the warp computes on matrix instructions
 // (mma.sync m16n8k16, bf16 x bf16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
 // query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
@@ -160,17 +160,17 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 //
 // Softmax statistics are fp32 in base 2.  The running maximum is only raised (and the sums rescaled) when a score
 // exceeds it by 8, so weights stay below 2^8 relative to it.  It is a whole number (rounded up), so that it and the
-// factors between the maxima of warps and CTAs are exact.  A warp takes two blocks per turn, which shares the
-// waits, votes and bookkeeping among 32 tokens.
+// factors between the maxima of warps and CTAs are exact.  A turn of several blocks shares the
+// waits, votes and bookkeeping among 32 (D = 128) or 64 tokens.
 struct Q4Cache {
   const uint8_t *k_pool, *v_pool;
   const int *tables, *lens;
   int Hkv, G, max_blocks, num_blocks, window;
+  int turn;  // blocks a warp takes at a time (q4_turn)
   float scale, softcap;
 };
 
 constexpr int kDecodeWarps = 4;
-constexpr int kPair = 2;                 // blocks a turn
 constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
 
 RLB_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2,
@@ -238,79 +238,76 @@ RLB_DEVICE int q4_len(const Q4Cache& c, int b, int* status) {
   return min(max(len, 0), most);
 }
 
-// First token that a sequence of `len` tokens attends to, and its pairs of blocks from there on.
+// First token that a sequence of `len` tokens attends to, and its turns from there on.
 RLB_DEVICE int q4_first(const Q4Cache& c, int len) { return c.window > 0 && len > c.window ? len - c.window : 0; }
-RLB_DEVICE int q4_pairs(const Q4Cache& c, int len) {
+RLB_DEVICE int q4_turns(const Q4Cache& c, int len) {
   if (len == 0) return 0;
   const int blocks = (len - 1) / kTok - q4_first(c, len) / kTok + 1;
-  return (blocks + kPair - 1) / kPair;
+  return (blocks + c.turn - 1) / c.turn;
 }
 
-// The pairs of all rows lie in a line: row (b, h) holds [base(b) + h n(b), + n(b)), and CTA k of C the stretch
+// The turns of all rows lie in a line: row (b, h) holds [base(b) + h n(b), + n(b)), and CTA k of C the stretch
 // [cut(k), cut(k + 1)).  A part (k, row) gets scratch slot k + row: along the line each next part raises one of the two.
 RLB_DEVICE long long q4_cut(long long k, long long total, int C) { return k * total / C; }
 RLB_DEVICE long long q4_owner(long long x, long long total, int C) { return ((x + 1) * C - 1) / total; }
 
-// Sums of the pairs before sequence `b` and in all, and the sequence that holds pair `x` (in units of Hkv: place
-// x / Hkv per head).  Every thread of the block calls it; scratch: 2 x 32 + 2 numbers.
+// Where CTA k of C begins: the turns of all sequences and of those before `seq` (of one KV head), `seq` being the
+// sequence that holds the CTA's first turn.  Every thread of the block calls it.
 struct Q4Line {
-  long long total;  // pairs of all sequences, one KV head
-  long long base;   // pairs before sequence `seq`, one KV head
+  long long total, base;
   int seq;
 };
-// find >= 0: the sequence that holds pair `find` of the line (all heads); else the sequence `seq` is given.
-RLB_DEVICE Q4Line q4_line(const Q4Cache& c, int B, long long k, int C, int seq, int* status) {
-  __shared__ long long warp_sum_[8], warp_base_[8];
+RLB_DEVICE Q4Line q4_line(const Q4Cache& c, int B, long long k, int C, int* status) {
+  __shared__ long long sums[32];
   __shared__ Q4Line found;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = (B + blockDim.x - 1) / blockDim.x;
   const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += q4_pairs(c, q4_len(c, b, status));
+  for (int b = b0; b < b1; ++b) mine += q4_turns(c, q4_len(c, b, status));
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long y = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += y;
   }
-  if (lane == 31) warp_sum_[warp] = incl;
+  if (lane == 31) sums[warp] = incl;
+  if (threadIdx.x == 0) found.seq = B;
   __syncthreads();
   long long before = incl - mine, total = 0;
   for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += warp_sum_[w];
-    total += warp_sum_[w];
+    if (w < warp) before += sums[w];
+    total += sums[w];
   }
-  if (threadIdx.x == 0) found = Q4Line{total, total, B};
-  __syncthreads();
-  if (seq >= 0) {
-    if (b0 <= seq && seq < b1) {
-      for (int b = b0; b < seq; ++b) before += q4_pairs(c, q4_len(c, b, nullptr));
-      found = Q4Line{total, before, seq};
-    }
-  } else {
-    const long long x = q4_cut(k, total * c.Hkv, C);
-    if (before * c.Hkv <= x && x < (before + mine) * c.Hkv) {
-      for (int b = b0; b < b1; ++b) {
-        const int n = q4_pairs(c, q4_len(c, b, nullptr));
-        if (x < (before + n) * c.Hkv) {
-          found = Q4Line{total, before, b};
-          break;
-        }
-        before += n;
+  const long long x = q4_cut(k, total * c.Hkv, C);
+  if (before * c.Hkv <= x && x < (before + mine) * c.Hkv) {
+    for (int b = b0; b < b1; ++b) {
+      const int n = q4_turns(c, q4_len(c, b, nullptr));
+      if (x < (before + n) * c.Hkv) {
+        found.base = before;
+        found.seq = b;
+        break;
       }
+      before += n;
     }
   }
   __syncthreads();
-  return found;
+  return Q4Line{total, found.base, found.seq};
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// One turn's work of a warp: the pair of blocks at `ks` (each K then V).  MASKED: some of the tokens are not seen.
+constexpr int q4_ctas(int D, int NT) { return NT == 2 ? 2 : D == 128 ? 3 : 4; }  // CTAs on an SM at a time
+template <int D>
+constexpr int q4_turn() { return D == 128 ? 2 : 4; }   // blocks a turn
+template <int D>
+constexpr int q4_stages() { return 2; }                // turns in a warp's ring
+
+// One turn's work of a warp: the blocks at `ks` (each K then V).  MASKED: some of the tokens are not seen.
 template <int D, int NT>
 struct Q4Warp {
   using L = Q4<D>;
-  static constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16;
+  static constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16, BT = q4_turn<D>();
   uint32_t qb[NT][NG][WPL][4];                   // Q^T's registers (column n = head g of each tile)
   float qs[NT][NG][2], qc[NT][NG][2], qf[NT][2]; // heads 2t, 2t + 1: sums of q, where S starts, the scores' factor
   float m[NT][2], mref[NT][2], l[NT][2];         // what a score may reach (8 above the maximum when that was last
@@ -386,14 +383,21 @@ struct Q4Warp {
       }
   }
 
-  // seen: bit 2k + i: this lane's token i of block k.  `scores`: this lane's token 0 of block 0, or null.
+  static RLB_DEVICE float largest(const float (&s)[BT][4], int e) {
+    float x = fmaxf(s[0][e], s[0][e + 2]);
+#pragma unroll
+    for (int k = 1; k < BT; ++k) x = fmaxf(x, fmaxf(s[k][e], s[k][e + 2]));
+    return x;
+  }
+
+  // seen: bit 2k + i: this lane's token i of block k is attended to, bit 8 + 2k + i: it has a place in `scores`.  `scores`: this lane's token 0 of block 0, or null.
   template <bool MASKED>
   RLB_DEVICE void turn(const uint8_t* ks, unsigned seen, float softcap, float* scores, int Gs) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int tok = (g & 1) * 4 + (g >> 1);  // this lane's tokens of a block in S^T: tok and tok + 8
-    float s[NT][kPair][4];
+    float s[NT][BT][4];
 #pragma unroll
-    for (int k = 0; k < kPair; ++k)
+    for (int k = 0; k < BT; ++k)
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
         const uint8_t* blk = ks + k * 2 * L::kBytes;
@@ -439,41 +443,40 @@ struct Q4Warp {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k = 0; k < kPair; ++k)
+      for (int k = 0; k < BT; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][k][e] *= qf[n][e & 1];
     if (softcap > 0.f) {  // (the factor then lacks log2 e)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int k = 0; k < kPair; ++k)
+        for (int k = 0; k < BT; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[n][k][e] = tanhf(s[n][k][e] / softcap) * (softcap * kLog2e);
     }
     bool raise = false;
-    uint32_t vm[kPair][NG][2], vmax = 0;  // V's (scale, minimum) of this lane's tokens
+    uint32_t vm[BT][NG][2], vmax = 0;  // V's (scale, minimum) of this lane's tokens
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int k = 0; k < kPair; ++k)
+      for (int k = 0; k < BT; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (MASKED && !((seen >> (2 * k + (e >> 1))) & 1)) s[n][k][e] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        raise |= fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2])) > m[n][e];
+      for (int e = 0; e < 2; ++e) raise |= largest(s[n], e) > m[n][e];
       if (scores != nullptr && n * 8 + 2 * t < Gs) {
 #pragma unroll
-        for (int k = 0; k < kPair; ++k)
+        for (int k = 0; k < BT; ++k)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (!MASKED || ((seen >> (4 + 2 * k + i)) & 1))
+            if (!MASKED || ((seen >> (8 + 2 * k + i)) & 1))
               *reinterpret_cast<float2*>(scores + (k * kTok + 8 * i) * Gs + n * 8 + 2 * t) =
                   make_float2(s[n][k][2 * i], s[n][k][2 * i + 1]);
       }
     }
 #pragma unroll
-    for (int k = 0; k < kPair; ++k)
+    for (int k = 0; k < BT; ++k)
 #pragma unroll
       for (int r = 0; r < NG; ++r)
 #pragma unroll
@@ -495,7 +498,7 @@ struct Q4Warp {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
+          float x = largest(s[n], e);
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
           const float was = m[n][e] - 8.f;
@@ -518,14 +521,14 @@ struct Q4Warp {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k = 0; k < kPair; ++k)
+      for (int k = 0; k < BT; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[n][k][e] = sm100::ex2_approx(s[n][k][e] - mref[n][e & 1]);
           l[n][e & 1] += s[n][k][e];
         }
 #pragma unroll
-    for (int k = 0; k < kPair; ++k)
+    for (int k = 0; k < BT; ++k)
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
         const uint8_t* blk = ks + (2 * k + 1) * L::kBytes;
@@ -567,20 +570,17 @@ struct Q4Warp {
   }
 };
 
-template <int D>
-constexpr int q4_stages() { return D == 128 ? 2 : 4; }  // pairs of blocks in a warp's ring
-
 // NT: tiles of 8 query heads.  Rows that lie in one CTA's stretch are finished here, the others' parts go to `part`
 // [slots][G][D] (unnormalised outputs) and `ml` [slots][G][2] (statistics).  `scores` [B][Hkv][tokens][Gs] receives the
 // base-2 scores for q4_finish_kernel, which then needs every row's statistics.
 template <int D, int NT>
-__global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_kernel(
+__global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_kernel(
     const __nv_bfloat16* __restrict__ q, Q4Cache c, int B, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
-    float* __restrict__ ml, float* __restrict__ scores, int Gs, int* status) {
+    float* __restrict__ ml, int2* __restrict__ plan, float* __restrict__ scores, int Gs, int* status) {
   using L = Q4<D>;
   using W = Q4Warp<D, NT>;
-  constexpr int HT = NT * 8, S = q4_stages<D>();
-  constexpr int kStage = kPair * 2 * L::kBytes;
+  constexpr int HT = NT * 8, S = q4_stages<D>(), BT = q4_turn<D>(), PER = 32 / BT;  // PER: turns whose ids a warp holds
+  constexpr int kStage = BT * 2 * L::kBytes;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kDecodeWarps][S];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_
     sm100::fence_barrier_init();
     sm100::fence_async_shared();
   }
-  const Q4Line line = q4_line(c, B, blockIdx.x, gridDim.x, -1, blockIdx.x == 0 ? status : nullptr);
+  const Q4Line line = q4_line(c, B, blockIdx.x, gridDim.x, blockIdx.x == 0 ? status : nullptr);
   const long long total = line.total * c.Hkv;
   long long x = q4_cut(blockIdx.x, total, gridDim.x);
   const long long x_end = q4_cut(blockIdx.x + 1, total, gridDim.x);
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_
   bool alive = true;
 
   for (int b = line.seq; x < x_end;) {
-    const int len = q4_len(c, b, nullptr), n = q4_pairs(c, len);
+    const int len = q4_len(c, b, nullptr), n = q4_turns(c, len);
     if (x >= base + (long long)n * c.Hkv) {  // sequences without tokens hold nothing
       base += (long long)n * c.Hkv;
       ++b;
@@ -609,32 +609,31 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_
     const int h = (int)((x - base) / n), p0 = (int)((x - base) % n);
     const int p1 = (int)min((long long)n, p0 + (x_end - x));
     x += p1 - p0;
-    const int t0 = q4_first(c, len), jb0 = t0 / kTok + p0 * kPair;
-    const int jb1 = min((len - 1) / kTok + 1, t0 / kTok + p1 * kPair);  // this part's blocks
+    const int t0 = q4_first(c, len), jb0 = t0 / kTok + p0 * BT;
+    const int jb1 = min((len - 1) / kTok + 1, t0 / kTok + p1 * BT);  // this part's blocks
     const int mine = p1 - p0 > warp ? (p1 - p0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's turns
     const int* table = c.tables + (long long)b * c.max_blocks;
 
-    int id = 0;         // lanes 2i and 2i + 1: the blocks of turn i of the current sixteen
-    uint32_t good = 0;  // bits 2 (i % 16), + 1: blocks of turn i that are there
+    int id = 0;                 // lane BT i + k: block k of turn i of the current PER turns
+    uint32_t good = 0, was = 0;  // bit BT i + k: that block is there; `was`: of the PER turns before
     auto issue = [&](int i) {
       if (i >= mine) return;
-      if ((i & 15) == 0) {
-        const int at = jb0 + ((i + (lane >> 1)) * kDecodeWarps + warp) * kPair + (lane & 1);
+      if (i % PER == 0) {
+        const int at = jb0 + ((i + lane / BT) * kDecodeWarps + warp) * BT + lane % BT;
         id = at < jb1 ? table[at] : -1;
-        const bool ok = id >= 0 && id < c.num_blocks;
-        if (!ok && at < jb1) report(status, kBadIndex);
-        if (!ok) id = -1;
+        if ((id < 0 || id >= c.num_blocks) && at < jb1) report(status, kBadIndex);
+        was = good;
+        good = __ballot_sync(0xffffffffu, at < jb1 && id >= 0 && id < c.num_blocks);
       }
-      const int shift = 2 * (i & 15), stage = (used + i) % S;
-      const unsigned ok = __ballot_sync(0xffffffffu, id >= 0) >> shift & 3u;
-      good = (good & ~(3u << shift)) | (ok << shift);
-      const int blk = __shfl_sync(0xffffffffu, id, shift + (lane & 1));
+      const int shift = i % PER * BT, stage = (used + i) % S;
+      const unsigned ok = good >> shift & ((1u << BT) - 1);
+      const int blk = __shfl_sync(0xffffffffu, id, shift + lane % BT);
       uint64_t* bar = &bars[warp][stage];
       if (lane == 0) sm100::mbar_arrive_expect_tx(bar, __popc(ok) * 2 * L::kBytes);
       __syncwarp();
-      if (lane < 4 && blk >= 0) {  // lane: block lane & 1, K (lanes 0, 1) or V (2, 3)
-        const uint8_t* src = (lane < 2 ? c.k_pool : c.v_pool) + ((long long)blk * c.Hkv + h) * L::kBytes;
-        bulk_load(ring + stage * kStage + ((lane & 1) * 2 + (lane >> 1)) * L::kBytes, src, L::kBytes, bar);
+      if (lane < 2 * BT && (ok >> lane % BT & 1)) {  // lane: block lane % BT, K (the first lanes) or V
+        const uint8_t* src = (lane < BT ? c.k_pool : c.v_pool) + ((long long)blk * c.Hkv + h) * L::kBytes;
+        bulk_load(ring + stage * kStage + (lane % BT * 2 + lane / BT) * L::kBytes, src, L::kBytes, bar);
       }
     };
 #pragma unroll
@@ -656,18 +655,19 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_
         break;
       }
       const uint8_t* ks = ring + stage * kStage;
-      const int jb = jb0 + (i * kDecodeWarps + warp) * kPair, at = jb * kTok;
-      const unsigned ok = good >> (2 * (i & 15)) & 3u;
+      const int jb = jb0 + (i * kDecodeWarps + warp) * BT, at = jb * kTok;
+      // (copies run S turns ahead, at most into the next PER turns)
+      const unsigned ok = (min(mine - 1, i + S - 1) / PER == i / PER ? good : was) >> (i % PER * BT) & ((1u << BT) - 1);
       float* sc = srow != nullptr ? srow + (long long)at * Gs : nullptr;
-      if (ok == 3u && at >= t0 && at + kPair * kTok <= len) {
+      if (ok == (1u << BT) - 1 && at >= t0 && at + BT * kTok <= len) {
         w.template turn<false>(ks, 0u, c.softcap, sc, Gs);
       } else {
         unsigned seen = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2 * BT; ++k) {
           const int y = at + (k >> 1) * kTok + tok + 8 * (k & 1);
           seen |= (unsigned)((ok >> (k >> 1) & 1) && y >= t0 && y < len) << k;
-          seen |= (unsigned)(y < len && jb + (k >> 1) < jb1) << (4 + k);  // a place in `scores` that is this CTA's
+          seen |= (unsigned)(y < len && jb + (k >> 1) < jb1) << (8 + k);
         }
         w.template turn<true>(ks, seen, c.softcap, sc, Gs);
       }
@@ -709,6 +709,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_
     __syncthreads();
     const long long row = (long long)b * c.Hkv + h, slot = blockIdx.x + row;
     const bool whole = p0 == 0 && p1 == n;
+    if (p0 == 0 && threadIdx.x == 0)  // the row's first slot and its parts, for q4_finish_kernel
+      plan[row] = make_int2((int)slot, (int)(q4_owner(x - (p1 - p0) + n - 1, total, gridDim.x) - blockIdx.x) + 1);
     for (int y = threadIdx.x; y < G * D; y += kDecodeWarps * 32) {
       const int head = y / D, d = y % D;
       float M = -INFINITY, sum = 0.f, acc = 0.f;
@@ -733,72 +735,85 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, NT == 1 ? 3 : 2) q4_decode_
   }
 }
 
-// Joins the parts of the rows that several CTAs of q4_decode_kernel (C in all) shared and clears those of empty
-// sequences: CTA 0 of a row's `gridDim.z` writes the outputs, and with `weights` each adds a stretch of the tokens'
-// attention weights, summed over the heads, to their accumulators.
+// Maximum and 1 / sum of one query head over a row's parts; a whole warp calls it.
+RLB_DEVICE float2 q4_join(const float* ml, int G, int parts) {
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY, sum = 0.f;
+  for (int s = lane; s < parts; s += 32) M = fmaxf(M, ml[2LL * s * G]);
+  M = warp_max(M);
+  for (int s = lane; s < parts; s += 32) {
+    const float ms = ml[2LL * s * G], ls = ml[2LL * s * G + 1];
+    sum += ms == -INFINITY ? ls : ls * sm100::ex2_approx(ms - M);
+  }
+  sum = warp_sum(sum);
+  return make_float2(M, sum != 0.f ? 1.f / sum : 0.f);
+}
+
+// Joins the parts of the rows that several CTAs of q4_decode_kernel shared, and writes zeros for empty sequences:
+// CTA z < G of a row does query head z, its four warps taking the parts in turn.  With `weights` the CTAs behind
+// add a stretch each of the tokens' attention weights, summed over the heads, to their accumulators.
 template <int D>
-__global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, int B, int C, const float* __restrict__ part,
-                                                        const float* __restrict__ ml,
+__global__ void __launch_bounds__(128) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
+                                                        const float* __restrict__ ml, const int2* __restrict__ plan,
                                                         __nv_bfloat16* __restrict__ out,
                                                         const float* __restrict__ scores, int Gs,
                                                         float* __restrict__ weights,
                                                         const int* __restrict__ weight_rows, long long w_rows,
                                                         int w_len, int* status) {
-  __shared__ float sm_m[16], sm_r[16];  // each head's maximum and 1 / sum
-  const int h = blockIdx.x, b = blockIdx.y, G = c.G;
-  const Q4Line line = q4_line(c, B, 0, C, b, nullptr);
-  const long long row = (long long)b * c.Hkv + h, total = line.total * c.Hkv;
-  const int len = q4_len(c, b, nullptr), n = q4_pairs(c, len);
-  if (n == 0) {
-    for (int x = threadIdx.x; x < G * D; x += 256) out[row * G * D + x] = __float2bfloat16(0.f);
+  constexpr int E = D / 32;
+  __shared__ float2 stat[16];
+  __shared__ float sums[4][D];
+  cudaGridDependencySynchronize();  // (every CTA: what follows this kernel must not overtake the one before)
+  const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, G = c.G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = (long long)b * c.Hkv + h;
+  const int len = q4_len(c, b, nullptr);
+  if (len == 0) {
+    if (z < G)
+      for (int d = threadIdx.x; d < D; d += 128) out[(row * G + z) * D + d] = __float2bfloat16(0.f);
     return;
   }
-  const long long start = line.base * c.Hkv + (long long)h * n;
-  const long long first = q4_owner(start, total, C), last = q4_owner(start + n - 1, total, C);
-  if (first == last && weights == nullptr) return;
-  const long long slot = first + row;
-  const int parts = (int)(last - first) + 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int head = warp; head < G; head += 8) {
-    const float* p = ml + (slot * G + head) * 2;
-    float M = -INFINITY, sum = 0.f;
-    for (int s = lane; s < parts; s += 32) M = fmaxf(M, p[2LL * s * G]);
-    M = warp_max(M);
-    for (int s = lane; s < parts; s += 32) {
-      const float ms = p[2LL * s * G], ls = p[2LL * s * G + 1];
-      sum += ms == -INFINITY ? ls : ls * sm100::ex2_approx(ms - M);
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) {
-      sm_m[head] = M;
-      sm_r[head] = sum != 0.f ? 1.f / sum : 0.f;
-    }
-  }
-  __syncthreads();
-  if (blockIdx.z == 0 && parts > 1)
-    for (int x = threadIdx.x; x < G * D; x += 256) {
-      const int head = x / D;
-      const float* p = ml + (slot * G + head) * 2;
-      const float* a = part + slot * G * D + x;
-      float acc = 0.f;
+  const int2 at = plan[row];  // first slot, parts
+  const float* stats = ml + (long long)at.x * G * 2;
+  if (z < G) {
+    if (at.y == 1) return;  // written already
+    const float M = q4_join(stats + 2 * z, G, at.y).x;
+    float acc[E] = {}, sum = 0.f;
 #pragma unroll 4
-      for (int s = 0; s < parts; ++s) {
-        const float ms = p[2LL * s * G];
-        acc += ms == -INFINITY ? a[(long long)s * G * D] : a[(long long)s * G * D] * sm100::ex2_approx(ms - sm_m[head]);
-      }
-      out[row * G * D + x] = __float2bfloat16(acc * sm_r[head]);
+    for (int s = warp; s < at.y; s += 4) {
+      const float ms = stats[2LL * s * G + 2 * z], f = ms == -INFINITY ? 1.f : sm100::ex2_approx(ms - M);
+      const float* a = part + (((long long)at.x + s) * G + z) * D + lane;
+      sum += stats[2LL * s * G + 2 * z + 1] * f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += a[32 * e] * f;
     }
-  if (weights == nullptr) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[warp][lane + 32 * e] = acc[e];
+    if (lane == 0) stat[warp].x = sum;
+    __syncthreads();
+    const float total = stat[0].x + stat[1].x + stat[2].x + stat[3].x;
+    for (int d = threadIdx.x; d < D; d += 128) {
+      const float a = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
+      out[(row * G + z) * D + d] = __float2bfloat16(total != 0.f ? a / total : 0.f);
+    }
+    return;
+  }
   const int r = weight_rows[b];
   if (r < 0) return;
-  if (threadIdx.x == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
+  if (threadIdx.x == 0 && z == G && h == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
   if (r >= w_rows) return;
-  const int t0 = q4_first(c, len);
+  for (int head = warp; head < G; head += 4) {
+    const float2 x = q4_join(stats + 2 * head, G, at.y);
+    if (lane == 0) stat[head] = x;
+  }
+  __syncthreads();
   float* w = weights + ((long long)r * c.Hkv + h) * w_len;
   const float* sc = scores + row * c.max_blocks * kTok * Gs;
-  for (int t = t0 + blockIdx.z * 256 + threadIdx.x; t < min(len, w_len); t += gridDim.z * 256) {
+  const int step = (gridDim.z - G) * 128;
+  for (int t = q4_first(c, len) + (z - G) * 128 + threadIdx.x; t < min(len, w_len); t += step) {
     float p = 0.f;
-    for (int head = 0; head < G; ++head) p += sm100::ex2_approx(sc[(long long)t * Gs + head] - sm_m[head]) * sm_r[head];
+    for (int head = 0; head < G; ++head)
+      p += sm100::ex2_approx(sc[(long long)t * Gs + head] - stat[head].x) * stat[head].y;
     if (p > 0.f) atomicAdd(w + t, p);
   }
 }
@@ -979,45 +994,69 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
 
 template <int D, int NT>
 static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, int B, int C, float* part, float* ml,
-                                    float* scores, int Gs, int* status, cudaStream_t s) {
-  constexpr int ring = kDecodeWarps * q4_stages<D>() * kPair * 2 * Q4<D>::kBytes;
+                                    int2* plan, float* scores, int Gs, int* status, cudaStream_t s) {
+  constexpr int ring = kDecodeWarps * q4_stages<D>() * q4_turn<D>() * 2 * Q4<D>::kBytes;
   constexpr int join = kDecodeWarps * NT * 8 * (D + 2) * 4;
   constexpr int smem = ring > join ? ring : join;
   static_assert(smem <= 47 * 1024, "above 48 KB a kernel has to ask for its shared memory");
   q4_decode_kernel<D, NT><<<C, kDecodeWarps * 32, smem, s>>>((const __nv_bfloat16*)q, c, B, (__nv_bfloat16*)out, part,
-                                                              ml, scores, Gs, status);
+                                                              ml, plan, scores, Gs, status);
   return cudaGetLastError();
 }
 
-int rlb_q4_decode_ctas(int B, int Hkv, int G, int max_blocks, int sms) {
-  // As many CTAs as fit at a time, but a pair of blocks for each warp if the tables are full.
-  const long long fit = (long long)sms * (G <= 8 ? 3 : 2);
-  const long long pairs = (long long)B * Hkv * ((max_blocks + kPair - 1) / kPair);
-  const long long want = (pairs + kDecodeWarps - 1) / kDecodeWarps;
+static int q4_turn_of(int D) { return D == 128 ? q4_turn<128>() : q4_turn<64>(); }
+
+int rlb_q4_decode_ctas(int B, int Hkv, int G, int D, int max_blocks, int sms) {
+  // As many CTAs as fit at a time, but a turn for each warp if the tables are full.
+  const long long fit = (long long)sms * q4_ctas(D, G <= 8 ? 1 : 2);
+  const long long turns = (long long)B * Hkv * ((max_blocks + q4_turn_of(D) - 1) / q4_turn_of(D));
+  const long long want = (turns + kDecodeWarps - 1) / kDecodeWarps;
   return (int)(want < 1 ? 1 : want < fit ? want : fit);
 }
 
 cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool, const int* tables, const int* lens,
                           void* out, int B, int Hkv, int G, int D, int max_blocks, int num_blocks, float scale,
-                          float softcap, int window, int ctas, float* part, float* ml, float* scores, float* weights,
+                          float softcap, int window, int ctas, float* scratch, bool weighted, float* weights,
                           const int* weight_rows, long long w_rows, int w_len, int sms, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
   const Q4Cache c{(const uint8_t*)k_pool, (const uint8_t*)v_pool, tables, lens, Hkv, G, max_blocks, num_blocks,
-                  window, scale, softcap};
+                  window, q4_turn_of(D), scale, softcap};
   const int Gs = (G + 1) & ~1;
+  const long long slots = ctas + (long long)B * Hkv;
+  float* scores = weighted ? scratch : nullptr;  // first: written in pairs
+  if (weighted) scratch += (long long)B * Hkv * max_blocks * kTok * Gs;
+  int2* plan = (int2*)scratch;
+  float* ml = scratch + 2LL * B * Hkv;
+  float* part = ml + slots * G * 2;
   cudaError_t e = cudaSuccess;
-  RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, ctas, part, ml, scores, Gs, status, s))
-                      : (q4_decode_launch<DD, 2>(q, c, out, B, ctas, part, ml, scores, Gs, status, s)));
+  RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, ctas, part, ml, plan, scores, Gs, status, s))
+                      : (q4_decode_launch<DD, 2>(q, c, out, B, ctas, part, ml, plan, scores, Gs, status, s)));
   if (e != cudaSuccess) return e;
-  int chunks = 1;  // CTAs per row that add weights: four waves of the GPU, 256 tokens each at least
-  if (weights != nullptr) {
-    const long long rows = (long long)B * Hkv, want = (16LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 255) / 256;
+  int chunks = 0;  // CTAs per row that add weights: four waves of the GPU, 128 tokens each at least
+  if (weighted) {
+    const long long rows = (long long)B * Hkv, want = (32LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 127) / 128;
     chunks = (int)(want < most ? want : most);
     if (chunks < 1) chunks = 1;
   }
-  RLB_Q4_D((q4_finish_kernel<DD><<<dim3(Hkv, B, chunks), 256, 0, s>>>(c, B, ctas, part, ml, (__nv_bfloat16*)out, scores,
-                                                                       Gs, weights, weight_rows, w_rows, w_len, status)));
-  return cudaGetLastError();
+  // launched while the decode kernel still runs; it waits for that one's end itself
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(Hkv, B, G + chunks);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  RLB_Q4_D(e = cudaLaunchKernelEx(&cfg, q4_finish_kernel<DD>, c, (const float*)part, (const float*)ml, (const int2*)plan,
+                                  (__nv_bfloat16*)out, (const float*)scores, Gs, weights, weight_rows, w_rows, w_len,
+                                  status));
+  return e;
+}
+
+long long rlb_q4_decode_scratch(int B, int Hkv, int G, int D, int max_blocks, int ctas, bool weighted) {
+  const long long rows = (long long)B * Hkv;
+  return (weighted ? rows * max_blocks * kTok * ((G + 1) & ~1) : 0) + 2 * rows + (ctas + rows) * G * (D + 2);
 }
 
 cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const int* lens, const int* new_tables,
