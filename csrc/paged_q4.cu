@@ -175,14 +175,14 @@ constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
 
 RLB_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2,
                         float c3) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 RLB_DEVICE uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -248,8 +248,11 @@ RLB_DEVICE int q4_turns(const Q4Cache& c, int len) {
 
 // The turns of all rows lie in a line: row (b, h) holds [base(b) + h n(b), + n(b)), and CTA k of C the stretch
 // [cut(k), cut(k + 1)).  A part (k, row) gets scratch slot k + row: along the line each next part raises one of the two.
-RLB_DEVICE long long q4_cut(long long k, long long total, int C) { return k * total / C; }
-RLB_DEVICE long long q4_owner(long long x, long long total, int C) { return ((x + 1) * C - 1) / total; }
+RLB_DEVICE long long q4_div(long long a, long long b) {  // of numbers that hardly ever need 64 bits
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+RLB_DEVICE long long q4_cut(long long k, long long total, int C) { return q4_div(k * total, C); }
+RLB_DEVICE long long q4_owner(long long x, long long total, int C) { return q4_div((x + 1) * C - 1, total); }
 
 // Where CTA k of C begins: the turns of all sequences and of those before `seq` (of one KV head), `seq` being the
 // sequence that holds the CTA's first turn.  Every thread of the block calls it.
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
       ++b;
       continue;
     }
-    const int h = (int)((x - base) / n), p0 = (int)((x - base) % n);
+    const int h = (int)q4_div(x - base, n), p0 = (int)(x - base - (long long)h * n);
     const int p1 = (int)min((long long)n, p0 + (x_end - x));
     x += p1 - p0;
     const int t0 = q4_first(c, len), jb0 = t0 / kTok + p0 * BT;
