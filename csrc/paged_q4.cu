@@ -131,13 +131,12 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 }
 
 // ---------------------------------------------------------------- decode attention
-// The work is the turns (2 or 4 blocks of 16 tokens) of all (sequence, KV head) rows in a line, cut into equal stretches, one
-// for each CTA that fits on the GPU: lengths are ragged and known on the device only, and a grid of whole rows or
-// fixed parts leaves SMs idle at the end (a fifth of the time at 32 sequences of 2048 to 8192 tokens).  A CTA walks
-// the rows of its stretch; each of its warps takes every fourth turn of a row and
-// works alone: its first lanes bring blocks (codes, scales and minima of K and V, one contiguous piece each) into the
-// warp's own ring of shared memory with bulk copies, and the warp computes on matrix instructions
-// (mma.sync m16n8k16, bf16 x bf16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
+// The work is the turns (2 or 4 blocks of 16 tokens) of all (sequence, KV head) rows in a line, cut into equal
+// stretches, one for each warp that fits on the GPU: lengths are ragged and known on the device only, and a grid of
+// whole rows or of fixed parts leaves SMs idle at the end.  A warp works alone, with no barrier: it brings blocks (codes,
+// scales and minima of K and V, one contiguous piece each) into its own ring of shared memory with bulk copies, which
+// run ahead across the rows' borders, and computes on matrix instructions
+// (mma.sync m16n8k16, fp16 x fp16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
 // query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
 // them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
 // memory) would need the unpacked values written back to shared memory first.
@@ -148,20 +147,20 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // is fp16 after division by a power of two per head (its largest element then lies in [2^13, 2^14)): bf16's 8 bits
 // fit, and what falls below 2^-24 is 2^-38 of the largest.  K's odd nibbles stay 1024 + 16 code: their q are divided by 16,
 // and the sums start at 8 sum(q even) - 64 sum(q odd) instead of zero, which leaves code . q.  The order of the
-// dimensions inside the
-// product is free as long as Q's registers use the same: a lane reads 16 consecutive dimensions of a token as two
+// dimensions inside the product is free as long as Q's registers use the same: a lane reads 16 consecutive dimensions of a token as two
 // words and takes nibbles j and j + 4 of a word as one operand register.
 // O^T = V^T P^T.  The token's scale goes into the weight and its minimum into a separate fp32 sum of p (m + 8 s).
 // The weights p s are rounded to fp16 (2^-11 of each, an eighth of what the output's own rounding to bf16 may
 // add); to stay in range, p is kept times a power of two that takes the largest scale so far below 2^4: p s <= 2^12.
-// The tokens' order is free too: row g of S^T is token (g & 1) * 4 + g / 2 (of each half of the block), which after
-// the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's gives lane t of a quad the tokens t,
-// t + 4, t + 8, t + 12, and the four V words that it reads for them lie in different banks.
+// The tokens' order is free too: row g of S^T (of each half of the block) is token g / 2 for even g and
+// 4 + (g / 2 ^ 2) for odd g.  After the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's, lane
+// t of a quad has the tokens t and 4 + (t ^ 2) of both halves; neither its four V words nor the K words that a half
+// warp reads at a time then share a bank.
 //
 // Softmax statistics are fp32 in base 2.  The running maximum is only raised (and the sums rescaled) when a score
 // exceeds it by 8, so weights stay below 2^8 relative to it.  It is a whole number (rounded up), so that it and the
-// factors between the maxima of warps and CTAs are exact.  A turn of several blocks shares the
-// waits, votes and bookkeeping among 32 (D = 128) or 64 tokens.
+// factors between the maxima of parts are exact.  A turn of several blocks shares the waits, votes and bookkeeping
+// among 32 (D = 128) or 64 tokens.
 struct Q4Cache {
   const uint8_t *k_pool, *v_pool;
   const int *tables, *lens;
@@ -186,9 +185,9 @@ RLB_DEVICE uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-RLB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+RLB_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
 
@@ -230,6 +229,8 @@ RLB_DEVICE uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+RLB_DEVICE int q4_token(int g) { return g & 1 ? 4 + (g >> 1 ^ 2) : g >> 1; }
+
 RLB_DEVICE float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 RLB_DEVICE int q4_len(const Q4Cache& c, int b, int* status) {
@@ -246,56 +247,47 @@ RLB_DEVICE int q4_turns(const Q4Cache& c, int len) {
   return (blocks + c.turn - 1) / c.turn;
 }
 
-// The turns of all rows lie in a line: row (b, h) holds [base(b) + h n(b), + n(b)), and CTA k of C the stretch
+// The turns of all rows lie in a line: row (b, h) holds [base(b) + h n(b), + n(b)), and warp k of C the stretch
 // [cut(k), cut(k + 1)).  A part (k, row) gets scratch slot k + row: along the line each next part raises one of the two.
-RLB_DEVICE long long q4_div(long long a, long long b) {  // of numbers that hardly ever need 64 bits
-  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+RLB_DEVICE int q4_cut(int k, int total, int C) { return k * (total / C) + k * (total % C) / C; }  // C^2 < 2^31
+RLB_DEVICE int q4_owner(int x, int total, int C) {  // ((x + 1) C - 1) / total: exact, the numbers have fewer than 53 bits
+  return (int)(((double)(x + 1) * C - 1) / total);
 }
-RLB_DEVICE long long q4_cut(long long k, long long total, int C) { return q4_div(k * total, C); }
-RLB_DEVICE long long q4_owner(long long x, long long total, int C) { return q4_div((x + 1) * C - 1, total); }
 
-// Where CTA k of C begins: the turns of all sequences and of those before `seq` (of one KV head), `seq` being the
-// sequence that holds the CTA's first turn.  Every thread of the block calls it.
+// Turns of all sequences (all KV heads), the warps that share them (each gets one at least, so that a row's slots follow
+// each other without a gap), and the sequence that holds turn x = cut(k), with the turns before it.
 struct Q4Line {
-  long long total, base;
-  int seq;
+  int total, warps, x, seq, base;
 };
-RLB_DEVICE Q4Line q4_line(const Q4Cache& c, int B, long long k, int C, int* status) {
-  __shared__ long long sums[32];
-  __shared__ Q4Line found;
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (B + blockDim.x - 1) / blockDim.x;
-  const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += q4_turns(c, q4_len(c, b, status));
-  long long incl = mine;
+RLB_DEVICE Q4Line q4_line(const Q4Cache& c, int B, int k, int C, int* status) {
+  const int lane = threadIdx.x & 31;
+  Q4Line r{0, 0, 0, B, 0};
+  int n = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    n = b0 + lane < B ? q4_turns(c, q4_len(c, b0 + lane, status)) * c.Hkv : 0;
+    r.total += __reduce_add_sync(0xffffffffu, n);
+  }
+  r.warps = min(C, r.total);
+  if (k >= r.warps) return r;
+  r.x = q4_cut(k, r.total, r.warps);
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    if (B > 32) n = b0 + lane < B ? q4_turns(c, q4_len(c, b0 + lane, nullptr)) * c.Hkv : 0;
+    int incl = n;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) sums[warp] = incl;
-  if (threadIdx.x == 0) found.seq = B;
-  __syncthreads();
-  long long before = incl - mine, total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += sums[w];
-    total += sums[w];
-  }
-  const long long x = q4_cut(k, total * c.Hkv, C);
-  if (before * c.Hkv <= x && x < (before + mine) * c.Hkv) {
-    for (int b = b0; b < b1; ++b) {
-      const int n = q4_turns(c, q4_len(c, b, nullptr));
-      if (x < (before + n) * c.Hkv) {
-        found.base = before;
-        found.seq = b;
-        break;
-      }
-      before += n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
     }
+    const unsigned behind = __ballot_sync(0xffffffffu, r.x < r.base + incl);
+    if (behind) {
+      const int at = __ffs(behind) - 1;
+      r.seq = b0 + at;
+      r.base += __shfl_sync(0xffffffffu, incl - n, at);
+      break;
+    }
+    r.base += __shfl_sync(0xffffffffu, incl, 31);
   }
-  __syncthreads();
-  return Q4Line{total, found.base, found.seq};
+  return r;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -313,8 +305,8 @@ struct Q4Warp {
   static constexpr int NG = L::kGroups, WPL = L::kGroup / 32, MT = L::kGroup / 16, BT = q4_turn<D>();
   uint32_t qb[NT][NG][WPL][4];                   // Q^T's registers (column n = head g of each tile)
   float qs[NT][NG][2], qc[NT][NG][2], qf[NT][2]; // heads 2t, 2t + 1: sums of q, where S starts, the scores' factor
-  float m[NT][2], mref[NT][2], l[NT][2];         // what a score may reach (8 above the maximum when that was last
-                                                 // raised), what exponents are taken against, sum of p
+  float m[NT][2], lim[NT][2];                    // maximum when it was last raised, the s that lies 8 above it
+  float mref[NT][2], l[NT][2];                   // what exponents are taken against, sum of p
   float z[NT][NG][2], o[NT][NG][MT][4];          // sums of p (m + 8 s) and of p s (code - 8)
   int ve;                                        // exponent field of the largest scale of V so far: p is kept times
                                                  // 2^(130 - ve), and so are the sums
@@ -341,8 +333,8 @@ struct Q4Warp {
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
       // q 2^e has its largest element in [2^13, 2^14)
       const int e = min(max(140 - (int)(__float_as_uint(big) >> 23), -126), 126);
-      const float up = pow2(e);
-      float factor = scale * pow2(-e);
+      const float up = scale < 0.f ? -pow2(e) : pow2(e);  // a negative scale's sign goes into q
+      float factor = fmaxf(fabsf(scale) * pow2(-e), 1e-37f);  // not 0, which -inf of unseen tokens could not take
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
         float sum = 0.f, odd = 0.f;
@@ -369,13 +361,16 @@ struct Q4Warp {
       qf[n][0] = __shfl_sync(0xffffffffu, factor, t * 8);
       qf[n][1] = __shfl_sync(0xffffffffu, factor, t * 8 + 4);
     }
+  }
+
+  RLB_DEVICE void reset() {
     ve = 70;  // (p is then at most 2^8 2^60)
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));  // kept in a register
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
+        m[n][e] = lim[n][e] = -INFINITY;
         mref[n][e] = l[n][e] = 0.f;
 #pragma unroll
         for (int r = 0; r < NG; ++r) {
@@ -397,7 +392,7 @@ struct Q4Warp {
   template <bool MASKED>
   RLB_DEVICE void turn(const uint8_t* ks, unsigned seen, float softcap, float* scores, int Gs) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int tok = (g & 1) * 4 + (g >> 1);  // this lane's tokens of a block in S^T: tok and tok + 8
+    const int tok = q4_token(g);  // this lane's tokens of a block in S^T: tok and tok + 8
     float s[NT][BT][4];
 #pragma unroll
     for (int k = 0; k < BT; ++k)
@@ -443,19 +438,17 @@ struct Q4Warp {
             s[n][k][e + 2] = fmaf(s1, acc[n][e + 2], y);
           }
       }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int k = 0; k < BT; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][k][e] *= qf[n][e & 1];
-    if (softcap > 0.f) {  // (the factor then lacks log2 e)
+    // from here on a score in base 2 is s qf
+    if (softcap > 0.f) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int k = 0; k < BT; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][k][e] = tanhf(s[n][k][e] / softcap) * (softcap * kLog2e);
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[n][k][e] * qf[n][e & 1] * (1.f / kLog2e);
+            s[n][k][e] = tanhf(x / softcap) * (softcap * kLog2e) / qf[n][e & 1];
+          }
     }
     bool raise = false;
     uint32_t vm[BT][NG][2], vmax = 0;  // V's (scale, minimum) of this lane's tokens
@@ -467,7 +460,7 @@ struct Q4Warp {
         for (int e = 0; e < 4; ++e)
           if (MASKED && !((seen >> (2 * k + (e >> 1))) & 1)) s[n][k][e] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) raise |= largest(s[n], e) > m[n][e];
+      for (int e = 0; e < 2; ++e) raise |= largest(s[n], e) > lim[n][e];
       if (scores != nullptr && n * 8 + 2 * t < Gs) {
 #pragma unroll
         for (int k = 0; k < BT; ++k)
@@ -475,7 +468,7 @@ struct Q4Warp {
           for (int i = 0; i < 2; ++i)
             if (!MASKED || ((seen >> (8 + 2 * k + i)) & 1))
               *reinterpret_cast<float2*>(scores + (k * kTok + 8 * i) * Gs + n * 8 + 2 * t) =
-                  make_float2(s[n][k][2 * i], s[n][k][2 * i + 1]);
+                  make_float2(s[n][k][2 * i] * qf[n][0], s[n][k][2 * i + 1] * qf[n][1]);
       }
     }
 #pragma unroll
@@ -501,13 +494,14 @@ struct Q4Warp {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = largest(s[n], e);
+          float x = largest(s[n], e) * qf[n][e];
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
-          const float was = m[n][e] - 8.f;
+          const float was = m[n][e];
           x = fmaxf(ceilf(x), was);
           const float f = (was == -INFINITY ? 0.f : sm100::ex2_approx(was - x)) * fv;
-          m[n][e] = x + 8.f;
+          m[n][e] = x;
+          lim[n][e] = (x + 8.f) / qf[n][e];
           mref[n][e] = (x == -INFINITY ? 0.f : x) - (float)(130 - ve);
           l[n][e] *= f;
 #pragma unroll
@@ -527,7 +521,7 @@ struct Q4Warp {
       for (int k = 0; k < BT; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[n][k][e] = sm100::ex2_approx(s[n][k][e] - mref[n][e & 1]);
+          s[n][k][e] = sm100::ex2_approx(fmaf(s[n][k][e], qf[n][e & 1], -mref[n][e & 1]));
           l[n][e & 1] += s[n][k][e];
         }
 #pragma unroll
@@ -545,19 +539,20 @@ struct Q4Warp {
           z[n][r][0] = fmaf(s[n][k][0], z0, fmaf(s[n][k][2], z1, z[n][r][0]));
           z[n][r][1] = fmaf(s[n][k][1], z0, fmaf(s[n][k][3], z1, z[n][r][1]));
         }
-        // the group's codes for this lane: dimensions 8 g .. 8 g + 7 (4 g .. 4 g + 3), tokens t, t + 4, t + 8, t + 12
-        uint32_t c[2][WPL][4];  // [tokens (t, t + 4) or (t + 8, t + 12)][dimensions 0-3 or 4-7], a token in each half
+        // the group's codes for this lane: dimensions 8 g .. 8 g + 7 (4 g .. 4 g + 3), tokens t and u of both halves
+        const int u = 4 + (t ^ 2);
+        uint32_t c[2][WPL][4];  // [half of the block][dimensions 0-3 or 4-7], a token in each half of the registers
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint8_t* row = blk + (r * kTok + t + 8 * i) * L::kRow + g * WPL * 2;
+          const uint8_t* row = blk + (r * kTok + 8 * i) * L::kRow + g * WPL * 2;
           if constexpr (WPL == 2) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(row);
-            const uint32_t y = *reinterpret_cast<const uint32_t*>(row + 4 * L::kRow);
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(row + t * L::kRow);
+            const uint32_t y = *reinterpret_cast<const uint32_t*>(row + u * L::kRow);
             codes_f16<true>(__byte_perm(x, y, 0x5410), c[i][0], magic);
             codes_f16<true>(__byte_perm(x, y, 0x7632), c[i][1], magic);
           } else {
-            codes_f16<true>(*reinterpret_cast<const uint16_t*>(row) |
-                          ((uint32_t)*reinterpret_cast<const uint16_t*>(row + 4 * L::kRow) << 16),
+            codes_f16<true>(*reinterpret_cast<const uint16_t*>(row + t * L::kRow) |
+                                ((uint32_t)*reinterpret_cast<const uint16_t*>(row + u * L::kRow) << 16),
                             c[i][0], magic);
           }
         }
@@ -573,94 +568,103 @@ struct Q4Warp {
   }
 };
 
-// NT: tiles of 8 query heads.  Rows that lie in one CTA's stretch are finished here, the others' parts go to `part`
-// [slots][G][D] (unnormalised outputs) and `ml` [slots][G][2] (statistics).  `scores` [B][Hkv][tokens][Gs] receives the
-// base-2 scores for q4_finish_kernel, which then needs every row's statistics.
+// NT: tiles of 8 query heads.  Rows that lie in one warp's stretch are finished here, the others' parts go to `part`
+// [slots][G][D] (unnormalised outputs) and `ml` [slots][G][2] (statistics); `plan` [row] = its first slot and its parts.
+// `scores` [B][Hkv][tokens][Gs] receives the base-2 scores for q4_finish_kernel, which then needs every row's statistics.
 template <int D, int NT>
 __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_kernel(
     const __nv_bfloat16* __restrict__ q, Q4Cache c, int B, __nv_bfloat16* __restrict__ out, float* __restrict__ part,
     float* __restrict__ ml, int2* __restrict__ plan, float* __restrict__ scores, int Gs, int* status) {
   using L = Q4<D>;
   using W = Q4Warp<D, NT>;
-  constexpr int HT = NT * 8, S = q4_stages<D>(), BT = q4_turn<D>(), PER = 32 / BT;  // PER: turns whose ids a warp holds
+  constexpr int S = q4_stages<D>(), BT = q4_turn<D>(), PER = 32 / BT;  // PER: turns whose blocks a warp has looked up
   constexpr int kStage = BT * 2 * L::kBytes;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kDecodeWarps][S];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = c.G;
+  const int G = c.G, me = blockIdx.x * kDecodeWarps + warp;
   uint8_t* ring = smem + warp * S * kStage;
   if (lane == 0) {
-    for (int s = 0; s < S; ++s) sm100::mbar_init(&bars[warp][s], 1);
+    for (int s = 0; s < S; ++s) sm100::mbar_init(&bars[warp][s], BT);
     sm100::fence_barrier_init();
     sm100::fence_async_shared();
   }
-  const Q4Line line = q4_line(c, B, blockIdx.x, gridDim.x, blockIdx.x == 0 ? status : nullptr);
-  const long long total = line.total * c.Hkv;
-  long long x = q4_cut(blockIdx.x, total, gridDim.x);
-  const long long x_end = q4_cut(blockIdx.x + 1, total, gridDim.x);
-  long long base = line.base * c.Hkv;
-  int used = 0;  // turns of this warp so far: the ring goes on from row to row
-  bool alive = true;
+  __syncwarp();
+  const Q4Line line = q4_line(c, B, me, gridDim.x * kDecodeWarps, me == 0 ? status : nullptr);
+  if (me >= line.warps) return;
+  const int turns = q4_cut(me + 1, line.total, line.warps) - line.x;
 
-  for (int b = line.seq; x < x_end;) {
-    const int len = q4_len(c, b, nullptr), n = q4_turns(c, len);
-    if (x >= base + (long long)n * c.Hkv) {  // sequences without tokens hold nothing
-      base += (long long)n * c.Hkv;
-      ++b;
-      continue;
+  // Where the warp's turns lie: lane BT i + k looks up block k of turn i of the next PER turns, one group ahead.
+  int lb = line.seq, lbase = line.base, llen = q4_len(c, lb, nullptr);
+  auto look = [&](int i0) {
+    const int i = i0 + lane / BT, x = line.x + i;
+    if (i >= turns) return -1;
+    int n = q4_turns(c, llen);
+    while (x >= lbase + n * c.Hkv) {  // ends: the last turn of the line is behind x
+      lbase += n * c.Hkv;
+      llen = q4_len(c, ++lb, nullptr);
+      n = q4_turns(c, llen);
     }
-    const int h = (int)q4_div(x - base, n), p0 = (int)(x - base - (long long)h * n);
-    const int p1 = (int)min((long long)n, p0 + (x_end - x));
-    x += p1 - p0;
-    const int t0 = q4_first(c, len), jb0 = t0 / kTok + p0 * BT;
-    const int jb1 = min((len - 1) / kTok + 1, t0 / kTok + p1 * BT);  // this part's blocks
-    const int mine = p1 - p0 > warp ? (p1 - p0 - warp + kDecodeWarps - 1) / kDecodeWarps : 0;  // this warp's turns
-    const int* table = c.tables + (long long)b * c.max_blocks;
-
-    int id = 0;                 // lane BT i + k: block k of turn i of the current PER turns
-    uint32_t good = 0, was = 0;  // bit BT i + k: that block is there; `was`: of the PER turns before
-    auto issue = [&](int i) {
-      if (i >= mine) return;
-      if (i % PER == 0) {
-        const int at = jb0 + ((i + lane / BT) * kDecodeWarps + warp) * BT + lane % BT;
-        id = at < jb1 ? table[at] : -1;
-        if ((id < 0 || id >= c.num_blocks) && at < jb1) report(status, kBadIndex);
-        was = good;
-        good = __ballot_sync(0xffffffffu, at < jb1 && id >= 0 && id < c.num_blocks);
+    const int h = (x - lbase) / n, p = x - lbase - h * n;
+    const int at = q4_first(c, llen) / kTok + p * BT + lane % BT;
+    if (at > (llen - 1) / kTok) return -1;
+    const int id = c.tables[(long long)lb * c.max_blocks + at];
+    if (id >= 0 && id < c.num_blocks) return id * c.Hkv + h;
+    report(status, kBadIndex);
+    return -1;
+  };
+  int unit = -1, next = look(0);  // block * Hkv + head, or -1
+  unsigned good = 0;              // bit BT i + k: that block is there
+  const uint32_t ring_at = sm100::smem_u32(ring) + lane % BT * 2 * L::kBytes, bar_at = sm100::smem_u32(&bars[warp][0]);
+  auto issue = [&](int i) {
+    if (i >= turns) return;
+    if (i % PER == 0) {
+      unit = next;
+      good = __ballot_sync(0xffffffffu, unit >= 0);
+      next = look(i + PER);
+    }
+    if (lane / BT == i % PER) {  // the lanes that looked the turn's blocks up
+      const uint32_t dst = ring_at + i % S * kStage, bar = bar_at + i % S * 8;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(unit >= 0 ? 2 * L::kBytes : 0) : "memory");
+      if (unit >= 0) {
+        const long long at = (long long)unit * L::kBytes;
+        bulk_load(dst, c.k_pool + at, L::kBytes, bar);
+        bulk_load(dst + L::kBytes, c.v_pool + at, L::kBytes, bar);
       }
-      const int shift = i % PER * BT, stage = (used + i) % S;
-      const unsigned ok = good >> shift & ((1u << BT) - 1);
-      const int blk = __shfl_sync(0xffffffffu, id, shift + lane % BT);
-      uint64_t* bar = &bars[warp][stage];
-      if (lane == 0) sm100::mbar_arrive_expect_tx(bar, __popc(ok) * 2 * L::kBytes);
-      __syncwarp();
-      if (lane < 2 * BT && (ok >> lane % BT & 1)) {  // lane: block lane % BT, K (the first lanes) or V
-        const uint8_t* src = (lane < BT ? c.k_pool : c.v_pool) + ((long long)blk * c.Hkv + h) * L::kBytes;
-        bulk_load(ring + stage * kStage + (lane % BT * 2 + lane / BT) * L::kBytes, src, L::kBytes, bar);
-      }
-    };
+    }
+  };
 #pragma unroll
-    for (int i = 0; i < S; ++i) issue(i);
+  for (int i = 0; i < S; ++i) issue(i);
 
-    W w;
-    w.load_q(q + ((long long)b * c.Hkv + h) * G * D, G, c.softcap > 0.f ? c.scale : c.scale * kLog2e);
-    const int tok = (g & 1) * 4 + (g >> 1);
-    float* srow = scores != nullptr ? scores + (((long long)b * c.Hkv + h) * c.max_blocks * kTok + tok) * Gs : nullptr;
-
-    for (int i = 0; i < mine; ++i) {
-      const int turn = used + i, stage = turn % S;
-      const bool here = sm100::mbar_wait_bounded(&bars[warp][stage], (turn / S) & 1, kWaitLimit);
+  const int tok = q4_token(g);
+  int b = line.seq, base = line.base, len = q4_len(c, b, nullptr), n = q4_turns(c, len);
+  while (n == 0) {  // (sequences without tokens hold nothing)
+    len = q4_len(c, ++b, nullptr);
+    n = q4_turns(c, len);
+  }
+  int h = (line.x - base) / n, p = line.x - base - h * n;
+  W w;
+  unsigned here_now = 0;  // `good` of the PER turns that are being worked on
+  for (int i = 0; i < turns;) {
+    // one part: turns p .. p1 of row (b, h)
+    const int p0 = p, p1 = min(n, p + turns - i), t0 = q4_first(c, len), jfirst = t0 / kTok;
+    const long long row = (long long)b * c.Hkv + h;
+    w.load_q(q + row * G * D, G, c.scale * kLog2e);
+    w.reset();
+    float* srow = scores != nullptr ? scores + (row * c.max_blocks * kTok + tok) * Gs : nullptr;
+    for (; p < p1; ++p, ++i) {
+      const int stage = i % S;
+      const bool here = sm100::mbar_wait_bounded(&bars[warp][stage], (i / S) & 1, kWaitLimit);
       if (!__all_sync(0xffffffffu, here)) {  // wait, bounded, for the copies still under way, then stop
         if (lane == 0) report(status, kTimeout);
-        for (int k = i + 1; k < min(mine, i + S); ++k)
-          sm100::mbar_wait_bounded(&bars[warp][(used + k) % S], ((used + k) / S) & 1, kWaitLimit);
-        alive = false;
-        break;
+        for (int k = i + 1; k < min(turns, i + S); ++k)
+          sm100::mbar_wait_bounded(&bars[warp][k % S], (k / S) & 1, kWaitLimit);
+        return;
       }
       const uint8_t* ks = ring + stage * kStage;
-      const int jb = jb0 + (i * kDecodeWarps + warp) * BT, at = jb * kTok;
-      // (copies run S turns ahead, at most into the next PER turns)
-      const unsigned ok = (min(mine - 1, i + S - 1) / PER == i / PER ? good : was) >> (i % PER * BT) & ((1u << BT) - 1);
+      const int jb = jfirst + p * BT, at = jb * kTok;
+      if (i % PER == 0) here_now = good;  // (copies run S - 1 < PER turns ahead: `good` is still this turn's)
+      const unsigned ok = here_now >> (i % PER * BT) & ((1u << BT) - 1);
       float* sc = srow != nullptr ? srow + (long long)at * Gs : nullptr;
       if (ok == (1u << BT) - 1 && at >= t0 && at + BT * kTok <= len) {
         w.template turn<false>(ks, 0u, c.softcap, sc, Gs);
@@ -670,71 +674,69 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
         for (int k = 0; k < 2 * BT; ++k) {
           const int y = at + (k >> 1) * kTok + tok + 8 * (k & 1);
           seen |= (unsigned)((ok >> (k >> 1) & 1) && y >= t0 && y < len) << k;
-          seen |= (unsigned)(y < len && jb + (k >> 1) < jb1) << (8 + k);
+          seen |= (unsigned)(y < len) << (8 + k);
         }
         w.template turn<true>(ks, seen, c.softcap, sc, Gs);
       }
       __syncwarp();  // every lane has read the stage
       issue(i + S);
     }
-    used += mine;
-
-    // the warps' sums, through shared memory (the ring is free once every warp is here)
-    if (!__syncthreads_and(alive)) return;
-    float* sm_o = reinterpret_cast<float*>(smem);                    // [warps][HT][D]
-    float* sm_ml = sm_o + kDecodeWarps * HT * D;                     // [warps][HT][2]
+    // the part's sums: over the quads for l and z, the outputs are whole in each lane (8 or 4 dimensions of two heads)
+    const long long slot = me + row;
+    const bool whole = p0 == 0 && p1 == n;
     const float back = pow2(w.ve - 130);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float y = w.l[n][e] * back;
+        const int head = nt * 8 + 2 * t + e;
+        float l = w.l[nt][e] * back;
 #pragma unroll
-        for (int k = 4; k < 32; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
-        const int head = n * 8 + 2 * t + e;
-        if (g == 0) {
-          sm_ml[(warp * HT + head) * 2] = w.m[n][e] - 8.f;
-          sm_ml[(warp * HT + head) * 2 + 1] = y;
-        }
+        for (int k = 4; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+        const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int r = 0; r < W::NG; ++r) {
-          float y = w.z[n][r][e] * back;
+          float z = w.z[nt][r][e] * back;
 #pragma unroll
-          for (int k = 4; k < 32; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
-          float* dst = sm_o + (warp * HT + head) * D + r * L::kGroup + g * W::MT * 2;
+          for (int k = 4; k < 32; k <<= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
+          if (head >= G) continue;
+          const int d = r * L::kGroup + g * W::MT * 2;
+          float x[W::MT * 2];
 #pragma unroll
           for (int k = 0; k < W::MT; ++k) {
-            dst[2 * k] = fmaf(w.o[n][r][k][e], back, y);
-            dst[2 * k + 1] = fmaf(w.o[n][r][k][e + 2], back, y);
+            x[2 * k] = fmaf(w.o[nt][r][k][e], back, z);
+            x[2 * k + 1] = fmaf(w.o[nt][r][k][e + 2], back, z);
+          }
+          if (whole) {
+            __nv_bfloat16* dst = out + (row * G + head) * D + d;
+#pragma unroll
+            for (int k = 0; k < W::MT * 2; k += 2)
+              *reinterpret_cast<__nv_bfloat162*>(dst + k) = __floats2bfloat162_rn(x[k] * inv, x[k + 1] * inv);
+          } else {
+            float* dst = part + (slot * G + head) * D + d;
+#pragma unroll
+            for (int k = 0; k < W::MT * 2; k += 4)
+              *reinterpret_cast<float4*>(dst + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
           }
         }
+        if (g == 0 && head < G && (!whole || scores != nullptr))
+          *reinterpret_cast<float2*>(ml + (slot * G + head) * 2) = make_float2(w.m[nt][e], l);
       }
-    __syncthreads();
-    const long long row = (long long)b * c.Hkv + h, slot = blockIdx.x + row;
-    const bool whole = p0 == 0 && p1 == n;
-    if (p0 == 0 && threadIdx.x == 0)  // the row's first slot and its parts, for q4_finish_kernel
-      plan[row] = make_int2((int)slot, (int)(q4_owner(x - (p1 - p0) + n - 1, total, gridDim.x) - blockIdx.x) + 1);
-    for (int y = threadIdx.x; y < G * D; y += kDecodeWarps * 32) {
-      const int head = y / D, d = y % D;
-      float M = -INFINITY, sum = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < kDecodeWarps; ++w) M = fmaxf(M, sm_ml[(w * HT + head) * 2]);
-#pragma unroll
-      for (int w = 0; w < kDecodeWarps; ++w) {
-        const float mw = sm_ml[(w * HT + head) * 2];
-        const float f = mw == -INFINITY ? 1.f : sm100::ex2_approx(mw - M);  // (an empty warp's sums are 0, or NaN)
-        sum += sm_ml[(w * HT + head) * 2 + 1] * f;
-        acc += sm_o[(w * HT + head) * D + d] * f;
-      }
-      if (whole) out[(row * G + head) * D + d] = __float2bfloat16(sum != 0.f ? acc / sum : 0.f);
-      else part[(slot * G + head) * D + d] = acc;
-      if (d == 0 && (!whole || scores != nullptr)) {
-        ml[(slot * G + head) * 2] = M;
-        ml[(slot * G + head) * 2 + 1] = sum;
+    if (p0 == 0 && lane == 0) {  // the row's first slot and its parts, for q4_finish_kernel
+      const int last = base + h * n + n - 1;
+      plan[row] = make_int2((int)slot, q4_owner(last, line.total, line.warps) - me + 1);
+    }
+    if (p == n) {  // the next row
+      p = 0;
+      if (++h == c.Hkv && i < turns) {
+        h = 0;
+        base += n * c.Hkv;
+        do {
+          len = q4_len(c, ++b, nullptr);
+          n = q4_turns(c, len);
+        } while (n == 0);
       }
     }
-    sm100::fence_async_shared();  // the next row's copies come after these reads and writes
-    __syncthreads();
   }
 }
 
@@ -742,8 +744,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
 RLB_DEVICE float2 q4_join(const float* ml, int G, int parts) {
   const int lane = threadIdx.x & 31;
   float M = -INFINITY, sum = 0.f;
+#pragma unroll 4
   for (int s = lane; s < parts; s += 32) M = fmaxf(M, ml[2LL * s * G]);
   M = warp_max(M);
+#pragma unroll 4
   for (int s = lane; s < parts; s += 32) {
     const float ms = ml[2LL * s * G], ls = ml[2LL * s * G + 1];
     sum += ms == -INFINITY ? ls : ls * sm100::ex2_approx(ms - M);
@@ -753,10 +757,10 @@ RLB_DEVICE float2 q4_join(const float* ml, int G, int parts) {
 }
 
 // Joins the parts of the rows that several CTAs of q4_decode_kernel shared, and writes zeros for empty sequences:
-// CTA z < G of a row does query head z, its four warps taking the parts in turn.  With `weights` the CTAs behind
+// CTA z < G of a row does query head z, its eight warps taking the parts in turn.  With `weights` the CTAs behind
 // add a stretch each of the tokens' attention weights, summed over the heads, to their accumulators.
 template <int D>
-__global__ void __launch_bounds__(128) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
+__global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
                                                         const float* __restrict__ ml, const int2* __restrict__ plan,
                                                         __nv_bfloat16* __restrict__ out,
                                                         const float* __restrict__ scores, int Gs,
@@ -765,7 +769,7 @@ __global__ void __launch_bounds__(128) q4_finish_kernel(Q4Cache c, const float* 
                                                         int w_len, int* status) {
   constexpr int E = D / 32;
   __shared__ float2 stat[16];
-  __shared__ float sums[4][D];
+  __shared__ float sums[8][D];
   cudaGridDependencySynchronize();  // (every CTA: what follows this kernel must not overtake the one before)
   const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, G = c.G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -773,30 +777,60 @@ __global__ void __launch_bounds__(128) q4_finish_kernel(Q4Cache c, const float* 
   const int len = q4_len(c, b, nullptr);
   if (len == 0) {
     if (z < G)
-      for (int d = threadIdx.x; d < D; d += 128) out[(row * G + z) * D + d] = __float2bfloat16(0.f);
+      for (int d = threadIdx.x; d < D; d += 256) out[(row * G + z) * D + d] = __float2bfloat16(0.f);
     return;
   }
   const int2 at = plan[row];  // first slot, parts
   const float* stats = ml + (long long)at.x * G * 2;
   if (z < G) {
     if (at.y == 1) return;  // written already
-    const float M = q4_join(stats + 2 * z, G, at.y).x;
-    float acc[E] = {}, sum = 0.f;
-#pragma unroll 4
-    for (int s = warp; s < at.y; s += 4) {
-      const float ms = stats[2LL * s * G + 2 * z], f = ms == -INFINITY ? 1.f : sm100::ex2_approx(ms - M);
-      const float* a = part + (((long long)at.x + s) * G + z) * D + lane;
-      sum += stats[2LL * s * G + 2 * z + 1] * f;
+    // each warp's share of the parts, 8 at a time, relative to the largest maximum so far (a part that saw nothing
+    // has none: its sums are 0, or NaN)
+    float M = -INFINITY, sum = 0.f, acc[E] = {};
+    for (int s0 = warp; s0 < at.y; s0 += 64) {
+      const int mine = s0 + 8 * (lane & 7);
+      const float2 x = mine < at.y ? *reinterpret_cast<const float2*>(stats + (2LL * mine * G + 2 * z)) : make_float2(-INFINITY, 0.f);
+      float a[8][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += a[32 * e] * f;
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          a[k][e] = s0 + 8 * k < at.y ? part[(((long long)at.x + s0 + 8 * k) * G + z) * D + lane + 32 * e] : 0.f;
+      float m = x.x;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      m = fmaxf(m, M);
+      const float was = M == -INFINITY ? 1.f : sm100::ex2_approx(M - m);
+      M = m;
+      sum *= was;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= was;
+      const float f = x.x == -INFINITY ? 1.f : sm100::ex2_approx(x.x - m);
+      const float l = x.y * f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sum += __shfl_sync(0xffffffffu, l, k);
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += a[k][e] * fk;
+      }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[warp][lane + 32 * e] = acc[e];
-    if (lane == 0) stat[warp].x = sum;
+    if (lane == 0) stat[warp] = make_float2(M, sum);
     __syncthreads();
-    const float total = stat[0].x + stat[1].x + stat[2].x + stat[3].x;
-    for (int d = threadIdx.x; d < D; d += 128) {
-      const float a = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
+    float most = -INFINITY, total = 0.f, f[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) most = fmaxf(most, stat[s].x);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      f[s] = stat[s].x == -INFINITY ? 1.f : sm100::ex2_approx(stat[s].x - most);
+      total += stat[s].y * f[s];
+    }
+    for (int d = threadIdx.x; d < D; d += 256) {
+      float a = 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) a += sums[s][d] * f[s];
       out[(row * G + z) * D + d] = __float2bfloat16(total != 0.f ? a / total : 0.f);
     }
     return;
@@ -805,15 +839,15 @@ __global__ void __launch_bounds__(128) q4_finish_kernel(Q4Cache c, const float* 
   if (r < 0) return;
   if (threadIdx.x == 0 && z == G && h == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
   if (r >= w_rows) return;
-  for (int head = warp; head < G; head += 4) {
+  for (int head = warp; head < G; head += 8) {
     const float2 x = q4_join(stats + 2 * head, G, at.y);
     if (lane == 0) stat[head] = x;
   }
   __syncthreads();
   float* w = weights + ((long long)r * c.Hkv + h) * w_len;
   const float* sc = scores + row * c.max_blocks * kTok * Gs;
-  const int step = (gridDim.z - G) * 128;
-  for (int t = q4_first(c, len) + (z - G) * 128 + threadIdx.x; t < min(len, w_len); t += step) {
+  const int step = (gridDim.z - G) * 256;
+  for (int t = q4_first(c, len) + (z - G) * 256 + threadIdx.x; t < min(len, w_len); t += step) {
     float p = 0.f;
     for (int head = 0; head < G; ++head)
       p += sm100::ex2_approx(sc[(long long)t * Gs + head] - stat[head].x) * stat[head].y;
@@ -998,9 +1032,7 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
 template <int D, int NT>
 static cudaError_t q4_decode_launch(const void* q, const Q4Cache& c, void* out, int B, int C, float* part, float* ml,
                                     int2* plan, float* scores, int Gs, int* status, cudaStream_t s) {
-  constexpr int ring = kDecodeWarps * q4_stages<D>() * q4_turn<D>() * 2 * Q4<D>::kBytes;
-  constexpr int join = kDecodeWarps * NT * 8 * (D + 2) * 4;
-  constexpr int smem = ring > join ? ring : join;
+  constexpr int smem = kDecodeWarps * q4_stages<D>() * q4_turn<D>() * 2 * Q4<D>::kBytes;
   static_assert(smem <= 47 * 1024, "above 48 KB a kernel has to ask for its shared memory");
   q4_decode_kernel<D, NT><<<C, kDecodeWarps * 32, smem, s>>>((const __nv_bfloat16*)q, c, B, (__nv_bfloat16*)out, part,
                                                               ml, plan, scores, Gs, status);
@@ -1022,22 +1054,26 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
                           float softcap, int window, int ctas, float* scratch, bool weighted, float* weights,
                           const int* weight_rows, long long w_rows, int w_len, int sms, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
+  // the kernel counts turns and blocks of all heads in 32 bits
+  if ((long long)B * Hkv * ((max_blocks + q4_turn_of(D) - 1) / q4_turn_of(D)) >= (1LL << 31) - (1 << 20) ||
+      (long long)num_blocks * Hkv >= 1LL << 31)
+    return cudaErrorInvalidValue;
   const Q4Cache c{(const uint8_t*)k_pool, (const uint8_t*)v_pool, tables, lens, Hkv, G, max_blocks, num_blocks,
                   window, q4_turn_of(D), scale, softcap};
   const int Gs = (G + 1) & ~1;
-  const long long slots = ctas + (long long)B * Hkv;
+  const long long slots = (long long)ctas * kDecodeWarps + (long long)B * Hkv;
   float* scores = weighted ? scratch : nullptr;  // first: written in pairs
   if (weighted) scratch += (long long)B * Hkv * max_blocks * kTok * Gs;
-  int2* plan = (int2*)scratch;
-  float* ml = scratch + 2LL * B * Hkv;
-  float* part = ml + slots * G * 2;
+  float* part = scratch;  // 16-byte pieces
+  float* ml = part + slots * G * D;
+  int2* plan = (int2*)(ml + slots * G * 2);
   cudaError_t e = cudaSuccess;
   RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, ctas, part, ml, plan, scores, Gs, status, s))
                       : (q4_decode_launch<DD, 2>(q, c, out, B, ctas, part, ml, plan, scores, Gs, status, s)));
   if (e != cudaSuccess) return e;
-  int chunks = 0;  // CTAs per row that add weights: four waves of the GPU, 128 tokens each at least
+  int chunks = 0;  // CTAs per row that add weights: four waves of the GPU, 256 tokens each at least
   if (weighted) {
-    const long long rows = (long long)B * Hkv, want = (32LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 127) / 128;
+    const long long rows = (long long)B * Hkv, want = (32LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 255) / 256;
     chunks = (int)(want < most ? want : most);
     if (chunks < 1) chunks = 1;
   }
@@ -1047,7 +1083,7 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(Hkv, B, G + chunks);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -1059,7 +1095,7 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
 
 long long rlb_q4_decode_scratch(int B, int Hkv, int G, int D, int max_blocks, int ctas, bool weighted) {
   const long long rows = (long long)B * Hkv;
-  return (weighted ? rows * max_blocks * kTok * ((G + 1) & ~1) : 0) + 2 * rows + (ctas + rows) * G * (D + 2);
+  return (weighted ? rows * max_blocks * kTok * ((G + 1) & ~1) : 0) + 2 * rows + (ctas * (long long)kDecodeWarps + rows) * G * (D + 2);
 }
 
 cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const int* lens, const int* new_tables,
