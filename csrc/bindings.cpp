@@ -944,7 +944,7 @@ std::vector<at::Tensor> token_logprob(const at::Tensor& logits, const at::Tensor
   float* st = stats.data_ptr<float>();
   CHECK_OK(rlb_token_logprob(logits.data_ptr(), logit_type(logits), logits.stride(0), N, (int)logits.size(1),
                              lptr(targets), (int)k, st, st + N, st + 2 * N, st + 3 * N, top_lp.data_ptr<float>(), lptr(top_ids),
-                             status_or_bounds(status, logits), cur_stream()),
+                             sm_count(), status_or_bounds(status, logits), cur_stream()),
            "token_logprob");
   return {stats[0], stats[1], stats[2], stats[3], top_lp, top_ids};
 }

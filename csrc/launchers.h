@@ -142,8 +142,8 @@ cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const in
 
 // Token log-probs, entropy and the k largest entries of each row of logits (dtype 0 fp32, 1 bf16, 2 fp16).
 cudaError_t rlb_token_logprob(const void* logits, int dtype, long long ld, long long rows, int V, const long long* tgt,
-                              int k, float* m, float* ls, float* lp, float* ent, float* top_lp, long long* top_ids, int* status,
-                              cudaStream_t s);
+                              int k, float* m, float* ls, float* lp, float* ent, float* top_lp, long long* top_ids,
+                              int sms, int* status, cudaStream_t s);
 cudaError_t rlb_token_logprob_bwd(const void* logits, int dtype, long long ld, long long rows, int V,
                                   const long long* tgt, const float* m, const float* ls, const float* ent,
                                   const long long* top_ids,

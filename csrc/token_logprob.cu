@@ -10,9 +10,11 @@
 // t = sum exp(x - m) (x - m) the entropy is log s - t / s.  Entries of -inf
 // (masked vocabulary) have p = 0 and add nothing; a row of nothing else has log-probs -inf, entropy 0 and no gradient.
 // A row with NaN or +inf gives NaN.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace rlb {
 
@@ -34,49 +36,243 @@ RLB_DEVICE unsigned long long rank_key(float x, int j) {
 }
 
 RLB_DEVICE unsigned long long max64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+RLB_DEVICE float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+RLB_DEVICE float exp_neg(float d) { return sm100::ex2_approx(d * 1.4426950408889634f); }  // d <= 0
 
 struct RowStats {
   float m, s, t;  // maximum, sum exp(x - m), sum exp(x - m) (x - m)
 };
 
-RLB_DEVICE RowStats merge(RowStats a, RowStats b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return RowStats{m, a.s + b.s, a.t + b.t};  // nothing yet (or NaN in the sums)
-  const float da = a.m - m, db = b.m - m;
-  const float fa = expf(da), fb = expf(db);
-  return RowStats{m, a.s * fa + b.s * fb,
-                  (fa == 0.f ? 0.f : fa * (a.t + da * a.s)) + (fb == 0.f ? 0.f : fb * (b.t + db * b.s))};
+// Statistics relative to a new, not smaller maximum.
+RLB_DEVICE void raise_to(RowStats& a, float m) {
+  const float d = a.m - m, f = a.m == m ? 1.f : a.m == -INFINITY ? 0.f : exp_neg(d);
+  a.t = f == 0.f ? 0.f : f * (a.t + d * a.s);
+  if (a.m == m) return;
+  a.s = f == 0.f && a.s == a.s ? 0.f : f * a.s;  // (NaN stays)
+  a.m = m;
 }
 
-RLB_DEVICE RowStats single(float x) {
-  return x == -INFINITY ? RowStats{-INFINITY, 0.f, 0.f} : RowStats{x, x - x + 1.f, 0.f};  // NaN and +inf: NaN
+RLB_DEVICE RowStats merge(RowStats a, RowStats b) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return RowStats{m, a.s + b.s, 0.f};  // nothing yet (or NaN in the sums)
+  if (a.m != m) raise_to(a, m);
+  if (b.m != m) raise_to(b, m);
+  return RowStats{m, a.s + b.s, a.t + b.t};
+}
+
+// VEC logits into the statistics; vm: their maximum, NaN if one is.
+template <int VEC>
+RLB_DEVICE void add_logits(RowStats& a, const float (&x)[VEC], float vm) {
+  if (vm > a.m) raise_to(a, vm);
+  const float m = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const float d = x[i] - m, e = exp_neg(d);
+    a.s += e;
+    a.t = fmaf(e, fmaxf(d, -1e30f), a.t);  // -inf: e is 0 and adds nothing
+  }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(512) token_logprob_kernel(const T* __restrict__ logits, long long ld, int V,
-                                                            const long long* __restrict__ tgt, int k,
-                                                            float* __restrict__ m_out, float* __restrict__ ls_out,
-                                                            float* __restrict__ lp_out,
-                                                            float* __restrict__ ent_out, float* __restrict__ top_lp,
-                                                            long long* __restrict__ top_ids, int* status) {
-  __shared__ RowStats red[16];
-  __shared__ unsigned long long best[16];
-  const long long r = blockIdx.x;
+RLB_DEVICE void load16(const T* p, float (&x)[16 / sizeof(T)]) {
+  const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));  // read once
+  const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) x[i] = to_f(e[i]);
+}
+
+template <typename T>
+RLB_DEVICE void store16(T* p, const float (&x)[16 / sizeof(T)]) {
+  uint4 v;
+  T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) e[i] = from_f<T>(x[i]);
+  __stcs(reinterpret_cast<uint4*>(p), v);
+}
+
+constexpr int kThreads = 512;
+constexpr int kHold = 256;                // candidates that may wait before the buffer is cut down
+constexpr int kRound = kThreads * 8;      // logits of a round, at most
+
+// The k largest keys of buf[0, c), largest first, into out (zeros behind).  The whole block calls it; keys differ.
+// Few candidates are ranked against each other, many are picked off one by one.
+RLB_DEVICE void pick_top(const unsigned long long* buf, int c, int k, unsigned long long* out,
+                         unsigned long long* scratch) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < k; i += kThreads) out[i] = 0;
+  __syncthreads();
+  if (c <= 2 * kThreads) {
+    for (int i = threadIdx.x; i < c; i += kThreads) {
+      const unsigned long long key = buf[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < c; ++j) rank += buf[j] > key;
+      if (rank < k) out[rank] = key;
+    }
+  } else {
+    unsigned long long below = ~0ull;
+    for (int n = 0; n < k; ++n) {
+      unsigned long long b = 0;
+      for (int i = threadIdx.x; i < c; i += kThreads)
+        if (buf[i] < below) b = max64(b, buf[i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) b = max64(b, __shfl_xor_sync(0xffffffffu, b, o));
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = b;
+      __syncthreads();
+      b = scratch[0];
+      for (int w = 1; w < kThreads / 32; ++w) b = max64(b, scratch[w]);
+      below = b;
+      if (threadIdx.x == 0) out[n] = b;
+    }
+  }
+  __syncthreads();
+}
+
+struct TopShared {
+  unsigned long long buf[kRound + kHold], out[kTopMost], scratch[kTopMost];
+  int count;
+};
+
+// A cluster of CTAs takes a row, each a slice (one CTA where there are rows enough to fill the GPU).  One pass: online
+// statistics per thread, and of the alternatives only those logits leave their registers that reach a bar known to
+// have k logits at or above it: at first the k-th largest of the maxima of 64 groups of 8 threads, later the k-th
+// largest candidate whenever more than kHold of them wait (checked once a round of 4096 logits, by the barrier
+// itself).  Rank 0 joins the slices over distributed shared memory.  Bound by the read of the logits.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprob_kernel(
+    const T* __restrict__ logits, long long ld, int V, const long long* __restrict__ tgt, int k,
+    float* __restrict__ m_out, float* __restrict__ ls_out, float* __restrict__ lp_out, float* __restrict__ ent_out,
+    float* __restrict__ top_lp, long long* __restrict__ top_ids, int* status) {
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(16) uint8_t dyn[];
+  TopShared& top = *reinterpret_cast<TopShared*>(dyn);
+  __shared__ RowStats red[kThreads / 32], mine;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int slices = cluster.num_blocks(), slice = cluster.block_rank();
+  const long long r = blockIdx.x / slices;
   const T* row = logits + r * ld;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
+  const int nvec = (V - head) / VEC;
+  const int v0 = (int)((long long)nvec * slice / slices), v1 = (int)((long long)nvec * (slice + 1) / slices);
   RowStats st{-INFINITY, 0.f, 0.f};
-  for (int j = threadIdx.x; j < V; j += 512) st = merge(st, single(to_f(row[j])));
+  unsigned long long bar = 0;  // keys from here on are candidates
+  float bar_x = -INFINITY;     // the bar's logit
+  bool full = false;           // this thread saw the buffer beyond kHold
+  if (TOP) {
+    if (tid == 0) top.count = 0;
+    __syncthreads();
+  }
+  auto offer = [&](float x, int j) {
+    const unsigned long long key = rank_key(x, j);
+    if (key >= bar) {
+      const int at = atomicAdd(&top.count, 1);
+      top.buf[at] = key;
+      full |= at >= kHold;
+    }
+  };
+  auto set_bar = [&](unsigned long long key) {
+    bar = key;
+    const uint32_t u = (uint32_t)(key >> 32);
+    bar_x = key == 0 ? -INFINITY : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+  };
+  // the row's unaligned ends, by single threads of the first and the last slice
+  auto ends = [&](int j) {
+    const float x[1] = {to_f(row[j])};
+    add_logits<1>(st, x, x[0]);
+    if (TOP) offer(x[0], j);
+  };
+  float x[VEC], next[VEC];
+  if (v0 + tid < v1) load16(row + head + (long long)(v0 + tid) * VEC, next);
+  for (int base = v0; base < v1; base += kThreads) {
+    const int v = base + tid;
+    const bool has = v < v1;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = next[i];
+    if (v + kThreads < v1) load16(row + head + (long long)(v + kThreads) * VEC, next);
+    float vm = -INFINITY;
+    if (has) {
+      vm = x[0];
+#pragma unroll
+      for (int i = 1; i < VEC; ++i) vm = max_nan(vm, x[i]);
+      add_logits<VEC>(st, x, vm);
+    }
+    if (TOP) {
+      const int j0 = head + v * VEC;
+      if (base == v0) {
+        unsigned long long best = 0;
+        if (has)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) best = max64(best, rank_key(x[i], j0 + i));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) best = max64(best, __shfl_xor_sync(0xffffffffu, best, o));
+        if ((tid & 7) == 0) top.scratch[tid >> 3] = best;
+        __syncthreads();
+        // the k-th largest of the 64 (absent groups: 0, so that fewer than k groups leave no bar)
+        if (tid < 64) {
+          const unsigned long long key = top.scratch[tid];
+          int rank = 0;
+          for (int i = 0; i < 64; ++i) rank += top.scratch[i] > key || (top.scratch[i] == key && i < tid);
+          if (rank == k - 1) top.out[0] = key;
+        }
+        __syncthreads();
+        set_bar(top.out[0]);
+      }
+      if (has && !(vm < bar_x))
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) offer(x[i], j0 + i);
+      if (__syncthreads_or(full)) {
+        const int c = top.count;
+        pick_top(top.buf, c, k, top.out, top.scratch);
+        if (tid < k) top.buf[tid] = top.out[tid];
+        if (tid == 0) top.count = k;  // (more than kHold >= k candidates waited)
+        set_bar(top.out[k - 1]);
+        full = false;
+        __syncthreads();
+      }
+    }
+  }
+  if (slice == 0 && tid < head) ends(tid);
+  if (slice == slices - 1 && tid < V - head - nvec * VEC) ends(head + nvec * VEC + tid);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     st = merge(st, RowStats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
                             __shfl_xor_sync(0xffffffffu, st.t, o)});
   if (lane == 0) red[warp] = st;
   __syncthreads();
-  st = red[0];
-  for (int w = 1; w < 16; ++w) st = merge(st, red[w]);
+  if (warp == 0) {
+    st = lane < kThreads / 32 ? red[lane] : RowStats{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+      st = merge(st, RowStats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+                              __shfl_xor_sync(0xffffffffu, st.t, o)});
+    if (lane == 0) mine = st;
+  }
+  if (TOP) pick_top(top.buf, top.count, k, top.out, top.scratch);
+  if (slices > 1) {
+    cluster.sync();
+    if (slice == 0) {
+      if (TOP) {
+        for (int i = tid; i < slices * k; i += kThreads) top.buf[i] = cluster.map_shared_rank(&top, i / k)->out[i % k];
+        pick_top(top.buf, slices * k, k, top.out, top.scratch);  // (zeros stand for nothing and rank last)
+      }
+      if (tid == 0)
+        for (int s = 1; s < slices; ++s) mine = merge(mine, *cluster.map_shared_rank(&mine, s));
+    }
+    cluster.sync();  // the others' shared memory is still read until here
+    if (slice != 0) return;
+  }
+  __syncthreads();
+  st = mine;
   const bool none = st.m == -INFINITY && st.s == 0.f;
   const float ls = logf(st.s);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     const long long tg = tgt[r];
     float lp = 0.f;
     if (tg >= V) report(status, kBadIndex);
@@ -86,61 +282,67 @@ __global__ void __launch_bounds__(512) token_logprob_kernel(const T* __restrict_
     lp_out[r] = lp;
     ent_out[r] = none ? 0.f : ls - st.t / st.s;
   }
-  unsigned long long below = ~0ull;  // the last one found; the next is the largest key under it
-  for (int i = 0; i < k; ++i) {
-    unsigned long long b = 0;
-    for (int j = threadIdx.x; j < V; j += 512) {
-      const unsigned long long key = rank_key(to_f(row[j]), j);
-      if (key < below) b = max64(b, key);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) b = max64(b, __shfl_xor_sync(0xffffffffu, b, o));
-    __syncthreads();
-    if (lane == 0) best[warp] = b;
-    __syncthreads();
-    b = best[0];
-    for (int w = 1; w < 16; ++w) b = max64(b, best[w]);
-    below = b;
-    if (threadIdx.x == 0) {
-      const int j = (int)~(uint32_t)b;
-      top_ids[r * k + i] = j;
-      top_lp[r * k + i] = none ? -INFINITY : to_f(row[j]) - st.m - ls;
-    }
+  if (TOP && tid < k) {
+    const int j = (int)~(uint32_t)top.out[tid];
+    top_ids[r * k + tid] = j;
+    top_lp[r * k + tid] = none ? -INFINITY : to_f(row[j]) - st.m - ls;
   }
 }
 
+// One CTA per stretch of a row.  Bound by the read of the logits and the write of their gradient.
+constexpr int kBwdThreads = 256;
+constexpr int kBwdStretch = kBwdThreads * 8 * 8;  // logits
+
 template <typename T>
-__global__ void __launch_bounds__(512) token_logprob_bwd_kernel(
-    const T* __restrict__ logits, long long ld, int V, const long long* __restrict__ tgt,
-    const float* __restrict__ row_m, const float* __restrict__ row_ls, const float* __restrict__ ent, const long long* __restrict__ top_ids, int k,
-    const float* __restrict__ g_lp, const float* __restrict__ g_ent, const float* __restrict__ g_top,
-    T* __restrict__ dx) {
-  const long long r = blockIdx.x;
+__global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_kernel(
+    const T* __restrict__ logits, long long ld, int V, int stretches, const long long* __restrict__ tgt,
+    const float* __restrict__ row_m, const float* __restrict__ row_ls, const float* __restrict__ ent,
+    const long long* __restrict__ top_ids, int k, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
+    const float* __restrict__ g_top, T* __restrict__ dx) {
+  constexpr int VEC = 16 / sizeof(T);
+  const long long r = blockIdx.x / stretches;
+  const int j0 = (int)(blockIdx.x % stretches) * kBwdStretch, j1 = (int)min((long long)V, (long long)j0 + kBwdStretch);
   const T* row = logits + r * ld;
   T* out = dx + r * V;
-  const float m = row_m[r], ls = row_ls[r];
+  const float m = row_m[r], ls = row_ls[r], H = ent[r];
   const long long tg = tgt[r];
   const bool has = tg >= 0 && tg < V;
-  const float g = g_lp && has ? g_lp[r] : 0.f, e = g_ent ? g_ent[r] : 0.f, H = ent[r];
+  const float g = g_lp && has ? g_lp[r] : 0.f, e = g_ent ? g_ent[r] : 0.f;
   float a = g;
   if (g_top)
     for (int i = 0; i < k; ++i) a += g_top[r * k + i];
+  const float c0 = -(a + e * H), c1 = -e;
   auto grad = [&](float x) {
-    const float logp = (x - m) - ls;
-    const float p = expf(logp);
-    return p == 0.f || m == -INFINITY ? 0.f : -p * (a + e * (logp + H));
+    // p is 0 from log p < -104 on: the bound keeps 0 times -inf out (a row of NaN stays NaN by its entropy)
+    const float logp = fmaxf((x - m) - ls, -200.f);
+    return exp_neg(logp) * fmaf(c1, logp, c0);
   };
-  for (int j = threadIdx.x; j < V; j += 512) out[j] = from_f<T>(grad(to_f(row[j])));
+  // whole vectors where the row and its gradient are aligned alike, single entries at the ends (or everywhere)
+  const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const int lead = (int)((16 - (reinterpret_cast<uintptr_t>(row + j0) & 15)) & 15) / (int)sizeof(T);
+  const int w0 = alike ? min(j1, j0 + lead) : j1, nvec = (j1 - w0) / VEC;
+#pragma unroll 2
+  for (int v = threadIdx.x; v < nvec; v += kBwdThreads) {
+    float x[VEC];
+    load16(row + w0 + v * VEC, x);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = grad(x[i]);
+    store16(out + w0 + v * VEC, x);
+  }
+  for (int j = j0 + threadIdx.x; j < w0; j += kBwdThreads) out[j] = from_f<T>(grad(to_f(row[j])));
+  for (int j = w0 + nvec * VEC + threadIdx.x; j < j1; j += kBwdThreads) out[j] = from_f<T>(grad(to_f(row[j])));
   __syncthreads();
   if (m == -INFINITY) return;
-  // the target's and the alternatives' entries again, with their own terms, rounded once
-  const int i = threadIdx.x - 1;
-  if (i >= (g_top ? k : 0) || (i < 0 && !has)) return;
-  const long long j = i < 0 ? tg : top_ids[r * k + i];
-  float d = grad(to_f(row[j])) + (has && j == tg ? g : 0.f);
-  if (g_top)
-    for (int u = 0; u < k; ++u) d += top_ids[r * k + u] == j ? g_top[r * k + u] : 0.f;
-  out[j] = from_f<T>(d);
+  // the target's and the alternatives' entries of this stretch again, with their own terms, rounded once
+  for (int i = (int)threadIdx.x - 1; i < (g_top ? k : 0); i += kBwdThreads) {
+    if (i < 0 && !has) continue;
+    const long long j = i < 0 ? tg : top_ids[r * k + i];
+    if (j < j0 || j >= j1) continue;
+    float d = grad(to_f(row[j])) + (has && j == tg ? g : 0.f);
+    if (g_top)
+      for (int u = 0; u < k; ++u) d += top_ids[r * k + u] == j ? g_top[r * k + u] : 0.f;
+    out[j] = from_f<T>(d);
+  }
 }
 
 }  // namespace rlb
@@ -155,23 +357,50 @@ using namespace rlb;
     else return cudaErrorNotSupported;                             \
   } while (0)
 
+template <typename T, bool TOP>
+static cudaError_t token_logprob_launch(const void* logits, long long ld, long long rows, int V, const long long* tgt,
+                                        int k, float* m, float* ls, float* lp, float* ent, float* top_lp,
+                                        long long* top_ids, int sms, int* status, cudaStream_t s) {
+  // Slices: as long as the CTAs fit on the GPU at a time and a slice keeps a round of logits (a single row of 128256 in
+  // bf16 takes 8 of them; from 3 rows per SM on a row stays whole).
+  int slices = 1;
+  while (slices < 8 && rows * slices * 2 <= 3LL * sms && V / (slices * 2) >= kRound) slices *= 2;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = slices;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * slices));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = TOP ? sizeof(TopShared) : 0;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, TOP>, (const T*)logits, ld, V, tgt, k, m, ls, lp, ent, top_lp,
+                            top_ids, status);
+}
+
 cudaError_t rlb_token_logprob(const void* logits, int dtype, long long ld, long long rows, int V, const long long* tgt,
-                              int k, float* m, float* ls, float* lp, float* ent, float* top_lp, long long* top_ids, int* status,
-                              cudaStream_t s) {
+                              int k, float* m, float* ls, float* lp, float* ent, float* top_lp, long long* top_ids,
+                              int sms, int* status, cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
-  if (k > kTopMost) return cudaErrorInvalidValue;
-  RLB_LOGIT_TYPE((token_logprob_kernel<T><<<(unsigned)rows, 512, 0, s>>>((const T*)logits, ld, V, tgt, k, m, ls, lp, ent,
-                                                                         top_lp, top_ids, status)));
-  return cudaGetLastError();
+  if (k > kTopMost || rows > (1LL << 31) - 1) return cudaErrorInvalidValue;
+  cudaError_t e = cudaSuccess;
+  RLB_LOGIT_TYPE((e = k > 0 ? token_logprob_launch<T, true>(logits, ld, rows, V, tgt, k, m, ls, lp, ent, top_lp, top_ids,
+                                                            sms, status, s)
+                            : token_logprob_launch<T, false>(logits, ld, rows, V, tgt, k, m, ls, lp, ent, top_lp,
+                                                             top_ids, sms, status, s)));
+  return e;
 }
 
 cudaError_t rlb_token_logprob_bwd(const void* logits, int dtype, long long ld, long long rows, int V,
                                   const long long* tgt, const float* m, const float* ls, const float* ent,
-                                  const long long* top_ids,
-                                  int k, const float* g_lp, const float* g_ent, const float* g_top, void* dx,
-                                  cudaStream_t s) {
+                                  const long long* top_ids, int k, const float* g_lp, const float* g_ent,
+                                  const float* g_top, void* dx, cudaStream_t s) {
   if (rows == 0) return cudaSuccess;
-  RLB_LOGIT_TYPE((token_logprob_bwd_kernel<T><<<(unsigned)rows, 512, 0, s>>>(
-      (const T*)logits, ld, V, tgt, m, ls, ent, top_ids, k, g_lp, g_ent, g_top, (T*)dx)));
+  const long long stretches = ((long long)V + kBwdStretch - 1) / kBwdStretch;
+  if (rows * stretches > (1LL << 31) - 1) return cudaErrorInvalidValue;
+  RLB_LOGIT_TYPE((token_logprob_bwd_kernel<T><<<(unsigned)(rows * stretches), kBwdThreads, 0, s>>>(
+      (const T*)logits, ld, V, (int)stretches, tgt, m, ls, ent, top_ids, k, g_lp, g_ent, g_top, (T*)dx)));
   return cudaGetLastError();
 }
