@@ -1,17 +1,18 @@
 // Log-probabilities of given tokens, entropy and the top alternatives from materialised logits, with the gradient.
 //
-//   log p_rj = (x_rj - m_r) - log sum_j exp(x_rj - m_r),  m_r = max_j x_rj
+//   log p_rj = (x_rj - m_r) - log sum_j exp(x_rj - m_r),  m_r about max_j x_rj
 //   lp[r] = log p_r,tgt  (0 where tgt < 0)      ent[r] = -sum_j p_rj log p_rj
 //   the k largest x_rj in falling order, the lowest index first among equals, as log-probs and ids
 // and, with incoming gradients g (log-prob), e (entropy) and u_i (alternatives with ids id_i),
 //   dx_j = g [j = tgt] + sum_i u_i [j = id_i] - (g + sum_i u_i) p_j - e p_j (log p_j + ent).
-// Everything is relative to the row's maximum, also what the backward pass gets (m and log s, with s the sum): a
+// Everything is relative to about the row's maximum, also what the backward pass gets (m and log s, s the sum): a
 // large common offset of the logits, up to rows of the type's lowest value, then cancels exactly.  With
 // t = sum exp(x - m) (x - m) the entropy is log s - t / s.  Entries of -inf
 // (masked vocabulary) have p = 0 and add nothing; a row of nothing else has log-probs -inf, entropy 0 and no gradient.
 // A row with NaN or +inf gives NaN.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -41,45 +42,47 @@ RLB_DEVICE float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-RLB_DEVICE float exp_neg(float d) { return sm100::ex2_approx(d * 1.4426950408889634f); }  // d <= 0
+RLB_DEVICE float fast_exp(float d) { return sm100::ex2_approx(d * 1.4426950408889634f); }
 
 struct RowStats {
-  float m, s, t;  // maximum, sum exp(x - m), sum exp(x - m) (x - m)
+  float m, s, t;  // a reference no more than kSlack below the maximum, sum exp(x - m), sum exp(x - m) (x - m)
 };
+constexpr float kSlack = 8.f;
 
 // Statistics relative to a new, not smaller maximum.
 RLB_DEVICE void raise_to(RowStats& a, float m) {
-  const float d = a.m - m, f = a.m == m ? 1.f : a.m == -INFINITY ? 0.f : exp_neg(d);
+  const float d = a.m - m, f = a.m == m ? 1.f : a.m == -INFINITY ? 0.f : fast_exp(d);
   a.t = f == 0.f ? 0.f : f * (a.t + d * a.s);
   if (a.m == m) return;
   a.s = f == 0.f && a.s == a.s ? 0.f : f * a.s;  // (NaN stays)
   a.m = m;
 }
 
-RLB_DEVICE RowStats merge(RowStats a, RowStats b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return RowStats{m, a.s + b.s, 0.f};  // nothing yet (or NaN in the sums)
-  if (a.m != m) raise_to(a, m);
-  if (b.m != m) raise_to(b, m);
-  return RowStats{m, a.s + b.s, a.t + b.t};
+// Statistics of a warp's lanes as one, in every lane: one common reference, then plain sums.
+RLB_DEVICE RowStats warp_stats(RowStats a) {
+  const float m = warp_max(a.m);
+  if (m != -INFINITY) raise_to(a, m);
+  return RowStats{m, warp_sum(a.s), warp_sum(a.t)};
 }
 
 // VEC logits into the statistics; vm: their maximum, NaN if one is.
 template <int VEC>
 RLB_DEVICE void add_logits(RowStats& a, const float (&x)[VEC], float vm) {
-  if (vm > a.m) raise_to(a, vm);
+  if (vm > a.m + kSlack) raise_to(a, vm);  // (rarely after the first logits: no new maximum costs a rescaling)
   const float m = a.m == -INFINITY ? 0.f : a.m;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const float d = x[i] - m, e = exp_neg(d);
+    const float d = x[i] - m, e = fast_exp(d);
     a.s += e;
     a.t = fmaf(e, fmaxf(d, -1e30f), a.t);  // -inf: e is 0 and adds nothing
   }
 }
 
 template <typename T>
-RLB_DEVICE void load16(const T* p, float (&x)[16 / sizeof(T)]) {
-  const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));  // read once
+RLB_DEVICE uint4 load16(const T* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }  // read once
+
+template <typename T>
+RLB_DEVICE void unpack16(const uint4& v, float* x) {
   const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
   for (int i = 0; i < (int)(16 / sizeof(T)); ++i) x[i] = to_f(e[i]);
@@ -95,8 +98,9 @@ RLB_DEVICE void store16(T* p, const float (&x)[16 / sizeof(T)]) {
 }
 
 constexpr int kThreads = 512;
-constexpr int kHold = 256;                // candidates that may wait before the buffer is cut down
-constexpr int kRound = kThreads * 8;      // logits of a round, at most
+constexpr int kHold = 160;                // candidates that may wait before the buffer is cut down, at most
+constexpr int kEach = 16;                 // logits of a thread in a round
+constexpr int kRound = kThreads * kEach;  // logits of a round, at most
 
 // The k largest keys of buf[0, c), largest first, into out (zeros behind).  The whole block calls it; keys differ.
 // Few candidates are ranked against each other, many are picked off one by one.
@@ -106,12 +110,16 @@ RLB_DEVICE void pick_top(const unsigned long long* buf, int c, int k, unsigned l
   for (int i = threadIdx.x; i < k; i += kThreads) out[i] = 0;
   __syncthreads();
   if (c <= 2 * kThreads) {
-    for (int i = threadIdx.x; i < c; i += kThreads) {
-      const unsigned long long key = buf[i];
+    // P neighbouring threads share a candidate's comparisons
+    const int P = c <= 64 ? 8 : c <= 128 ? 4 : c <= 256 ? 2 : 1, part = threadIdx.x % P;
+    for (int i0 = 0; i0 < c; i0 += kThreads / P) {
+      const int i = i0 + threadIdx.x / P;
+      const unsigned long long key = i < c ? buf[i] : ~0ull;
       int rank = 0;
 #pragma unroll 8
-      for (int j = 0; j < c; ++j) rank += buf[j] > key;
-      if (rank < k) out[rank] = key;
+      for (int j = part; j < c; j += P) rank += buf[j] > key;
+      for (int o = 1; o < P; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      if (i < c && part == 0 && rank < k) out[rank] = key;
     }
   } else {
     unsigned long long below = ~0ull;
@@ -141,14 +149,14 @@ struct TopShared {
 // A cluster of CTAs takes a row, each a slice (one CTA where there are rows enough to fill the GPU).  One pass: online
 // statistics per thread, and of the alternatives only those logits leave their registers that reach a bar known to
 // have k logits at or above it: at first the k-th largest of the maxima of 64 groups of 8 threads, later the k-th
-// largest candidate whenever more than kHold of them wait (checked once a round of 4096 logits, by the barrier
+// largest candidate whenever more than 2 k + 32 of them wait (checked once a round of 8192 logits, by the barrier
 // itself).  Rank 0 joins the slices over distributed shared memory.  Bound by the read of the logits.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprob_kernel(
+__global__ void __launch_bounds__(kThreads, 2) token_logprob_kernel(
     const T* __restrict__ logits, long long ld, int V, const long long* __restrict__ tgt, int k,
     float* __restrict__ m_out, float* __restrict__ ls_out, float* __restrict__ lp_out, float* __restrict__ ent_out,
     float* __restrict__ top_lp, long long* __restrict__ top_ids, int* status) {
-  constexpr int VEC = 16 / sizeof(T);
+  constexpr int VEC = 16 / sizeof(T), U = kEach / VEC;
   extern __shared__ __align__(16) uint8_t dyn[];
   TopShared& top = *reinterpret_cast<TopShared*>(dyn);
   __shared__ RowStats red[kThreads / 32], mine;
@@ -164,7 +172,8 @@ __global__ void __launch_bounds__(kThreads) token_logprob_kernel(
   RowStats st{-INFINITY, 0.f, 0.f};
   unsigned long long bar = 0;  // keys from here on are candidates
   float bar_x = -INFINITY;     // the bar's logit
-  bool full = false;           // this thread saw the buffer beyond kHold
+  bool full = false;           // this thread saw more than `hold` candidates wait
+  const int hold = 2 * k + 32;
   if (TOP) {
     if (tid == 0) top.count = 0;
     __syncthreads();
@@ -174,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) token_logprob_kernel(
     if (key >= bar) {
       const int at = atomicAdd(&top.count, 1);
       top.buf[at] = key;
-      full |= at >= kHold;
+      full |= at >= hold;
     }
   };
   auto set_bar = [&](unsigned long long key) {
@@ -188,50 +197,62 @@ __global__ void __launch_bounds__(kThreads) token_logprob_kernel(
     add_logits<1>(st, x, x[0]);
     if (TOP) offer(x[0], j);
   };
-  float x[VEC], next[VEC];
-  if (v0 + tid < v1) load16(row + head + (long long)(v0 + tid) * VEC, next);
-  for (int base = v0; base < v1; base += kThreads) {
-    const int v = base + tid;
-    const bool has = v < v1;
+  const uint4 absent = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)  // -inf
+                       : std::is_same<T, __half>::value ? make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u)
+                                                        : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+  const T* data = row + head;
+  uint4 next[U];
+  auto fetch = [&](int base) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = next[i];
-    if (v + kThreads < v1) load16(row + head + (long long)(v + kThreads) * VEC, next);
-    float vm = -INFINITY;
-    if (has) {
-      vm = x[0];
-#pragma unroll
-      for (int i = 1; i < VEC; ++i) vm = max_nan(vm, x[i]);
-      add_logits<VEC>(st, x, vm);
+    for (int u = 0; u < U; ++u) {
+      const int v = base + u * kThreads + tid;
+      next[u] = v < v1 ? load16(data + (long long)v * VEC) : absent;
     }
-    if (TOP) {
-      const int j0 = head + v * VEC;
-      if (base == v0) {
-        unsigned long long best = 0;
-        if (has)
+  };
+  fetch(v0);
+  for (int base = v0; base < v1; base += U * kThreads) {
+    float x[U * VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) best = max64(best, rank_key(x[i], j0 + i));
+    for (int u = 0; u < U; ++u) unpack16<T>(next[u], x + u * VEC);
+    if (base + U * kThreads < v1) fetch(base + U * kThreads);
+    float vm = x[0];
+#pragma unroll
+    for (int i = 1; i < U * VEC; ++i) vm = max_nan(vm, x[i]);
+    add_logits<U * VEC>(st, x, vm);
+    if (TOP) {
+      const int j0 = head + (base + tid) * VEC;  // vector u begins u * kThreads * VEC behind
+      if (base == v0) {
+        // (a key no larger than the maximum's: the last place that this thread could have it at)
+        const bool has = base + tid < v1;
+        unsigned long long best = has ? rank_key(vm, V - 1) : 0;
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) best = max64(best, __shfl_xor_sync(0xffffffffu, best, o));
         if ((tid & 7) == 0) top.scratch[tid >> 3] = best;
         __syncthreads();
         // the k-th largest of the 64 (absent groups: 0, so that fewer than k groups leave no bar)
-        if (tid < 64) {
-          const unsigned long long key = top.scratch[tid];
-          int rank = 0;
-          for (int i = 0; i < 64; ++i) rank += top.scratch[i] > key || (top.scratch[i] == key && i < tid);
-          if (rank == k - 1) top.out[0] = key;
-        }
+        const int at = tid >> 3;
+        const unsigned long long key = top.scratch[at];
+        int rank = 0;
+#pragma unroll
+        for (int i = tid & 7; i < 64; i += 8) rank += top.scratch[i] > key || (top.scratch[i] == key && i < at);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (rank == k - 1 && (tid & 7) == 0) top.out[0] = key;
         __syncthreads();
         set_bar(top.out[0]);
       }
-      if (has && !(vm < bar_x))
+      if (!(vm < bar_x))
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) offer(x[i], j0 + i);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (!(x[u * VEC + i] < bar_x) && base + u * kThreads + tid < v1)
+              offer(x[u * VEC + i], j0 + u * kThreads * VEC + i);
       if (__syncthreads_or(full)) {
         const int c = top.count;
         pick_top(top.buf, c, k, top.out, top.scratch);
         if (tid < k) top.buf[tid] = top.out[tid];
-        if (tid == 0) top.count = k;  // (more than kHold >= k candidates waited)
+        if (tid == 0) top.count = k;  // (more than k candidates waited)
         set_bar(top.out[k - 1]);
         full = false;
         __syncthreads();
@@ -240,18 +261,11 @@ __global__ void __launch_bounds__(kThreads) token_logprob_kernel(
   }
   if (slice == 0 && tid < head) ends(tid);
   if (slice == slices - 1 && tid < V - head - nvec * VEC) ends(head + nvec * VEC + tid);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    st = merge(st, RowStats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                            __shfl_xor_sync(0xffffffffu, st.t, o)});
+  st = warp_stats(st);
   if (lane == 0) red[warp] = st;
   __syncthreads();
   if (warp == 0) {
-    st = lane < kThreads / 32 ? red[lane] : RowStats{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
-      st = merge(st, RowStats{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                              __shfl_xor_sync(0xffffffffu, st.t, o)});
+    st = warp_stats(lane < kThreads / 32 ? red[lane] : RowStats{-INFINITY, 0.f, 0.f});
     if (lane == 0) mine = st;
   }
   if (TOP) pick_top(top.buf, top.count, k, top.out, top.scratch);
@@ -262,8 +276,11 @@ __global__ void __launch_bounds__(kThreads) token_logprob_kernel(
         for (int i = tid; i < slices * k; i += kThreads) top.buf[i] = cluster.map_shared_rank(&top, i / k)->out[i % k];
         pick_top(top.buf, slices * k, k, top.out, top.scratch);  // (zeros stand for nothing and rank last)
       }
-      if (tid == 0)
-        for (int s = 1; s < slices; ++s) mine = merge(mine, *cluster.map_shared_rank(&mine, s));
+      if (warp == 0) {
+        st = warp_stats(lane < slices ? *cluster.map_shared_rank(&mine, lane) : RowStats{-INFINITY, 0.f, 0.f});
+        __syncwarp();
+        if (lane == 0) mine = st;
+      }
     }
     cluster.sync();  // the others' shared memory is still read until here
     if (slice != 0) return;
@@ -315,7 +332,7 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_kernel(
   auto grad = [&](float x) {
     // p is 0 from log p < -104 on: the bound keeps 0 times -inf out (a row of NaN stays NaN by its entropy)
     const float logp = fmaxf((x - m) - ls, -200.f);
-    return exp_neg(logp) * fmaf(c1, logp, c0);
+    return fast_exp(logp) * fmaf(c1, logp, c0);
   };
   // whole vectors where the row and its gradient are aligned alike, single entries at the ends (or everywhere)
   const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
@@ -324,7 +341,7 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_kernel(
 #pragma unroll 2
   for (int v = threadIdx.x; v < nvec; v += kBwdThreads) {
     float x[VEC];
-    load16(row + w0 + v * VEC, x);
+    unpack16<T>(load16(row + w0 + v * VEC), x);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) x[i] = grad(x[i]);
     store16(out + w0 + v * VEC, x);
@@ -361,10 +378,10 @@ template <typename T, bool TOP>
 static cudaError_t token_logprob_launch(const void* logits, long long ld, long long rows, int V, const long long* tgt,
                                         int k, float* m, float* ls, float* lp, float* ent, float* top_lp,
                                         long long* top_ids, int sms, int* status, cudaStream_t s) {
-  // Slices: as long as the CTAs fit on the GPU at a time and a slice keeps a round of logits (a single row of 128256 in
-  // bf16 takes 8 of them; from 3 rows per SM on a row stays whole).
+  // Slices: as long as the CTAs fit on the GPU at a time and a slice keeps half a round of logits (a single row of 128256 in
+  // bf16 takes 8 of them; with more rows than SMs a row stays whole).
   int slices = 1;
-  while (slices < 8 && rows * slices * 2 <= 3LL * sms && V / (slices * 2) >= kRound) slices *= 2;
+  while (slices < 8 && rows * slices * 2 <= 2LL * sms && V / (slices * 2) >= kRound / 2) slices *= 2;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = slices;
@@ -376,6 +393,11 @@ static cudaError_t token_logprob_launch(const void* logits, long long ld, long l
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  if (TOP) {
+    const cudaError_t e = cudaFuncSetAttribute(token_logprob_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)sizeof(TopShared));
+    if (e != cudaSuccess) return e;
+  }
   return cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, TOP>, (const T*)logits, ld, V, tgt, k, m, ls, lp, ent, top_lp,
                             top_ids, status);
 }
