@@ -924,29 +924,36 @@ static int logit_type(const at::Tensor& x) {
   return x.scalar_type() == at::kFloat ? 0 : x.scalar_type() == at::kBFloat16 ? 1 : x.scalar_type() == at::kHalf ? 2 : -1;
 }
 
-// logits [N, V] (unit inner stride), targets [N] int64 -> {maximum, log of the sum, lp, ent [N], top_lp [N, k] fp32,
-// top_ids [N, k] int64}
-std::vector<at::Tensor> token_logprob(const at::Tensor& logits, const at::Tensor& targets, int64_t k,
+// logits [N, V] (unit inner stride), targets [N] int64 -> {lp, ent [N], top_lp [N, k] fp32, top_ids [N, k] int64}, and with
+// `stats` what the backward pass needs: {reference, log of the sum [N] fp32}
+std::vector<at::Tensor> token_logprob(const at::Tensor& logits, const at::Tensor& targets, int64_t k, bool stats,
                                       const c10::optional<at::Tensor>& status) {
   check_cuda(logits, "logits");
   TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) < (1LL << 31) && logits.stride(1) == 1 &&
-                        logits.size(0) < (1LL << 31), "logits: [N, V] with unit inner stride");
+                  logits.size(0) < (1LL << 31), "logits: [N, V] with unit inner stride");
   TORCH_CHECK(logit_type(logits) >= 0, "logits: fp32, bf16 or fp16");
   check_dev(targets, logits, "targets");
   TORCH_CHECK(targets.scalar_type() == at::kLong && targets.is_contiguous() && targets.dim() == 1 &&
-                        targets.size(0) == logits.size(0), "targets: contiguous int64 [N]");
+                  targets.size(0) == logits.size(0), "targets: contiguous int64 [N]");
   TORCH_CHECK(k >= 0 && k <= 64 && k <= logits.size(1), "top: 0 to 64, and no more than the vocabulary");
   const c10::cuda::CUDAGuard g(logits.device());
   const int64_t N = logits.size(0);
   auto fopt = logits.options().dtype(at::kFloat);
-  auto stats = at::empty({4, N}, fopt);
-  auto top_lp = at::empty({N, k}, fopt), top_ids = at::empty({N, k}, logits.options().dtype(at::kLong));
-  float* st = stats.data_ptr<float>();
+  auto lp = at::empty({N}, fopt), ent = at::empty({N}, fopt), top_lp = at::empty({N, k}, fopt);
+  auto top_ids = at::empty({N, k}, logits.options().dtype(at::kLong));
+  at::Tensor m, ls;
+  if (stats) {
+    m = at::empty({N}, fopt);
+    ls = at::empty({N}, fopt);
+  }
   CHECK_OK(rlb_token_logprob(logits.data_ptr(), logit_type(logits), logits.stride(0), N, (int)logits.size(1),
-                             lptr(targets), (int)k, st, st + N, st + 2 * N, st + 3 * N, top_lp.data_ptr<float>(), lptr(top_ids),
-                             sm_count(), status_or_bounds(status, logits), cur_stream()),
+                             lptr(targets), (int)k, stats ? m.data_ptr<float>() : nullptr,
+                             stats ? ls.data_ptr<float>() : nullptr, lp.data_ptr<float>(), ent.data_ptr<float>(),
+                             top_lp.data_ptr<float>(), lptr(top_ids), sm_count(), status_or_bounds(status, logits),
+                             cur_stream()),
            "token_logprob");
-  return {stats[0], stats[1], stats[2], stats[3], top_lp, top_ids};
+  if (stats) return {lp, ent, top_lp, top_ids, m, ls};
+  return {lp, ent, top_lp, top_ids};
 }
 
 at::Tensor token_logprob_bwd(const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& m,

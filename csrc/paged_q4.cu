@@ -32,6 +32,41 @@ RLB_DEVICE float bf16_hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u)
 // ---------------------------------------------------------------- storing rows
 // A group's threads reduce its minimum and maximum by shuffles (NaN-propagating), then each quantises its 8
 // elements to one 32-bit word.  Bound by memory: 2 bytes read and about 0.56 written per element.
+//
+// code = clamp(rint((x - lo) / s)) without a division per element: y = fma(x - lo, 1 / s, 1.5 2^23) rounds to a whole
+// number c, and the remainder r = fma(-c, s, x - lo) tells whether that is the nearest (|r| <= s / 2, and c even
+// where both are equal); only then a neighbour is taken.
+RLB_DEVICE uint32_t q4_codes(const bf16x8& x, float lo, float s) {
+  float f[8];
+  unpack8(x, f);
+  uint32_t word = 0;
+  if (!(s >= 1e-36f && s < INFINITY)) {  // no spread, one too small for 1 / s, or not finite (all codes are 0)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(f[e] - lo, s)), 0.f), 15.f) << (4 * e);  // NaN becomes 0
+    return word;
+  }
+  const float inv = __fdividef(1.f, s), h = 0.5f * s;
+  float r[8], far = 0.f;
+  int c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float d = f[e] - lo, y = fmaf(d, inv, 12582912.f);
+    c[e] = __float_as_int(y) - 0x4b400000;
+    r[e] = fmaf(12582912.f - y, s, d);
+    far = fmaxf(far, fabsf(r[e]));
+  }
+  if (far >= h) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (fabsf(r[e]) > h || (fabsf(r[e]) == h && (c[e] & 1))) c[e] += r[e] > 0.f ? 1 : -1;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) word |= (uint32_t)min(c[e], 15) << (4 * e);
+  return word;
+}
+
+// A block of threads takes one KV head of 2048 / D rows, keys and values alike; blocks of a row's heads are neighbours.
 template <int D>
 __global__ void __launch_bounds__(256) q4_write_kernel(
     const __nv_bfloat16* __restrict__ k_new, const __nv_bfloat16* __restrict__ v_new, long long k_sn, long long k_sh,
@@ -39,52 +74,59 @@ __global__ void __launch_bounds__(256) q4_write_kernel(
     const int* __restrict__ slot_block, const int* __restrict__ slot_off, long long N, int Hkv, int num_blocks,
     int* status) {
   using L = Q4<D>;
-  const bool is_v = blockIdx.y != 0;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int lane = (int)(i % L::kLanes);
-  const long long team = i / L::kLanes;
-  const int grp = (int)(team % L::kGroups);
-  const int h = (int)(team / L::kGroups % Hkv);
-  const long long n = team / L::kGroups / Hkv;
-  if (n >= N) return;  // whole teams leave together: kLanes divides the block
+  const int h = blockIdx.x % Hkv;
+  const long long n = (long long)(blockIdx.x / Hkv) * (2048 / D) + threadIdx.x / (D / 8);
+  const int grp = threadIdx.x % (D / 8) / L::kLanes, lane = threadIdx.x % L::kLanes;
+  if (n >= N) return;  // whole groups leave together: kLanes divides the block
+  const bf16x8 k = ldg8(k_new + n * k_sn + h * k_sh + threadIdx.x % (D / 8) * 8);
+  const bf16x8 v = ldg8(v_new + n * v_sn + h * v_sh + threadIdx.x % (D / 8) * 8);
   const int blk = slot_block[n], off = slot_off[n];
   if (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok) {
     if (lane == 0) report(status, kBadIndex);
     return;
   }
-  const __nv_bfloat16* src = is_v ? v_new + n * v_sn + h * v_sh : k_new + n * k_sn + h * k_sh;
-  const bf16x8 x = ldg8(src + grp * L::kGroup + lane * 8);
-  __nv_bfloat162 mn = __hmin2_nan(__hmin2_nan(x.h[0], x.h[1]), __hmin2_nan(x.h[2], x.h[3]));
-  __nv_bfloat162 mx = __hmax2_nan(__hmax2_nan(x.h[0], x.h[1]), __hmax2_nan(x.h[2], x.h[3]));
-  const unsigned mask = (L::kLanes == 32 ? 0xffffffffu : ((1u << L::kLanes) - 1)) << (threadIdx.x & 31 & ~(L::kLanes - 1));
+  const unsigned mask = ((1u << L::kLanes) - 1) << (threadIdx.x & 31 & ~(L::kLanes - 1));
+  const long long at = ((long long)blk * Hkv + h) * L::kBytes + (grp * kTok + off) * L::kRow + lane * 4;
+  const long long meta = ((long long)blk * Hkv + h) * L::kBytes + L::kCodes + (grp * kTok + off) * 4;
 #pragma unroll
-  for (int o = 1; o < L::kLanes; o <<= 1) {
-    mn = __hmin2_nan(mn, __shfl_xor_sync(mask, mn, o));
-    mx = __hmax2_nan(mx, __shfl_xor_sync(mask, mx, o));
-  }
-  const __nv_bfloat16 lo = __hmin_nan(mn.x, mn.y);
-  const float lof = __bfloat162float(lo);
-  const __nv_bfloat16 scale = __float2bfloat16(__fdiv_rn(__bfloat162float(__hmax_nan(mx.x, mx.y)) - lof, 15.f));
-  const float sf = __bfloat162float(scale);
-  float f[8];
-  unpack8(x, f);
-  uint32_t word = 0;
+  for (int i = 0; i < 2; ++i) {
+    const bf16x8& x = i ? v : k;
+    uint8_t* pool = i ? v_pool : k_pool;
+    __nv_bfloat162 mn = __hmin2_nan(__hmin2_nan(x.h[0], x.h[1]), __hmin2_nan(x.h[2], x.h[3]));
+    __nv_bfloat162 mx = __hmax2_nan(__hmax2_nan(x.h[0], x.h[1]), __hmax2_nan(x.h[2], x.h[3]));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float c = rintf(__fdiv_rn(f[e] - lof, sf));
-    const float cl = fminf(fmaxf(c, 0.f), 15.f);  // NaN (a group without spread, or not finite) becomes 0
-    word |= (uint32_t)cl << (4 * e);
+    for (int o = 1; o < L::kLanes; o <<= 1) {
+      mn = __hmin2_nan(mn, __shfl_xor_sync(mask, mn, o));
+      mx = __hmax2_nan(mx, __shfl_xor_sync(mask, mx, o));
+    }
+    const __nv_bfloat16 lo = __hmin_nan(mn.x, mn.y);
+    const float lof = __bfloat162float(lo);
+    const __nv_bfloat16 scale = __float2bfloat16(__fdiv_rn(__bfloat162float(__hmax_nan(mx.x, mx.y)) - lof, 15.f));
+    *reinterpret_cast<uint32_t*>(pool + at) = q4_codes(x, lof, __bfloat162float(scale));
+    if (lane == 0)
+      *reinterpret_cast<uint32_t*>(pool + meta) =
+          (uint32_t)__bfloat16_as_ushort(scale) | ((uint32_t)__bfloat16_as_ushort(lo) << 16);
   }
-  uint8_t* dst = (is_v ? v_pool : k_pool) + ((long long)blk * Hkv + h) * L::kBytes;
-  *reinterpret_cast<uint32_t*>(dst + (grp * kTok + off) * L::kRow + lane * 4) = word;
-  if (lane == 0)
-    *reinterpret_cast<uint32_t*>(dst + L::kCodes + (grp * kTok + off) * 4) =
-        (uint32_t)__bfloat16_as_ushort(scale) | ((uint32_t)__bfloat16_as_ushort(lo) << 16);
 }
 
 // ---------------------------------------------------------------- reading rows
-// One thread per 8 elements.  Row r is slot (slot_block[r], slot_off[r]), or, with a block table, position
-// r % max_len of sequence r / max_len.  Rows without a place in the pool read as zeros.
+// The 8 elements of a word: codes become fp16 numbers by their bits (0x6400 | code is 1024 + code).
+RLB_DEVICE bf16x8 q4_elements(uint32_t word, uint32_t meta) {
+  const float s = bf16_lo_f(meta), lo = bf16_hi_f(meta);
+  const __half2 off = __half2half2(__ushort_as_half(0xe400));  // -1024
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t two = ((word >> (4 * j)) & 0x000f000fu) | 0x64006400u;  // elements j and j + 4
+    const float2 n = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&two), off));
+    f[j] = fmaf(n.x, s, lo);
+    f[j + 4] = fmaf(n.y, s, lo);
+  }
+  return pack8(f);
+}
+
+// One thread per 8 elements of a key and of a value, blocks as above.  Row n is slot (slot_block[n], slot_off[n]), or,
+// with a block table, position n % max_len of sequence n / max_len.  Rows without a place in the pool read as zeros.
 template <int D>
 __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict__ k_pool,
                                                       const uint8_t* __restrict__ v_pool,
@@ -95,11 +137,8 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
                                                       __nv_bfloat16* __restrict__ k_out,
                                                       __nv_bfloat16* __restrict__ v_out, int* status) {
   using L = Q4<D>;
-  const bool is_v = blockIdx.y != 0;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int d8 = (int)(i % (D / 8));
-  const int h = (int)(i / (D / 8) % Hkv);
-  const long long n = i / (D / 8) / Hkv;
+  const int h = blockIdx.x % Hkv, d8 = threadIdx.x % (D / 8);
+  const long long n = (long long)(blockIdx.x / Hkv) * (2048 / D) + threadIdx.x / (D / 8);
   if (n >= N) return;
   int blk = -1, off = 0;
   bool absent = false;
@@ -107,27 +146,30 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
     blk = slot_block[n];
     off = slot_off[n];
   } else {
-    const long long b = n / max_len;
-    const int pos = (int)(n % max_len);
+    const long long b = n >> 31 == 0 ? (long long)((unsigned)n / (unsigned)max_len) : n / max_len;
+    const int pos = (int)(n - b * max_len);
     off = pos % kTok;
     absent = pos >= lens[b];
     if (!absent && pos / kTok < max_blocks) blk = tables[b * max_blocks + pos / kTok];
   }
-  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  bf16x8 k, v;
+  *reinterpret_cast<uint4*>(&k) = *reinterpret_cast<uint4*>(&v) = make_uint4(0, 0, 0, 0);
   if (!absent) {
     if (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok) {
       if (d8 == 0 && h == 0) report(status, kBadIndex);
     } else {
-      const uint8_t* src = (is_v ? v_pool : k_pool) + ((long long)blk * Hkv + h) * L::kBytes;
-      const int grp = d8 * 8 / L::kGroup, lane = d8 % L::kLanes;
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(src + (grp * kTok + off) * L::kRow + lane * 4);
-      const uint32_t meta = *reinterpret_cast<const uint32_t*>(src + L::kCodes + (grp * kTok + off) * 4);
-      const float s = bf16_lo_f(meta), lo = bf16_hi_f(meta);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = fmaf((float)((word >> (4 * e)) & 15u), s, lo);
+      const int grp = d8 / L::kLanes, lane = d8 % L::kLanes;
+      const long long at = ((long long)blk * Hkv + h) * L::kBytes, code = at + (grp * kTok + off) * L::kRow + lane * 4;
+      const long long meta = at + L::kCodes + (grp * kTok + off) * 4;
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(k_pool + code), km = *reinterpret_cast<const uint32_t*>(k_pool + meta);
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(v_pool + code), vm = *reinterpret_cast<const uint32_t*>(v_pool + meta);
+      k = q4_elements(kw, km);
+      v = q4_elements(vw, vm);
     }
   }
-  stg8((is_v ? v_out : k_out) + (n * Hkv + h) * D + d8 * 8, pack8(f));
+  const long long to = (n * Hkv + h) * D + d8 * 8;
+  stg8(k_out + to, k);
+  stg8(v_out + to, v);
 }
 
 // ---------------------------------------------------------------- decode attention
@@ -863,39 +905,20 @@ RLB_DEVICE uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix sum of one flag per thread over a 1024-thread block (`scratch`: 33 ints), and the total.
-RLB_DEVICE int block_rank(bool flag, int* scratch, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned vote = __ballot_sync(0xffffffffu, flag);
-  __syncthreads();
-  if (lane == 0) scratch[warp] = __popc(vote);
-  __syncthreads();
-  if (warp == 0) {
-    const int c = scratch[lane];
-    int s = c;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    scratch[lane] = s - c;
-    if (lane == 31) scratch[32] = s;
-  }
-  __syncthreads();
-  total = scratch[32];
-  return scratch[warp] + __popc(vote & ((1u << lane) - 1));
-}
+// One CTA per (KV head, sequence).  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
+// a histogram in shared memory, whose bins a scan then walks from the top).  Each warp then takes a stretch of the
+// tokens: it counts the tokens above that weight and those equal to it, a scan over the warps gives it its place, and
+// it writes its kept positions in order.  The weights move to the front last, tile by tile: a token never moves to a
+// higher place, so a tile is read before anything that a later one reads is written.
+constexpr int kSelect = 1024, kTile = 8;  // threads; weights a thread moves at a time
 
-// One CTA per (KV head, sequence): finds the weight of the last kept token by a radix selection over 8-bit digits,
-// then walks the tokens in order, writing the kept ones' positions and moving their weights to the front.  Moving
-// in place is safe because a token never moves backwards past one that is still to be read: a tile's weights are
-// all read before any of it is written.
-__global__ void __launch_bounds__(1024) q4_select_kernel(const int* __restrict__ lens, float* __restrict__ weights,
-                                                         const int* __restrict__ weight_rows, int* __restrict__ kept,
-                                                         int* __restrict__ new_lens, int Hkv, long long w_rows,
-                                                         int w_len, int keep, int recent, int sink, int* status) {
-  __shared__ int hist[256], scratch[33], pick[2];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+__global__ void __launch_bounds__(kSelect) q4_select_kernel(const int* __restrict__ lens, float* __restrict__ weights,
+                                                            const int* __restrict__ weight_rows,
+                                                            int* __restrict__ kept, int* __restrict__ new_lens,
+                                                            int Hkv, long long w_rows, int w_len, int keep, int recent,
+                                                            int sink, int* status) {
+  __shared__ int hist[2048], part[33], part2[33], pick[2];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int n = lens[b];
   const int r = weight_rows[b];
   if (n > w_len || (n > 0 && (r < 0 || r >= w_rows))) {
@@ -906,91 +929,142 @@ __global__ void __launch_bounds__(1024) q4_select_kernel(const int* __restrict__
   int* out = kept + ((long long)b * Hkv + h) * keep;
   if (h == 0 && tid == 0) new_lens[b] = min(n, keep);
   if (n <= keep) {
-    for (int j = tid; j < keep; j += 1024) out[j] = j < n ? j : -1;
+    for (int j = tid; j < keep; j += kSelect) out[j] = j < n ? j : -1;
     return;
   }
   float* w = weights + ((long long)r * Hkv + h) * w_len;
   const int first = sink, last = n - recent;  // tokens [first, last) compete for `need` places
   int need = keep - sink - recent;
+  const bool any = need > 0;
   uint32_t prefix = 0, known = 0;
-  for (int shift = 24; need > 0 && shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  for (int step = 0; any && step < 3; ++step) {
+    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bins = step == 2 ? 1024 : 2048;
+    hist[tid] = hist[tid + kSelect] = 0;
     __syncthreads();
-    for (int t = first + tid; t < last; t += 1024) {
+#pragma unroll 8
+    for (int t = first + tid; t < last; t += kSelect) {
       const uint32_t key = weight_key(w[t]);
-      if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+      if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    if (tid == 0) {
-      int left = need, d = 255;
-      while (hist[d] < left) left -= hist[d--];  // the digits above hold fewer than `need`: ends at d >= 0
+    // this thread's two bins, counted from the top; how many lie in higher bins
+    const int d = bins - 1 - 2 * tid;
+    const int c0 = d > 0 ? hist[d] : 0, c1 = d > 0 ? hist[d - 1] : 0;
+    int incl = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    int above = incl - c0 - c1;
+    for (int i = 0; i < warp; ++i) above += part[i];
+    if (above < need && need <= above + c0) {
       pick[0] = d;
-      pick[1] = left;
+      pick[1] = need - above;
+    } else if (above + c0 < need && need <= above + c0 + c1) {
+      pick[0] = d - 1;
+      pick[1] = need - above - c0;
     }
     __syncthreads();
     prefix |= (uint32_t)pick[0] << shift;
-    known |= 255u << shift;
+    known |= (uint32_t)(bins - 1) << shift;
     need = pick[1];
-    __syncthreads();
   }
   // every competitor above `prefix` is kept, and the first `need` of those equal to it
-  const bool any = keep - sink - recent > 0;
-  int done = 0, ties = 0;
-  for (int base = 0; base < n; base += 1024) {
-    const int t = base + tid;
-    const float x = t < n ? w[t] : 0.f;
-    const bool competes = t >= first && t < last;
-    const uint32_t key = weight_key(x);
-    int total;
-    const bool tie = any && competes && key == prefix;
-    const int rank = block_rank(tie, scratch, total);
-    const bool keep_it = t < n && (!competes || (any && (key > prefix || (tie && ties + rank < need))));
-    ties += total;
-    const int at = done + block_rank(keep_it, scratch, total);
-    if (keep_it) {  // every thread has read its weight: block_rank() synchronised
-      w[at] = x;
-      out[at] = t;
-    }
-    done += total;
-    __syncthreads();
+  auto state = [&](int t, bool& tie) {  // whether token t is kept whatever the ties, and whether it is one
+    tie = false;
+    if (t >= n) return false;
+    if (t < first || t >= last) return true;
+    const uint32_t key = weight_key(w[t]);
+    tie = any && key == prefix;
+    return any && key > prefix;
+  };
+  const int per = (n + 32 * 32 - 1) / (32 * 32) * 32, s0 = min(n, warp * per), s1 = min(n, s0 + per);
+  int sure = 0, ties = 0;
+#pragma unroll 8
+  for (int t = s0 + lane; t < s0 + per; t += 32) {
+    bool tie;
+    sure += state(t < s1 ? t : n, tie);
+    ties += tie;
   }
-  for (int t = keep + tid; t < n; t += 1024) w[t] = 0.f;
+  sure = __reduce_add_sync(0xffffffffu, sure);
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  if (lane == 0) {
+    part[warp] = sure;
+    part2[warp] = ties;
+  }
+  __syncthreads();
+  int done = 0, ties_before = 0;
+  for (int i = 0; i < warp; ++i) {
+    done += part[i];
+    ties_before += part2[i];
+  }
+  done += min(need, ties_before);
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll 4
+  for (int t0 = s0; t0 < s1; t0 += 32) {
+    bool tie;
+    const bool keep_it = state(t0 + lane < s1 ? t0 + lane : n, tie);
+    const unsigned tied = __ballot_sync(0xffffffffu, tie);
+    const bool in = keep_it || (tie && ties_before + __popc(tied & below) < need);
+    const unsigned all = __ballot_sync(0xffffffffu, in);
+    if (in) out[done + __popc(all & below)] = t0 + lane;
+    done += __popc(all);
+    ties_before += __popc(tied);
+  }
+  __syncthreads();
+  for (int j0 = 0; j0 < keep; j0 += kSelect * kTile) {
+    float x[kTile];
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) {
+      const int j = j0 + i * kSelect + tid;
+      x[i] = j < keep ? w[out[j]] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTile; ++i)
+      if (j0 + i * kSelect + tid < keep) w[j0 + i * kSelect + tid] = x[i];
+  }
+  __syncthreads();  // (the last tile may have read from behind `keep`)
+  for (int t = keep + tid; t < n; t += kSelect) w[t] = 0.f;
 }
 
-// Moves the kept tokens' stored rows (codes and scales) to the new blocks, 16 bytes a thread.
+// Moves the kept tokens' stored rows (codes and scales) to the new blocks: 16 bytes of a key and of a value a thread.
 template <int D>
 __global__ void __launch_bounds__(256) q4_move_kernel(uint8_t* k_pool, uint8_t* v_pool, const int* __restrict__ tables,
                                                       const int* __restrict__ new_tables, const int* __restrict__ kept,
-                                                      const int* __restrict__ new_lens, int B, int Hkv, int max_blocks,
+                                                      const int* __restrict__ new_lens, int Hkv, int max_blocks,
                                                       int new_blocks, int num_blocks, int keep, int* status) {
   using L = Q4<D>;
-  constexpr int UNITS = L::kRow / 16;  // 16-byte units of a token in a group
-  uint8_t* pool = blockIdx.y ? v_pool : k_pool;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int unit = (int)(i % UNITS);
-  const long long tok = i / UNITS;
-  const int slot = (int)(tok % kTok);
-  const int grp = (int)(tok / kTok % L::kGroups);
-  const int nb = (int)(tok / kTok / L::kGroups % new_blocks);
-  const long long bh = tok / kTok / L::kGroups / new_blocks;
-  if (bh >= (long long)B * Hkv) return;
-  const int b = (int)(bh / Hkv), h = (int)(bh % Hkv), j = nb * kTok + slot;
-  if (j >= new_lens[b]) return;
-  const int t = kept[bh * keep + j];
-  const int from = t / kTok < max_blocks ? tables[(long long)b * max_blocks + t / kTok] : -1;
+  constexpr int UNITS = L::kRow / 16;                  // 16-byte units of a token in a group
+  constexpr int PER = kTok * UNITS * L::kGroups;       // threads for a block
+  const int h = blockIdx.y, b = blockIdx.z, len = new_lens[b];
+  const int nb = blockIdx.x * (256 / PER) + threadIdx.x / PER, x = threadIdx.x % PER;
+  const int unit = x % UNITS, slot = x / UNITS % kTok, grp = x / UNITS / kTok, j = nb * kTok + slot;
+  if (j >= len) return;
+  const int t = kept[((long long)b * Hkv + h) * keep + j];
   const int to = new_tables[(long long)b * new_blocks + nb];
+  const int from = t >= 0 && t / kTok < max_blocks ? tables[(long long)b * max_blocks + t / kTok] : -1;
   if (from < 0 || from >= num_blocks || to < 0 || to >= num_blocks) {
     report(status, kBadIndex);
     return;
   }
-  const uint8_t* src = pool + ((long long)from * Hkv + h) * L::kBytes;
-  uint8_t* dst = pool + ((long long)to * Hkv + h) * L::kBytes;
   const int off = t % kTok;
-  *reinterpret_cast<uint4*>(dst + (grp * kTok + slot) * L::kRow + unit * 16) =
-      *reinterpret_cast<const uint4*>(src + (grp * kTok + off) * L::kRow + unit * 16);
-  if (unit == 0)
-    *reinterpret_cast<uint32_t*>(dst + L::kCodes + (grp * kTok + slot) * 4) =
-        *reinterpret_cast<const uint32_t*>(src + L::kCodes + (grp * kTok + off) * 4);
+  const long long src = ((long long)from * Hkv + h) * L::kBytes, dst = ((long long)to * Hkv + h) * L::kBytes;
+  const int code_from = (grp * kTok + off) * L::kRow + unit * 16, code_to = (grp * kTok + slot) * L::kRow + unit * 16;
+  const uint4 k = *reinterpret_cast<const uint4*>(k_pool + src + code_from);
+  const uint4 v = *reinterpret_cast<const uint4*>(v_pool + src + code_from);
+  *reinterpret_cast<uint4*>(k_pool + dst + code_to) = k;
+  *reinterpret_cast<uint4*>(v_pool + dst + code_to) = v;
+  if (unit == 0) {
+    const int meta_from = L::kCodes + (grp * kTok + off) * 4, meta_to = L::kCodes + (grp * kTok + slot) * 4;
+    const uint32_t km = *reinterpret_cast<const uint32_t*>(k_pool + src + meta_from);
+    const uint32_t vm = *reinterpret_cast<const uint32_t*>(v_pool + src + meta_from);
+    *reinterpret_cast<uint32_t*>(k_pool + dst + meta_to) = km;
+    *reinterpret_cast<uint32_t*>(v_pool + dst + meta_to) = vm;
+  }
 }
 
 }  // namespace rlb
@@ -1009,9 +1083,9 @@ cudaError_t rlb_q4_write(const void* k_new, const void* v_new, long long k_sn, l
                          long long v_sh, void* k_pool, void* v_pool, const int* slot_block, const int* slot_off,
                          long long N, int Hkv, int D, int num_blocks, int* status, cudaStream_t s) {
   if (N == 0) return cudaSuccess;
-  const long long threads = N * Hkv * (D / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256), 2);
-  RLB_Q4_D((q4_write_kernel<DD><<<grid, 256, 0, s>>>(
+  const long long grid = (N + 2048 / D - 1) / (2048 / D) * Hkv;
+  if (grid > (1LL << 31) - 1) return cudaErrorInvalidValue;
+  RLB_Q4_D((q4_write_kernel<DD><<<(unsigned)grid, 256, 0, s>>>(
       (const __nv_bfloat16*)k_new, (const __nv_bfloat16*)v_new, k_sn, k_sh, v_sn, v_sh, (uint8_t*)k_pool,
       (uint8_t*)v_pool, slot_block, slot_off, N, Hkv, num_blocks, status)));
   return cudaGetLastError();
@@ -1021,9 +1095,9 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
                         const int* tables, const int* lens, int max_blocks, int max_len, long long N, int Hkv, int D,
                         int num_blocks, void* k_out, void* v_out, int* status, cudaStream_t s) {
   if (N == 0) return cudaSuccess;
-  const long long threads = N * Hkv * (D / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256), 2);
-  RLB_Q4_D((q4_read_kernel<DD><<<grid, 256, 0, s>>>((const uint8_t*)k_pool, (const uint8_t*)v_pool, slot_block,
+  const long long grid = (N + 2048 / D - 1) / (2048 / D) * Hkv;
+  if (grid > (1LL << 31) - 1) return cudaErrorInvalidValue;
+  RLB_Q4_D((q4_read_kernel<DD><<<(unsigned)grid, 256, 0, s>>>((const uint8_t*)k_pool, (const uint8_t*)v_pool, slot_block,
                                                     slot_off, tables, lens, max_blocks, max_len, N, Hkv, num_blocks,
                                                     (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, status)));
   return cudaGetLastError();
@@ -1103,11 +1177,11 @@ cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const in
                          int max_blocks, int new_blocks, int num_blocks, long long w_rows, int w_len, int keep,
                          int recent, int sink, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
-  q4_select_kernel<<<dim3(Hkv, B), 1024, 0, s>>>(lens, weights, weight_rows, kept, new_lens, Hkv, w_rows, w_len, keep,
-                                                 recent, sink, status);
-  const long long rows = (long long)B * Hkv * new_blocks * kTok;
-  RLB_Q4_D((q4_move_kernel<DD><<<dim3((unsigned)((rows * Q4<DD>::kGroups * (Q4<DD>::kRow / 16) + 255) / 256), 2), 256, 0, s>>>(
-      (uint8_t*)k_pool, (uint8_t*)v_pool, tables, new_tables, kept, new_lens, B, Hkv, max_blocks, new_blocks,
-      num_blocks, keep, status)));
+  q4_select_kernel<<<dim3(Hkv, B), kSelect, 0, s>>>(lens, weights, weight_rows, kept, new_lens, Hkv, w_rows, w_len,
+                                                     keep, recent, sink, status);
+  const int rows = (keep + kTok - 1) / kTok * kTok;  // the new blocks that can hold a token
+  RLB_Q4_D((q4_move_kernel<DD><<<dim3((unsigned)(((long long)rows * Q4<DD>::kGroups * (Q4<DD>::kRow / 16) + 255) / 256), Hkv, B),
+                                 256, 0, s>>>((uint8_t*)k_pool, (uint8_t*)v_pool, tables, new_tables, kept, new_lens,
+                                              Hkv, max_blocks, new_blocks, num_blocks, keep, status)));
   return cudaGetLastError();
 }

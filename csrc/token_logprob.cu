@@ -294,8 +294,10 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprob_kernel(
     float lp = 0.f;
     if (tg >= V) report(status, kBadIndex);
     else if (tg >= 0) lp = none ? -INFINITY : to_f(row[tg]) - st.m - ls;
-    m_out[r] = st.m;
-    ls_out[r] = ls;
+    if (m_out != nullptr) {
+      m_out[r] = st.m;
+      ls_out[r] = ls;
+    }
     lp_out[r] = lp;
     ent_out[r] = none ? 0.f : ls - st.t / st.s;
   }

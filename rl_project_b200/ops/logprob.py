@@ -166,7 +166,7 @@ class TokenLogprobs(NamedTuple):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, targets, top, status):
-        m, ls, lp, ent, top_lp, top_ids = native().token_logprob(x, targets, top, status)
+        lp, ent, top_lp, top_ids, m, ls = native().token_logprob(x, targets, top, True, status)
         ctx.save_for_backward(x, targets, m, ls, ent, top_ids)
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
@@ -203,7 +203,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
         if x.requires_grad and torch.is_grad_enabled():
             lp, ent, top_lp, ids = _TokenLogprobs.apply(x, t, int(top), status)
         else:
-            _, _, lp, ent, top_lp, ids = native().token_logprob(x.detach(), t, int(top), status)
+            lp, ent, top_lp, ids = native().token_logprob(x.detach(), t, int(top), False, status)
     else:
         if t.numel() and t.max() >= V:
             raise IndexError("a target lies outside the vocabulary")
