@@ -29,13 +29,48 @@ struct Q4 {
 RLB_DEVICE float bf16_lo_f(uint32_t v) { return __uint_as_float(v << 16); }
 RLB_DEVICE float bf16_hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// Two nibbles of a word in one instruction: (w & mask) | 0x64006400.  (Written out because the compiler takes two
+// where both constants are immediates; `magic` comes from a register.)
+template <uint32_t MASK>
+RLB_DEVICE uint32_t nibbles(uint32_t w, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));
+  return r;
+}
+
+RLB_DEVICE uint32_t half2_add(uint32_t x, uint32_t both) {
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&both));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// Nibbles j and j + 4 of a word as two fp16 numbers: code - MINUS for j = 0 and 2, for j = 1 and 3 the same (ALL) or
+// 1024 + 16 code.
+template <bool ALL, int MINUS = 8>
+RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
+  static_assert(MINUS == 0 || MINUS == 8, "-1024 and -64, or -1032 and -72");
+  constexpr uint32_t off = MINUS == 8 ? 0xe408e408u : 0xe400e400u;
+  const uint32_t x = w >> 8;
+  r[0] = half2_add(nibbles<0x000f000fu>(w, magic), off);
+  r[1] = nibbles<0x00f000f0u>(w, magic);
+  r[2] = half2_add(nibbles<0x000f000fu>(x, magic), off);
+  r[3] = nibbles<0x00f000f0u>(x, magic);
+  if (ALL) {
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+    const __half2 off16 = __half2half2(__ushort_as_half(MINUS == 8 ? 0xd480 : 0xd400));
+#pragma unroll
+    for (int j = 1; j < 4; j += 2) {
+      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&r[j]), sixteenth, off16);
+      r[j] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- storing rows
 // A group's threads reduce its minimum and maximum by shuffles (NaN-propagating), then each quantises its 8
 // elements to one 32-bit word.  Bound by memory: 2 bytes read and about 0.56 written per element.
 //
-// code = clamp(rint((x - lo) / s)) without a division per element: y = fma(x - lo, 1 / s, 1.5 2^23) rounds to a whole
-// number c, and the remainder r = fma(-c, s, x - lo) tells whether that is the nearest (|r| <= s / 2, and c even
-// where both are equal); only then a neighbour is taken.
+// code = clamp(rint((x - lo) / s)) without a division per element: q = (x - lo) (1 / s) and its remainder's share
+// q + (x - lo - q s) (1 / s) is the correctly rounded quotient, and adding 1.5 2^23 rounds that to a whole number.
 RLB_DEVICE uint32_t q4_codes(const bf16x8& x, float lo, float s) {
   float f[8];
   unpack8(x, f);
@@ -46,24 +81,14 @@ RLB_DEVICE uint32_t q4_codes(const bf16x8& x, float lo, float s) {
       word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(f[e] - lo, s)), 0.f), 15.f) << (4 * e);  // NaN becomes 0
     return word;
   }
-  const float inv = __fdividef(1.f, s), h = 0.5f * s;
-  float r[8], far = 0.f;
-  int c[8];
+  const float inv = __frcp_rn(s);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float d = f[e] - lo, y = fmaf(d, inv, 12582912.f);
-    c[e] = __float_as_int(y) - 0x4b400000;
-    r[e] = fmaf(12582912.f - y, s, d);
-    far = fmaxf(far, fabsf(r[e]));
+    const float d = f[e] - lo, q = d * inv, y = fmaf(fmaf(-q, s, d), inv, q) + 12582912.f;
+    word += __float_as_uint(y) << (4 * e);
   }
-  if (far >= h) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (fabsf(r[e]) > h || (fabsf(r[e]) == h && (c[e] & 1))) c[e] += r[e] > 0.f ? 1 : -1;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) word |= (uint32_t)min(c[e], 15) << (4 * e);
-  return word;
+  // y's bits are 0x4b400000 + code; no code is above 15, s being within 2^-9 of a 15th of the spread
+  return word - 0x4b400000u * 0x11111111u;
 }
 
 // A block of threads takes one KV head of 2048 / D rows, keys and values alike; blocks of a row's heads are neighbours.
@@ -101,7 +126,9 @@ __global__ void __launch_bounds__(256) q4_write_kernel(
     }
     const __nv_bfloat16 lo = __hmin_nan(mn.x, mn.y);
     const float lof = __bfloat162float(lo);
-    const __nv_bfloat16 scale = __float2bfloat16(__fdiv_rn(__bfloat162float(__hmax_nan(mx.x, mx.y)) - lof, 15.f));
+    // the range over 15, correctly rounded (a quotient and its remainder's)
+    const float range = __bfloat162float(__hmax_nan(mx.x, mx.y)) - lof, q0 = range * (1.f / 15.f);
+    const __nv_bfloat16 scale = __float2bfloat16(fmaf(fmaf(-15.f, q0, range), 1.f / 15.f, q0));
     *reinterpret_cast<uint32_t*>(pool + at) = q4_codes(x, lof, __bfloat162float(scale));
     if (lane == 0)
       *reinterpret_cast<uint32_t*>(pool + meta) =
@@ -110,15 +137,14 @@ __global__ void __launch_bounds__(256) q4_write_kernel(
 }
 
 // ---------------------------------------------------------------- reading rows
-// The 8 elements of a word: codes become fp16 numbers by their bits (0x6400 | code is 1024 + code).
 RLB_DEVICE bf16x8 q4_elements(uint32_t word, uint32_t meta) {
   const float s = bf16_lo_f(meta), lo = bf16_hi_f(meta);
-  const __half2 off = __half2half2(__ushort_as_half(0xe400));  // -1024
+  uint32_t two[4];
+  codes_f16<true, 0>(word, two, 0x64006400u);
   float f[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t two = ((word >> (4 * j)) & 0x000f000fu) | 0x64006400u;  // elements j and j + 4
-    const float2 n = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&two), off));
+    const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&two[j]));
     f[j] = fmaf(n.x, s, lo);
     f[j + 4] = fmaf(n.y, s, lo);
   }
@@ -231,39 +257,6 @@ RLB_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
-}
-
-// Two nibbles of a word in one instruction: (w & mask) | 0x64006400.  (Written out because the compiler takes two
-// where both constants are immediates; `magic` comes from a register.)
-template <uint32_t MASK>
-RLB_DEVICE uint32_t nibbles(uint32_t w, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));
-  return r;
-}
-
-RLB_DEVICE uint32_t half2_add(uint32_t x, uint32_t both) {
-  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&both));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-
-// Nibbles j and j + 4 of a word as two fp16 numbers: code - 8 for j = 0 and 2, for j = 1 and 3 code - 8 too (CENTRED)
-// or 1024 + 16 code.
-template <bool CENTRED>
-RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
-  const uint32_t x = w >> 8;
-  r[0] = half2_add(nibbles<0x000f000fu>(w, magic), 0xe408e408u);  // -1032
-  r[1] = nibbles<0x00f000f0u>(w, magic);
-  r[2] = half2_add(nibbles<0x000f000fu>(x, magic), 0xe408e408u);
-  r[3] = nibbles<0x00f000f0u>(x, magic);
-  if (CENTRED) {
-    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00)), off = __half2half2(__ushort_as_half(0xd480));  // -72
-#pragma unroll
-    for (int j = 1; j < 4; j += 2) {
-      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&r[j]), sixteenth, off);
-      r[j] = *reinterpret_cast<const uint32_t*>(&y);
-    }
-  }
 }
 
 RLB_DEVICE uint32_t pack_f16(float lo, float hi) {
@@ -905,7 +898,8 @@ RLB_DEVICE uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per (KV head, sequence).  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
+// Choosing what stays has two forms.  This one, a CTA per (KV head, sequence), takes sequences whose weights do not fit
+// into a CTA's registers.  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
 // a histogram in shared memory, whose bins a scan then walks from the top).  Each warp then takes a stretch of the
 // tokens: it counts the tokens above that weight and those equal to it, a scan over the warps gives it its place, and
 // it writes its kept positions in order.  The weights move to the front last, tile by tile: a token never moves to a
@@ -1028,6 +1022,116 @@ __global__ void __launch_bounds__(kSelect) q4_select_kernel(const int* __restric
       if (j0 + i * kSelect + tid < keep) w[j0 + i * kSelect + tid] = x[i];
   }
   __syncthreads();  // (the last tile may have read from behind `keep`)
+  for (int t = keep + tid; t < n; t += kSelect) w[t] = 0.f;
+}
+
+// The same with K keys a thread in registers: the weights are read once.  A bar that exactly
+// `keep` keys reach is searched by halving the interval of keys and counting: 10 to 20 times K compares and a barrier
+// (32 where many weights are equal), where histograms pay for colliding atomics, weights crowding in few exponents.  Warp w holds tokens [32 K w, 32 K (w + 1)), 32 neighbours at a
+// time.  (A cluster of 8 CTAs a row, exchanging its counts over distributed shared memory, took 35 us for 8 rows of 40000
+// tokens where one CTA takes 40: the barriers of the cluster eat what the additional SMs bring.)
+template <int K>
+__global__ void __launch_bounds__(kSelect) q4_select_regs_kernel(const int* __restrict__ lens, float* __restrict__ weights,
+                                                                 const int* __restrict__ weight_rows,
+                                                                 int* __restrict__ kept, int* __restrict__ new_lens,
+                                                                 int Hkv, long long w_rows, int w_len, int keep,
+                                                                 int recent, int sink, int* status) {
+  __shared__ int part[2][32], place[2][32];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int n = lens[b];
+  const int r = weight_rows[b];
+  if (n > min(w_len, K * kSelect) || (n > 0 && (r < 0 || r >= w_rows))) {
+    if (tid == 0) report(status, kBadIndex);
+    n = 0;
+  }
+  n = max(n, 0);
+  int* out = kept + ((long long)b * Hkv + h) * keep;
+  if (h == 0 && tid == 0) new_lens[b] = min(n, keep);
+  if (n <= keep) {
+    for (int j = tid; j < keep; j += kSelect) out[j] = j < n ? j : -1;
+    return;
+  }
+  float* w = weights + ((long long)r * Hkv + h) * w_len;
+  const int t0 = warp * 32 * K + lane;
+  uint32_t key[K];  // above all for protected tokens, 0 for absent ones (a NaN's is 1)
+#pragma unroll
+  for (int i = 0; i < K; ++i) key[i] = t0 + 32 * i < n ? __float_as_uint(w[t0 + 32 * i]) : 0u;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int t = t0 + 32 * i;
+    key[i] = t >= n ? 0u : t < sink || t >= n - recent ? 0xffffffffu : max(weight_key(__uint_as_float(key[i])), 1u);
+  }
+  int turn = 0;
+  auto count = [&](uint32_t least) {  // keys of at least `least`, in the block
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) c += key[i] >= least;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) part[turn & 1][warp] = c;
+    __syncthreads();
+    c = __reduce_add_sync(0xffffffffu, part[turn & 1][lane]);
+    ++turn;
+    return c;
+  };
+  // at_bar >= keep keys are at least `bar`, fewer at least `over`
+  uint32_t bar = 1, over = 0xffffffffu;
+  int at_bar = n;
+  if (sink + recent == keep) {
+    bar = over;
+    at_bar = keep;
+  }
+  while (over - bar > 1 && at_bar > keep) {
+    const uint32_t least = bar + (over - bar) / 2;
+    const int c = count(least);
+    if (c >= keep) {
+      bar = least;
+      at_bar = c;
+    } else {
+      over = least;
+    }
+  }
+  const unsigned below = (1u << lane) - 1;
+  if (at_bar > keep) {  // of the keys equal to the bar only the first find a place: the others fall below it
+    const int taken = keep - count(bar + 1);
+    int ties = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) ties += key[i] == bar;
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) place[1][warp] = ties;
+    __syncthreads();
+    int before = __reduce_add_sync(0xffffffffu, lane < warp ? place[1][lane] : 0);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const unsigned tied = __ballot_sync(0xffffffffu, key[i] == bar);
+      if (key[i] == bar && before + __popc(tied & below) >= taken) key[i] = 0;
+      before += __popc(tied);
+    }
+  }
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < K; ++i) mine += key[i] >= bar;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) place[0][warp] = mine;
+  float x[K];  // the kept tokens' weights
+  unsigned in[(K + 31) / 32] = {};
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    if (key[i] >= bar) in[i / 32] |= 1u << (i % 32);
+    x[i] = key[i] >= bar ? w[t0 + 32 * i] : 0.f;
+  }
+  __syncthreads();  // every weight has been read
+  int done = __reduce_add_sync(0xffffffffu, lane < warp ? place[0][lane] : 0);
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const bool keep_it = in[i / 32] >> (i % 32) & 1;
+    const unsigned all = __ballot_sync(0xffffffffu, keep_it);
+    const int to = done + __popc(all & below);
+    if (keep_it) {
+      out[to] = t0 + 32 * i;
+      w[to] = x[i];
+    }
+    done += __popc(all);
+  }
   for (int t = keep + tid; t < n; t += kSelect) w[t] = 0.f;
 }
 
@@ -1177,8 +1281,13 @@ cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const in
                          int max_blocks, int new_blocks, int num_blocks, long long w_rows, int w_len, int keep,
                          int recent, int sink, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
-  q4_select_kernel<<<dim3(Hkv, B), kSelect, 0, s>>>(lens, weights, weight_rows, kept, new_lens, Hkv, w_rows, w_len,
-                                                     keep, recent, sink, status);
+  const long long most = (long long)max_blocks * kTok < w_len ? (long long)max_blocks * kTok : w_len;  // tokens
+  auto select = most <= 4 * kSelect    ? q4_select_regs_kernel<4>
+                : most <= 16 * kSelect ? q4_select_regs_kernel<16>
+                : most <= 40 * kSelect ? q4_select_regs_kernel<40>  // (64 registers a thread hold no more)
+                                       : q4_select_kernel;
+  select<<<dim3(Hkv, B), kSelect, 0, s>>>(lens, weights, weight_rows, kept, new_lens, Hkv, w_rows, w_len, keep, recent,
+                                          sink, status);
   const int rows = (keep + kTok - 1) / kTok * kTok;  // the new blocks that can hold a token
   RLB_Q4_D((q4_move_kernel<DD><<<dim3((unsigned)(((long long)rows * Q4<DD>::kGroups * (Q4<DD>::kRow / 16) + 255) / 256), Hkv, B),
                                  256, 0, s>>>((uint8_t*)k_pool, (uint8_t*)v_pool, tables, new_tables, kept, new_lens,

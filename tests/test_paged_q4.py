@@ -312,10 +312,19 @@ def chosen(w, n, keep, sink, recent):
     ([50, 80], 2, 128, 1, 0, 0, "random"),
     ([2500, 1025, 1024, 1023], 2, 64, 1000, 4, 64, "ties"),
     ([5000], 1, 64, 4100, 1, 10, "zeros"),
+    ([9000, 4097, 8999], 1, 32, 4096, 3, 100, "ties"),
+    ([17000], 2, 32, 3001, 0, 1, "random"),
+    ([41000, 40960], 1, 32, 2000, 2, 9, "random"),
+    ([41000], 1, 32, 40000, 2, 9, "odd"),
+    ([16384], 1, 32, 16000, 0, 0, "ties"),
+    ([132000, 131073], 1, 32, 3000, 2, 9, "random"),
+    ([132000], 1, 32, 131000, 2, 9, "odd"),
     ([90, 33], 2, 64, 30, 1, 1, "odd"),
     ([70], 2, 64, 90, 1, 1, "random"),
 ])
 def test_evict(dev, lens, Hkv, D, keep, sink, recent, kind):
+    if dev == "cpu" and max(lens) > 50000:
+        pytest.skip("long sequences are for the kernels")
     new_w = -(-keep // 16)
     ks, vs, pools, tables, n, ids = cache(lens, Hkv, D, dev, extra=len(lens) * new_w)
     new = ids[-len(lens) * new_w:].view(len(lens), new_w).int().to(dev)
