@@ -281,7 +281,8 @@ def cmd_serve(args: argparse.Namespace) -> int:
     from rl_project_b200.serving import EngineBackend, Router, ServingServer
 
     policy = _load_policy(args)
-    engine = InferenceEngine(policy.model, max_batch=args.max_batch, max_seq_len=args.max_seq_len)
+    engine = InferenceEngine(policy.model, max_batch=args.max_batch, max_seq_len=args.max_seq_len,
+                             kv_cache=args.kv_cache, kv_budget=args.kv_budget)
     backend = EngineBackend(args.model_name, engine, policy.tokenizer)
     route_fn = None
     if args.routing:
@@ -546,6 +547,9 @@ _EVALUATE = _POLICY_SOURCE + [
 _SERVE = _POLICY_SOURCE + [
     A("--host", default="127.0.0.1"), A("--port", type=int, default=8000), A("--model-name", default="forgeline-model"),
     A("--max-batch", type=int, default=8), A("--max-seq-len", type=int, default=None),
+    A("--kv-cache", default="bf16", choices=["bf16", "q4"], help="how keys and values are held (q4: 4 bits)"),
+    A("--kv-budget", type=int, default=None,
+      help="tokens a sequence keeps cached, by accumulated attention weight (needs --kv-cache q4)"),
     A("--routing", default=None, help="routing policy JSON"), A("--metrics", default="none"),
     A("--output-dir", default="runs/serve")]
 

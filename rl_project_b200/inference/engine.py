@@ -29,6 +29,14 @@ captured on first use.  Padding rows decode a dummy token into a block reserved 
 never touch a live sequence's K/V.  Graphs hold the model's weight and KV-pool addresses: call
 ``reset_graphs()`` after replacing (not updating in place) a weight tensor.  Measured on B200 with
 the dense 1B model, batch 64: 26.9k generated tokens/s against 13.5k eager, identical greedy tokens.
+
+``kv_cache="q4"`` keeps the cache in 4 bits (ops/paged_q4.py): 3.6 times the tokens in the same memory, and as much
+less to read per step.  ``kv_budget`` bounds it further: each decode step accumulates every cached token's attention
+weight, and a sequence whose cache has grown an eighth (at least a block) beyond the budget is cut back to it, per layer
+and KV head, keeping its first ``kv_sink`` and last ``kv_recent`` tokens and those with the most weight.  Prompts
+longer than the budget are read whole and cut after their first decode step.
+
+``SamplingParams.logprobs`` records each generated token's log-prob and its most likely alternatives.
 """
 
 from __future__ import annotations
@@ -43,19 +51,22 @@ import numpy as np
 import torch
 
 from rl_project_b200.core.errors import ServingError
-from rl_project_b200.inference.paged_memory import KERNEL_BLOCK, OutOfBlocksError, PagedBlockAllocator, PagedKVCache
+from rl_project_b200.inference.paged_memory import (KERNEL_BLOCK, OutOfBlocksError, PagedBlockAllocator, PagedKVCache,
+                                                    PagedQ4KVCache)
 from rl_project_b200.inference.requests import GenerationRequest, SamplingParams
 from rl_project_b200.inference.scheduler import Scheduler
 from rl_project_b200.models.generation.sampling import apply_sampling_filters, sample_from_logits
 from rl_project_b200.observability.logging import get_logger
 from rl_project_b200.observability.tracing import Tracer
+from rl_project_b200.ops.logprob import token_logprobs
 from rl_project_b200.ops.paged_attention import paged_write
+from rl_project_b200.ops.paged_q4 import paged_write_q4
 
 log = get_logger("forgeline.inference")
 
 
 class _Seq:
-    __slots__ = ("req", "position", "last_logits", "tokens", "cache")
+    __slots__ = ("req", "position", "last_logits", "tokens", "cache", "evicted", "row")
 
     def __init__(self, req: GenerationRequest):
         self.req = req
@@ -63,13 +74,21 @@ class _Seq:
         self.last_logits: Optional[torch.Tensor] = None  # [1, V] logits of the prompt's last token
         self.tokens: List[int] = list(req.prompt_tokens)
         self.cache: Optional[List[Any]] = None  # contiguous per-layer cache (non-paged models only)
+        self.evicted = 0  # tokens dropped from the cache
+        self.row = -1  # accumulator row of attention weights
+
+    @property
+    def cached(self) -> int:
+        """Tokens in the cache (the next token's place in it; its position counts the evicted ones too)."""
+        return self.position - self.evicted
 
 
 class InferenceEngine:
     def __init__(self, model: Any, *, max_batch: int = 8, max_seq_len: Optional[int] = None, block_size: int = 16,
                  max_blocks: Optional[int] = None, device: Optional[torch.device] = None,
                  eos_token_id: Optional[int] = None, share_prefixes: bool = True, profile: bool = False,
-                 decode_graphs: Optional[bool] = None):
+                 decode_graphs: Optional[bool] = None, kv_cache: str = "bf16", kv_budget: Optional[int] = None,
+                 kv_sink: int = 4, kv_recent: Optional[int] = None):
         self.model = model.eval()
         self.device = device or next(model.parameters()).device
         self.max_seq_len = min(max_seq_len or model.spec.block_size, model.spec.block_size)
@@ -80,10 +99,19 @@ class InferenceEngine:
         self.allocator = PagedBlockAllocator(block_size=block_size, max_blocks=max_blocks)
         self.scheduler = Scheduler(self.allocator, max_batch=max_batch, max_seq_len=self.max_seq_len)
         self.kv: Optional[PagedKVCache] = None
+        self._check_kv(kv_cache, kv_budget, kv_sink, kv_recent)
+        self.kv_budget, self.kv_sink = kv_budget, kv_sink
+        self.kv_recent = 0 if kv_budget is None else kv_budget // 4 if kv_recent is None else kv_recent
+        self.evictions = 0
+        self._free_rows: List[int] = list(range(max_batch)) if kv_budget is not None else []
         if self.paged:
             n_layer, n_kv, hd = model.kv_layout()
             dtype = next(model.parameters()).dtype
-            self.kv = PagedKVCache(n_layer, n_kv, hd, max_blocks, self.device, dtype=dtype)
+            if kv_cache == "q4":
+                self.kv = PagedQ4KVCache(n_layer, n_kv, hd, max_blocks, self.device, weight_rows=len(self._free_rows),
+                                         weight_tokens=-(-self.max_seq_len // block_size) * block_size)
+            else:
+                self.kv = PagedKVCache(n_layer, n_kv, hd, max_blocks, self.device, dtype=dtype)
         self.eos_token_id = eos_token_id
         self.share_prefixes = share_prefixes and self.paged
         self.states: Dict[str, _Seq] = {}
@@ -114,6 +142,26 @@ class InferenceEngine:
         self.decode_graphs = bool(decode_graphs) and self.paged and self.device.type == "cuda"
         if self.decode_graphs:
             self._pad_block = self.allocator.allocate("__graph_padding__", 1)[0]
+
+    def _check_kv(self, kv_cache: str, budget: Optional[int], sink: int, recent: Optional[int]) -> None:
+        if kv_cache not in ("bf16", "q4"):
+            raise ServingError(f"kv_cache must be 'bf16' or 'q4', got {kv_cache!r}")
+        if kv_cache == "q4":
+            if not self.paged:
+                raise ServingError("kv_cache='q4' needs a model with paged grouped-query attention")
+            attn = self.model.transformer.h[0].attn
+            if attn.n_head // attn.n_kv_head > 16:
+                raise ServingError("kv_cache='q4' serves up to 16 query heads per KV head")
+            if self.device.type == "cuda" and next(self.model.parameters()).dtype != torch.bfloat16:
+                raise ServingError("kv_cache='q4' takes the keys and values of a bf16 model on CUDA")
+        if budget is None:
+            return
+        if kv_cache != "q4":
+            raise ServingError("kv_budget needs kv_cache='q4'")
+        if any(blk.attn.window_size for blk in self.model.transformer.h):
+            raise ServingError("kv_budget does not go with sliding windows, which count cached tokens")
+        if sink < 0 or (recent is not None and recent < 0) or sink + (recent or 0) > budget or budget < KERNEL_BLOCK:
+            raise ServingError(f"kv_budget must hold kv_sink + kv_recent tokens and at least {KERNEL_BLOCK}")
 
     # ------------------------------------------------------------ submission
     def submit(self, prompt_tokens: List[int], params: Optional[SamplingParams] = None,
@@ -156,6 +204,9 @@ class InferenceEngine:
         for req in reqs:
             st = _Seq(req)
             self.states[req.id] = st
+            if self.kv_budget is not None:
+                st.row = self._free_rows.pop()
+                self.kv.weights[:, st.row].zero_()
             req.started_at = time.time()
             if min(req.prompt_tokens) < 0 or max(req.prompt_tokens) >= vocab:
                 # fail this request alone, before its ids reach a batched forward with other requests
@@ -246,12 +297,13 @@ class InferenceEngine:
         n_tok = packed.numel() // 3
         flat_d = packed[:n_tok]
         blk_d, off_d = packed[n_tok:2 * n_tok].to(torch.int32), packed[2 * n_tok:].to(torch.int32)
+        write = paged_write_q4 if isinstance(self.kv, PagedQ4KVCache) else paged_write
         for layer, (k, v) in enumerate(cache):
             B, H, _, D = k.shape
             kk = k.transpose(1, 2).reshape(B * L, H, D).index_select(0, flat_d)
             vv = v.transpose(1, 2).reshape(B * L, H, D).index_select(0, flat_d)
-            kl, vl = self.kv.layer(layer)
-            paged_write(kk, vv, kl, vl, blk_d, off_d)
+            kl, vl = self.kv.layer(layer)[:2]
+            write(kk, vv, kl, vl, blk_d, off_d)
 
     # ------------------------------------------------------------ profiling (CUDA events per decode step)
     @staticmethod
@@ -278,7 +330,34 @@ class InferenceEngine:
         p["steps"] = p.get("steps", 0.0) + 1
 
     # ------------------------------------------------------------ decode
+    def _evict(self, seqs: List[_Seq]) -> None:
+        """Cut the caches that have outgrown the budget (see the module's notes)."""
+        due = [s for s in seqs if s.cached >= self.kv_budget + max(KERNEL_BLOCK, self.kv_budget // 8)]
+        plan = []
+        for s in due:
+            try:  # the token that the coming step adds has its place in the new blocks too
+                plan.append((s, *self.allocator.replace(s.req.id, self.kv_budget + 1)))
+            except OutOfBlocksError:  # no room to copy to now: the cache keeps growing until there is
+                continue
+        if not plan:
+            return
+        width, new_width = max(len(old) for _, old, _ in plan), max(len(new) for _, _, new in plan)
+        table = torch.tensor([old + [0] * (width - len(old)) for _, old, _ in plan], dtype=torch.int32)
+        new = torch.tensor([new + [0] * (new_width - len(new)) for _, _, new in plan], dtype=torch.int32)
+        lens, rows = (torch.tensor(x, dtype=torch.int32) for x in ([s.cached for s, _, _ in plan],
+                                                                    [s.row for s, _, _ in plan]))
+        dev = self.device
+        self.kv.evict(table.to(dev), lens.to(dev), new.to(dev), rows.to(dev), self.kv_budget, self.kv_recent,
+                      self.kv_sink)
+        for s, old, _ in plan:
+            self.allocator.release(old)  # (their next user's writes come behind the copies, on the same stream)
+            s.evicted += s.cached - self.kv_budget
+            self.evictions += 1
+            self._unshare(s)
+
     def _decode(self, seqs: List[_Seq]) -> int:
+        if self.kv_budget is not None:
+            self._evict(seqs)
         if self.decode_graphs and not self.profile:
             try:
                 done = self._decode_graph(seqs)
@@ -297,7 +376,7 @@ class InferenceEngine:
         bs = self.allocator.block_size
         tables = [self.allocator.tables[s.req.id] for s in seqs]
         width = max(len(t) for t in tables)
-        n = 5 * B + B * width
+        n = 6 * B + B * width
         if self._pinned is None or self._pinned.numel() < n:
             self._pinned = torch.empty(max(n, 1024), dtype=torch.int32,
                                        pin_memory=self.device.type == "cuda")
@@ -305,22 +384,25 @@ class InferenceEngine:
         hv = host.numpy()
         pos = np.fromiter((s.position for s in seqs), dtype=np.int64, count=B)
         hv[:B] = np.fromiter((s.tokens[-1] for s in seqs), dtype=np.int64, count=B)
+        at = np.fromiter((s.cached for s in seqs), dtype=np.int64, count=B)
         hv[B:2 * B] = pos
-        hv[2 * B:3 * B] = pos + 1
-        hv[4 * B:5 * B] = pos % bs
-        grid = hv[5 * B:].reshape(B, width)
+        hv[2 * B:3 * B] = at + 1
+        hv[4 * B:5 * B] = at % bs
+        hv[5 * B + B * width:] = [s.row for s in seqs]
+        grid = hv[5 * B:5 * B + B * width].reshape(B, width)
         grid[:] = 0
         for b, t in enumerate(tables):
             grid[b, :len(t)] = t
-        hv[3 * B:4 * B] = grid[np.arange(B), pos // bs]
+        hv[3 * B:4 * B] = grid[np.arange(B), at // bs]
         max_pos = int(pos.max())
         dev = host.to(self.device, non_blocking=True)
         from rl_project_b200.models.attention.causal import PagedDecodeMeta
 
         meta = PagedDecodeMeta(positions=dev[B:2 * B].view(B, 1), max_pos=max_pos, ctx_lens=dev[2 * B:3 * B],
                                slot_block=dev[3 * B:4 * B], slot_off=dev[4 * B:5 * B],
-                               block_tables=dev[5 * B:].view(B, width),
-                               split_tokens=self._split_tokens(B, max_pos + 1))
+                               block_tables=dev[5 * B:5 * B + B * width].view(B, width),
+                               split_tokens=self._split_tokens(B, max_pos + 1),
+                               weight_rows=dev[5 * B + B * width:])
         evs = [self._event()] if self.profile else None
         try:
             with self.tracer.span("decode", batch=B):
@@ -351,24 +433,30 @@ class InferenceEngine:
 
     @staticmethod
     def stage_graph_inputs(hv: np.ndarray, tokens: List[int], positions: List[int], tables: List[List[int]],
-                           Bb: int, Wb: int, pad_block: int, bs: int) -> None:
+                           Bb: int, Wb: int, pad_block: int, bs: int, cached: Optional[List[int]] = None,
+                           rows: Optional[List[int]] = None) -> None:
         """Fill the int32 staging buffer of a (Bb, Wb) decode graph: tokens, positions, context lengths,
-        slot blocks, slot offsets ([Bb] each), then the [Bb, Wb] block tables.  Rows past the real batch
-        decode token 0 at position 0 with a one-token context in ``pad_block``."""
+        slot blocks, slot offsets ([Bb] each), then the [Bb, Wb] block tables and, with ``rows``, the accumulator
+        rows ([Bb]).  ``cached``: tokens in each cache, where evictions made them fewer than the positions.  Rows
+        past the real batch decode token 0 at position 0 with a one-token context in ``pad_block``."""
         B = len(tokens)
         hv[:5 * Bb + Bb * Wb] = 0
+        if rows is not None:
+            hv[5 * Bb + Bb * Wb:6 * Bb + Bb * Wb] = -1
+            hv[5 * Bb + Bb * Wb:5 * Bb + Bb * Wb + B] = rows
         pos = np.asarray(positions, dtype=np.int64)
+        at = pos if cached is None else np.asarray(cached, dtype=np.int64)
         hv[:B] = np.asarray(tokens, dtype=np.int64)
         hv[Bb:Bb + B] = pos
         hv[2 * Bb:3 * Bb] = 1
-        hv[2 * Bb:2 * Bb + B] = pos + 1
+        hv[2 * Bb:2 * Bb + B] = at + 1
         hv[3 * Bb:4 * Bb] = pad_block
-        hv[4 * Bb:4 * Bb + B] = pos % bs
+        hv[4 * Bb:4 * Bb + B] = at % bs
         grid = hv[5 * Bb:5 * Bb + Bb * Wb].reshape(Bb, Wb)
         grid[:, 0] = pad_block
         for b, t in enumerate(tables):
             grid[b, :len(t)] = t
-        hv[3 * Bb:3 * Bb + B] = grid[np.arange(B), pos // bs]
+        hv[3 * Bb:3 * Bb + B] = grid[np.arange(B), at // bs]
 
     def reset_graphs(self) -> None:
         """Drop the captured decode graphs (they are captured again on use)."""
@@ -385,14 +473,17 @@ class InferenceEngine:
             rope = getattr(getattr(blk, "attn", None), "rope", None)
             if rope is not None:
                 rope.tables(self.max_seq_len + 1, dev)
-        buf = torch.zeros(5 * Bb + Bb * Wb, dtype=torch.int32, device=dev)
+        buf = torch.zeros(6 * Bb + Bb * Wb, dtype=torch.int32, device=dev)
+        buf[5 * Bb + Bb * Wb:] = -1  # nobody's attention weights
         buf[2 * Bb:3 * Bb] = 1  # padding rows: context of one token...
         buf[3 * Bb:4 * Bb] = self._pad_block  # ...written into the padding block
-        buf[5 * Bb:].view(Bb, Wb)[:, 0] = self._pad_block
+        tables = buf[5 * Bb:5 * Bb + Bb * Wb].view(Bb, Wb)
+        tables[:, 0] = self._pad_block
         meta = PagedDecodeMeta(positions=buf[Bb:2 * Bb].view(Bb, 1), max_pos=self.max_seq_len - 1,
                                ctx_lens=buf[2 * Bb:3 * Bb], slot_block=buf[3 * Bb:4 * Bb], slot_off=buf[4 * Bb:5 * Bb],
-                               block_tables=buf[5 * Bb:].view(Bb, Wb),
-                               split_tokens=self._split_tokens(Bb, Wb * self.allocator.block_size))
+                               block_tables=tables,
+                               split_tokens=self._split_tokens(Bb, Wb * self.allocator.block_size),
+                               weight_rows=buf[5 * Bb + Bb * Wb:])
         cur = torch.cuda.current_stream(dev)
         side = torch.cuda.Stream(dev)
         side.wait_stream(cur)
@@ -430,12 +521,12 @@ class InferenceEngine:
                 self._graph_fail.add(key)
                 return None
             self._graphs[key] = gr
-        n = 5 * Bb + Bb * Wb
+        n = 6 * Bb + Bb * Wb
         if self._pinned is None or self._pinned.numel() < n:
             self._pinned = torch.empty(max(n, 1024), dtype=torch.int32, pin_memory=True)
         host = self._pinned[:n]
         self.stage_graph_inputs(host.numpy(), [s.tokens[-1] for s in seqs], [s.position for s in seqs], tables,
-                                Bb, Wb, self._pad_block, bs)
+                                Bb, Wb, self._pad_block, bs, [s.cached for s in seqs], [s.row for s in seqs])
         gr["buf"].copy_(host, non_blocking=True)
         with self.tracer.span("decode", batch=B, graph=1):
             gr["graph"].replay()
@@ -536,15 +627,31 @@ class InferenceEngine:
                 out.index_copy_(0, idx, tok)
         if evs is not None:
             evs.append(self._event())
+        said = self._logprobs(seqs, logits, out)
         tokens = out.tolist()
         produced = 0
-        for s, tok in zip(seqs, tokens):
-            produced += self._emit(s, int(tok))
+        for i, (s, tok) in enumerate(zip(seqs, tokens)):
+            produced += self._emit(s, int(tok), *said.get(i, ()))
         return produced
 
-    def _emit(self, st: _Seq, token: int) -> int:
+    @staticmethod
+    def _logprobs(seqs: List[_Seq], logits: torch.Tensor, tokens: torch.Tensor) -> Dict[int, tuple]:
+        """Row -> (log-prob of its token, alternatives) of the rows whose request asks for them."""
+        rows = [i for i, s in enumerate(seqs) if s.req.params.logprobs is not None]
+        if not rows:
+            return {}
+        if len(rows) < len(seqs):
+            at = torch.as_tensor(rows, device=logits.device)
+            logits, tokens = logits.index_select(0, at), tokens.index_select(0, at)
+        top = min(max(seqs[i].req.params.logprobs for i in rows), logits.shape[-1])
+        r = token_logprobs(logits, tokens, top=top)
+        lp, ids, top_lp = r.logprobs.tolist(), r.top_ids.tolist(), r.top_logprobs.tolist()
+        return {i: (lp[j], list(zip(ids[j], top_lp[j]))[:seqs[i].req.params.logprobs]) for j, i in enumerate(rows)}
+
+    def _emit(self, st: _Seq, token: int, logprob: Optional[float] = None,
+              top: Optional[List[Tuple[int, float]]] = None) -> int:
         req, p = st.req, st.req.params
-        req.push_token(token)
+        req.push_token(token, logprob, top)
         st.tokens.append(token)
         stop = set(p.stop_token_ids)
         if self.eos_token_id is not None:
@@ -567,13 +674,20 @@ class InferenceEngine:
         return 1
 
     # ------------------------------------------------------------ retirement
-    def _forget(self, st: _Seq) -> None:
+    def _unshare(self, st: _Seq) -> None:
+        """No new request shares this sequence's prompt from here on."""
         rid = st.req.id
-        self.states.pop(rid, None)
         self._prompt_logits.pop(rid, None)
         key = tuple(st.req.prompt_tokens)
         if self._prefix_owner.get(key) == rid:
             del self._prefix_owner[key]
+
+    def _forget(self, st: _Seq) -> None:
+        self.states.pop(st.req.id, None)
+        self._unshare(st)
+        if st.row >= 0:
+            self._free_rows.append(st.row)
+            st.row = -1
         st.cache = None
 
     def _retire(self, st: _Seq, reason: str) -> None:
@@ -634,4 +748,6 @@ class InferenceEngine:
                "decode_graphs": len(self._graphs) if self.decode_graphs else 0, "spans": self.tracer.summary()}
         if self.kv is not None:
             out["kv_cache_bytes"] = self.kv.nbytes
+        if self.kv_budget is not None:
+            out["evictions"] = self.evictions
         return out

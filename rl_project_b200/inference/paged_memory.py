@@ -7,6 +7,9 @@ pool per layer for K and V, sequences address it through block tables, and
 the decode kernel (csrc/paged_attention.cu) reads it directly, so sequences
 of different lengths decode in one batch and nothing is concatenated or split.
 
+``PagedQ4KVCache`` holds the same blocks in 4 bits (ops/paged_q4.py: 0.28 of the bytes at head sizes 64 and 128),
+optionally with accumulators of the cached tokens' attention weights, by which the engine evicts.
+
 ``PagedBlockAllocator`` keeps the reference's interface (``blocks_needed``,
 ``can_allocate``, ``allocate``, ``append_token``, ``free``, ``stats``) and adds
 reference counts: ``share_prefix`` lets a new sequence reuse the blocks of a
@@ -109,6 +112,22 @@ class PagedBlockAllocator:
         self.lengths[child_id] = n_tokens
         return self.tables[child_id]
 
+    def replace(self, seq_id: str, n_tokens: int) -> Tuple[List[int], List[int]]:
+        """Give ``seq_id`` fresh blocks for ``n_tokens`` and return ``(old, new)`` tables.  The old blocks stay
+        referenced until the caller, done copying from them, passes them to ``release``."""
+        need = self.blocks_needed(n_tokens)
+        if need > len(self.free_blocks):
+            raise OutOfBlocksError(f"sequence {seq_id} needs {need} fresh blocks, {len(self.free_blocks)} free")
+        old, new = self.tables[seq_id], [self._take() for _ in range(need)]
+        self.tables[seq_id] = list(new)
+        self.lengths[seq_id] = n_tokens
+        return old, new
+
+    def release(self, blocks: List[int]) -> None:
+        """Drop one reference of each block (of a table that ``replace`` returned)."""
+        for b in blocks:
+            self._release(b)
+
     def free(self, seq_id: str) -> None:
         for b in self.tables.pop(seq_id, []):
             self._release(b)
@@ -164,3 +183,50 @@ class PagedKVCache:
         kl, vl = self.layer(layer)
         paged_write(k.transpose(0, 1), v.transpose(0, 1), kl, vl, blocks.to(dev, non_blocking=True),
                     offs.to(dev, non_blocking=True))
+
+
+class PagedQ4KVCache:
+    """K/V pools in 4 bits, uint8 ``[n_layer, num_blocks, Hkv, block bytes]`` (layout: ops/paged_q4.py), with the
+    interface of ``PagedKVCache``.
+
+    With ``weight_rows`` sequences of up to ``weight_tokens`` cached tokens each have an accumulator row of
+    attention weights per layer and KV head (fp32 ``[n_layer, rows, Hkv, tokens]``).
+    """
+
+    def __init__(self, n_layer: int, n_kv_head: int, head_dim: int, num_blocks: int, device: torch.device,
+                 block_size: int = KERNEL_BLOCK, weight_rows: int = 0, weight_tokens: int = 0):
+        from rl_project_b200.ops.paged_q4 import HEAD_DIMS, q4_block_bytes
+
+        if block_size != KERNEL_BLOCK:
+            raise ServingError(f"the paged KV cache uses {KERNEL_BLOCK}-token blocks (got {block_size})")
+        if head_dim not in HEAD_DIMS:
+            raise ServingError(f"the 4-bit KV cache has heads of {HEAD_DIMS} (got {head_dim})")
+        shape = (n_layer, num_blocks, n_kv_head, q4_block_bytes(head_dim))
+        self.k = torch.zeros(shape, dtype=torch.uint8, device=device)
+        self.v = torch.zeros(shape, dtype=torch.uint8, device=device)
+        self.weights: Optional[torch.Tensor] = None
+        if weight_rows:
+            self.weights = torch.zeros(n_layer, weight_rows, n_kv_head, weight_tokens, device=device)
+        self.head_dim = head_dim
+        self.block_size = block_size
+        self.num_blocks = num_blocks
+
+    def layer(self, i: int) -> Tuple[torch.Tensor, ...]:
+        return (self.k[i], self.v[i]) if self.weights is None else (self.k[i], self.v[i], self.weights[i])
+
+    @property
+    def nbytes(self) -> int:
+        return 2 * self.k.numel() + (0 if self.weights is None else 4 * self.weights.numel())
+
+    def copy_block(self, src: int, dst: int) -> None:
+        self.k[:, dst].copy_(self.k[:, src])
+        self.v[:, dst].copy_(self.v[:, src])
+
+    def evict(self, tables: torch.Tensor, lens: torch.Tensor, new_tables: torch.Tensor, rows: torch.Tensor, keep: int,
+              recent: int, sink: int) -> None:
+        """Cut the given sequences to ``keep`` tokens in every layer (``ops.paged_q4.paged_evict_q4``)."""
+        from rl_project_b200.ops.paged_q4 import paged_evict_q4
+
+        for i in range(self.k.shape[0]):
+            k, v, w = self.layer(i)
+            paged_evict_q4(k, v, tables, lens, new_tables, w, rows, keep, self.head_dim, recent=recent, sink=sink)

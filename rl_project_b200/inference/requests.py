@@ -38,6 +38,9 @@ _ALLOWED = {
 }
 
 
+MAX_LOGPROBS = 20  # alternatives per token (the limit of the API that the server speaks)
+
+
 def _in_range(value, lo, hi, lo_open=False) -> bool:
     return (lo < value if lo_open else lo <= value) and value <= hi
 
@@ -51,6 +54,7 @@ class SamplingParams:
     min_p: Optional[float] = None
     repetition_penalty: float = 1.0
     stop_token_ids: List[int] = field(default_factory=list)
+    logprobs: Optional[int] = None  # record each generated token's log-prob and this many alternatives
 
     def validate(self) -> None:
         problems = []
@@ -64,6 +68,8 @@ class SamplingParams:
             problems.append("top_p must be in (0, 1]")
         if self.min_p is not None and not _in_range(self.min_p, 0.0, 1.0):
             problems.append("min_p must be in [0, 1]")
+        if self.logprobs is not None and not _in_range(self.logprobs, 0, MAX_LOGPROBS):
+            problems.append(f"logprobs must be between 0 and {MAX_LOGPROBS}")
         if self.repetition_penalty <= 0:
             problems.append("repetition_penalty must be > 0")
         if problems:
@@ -93,6 +99,10 @@ class GenerationRequest:
     started_at: Optional[float] = None
     finished_at: Optional[float] = None
     meta: dict = field(default_factory=dict)
+    # with params.logprobs: per generated token its log-prob under the model's distribution (temperature 1, no filters)
+    # and the most likely tokens as (id, log-prob), falling
+    token_logprobs: List[float] = field(default_factory=list)
+    top_logprobs: List[List[Tuple[int, float]]] = field(default_factory=list)
     _cv: threading.Condition = field(default_factory=threading.Condition, repr=False, compare=False)
 
     # ------------------------------------------------------------ state
@@ -115,8 +125,12 @@ class GenerationRequest:
             self._move(RequestStatus.RUNNING)
             self.started_at = time.time()
 
-    def push_token(self, token: int) -> None:
+    def push_token(self, token: int, logprob: Optional[float] = None,
+                   top: Optional[List[Tuple[int, float]]] = None) -> None:
         with self._cv:
+            if logprob is not None:
+                self.token_logprobs.append(logprob)
+                self.top_logprobs.append(top or [])
             self.generated_tokens.append(int(token))
             self._cv.notify_all()
 

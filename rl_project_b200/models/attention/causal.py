@@ -21,6 +21,7 @@ from rl_project_b200.ops import gemm
 from rl_project_b200.ops.attention import attention_reference, causal_attention
 from rl_project_b200.ops.linear import linear
 from rl_project_b200.ops.paged_attention import paged_decode, paged_write
+from rl_project_b200.ops.paged_q4 import paged_decode_q4, paged_write_q4
 from rl_project_b200.ops.rope import RopeTable, rope_split_qkv
 
 KVCache = Tuple[torch.Tensor, torch.Tensor]
@@ -33,7 +34,9 @@ class PagedDecodeMeta:
     ``positions [B, 1]`` is each new token's position (= cached tokens before
     it); its K/V go to block ``slot_block[b]``, offset ``slot_off[b]``; attention
     then covers ``ctx_lens[b] = positions[b] + 1`` tokens through
-    ``block_tables [B, max_blocks]``.  All int32 on the model's device.
+    ``block_tables [B, max_blocks]``.  All int32 on the model's device.  After an eviction a sequence has fewer
+    cached tokens than positions; ``ctx_lens`` and the slots count the cached ones.  ``weight_rows [B]`` are the
+    accumulator rows of a cache with attention weights (-1: none).
     """
 
     positions: torch.Tensor
@@ -43,6 +46,7 @@ class PagedDecodeMeta:
     slot_block: torch.Tensor
     slot_off: torch.Tensor
     split_tokens: int = 0
+    weight_rows: Optional[torch.Tensor] = None
 
 
 def layer_window(spec: ModelSpec, layer_id: int) -> int:
@@ -143,12 +147,19 @@ class CausalSelfAttention(nn.Module):
         return self._out(y), present
 
     def forward_paged(self, x: torch.Tensor, kv: KVCache, meta: PagedDecodeMeta) -> torch.Tensor:
-        """One new token per sequence (``x [B, 1, C]``) against this layer's paged K/V pools."""
+        """One new token per sequence (``x [B, 1, C]``) against this layer's paged K/V pools (uint8 pools: held in
+        4 bits, followed by the accumulators of attention weights if the cache has them)."""
         B = x.shape[0]
         qkv = self._qkv(x)
         q, k, v = rope_split_qkv(qkv, self.rope, self.n_head, self.n_kv_head, self.head_dim,
                                  positions=meta.positions, rotate=self.use_rope, heads_major=False,
                                  max_pos=meta.max_pos)
+        if kv[0].dtype == torch.uint8:
+            paged_write_q4(k[:, 0], v[:, 0], kv[0], kv[1], meta.slot_block, meta.slot_off)
+            y = paged_decode_q4(q[:, 0], kv[0], kv[1], meta.block_tables, meta.ctx_lens, 1.0 / math.sqrt(self.head_dim),
+                                self.attn_logit_cap, self.window_size, weights=kv[2] if len(kv) > 2 else None,
+                                weight_rows=meta.weight_rows if len(kv) > 2 else None)
+            return self._out(y.reshape(B, 1, self.n_head * self.head_dim))
         paged_write(k[:, 0], v[:, 0], kv[0], kv[1], meta.slot_block, meta.slot_off)
         y = paged_decode(q[:, 0], kv[0], kv[1], meta.block_tables, meta.ctx_lens, 1.0 / math.sqrt(self.head_dim),
                          self.attn_logit_cap, self.window_size, meta.split_tokens)

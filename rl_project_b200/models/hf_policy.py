@@ -14,7 +14,7 @@ import torch.nn as nn
 from rl_project_b200.core.errors import ConfigError, OptionalDependencyError
 from rl_project_b200.core.protocols import GenerationSettings
 from rl_project_b200.models.policy import ValueHead
-from rl_project_b200.ops.logprob import logprobs_from_logits
+from rl_project_b200.ops.logprob import logprobs_from_logits, token_logprobs
 
 
 class _TokenizerAdapter:
@@ -148,10 +148,8 @@ class HFPolicy(nn.Module):
 
     def token_logprobs(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         """Per-position ``log p(targets | input_ids)`` ``[B, T]``; 0 where ``targets == -1``."""
-        logits = self.token_logits(input_ids).float()
-        tg = targets.to(logits.device)
-        lp = torch.log_softmax(logits, -1).gather(-1, tg.clamp(min=0)[..., None])[..., 0]
-        return lp * (tg >= 0)
+        logits = self.token_logits(input_ids)
+        return token_logprobs(logits, targets.to(logits.device)).logprobs
 
     def token_ce(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         """Mean next-token cross-entropy over ``targets != -1`` (the SFT / pretrain loss)."""
@@ -162,11 +160,8 @@ class HFPolicy(nn.Module):
     def logprobs_with_entropy(self, prompt_ids, response_ids):
         """Response-token log-probs and the policy's entropy at each response position."""
         full, out = self._forward(prompt_ids, response_ids)
-        logits = out.logits[:, prompt_ids.shape[1] - 1:-1].float()
-        logp = torch.log_softmax(logits, -1)
-        lp = logp.gather(-1, full[:, prompt_ids.shape[1]:, None])[..., 0]
-        ent = -(logp.exp() * logp).sum(-1)
-        return lp, ent
+        r = token_logprobs(out.logits[:, prompt_ids.shape[1] - 1:-1], full[:, prompt_ids.shape[1]:])
+        return r.logprobs, r.entropy
 
     def with_frozen_reference(self) -> "HFPolicy":
         """A frozen copy of the initial weights as the KL reference when no adapter is attached (with LoRA the

@@ -220,7 +220,10 @@ def _token_logprobs_reference(x: torch.Tensor, t: torch.Tensor, top: int):
     lp = logp.gather(-1, t.clamp(min=0)[:, None])[:, 0]
     p = logp.exp()
     ent = -torch.where(p == 0, torch.zeros_like(p), p * logp.masked_fill(p == 0, 0.0)).sum(-1)
-    ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top]
+    if top:
+        ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top]
+    else:
+        ids = torch.empty(x.shape[0], 0, dtype=torch.long)
     inf, zero = torch.full_like(lp, float("-inf")), torch.zeros_like(lp)
     lp = torch.where(t >= 0, torch.where(dead[:, 0], inf, lp), zero)
     return lp, torch.where(dead[:, 0], zero, ent), logp.gather(-1, ids).masked_fill(dead, float("-inf")), ids

@@ -45,6 +45,7 @@ class RolloutConfig:
     # > 0 in a distributed run: the ranks form world / replica_tp tensor-parallel generation replicas of this
     # many GPUs (rollouts/replicas.py) that share each step's prompts; 0: every rank generates its own
     replica_tp: int = 0
+    engine_kv_cache: str = "bf16"  # how the paged engine holds keys and values: bf16 | q4 (4 bits)
 
 
 class RolloutEngine:
@@ -76,7 +77,8 @@ class RolloutEngine:
             per_seq = (model.spec.block_size + 15) // 16 + 1
             self._engine = InferenceEngine(model, max_batch=self.cfg.engine_max_batch,
                                            max_blocks=self.cfg.engine_kv_blocks or self.cfg.engine_max_batch * per_seq,
-                                           decode_graphs=self.cfg.engine_decode_graphs)
+                                           decode_graphs=self.cfg.engine_decode_graphs,
+                                           kv_cache=self.cfg.engine_kv_cache)
         return self._engine
 
     def release_engine(self) -> None:

@@ -115,7 +115,8 @@ class Router:
             return 200, self._sse(pieces, lambda t, fr: chunk(rid, name, t, fr), t0, name)
         res = backend.complete(prompt, req.sampling(), rid, stop=req.stop)
         self._record(t0, res.completion_tokens, name)
-        return 200, respond(rid, name, res.text, res.prompt_tokens, res.completion_tokens, res.finish_reason, name)
+        return 200, respond(rid, name, res.text, res.prompt_tokens, res.completion_tokens, res.finish_reason, name,
+                            logprobs=getattr(res, "logprobs", None))
 
     def completions(self, body: Dict[str, Any]) -> Response:
         req = CompletionRequest.from_dict(body)

@@ -15,6 +15,7 @@ from typing import Any, Dict, Iterator, List, Optional, Protocol, Sequence
 
 from rl_project_b200.core.errors import BackendUnavailableError, ServingError
 from rl_project_b200.inference.requests import GenerationRequest, SamplingParams
+from rl_project_b200.serving.schemas import TokenLogprob
 
 
 @dataclass
@@ -25,6 +26,7 @@ class CompletionResult:
     finish_reason: str
     backend: str
     request_id: str
+    logprobs: Optional[List[TokenLogprob]] = None  # with SamplingParams.logprobs
 
 
 class Backend(Protocol):
@@ -125,7 +127,20 @@ class EngineBackend(_Toggle):
             text, finish = text[:cut], "stop"
         return CompletionResult(text=text, prompt_tokens=len(req.prompt_tokens), completion_tokens=len(tokens),
                                 finish_reason=finish or req.finish_reason or "length", backend=self.name,
-                                request_id=req.id)
+                                request_id=req.id, logprobs=self._token_logprobs(req, tokens, len(text)))
+
+    def _token_logprobs(self, req: GenerationRequest, tokens: List[int], end: int) -> Optional[List[TokenLogprob]]:
+        """The recorded log-probs of the tokens that begin within the first ``end`` characters of the text."""
+        if req.params.logprobs is None:
+            return None
+        decode, out = self.tokenizer.decode, []
+        for i, lp in enumerate(req.token_logprobs[:len(tokens)]):
+            offset = len(decode(tokens[:i]))
+            if offset >= end:
+                break
+            out.append(TokenLogprob(decode([tokens[i]]), offset, lp,
+                                    [(decode([t]), x) for t, x in req.top_logprobs[i]]))
+        return out
 
     def stream(self, prompt: str, params: SamplingParams, request_id: Optional[str] = None,
                stop: Sequence[str] = ()) -> Iterator[str]:

@@ -12,7 +12,7 @@ from __future__ import annotations
 import time
 import uuid
 from dataclasses import dataclass, field
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, Optional, Tuple
 
 from rl_project_b200.core.errors import ServingError
 from rl_project_b200.inference.requests import SamplingParams
@@ -30,14 +30,35 @@ def _stop_list(value: Any) -> List[str]:
     raise ServingError("'stop' must be a string or a list of strings")
 
 
+def _logprobs(d: Dict[str, Any]) -> Optional[int]:
+    """Alternatives per token to report, None for no log-probs: ``logprobs: n`` (completions), or ``logprobs: true``
+    with ``top_logprobs: n`` (chat)."""
+    want, top = d.get("logprobs"), d.get("top_logprobs")
+    if want is None or want is False:
+        if top:
+            raise ServingError("'top_logprobs' needs 'logprobs'")
+        return None
+    return int(top or 0) if want is True else int(want)
+
+
 def _common(d: Dict[str, Any]) -> Dict[str, Any]:
     try:
         return {"model": d.get("model"), "max_tokens": int(d.get("max_tokens", 64)),
                 "temperature": float(d.get("temperature", 0.8)), "top_k": d.get("top_k", 50),
                 "top_p": d.get("top_p"), "stream": bool(d.get("stream", False)), "stop": _stop_list(d.get("stop")),
-                "user": d.get("user"), "request_id": d.get("request_id")}
+                "user": d.get("user"), "request_id": d.get("request_id"), "logprobs": _logprobs(d)}
     except (TypeError, ValueError) as exc:
         raise ServingError(f"invalid numeric field: {exc}") from exc
+
+
+@dataclass
+class TokenLogprob:
+    """One generated token: its text, where it begins in the completion, its log-prob and alternatives (text, log-prob)."""
+
+    text: str
+    offset: int
+    logprob: float
+    top: List[Tuple[str, float]]
 
 
 @dataclass
@@ -51,10 +72,11 @@ class _SamplingFields:
     stop: List[str] = field(default_factory=list)
     user: Optional[str] = None
     request_id: Optional[str] = None
+    logprobs: Optional[int] = None
 
     def sampling(self) -> SamplingParams:
         return SamplingParams(max_tokens=self.max_tokens, temperature=self.temperature, top_k=self.top_k,
-                              top_p=self.top_p)
+                              top_p=self.top_p, logprobs=self.logprobs)
 
 
 @dataclass
@@ -116,10 +138,14 @@ def _usage(prompt_tokens: int, completion_tokens: int) -> Dict[str, int]:
 
 
 def completion_response(request_id: str, model: str, text: str, prompt_tokens: int, completion_tokens: int,
-                        finish_reason: str, backend: Optional[str] = None) -> Dict[str, Any]:
+                        finish_reason: str, backend: Optional[str] = None,
+                        logprobs: Optional[List[TokenLogprob]] = None) -> Dict[str, Any]:
+    said = None if logprobs is None else {
+        "tokens": [t.text for t in logprobs], "token_logprobs": [t.logprob for t in logprobs],
+        "top_logprobs": [dict(t.top) for t in logprobs], "text_offset": [t.offset for t in logprobs]}
     out: Dict[str, Any] = {"id": f"cmpl-{request_id}", "object": "text_completion", "created": int(time.time()),
                            "model": model,
-                           "choices": [{"text": text, "index": 0, "finish_reason": finish_reason, "logprobs": None}],
+                           "choices": [{"text": text, "index": 0, "finish_reason": finish_reason, "logprobs": said}],
                            "usage": _usage(prompt_tokens, completion_tokens)}
     if backend:
         out["forgeline"] = {"backend": backend}
@@ -127,12 +153,19 @@ def completion_response(request_id: str, model: str, text: str, prompt_tokens: i
 
 
 def chat_response(request_id: str, model: str, text: str, prompt_tokens: int, completion_tokens: int,
-                  finish_reason: str, backend: Optional[str] = None) -> Dict[str, Any]:
+                  finish_reason: str, backend: Optional[str] = None,
+                  logprobs: Optional[List[TokenLogprob]] = None) -> Dict[str, Any]:
     out: Dict[str, Any] = {"id": f"chatcmpl-{request_id}", "object": "chat.completion", "created": int(time.time()),
                            "model": model,
                            "choices": [{"index": 0, "message": {"role": "assistant", "content": text},
                                         "finish_reason": finish_reason}],
                            "usage": _usage(prompt_tokens, completion_tokens)}
+    if logprobs is not None:
+        def entry(text: str, lp: float) -> Dict[str, Any]:
+            return {"token": text, "logprob": lp, "bytes": list(text.encode())}
+
+        out["choices"][0]["logprobs"] = {"content": [
+            {**entry(t.text, t.logprob), "top_logprobs": [entry(*x) for x in t.top]} for t in logprobs]}
     if backend:
         out["forgeline"] = {"backend": backend}
     return out

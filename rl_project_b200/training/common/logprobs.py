@@ -96,10 +96,9 @@ def packed_response_logprobs(policy, trajectories, width: int, with_entropy: boo
     elif hasattr(policy.model, "token_logprobs"):  # the native model: entropy from the same fused pass
         lp, ent = policy.model.token_logprobs(inputs, targets, with_entropy=True)
     else:  # other backends: from full logits
-        logits = policy.token_logits(inputs).float()
-        logp = logits.log_softmax(-1)
-        lp = logp.gather(-1, targets.clamp(min=0)[..., None])[..., 0] * (targets >= 0)
-        ent = -(logp.exp() * logp).sum(-1)
+        from rl_project_b200.ops.logprob import token_logprobs
+
+        lp, ent = token_logprobs(policy.token_logits(inputs), targets)[:2]
     starts = torch.tensor([len(p) - 1 for p, _ in pairs], device=dev)
     cols = (starts[:, None] + torch.arange(width, device=dev)[None, :]).clamp(max=lp.shape[1] - 1)
     return lp.float().gather(1, cols), (ent.float().gather(1, cols) if ent is not None else None)

@@ -1,0 +1,231 @@
+"""The inference engine over the 4-bit KV cache, with evictions, and the log-probabilities it records."""
+
+import math
+
+import pytest
+import torch
+
+from rl_project_b200.core.config import ModelSpec
+from rl_project_b200.core.errors import ServingError
+from rl_project_b200.inference import InferenceEngine, PagedQ4KVCache, SamplingParams
+from rl_project_b200.models.transformer.model import TransformerLM
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def model(dev, n_embd=128, n_head=4, n_kv_head=2, block_size=256, **kw):
+    torch.manual_seed(0)
+    spec = ModelSpec(n_layer=2, n_head=n_head, n_kv_head=n_kv_head, n_embd=n_embd, block_size=block_size, dropout=0.0,
+                     vocab_size=97, **kw)
+    m = TransformerLM(spec).eval()
+    return m.cuda().bfloat16() if dev == "cuda" else m
+
+
+GREEDY = dict(temperature=0.0, top_k=None)
+PROMPTS = [[1, 2, 3], list(range(5, 75)), [7] * 33, list(range(40, 57))]
+
+
+@pytest.mark.parametrize("extra", [{}, {"sliding_window": 24, "alternating_layers": True, "attn_logit_cap": 30.0}])
+def test_same_tokens_as_a_cache_of_rounded_rows(monkeypatch, extra):
+    """The 4-bit engine generates what the plain cache does when every key and value is rounded on its way in."""
+    from rl_project_b200.inference import engine as eng_mod
+    from rl_project_b200.models.attention import causal
+    from rl_project_b200.ops import paged_q4
+    from rl_project_b200.ops.paged_attention import paged_write
+
+    m = model("cpu", **extra)
+    params = SamplingParams(max_tokens=20, **GREEDY)
+    eng = InferenceEngine(m, max_batch=4, kv_cache="q4")
+    assert isinstance(eng.kv, PagedQ4KVCache) and eng.kv.nbytes < 0.3 * InferenceEngine(m, max_batch=4).kv.nbytes
+    got = [r.generated_tokens for r in eng.generate_batch(PROMPTS, params)]
+    assert eng.allocator.used_blocks == 0
+
+    def rounded(x):
+        pools = [torch.zeros(-(-len(x) // 16), x.shape[1], paged_q4.q4_block_bytes(x.shape[2]), dtype=torch.uint8)
+                 for _ in range(2)]
+        at = torch.arange(len(x), dtype=torch.int32)
+        paged_q4.paged_write_q4(x, x, *pools, at // 16, at % 16)
+        return paged_q4._values(pools[0], x.shape[2]).transpose(1, 2).flatten(0, 1)[:len(x)]
+
+    def write(k, v, k_pool, v_pool, blk, off, status=None):
+        paged_write(rounded(k), rounded(v), k_pool, v_pool, blk, off)
+
+    monkeypatch.setattr(causal, "paged_write", write)
+    monkeypatch.setattr(eng_mod, "paged_write", write)
+    ref = InferenceEngine(m, max_batch=4)
+    assert [r.generated_tokens for r in ref.generate_batch(PROMPTS, params)] == got
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_evictions(dev):
+    """Caches stay within the budget's bounds while positions go on; everything is returned at the end."""
+    m = model(dev)
+    eng = InferenceEngine(m, max_batch=4, kv_cache="q4", kv_budget=32, kv_sink=2, kv_recent=8)
+    reqs = [eng.submit(p, SamplingParams(max_tokens=90, **GREEDY)) for p in PROMPTS]
+    seen = {}
+    while not all(r.finished for r in reqs):
+        eng.step()
+        for st in eng.states.values():
+            n = len(st.req.generated_tokens)
+            assert st.position == len(st.req.prompt_tokens) + n - 1
+            if n > 2:
+                assert st.cached <= 32 + 16
+            seen[st.req.id] = max(seen.get(st.req.id, 0), st.evicted)
+            assert len(eng.allocator.tables[st.req.id]) == -(-(st.cached + 1) // 16)
+    assert all(len(r.generated_tokens) == 90 for r in reqs)
+    # a prompt of 70 is cut to 32 at its second decode step at the latest, then after every 16 tokens
+    by_prompt = {tuple(r.prompt_tokens): seen[r.id] for r in reqs}
+    assert by_prompt[tuple(PROMPTS[1])] >= 70 + 88 - 48 and by_prompt[tuple(PROMPTS[0])] >= 3 + 88 - 48
+    assert eng.stats()["evictions"] == eng.evictions > 8
+    assert eng.allocator.used_blocks == (1 if eng.decode_graphs else 0)  # graph decode keeps a padding block
+    assert sorted(eng._free_rows) == [0, 1, 2, 3]
+
+
+def test_budget_never_reached_changes_nothing():
+    m = model("cpu")
+    params = SamplingParams(max_tokens=24, **GREEDY)
+    outs = [[r.generated_tokens for r in InferenceEngine(m, max_batch=4, kv_cache="q4", **kw).generate_batch(PROMPTS, params)]
+            for kw in ({}, {"kv_budget": 200})]
+    assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_shared_prompts_with_evictions(dev):
+    """Samples of one prompt share its blocks until the first is cut; what it is cut from stays whole for the rest."""
+    m = model(dev)
+    prompt = list(range(3, 60))
+    kw = dict(max_batch=4, kv_cache="q4", kv_budget=32, kv_sink=2, kv_recent=8)
+    params = SamplingParams(max_tokens=40, **GREEDY)
+    eng = InferenceEngine(m, **kw)
+    reqs = [eng.submit(prompt, params) for _ in range(3)]
+    eng.step()
+    late = eng.submit(prompt, params)  # joins after the others were prefilled, maybe cut
+    eng.run_until_idle()
+    assert eng.shared_prefills >= 2
+    alone = InferenceEngine(m, **kw).generate(prompt, params).generated_tokens
+    if dev == "cpu":  # (bf16 products of another batch size round differently)
+        assert all(r.generated_tokens == alone for r in reqs + [late])
+    assert eng.allocator.used_blocks == (1 if eng.decode_graphs else 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget", [None, 48])
+@pytest.mark.parametrize("shape", [(256, 4, 1), (512, 4, 2), (128, 4, 4)])
+def test_graph_decode_matches_eager_decode(shape, budget):
+    """The same greedy requests decoded eagerly and from captured graphs, caches cut in between."""
+    m = model("cuda", *shape)
+    outs = {}
+    for graphs in (False, True):
+        eng = InferenceEngine(m, max_batch=8, decode_graphs=graphs, kv_cache="q4", kv_budget=budget)
+        reqs = eng.generate_batch(PROMPTS, SamplingParams(max_tokens=60, **GREEDY))
+        outs[graphs] = [r.generated_tokens for r in reqs]
+        assert (eng.evictions > 3) == (budget is not None)
+        if graphs:
+            assert eng._graphs and eng.allocator.used_blocks == 1
+    assert outs[True] == outs[False]
+    from rl_project_b200.ops._ext import check_bounds
+
+    check_bounds(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kv", ["bf16", "q4"])
+def test_recorded_logprobs(dev, kv):
+    """Log-probs and alternatives of every generated token, for the requests that ask for them."""
+    m = model(dev)
+    eng = InferenceEngine(m, max_batch=4, kv_cache=kv)
+    asks = [3, None, 0, 20]
+    reqs = [eng.submit(p, SamplingParams(max_tokens=6, temperature=t, top_k=None, logprobs=n))
+            for p, n, t in zip(PROMPTS, asks, (0.0, 1.0, 1.0, 0.7))]
+    eng.run_until_idle()
+    for r, n in zip(reqs, asks):
+        if n is None:
+            assert not r.token_logprobs and not r.top_logprobs
+            continue
+        assert len(r.token_logprobs) == len(r.top_logprobs) == len(r.generated_tokens) == 6
+        assert all(len(t) == n for t in r.top_logprobs)
+        ids = torch.tensor([r.prompt_tokens + r.generated_tokens], device=dev)
+        with torch.no_grad():
+            want = m.full_logits(ids)[0].float().log_softmax(-1).cpu()
+        # the model's own rounding (bf16 on the GPU, keys and values in 4 bits) moves log-probs; the first token's come
+        # from the prompt's forward, which neither touches
+        tol = {"cpu": {"bf16": 1e-3, "q4": 1.0}, "cuda": {"bf16": 0.15, "q4": 1.0}}[dev][kv]
+        for i, tok in enumerate(r.generated_tokens):
+            row = want[len(r.prompt_tokens) - 1 + i]
+            bound = (1e-4 if dev == "cpu" else 0.1) if i == 0 else tol
+            assert abs(r.token_logprobs[i] - float(row[tok])) <= bound
+            top = r.top_logprobs[i]
+            assert all(a[1] >= b[1] for a, b in zip(top, top[1:]))
+            for t, lp in top:
+                assert abs(lp - float(row[t])) <= bound
+    assert [t[0][0] for t in reqs[0].top_logprobs] == reqs[0].generated_tokens  # greedy: the likeliest
+
+
+def test_served_logprobs():
+    from rl_project_b200.data.tokenizers import CharTokenizer
+    from rl_project_b200.serving import EngineBackend, Router
+
+    tok = CharTokenizer.ascii()
+    torch.manual_seed(0)
+    spec = ModelSpec(n_layer=1, n_head=2, n_kv_head=1, n_embd=64, block_size=128, dropout=0.0, vocab_size=tok.vocab_size)
+    eng = InferenceEngine(TransformerLM(spec).eval(), max_batch=2, kv_cache="q4", kv_budget=16)
+    router = Router({"m": EngineBackend("m", eng, tok, background=False)}, "m")
+    status, out = router.handle("POST", "/v1/completions", {"prompt": "abc", "max_tokens": 30, "logprobs": 2})
+    assert status == 200
+    said, text = out["choices"][0]["logprobs"], out["choices"][0]["text"]
+    assert "".join(said["tokens"]) == text and len(said["token_logprobs"]) == len(said["text_offset"]) == 30
+    assert all(text[o:].startswith(t) for o, t in zip(said["text_offset"], said["tokens"]))
+    assert all(len(t) == 2 for t in said["top_logprobs"]) and all(x <= 0 for x in said["token_logprobs"])
+    stop = text[7]
+    status, out = router.handle("POST", "/v1/chat/completions", {
+        "messages": [{"role": "user", "content": "hi"}], "max_tokens": 5, "logprobs": True, "top_logprobs": 3})
+    said = out["choices"][0]["logprobs"]["content"]
+    assert status == 200 and len(said) == 5 and all(len(e["top_logprobs"]) == 3 for e in said)
+    assert said[0]["bytes"] == list(said[0]["token"].encode())
+    status, out = router.handle("POST", "/v1/completions", {"prompt": "abc", "max_tokens": 30, "temperature": 0,
+                                                            "logprobs": 0, "stop": stop})
+    said = out["choices"][0]["logprobs"]
+    assert "".join(said["tokens"]) == out["choices"][0]["text"] and said["top_logprobs"] == [{}] * len(said["tokens"])
+    status, out = router.handle("POST", "/v1/completions", {"prompt": "abc", "max_tokens": 3})
+    assert out["choices"][0]["logprobs"] is None
+    for bad in ({"logprobs": 21}, {"logprobs": -1}, {"logprobs": "x"}, {"top_logprobs": 3}):
+        assert router.handle("POST", "/v1/completions", {"prompt": "abc", **bad})[0] == 400
+
+
+def test_refusals():
+    m = model("cpu")
+    for kw in ({"kv_cache": "int4"}, {"kv_budget": 64}, {"kv_cache": "q4", "kv_budget": 8},
+               {"kv_cache": "q4", "kv_budget": 64, "kv_sink": 40, "kv_recent": 40},
+               {"kv_cache": "q4", "kv_budget": 64, "kv_sink": -1}):
+        with pytest.raises(ServingError):
+            InferenceEngine(m, **kw)
+    with pytest.raises(ServingError):  # heads of 16
+        InferenceEngine(model("cpu", n_embd=64), kv_cache="q4")
+    with pytest.raises(ServingError):  # windows count cached tokens
+        InferenceEngine(model("cpu", sliding_window=24), kv_cache="q4", kv_budget=64)
+    with pytest.raises(ServingError):
+        SamplingParams(logprobs=21).validate()
+
+
+def test_packed_scoring_through_logits():
+    """The scoring path of policies that have logits only: values and gradients as from a plain log-softmax."""
+    from types import SimpleNamespace
+
+    from rl_project_b200.training.common.logprobs import pack_prompt_response, packed_response_logprobs
+
+    torch.manual_seed(1)
+    table = torch.randn(30, 30, requires_grad=True)
+    policy = SimpleNamespace(pad_token_id=0, device=torch.device("cpu"), model=object(),
+                             token_logits=lambda ids: table[ids])
+    trajs = [SimpleNamespace(prompt_ids=torch.tensor(p), response_ids=torch.tensor(r))
+             for p, r in (([1, 2], [3, 4, 5]), ([6], [7, 8]))]
+    lp, ent = packed_response_logprobs(policy, trajs, 3, with_entropy=True)
+    (lp[0].sum() + lp[1, :2].sum() + ent[0].sum() - ent[1, :2].sum()).backward()
+    got, table.grad = table.grad, None
+    inputs, targets = pack_prompt_response([([1, 2], [3, 4, 5]), ([6], [7, 8])], 0)
+    logp = table[inputs].log_softmax(-1)
+    want = logp.gather(-1, targets.clamp(min=0)[..., None])[..., 0]
+    h = -(logp.exp() * logp).sum(-1)
+    (want[0, 1:4].sum() + want[1, :2].sum() + h[0, 1:4].sum() - h[1, :2].sum()).backward()
+    assert torch.allclose(lp[0], want[0, 1:4], atol=1e-5) and torch.allclose(ent[1, :2], h[1, :2], atol=1e-5)
+    assert torch.allclose(got, table.grad, atol=1e-5) and math.isfinite(float(got.sum()))
