@@ -791,10 +791,50 @@ RLB_DEVICE float2 q4_join(const float* ml, int G, int parts) {
   return make_float2(M, sum != 0.f ? 1.f / sum : 0.f);
 }
 
-// Joins the parts of the rows that several CTAs of q4_decode_kernel shared, and writes zeros for empty sequences:
-// CTA z < G of a row does query head z, its eight warps taking the parts in turn.  With `weights` the CTAs behind
-// add a stretch each of the tokens' attention weights, summed over the heads, to their accumulators.
+// Unnormalised output (dimensions lane + 32 e) and statistics of parts first, first + step, ... of one query head, by a
+// whole warp, 8 parts at a time, relative to the largest maximum so far.  (A part that saw nothing has none: its
+// sums are 0, or NaN.)
 template <int D>
+RLB_DEVICE float2 q4_add_parts(const float* part, const float* stats, int G, int first, int step, int parts,
+                               float (&acc)[D / 32]) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY, sum = 0.f;
+  for (int s0 = first; s0 < parts; s0 += 8 * step) {
+    const int mine = s0 + step * (lane & 7);
+    const float2 x = mine < parts ? *reinterpret_cast<const float2*>(stats + 2LL * mine * G) : make_float2(-INFINITY, 0.f);
+    float a[8][E];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        a[k][e] = s0 + step * k < parts ? part[(long long)(s0 + step * k) * G * D + lane + 32 * e] : 0.f;
+    float m = x.x;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = fmaxf(m, M);
+    const float was = M == -INFINITY ? 1.f : sm100::ex2_approx(M - m);
+    M = m;
+    sum *= was;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= was;
+    const float f = x.x == -INFINITY ? 1.f : sm100::ex2_approx(x.x - m), l = x.y * f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      sum += __shfl_sync(0xffffffffu, l, k);
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += a[k][e] * fk;
+    }
+  }
+  return make_float2(M, sum);
+}
+
+// Joins the parts of the rows that several warps of q4_decode_kernel shared, and writes zeros for empty sequences.
+// WIDE: CTA z of a row does query head z, its eight warps taking the parts in turn (few rows, long contexts);
+// otherwise a warp does a query head.  With `weights` the CTAs behind add a stretch each of the tokens' attention
+// weights, summed over the heads, to their accumulators.
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
                                                         const float* __restrict__ ml, const int2* __restrict__ plan,
                                                         __nv_bfloat16* __restrict__ out,
@@ -804,75 +844,51 @@ __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* 
                                                         int w_len, int* status) {
   constexpr int E = D / 32;
   __shared__ float2 stat[16];
-  __shared__ float sums[8][D];
+  __shared__ float sums[WIDE ? 8 : 1][D];
   cudaGridDependencySynchronize();  // (every CTA: what follows this kernel must not overtake the one before)
-  const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, G = c.G;
+  const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, G = c.G, joins = WIDE ? G : (G + 7) / 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = (long long)b * c.Hkv + h;
   const int len = q4_len(c, b, nullptr);
-  if (len == 0) {
-    if (z < G)
-      for (int d = threadIdx.x; d < D; d += 256) out[(row * G + z) * D + d] = __float2bfloat16(0.f);
-    return;
-  }
-  const int2 at = plan[row];  // first slot, parts
+  const int2 at = len > 0 ? plan[row] : make_int2(0, 0);  // first slot, parts
   const float* stats = ml + (long long)at.x * G * 2;
-  if (z < G) {
-    if (at.y == 1) return;  // written already
-    // each warp's share of the parts, 8 at a time, relative to the largest maximum so far (a part that saw nothing
-    // has none: its sums are 0, or NaN)
-    float M = -INFINITY, sum = 0.f, acc[E] = {};
-    for (int s0 = warp; s0 < at.y; s0 += 64) {
-      const int mine = s0 + 8 * (lane & 7);
-      const float2 x = mine < at.y ? *reinterpret_cast<const float2*>(stats + (2LL * mine * G + 2 * z)) : make_float2(-INFINITY, 0.f);
-      float a[8][E];
+  if (z < joins) {
+    const int head = WIDE ? z : z * 8 + warp;
+    if (head >= G || at.y == 1) return;  // (one part: written already)
+    __nv_bfloat16* dst = out + (row * G + head) * D;
+    float acc[E] = {};
+    const float* from = part + ((long long)at.x * G + head) * D;
+    float2 s = q4_add_parts<D>(from, stats + 2 * head, G, WIDE ? warp : 0, WIDE ? 8 : 1, at.y, acc);
+    if (!WIDE) {
+      const float inv = s.y != 0.f ? 1.f / s.y : 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          a[k][e] = s0 + 8 * k < at.y ? part[(((long long)at.x + s0 + 8 * k) * G + z) * D + lane + 32 * e] : 0.f;
-      float m = x.x;
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      m = fmaxf(m, M);
-      const float was = M == -INFINITY ? 1.f : sm100::ex2_approx(M - m);
-      M = m;
-      sum *= was;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= was;
-      const float f = x.x == -INFINITY ? 1.f : sm100::ex2_approx(x.x - m);
-      const float l = x.y * f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        sum += __shfl_sync(0xffffffffu, l, k);
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += a[k][e] * fk;
-      }
+      for (int e = 0; e < E; ++e) dst[lane + 32 * e] = __float2bfloat16(acc[e] * inv);
+      return;
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[warp][lane + 32 * e] = acc[e];
-    if (lane == 0) stat[warp] = make_float2(M, sum);
+    if (lane == 0) stat[warp] = s;
     __syncthreads();
     float most = -INFINITY, total = 0.f, f[8];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) most = fmaxf(most, stat[s].x);
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, stat[i].x);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      f[s] = stat[s].x == -INFINITY ? 1.f : sm100::ex2_approx(stat[s].x - most);
-      total += stat[s].y * f[s];
+    for (int i = 0; i < 8; ++i) {
+      f[i] = stat[i].x == -INFINITY ? 1.f : sm100::ex2_approx(stat[i].x - most);
+      total += stat[i].y * f[i];
     }
     for (int d = threadIdx.x; d < D; d += 256) {
       float a = 0.f;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) a += sums[s][d] * f[s];
-      out[(row * G + z) * D + d] = __float2bfloat16(total != 0.f ? a / total : 0.f);
+      for (int i = 0; i < 8; ++i) a += sums[i][d] * f[i];
+      dst[d] = __float2bfloat16(total != 0.f ? a / total : 0.f);
     }
     return;
   }
+  if (len == 0) return;
   const int r = weight_rows[b];
   if (r < 0) return;
-  if (threadIdx.x == 0 && z == G && h == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
+  if (threadIdx.x == 0 && z == joins && h == 0 && (r >= w_rows || len > w_len)) report(status, kBadIndex);
   if (r >= w_rows) return;
   for (int head = warp; head < G; head += 8) {
     const float2 x = q4_join(stats + 2 * head, G, at.y);
@@ -881,8 +897,8 @@ __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* 
   __syncthreads();
   float* w = weights + ((long long)r * c.Hkv + h) * w_len;
   const float* sc = scores + row * c.max_blocks * kTok * Gs;
-  const int step = (gridDim.z - G) * 256;
-  for (int t = q4_first(c, len) + (z - G) * 256 + threadIdx.x; t < min(len, w_len); t += step) {
+  const int step = (gridDim.z - joins) * 256;
+  for (int t = q4_first(c, len) + (z - joins) * 256 + threadIdx.x; t < min(len, w_len); t += step) {
     float p = 0.f;
     for (int head = 0; head < G; ++head)
       p += sm100::ex2_approx(sc[(long long)t * Gs + head] - stat[head].x) * stat[head].y;
@@ -1260,12 +1276,15 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(Hkv, B, G + chunks);
+  // wide where more than about 6 parts fall on a row (at 7, 32 x 8192 tokens of 128: 8.6 us wide, 10.4 narrow; at 4.6,
+  // 64 x 4096 of 64: 9.7 wide, 7.2 narrow)
+  const bool wide = (long long)ctas * kDecodeWarps > 6LL * B * Hkv;
+  cfg.gridDim = dim3(Hkv, B, (wide ? G : (G + 7) / 8) + chunks);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  RLB_Q4_D(e = cudaLaunchKernelEx(&cfg, q4_finish_kernel<DD>, c, (const float*)part, (const float*)ml, (const int2*)plan,
+  RLB_Q4_D(e = cudaLaunchKernelEx(&cfg, wide ? q4_finish_kernel<DD, true> : q4_finish_kernel<DD, false>, c, (const float*)part, (const float*)ml, (const int2*)plan,
                                   (__nv_bfloat16*)out, (const float*)scores, Gs, weights, weight_rows, w_rows, w_len,
                                   status));
   return e;

@@ -65,16 +65,53 @@ RLB_DEVICE RowStats warp_stats(RowStats a) {
   return RowStats{m, warp_sum(a.s), warp_sum(a.t)};
 }
 
+// Pairs of fp32 numbers in one instruction.
+RLB_DEVICE float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+RLB_DEVICE float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+RLB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return r;
+}
+
 // VEC logits into the statistics; vm: their maximum, NaN if one is.
 template <int VEC>
 RLB_DEVICE void add_logits(RowStats& a, const float (&x)[VEC], float vm) {
   if (vm > a.m + kSlack) raise_to(a, vm);  // (rarely after the first logits: no new maximum costs a rescaling)
   const float m = a.m == -INFINITY ? 0.f : a.m;
+  if constexpr (VEC % 2 == 0) {
+    float2 s = make_float2(0.f, 0.f), t = s;
+    const float2 mm = make_float2(-m, -m), l2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const float d = x[i] - m, e = fast_exp(d);
-    a.s += e;
-    a.t = fmaf(e, fmaxf(d, -1e30f), a.t);  // -inf: e is 0 and adds nothing
+    for (int i = 0; i < VEC; i += 2) {
+      float2 d = add2(make_float2(x[i], x[i + 1]), mm);
+      const float2 y = mul2(d, l2e), e = make_float2(sm100::ex2_approx(y.x), sm100::ex2_approx(y.y));
+      d.x = fmaxf(d.x, -1e30f);  // -inf: e is 0 and adds nothing
+      d.y = fmaxf(d.y, -1e30f);
+      s = add2(s, e);
+      t = fma2(e, d, t);
+    }
+    a.s += s.x + s.y;
+    a.t += t.x + t.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float d = x[i] - m, e = fast_exp(d);
+      a.s += e;
+      a.t = fmaf(e, fmaxf(d, -1e30f), a.t);
+    }
   }
 }
 
@@ -97,7 +134,9 @@ RLB_DEVICE void store16(T* p, const float (&x)[16 / sizeof(T)]) {
   __stcs(reinterpret_cast<uint4*>(p), v);
 }
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kCtas = 1024 / kThreads;    // on an SM at a time
+constexpr int kGroup = kThreads / 64;     // threads of each of 64 groups
 constexpr int kHold = 160;                // candidates that may wait before the buffer is cut down, at most
 constexpr int kEach = 16;                 // logits of a thread in a round
 constexpr int kRound = kThreads * kEach;  // logits of a round, at most
@@ -148,11 +187,11 @@ struct TopShared {
 
 // A cluster of CTAs takes a row, each a slice (one CTA where there are rows enough to fill the GPU).  One pass: online
 // statistics per thread, and of the alternatives only those logits leave their registers that reach a bar known to
-// have k logits at or above it: at first the k-th largest of the maxima of 64 groups of 8 threads, later the k-th
-// largest candidate whenever more than 2 k + 32 of them wait (checked once a round of 8192 logits, by the barrier
+// have k logits at or above it: at first the k-th largest of the maxima of 64 groups of 4 threads, later the k-th
+// largest candidate whenever more than 2 k + 32 of them wait (checked once a round of 4096 logits, by the barrier
 // itself).  Rank 0 joins the slices over distributed shared memory.  Bound by the read of the logits.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) token_logprob_kernel(
+__global__ void __launch_bounds__(kThreads, kCtas) token_logprob_kernel(
     const T* __restrict__ logits, long long ld, int V, const long long* __restrict__ tgt, int k,
     float* __restrict__ m_out, float* __restrict__ ls_out, float* __restrict__ lp_out, float* __restrict__ ent_out,
     float* __restrict__ top_lp, long long* __restrict__ top_ids, int* status) {
@@ -215,9 +254,14 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprob_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) unpack16<T>(next[u], x + u * VEC);
     if (base + U * kThreads < v1) fetch(base + U * kThreads);
-    float vm = x[0];
+    float vec_max[U], vm;
 #pragma unroll
-    for (int i = 1; i < U * VEC; ++i) vm = max_nan(vm, x[i]);
+    for (int u = 0; u < U; ++u) {
+      vec_max[u] = x[u * VEC];
+#pragma unroll
+      for (int i = 1; i < VEC; ++i) vec_max[u] = max_nan(vec_max[u], x[u * VEC + i]);
+      vm = u == 0 ? vec_max[0] : max_nan(vm, vec_max[u]);
+    }
     add_logits<U * VEC>(st, x, vm);
     if (TOP) {
       const int j0 = head + (base + tid) * VEC;  // vector u begins u * kThreads * VEC behind
@@ -226,28 +270,27 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprob_kernel(
         const bool has = base + tid < v1;
         unsigned long long best = has ? rank_key(vm, V - 1) : 0;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) best = max64(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if ((tid & 7) == 0) top.scratch[tid >> 3] = best;
+        for (int o = 1; o < kGroup; o <<= 1) best = max64(best, __shfl_xor_sync(0xffffffffu, best, o));
+        if (tid % kGroup == 0) top.scratch[tid / kGroup] = best;
         __syncthreads();
         // the k-th largest of the 64 (absent groups: 0, so that fewer than k groups leave no bar)
-        const int at = tid >> 3;
+        const int at = tid / kGroup;
         const unsigned long long key = top.scratch[at];
         int rank = 0;
 #pragma unroll
-        for (int i = tid & 7; i < 64; i += 8) rank += top.scratch[i] > key || (top.scratch[i] == key && i < at);
+        for (int i = tid % kGroup; i < 64; i += kGroup) rank += top.scratch[i] > key || (top.scratch[i] == key && i < at);
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-        if (rank == k - 1 && (tid & 7) == 0) top.out[0] = key;
+        for (int o = 1; o < kGroup; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (rank == k - 1 && tid % kGroup == 0) top.out[0] = key;
         __syncthreads();
         set_bar(top.out[0]);
       }
-      if (!(vm < bar_x))
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
+        if (!(vec_max[u] < bar_x) && base + u * kThreads + tid < v1)
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            if (!(x[u * VEC + i] < bar_x) && base + u * kThreads + tid < v1)
-              offer(x[u * VEC + i], j0 + u * kThreads * VEC + i);
+            if (!(x[u * VEC + i] < bar_x)) offer(x[u * VEC + i], j0 + u * kThreads * VEC + i);
       if (__syncthreads_or(full)) {
         const int c = top.count;
         pick_top(top.buf, c, k, top.out, top.scratch);
@@ -345,7 +388,15 @@ __global__ void __launch_bounds__(kBwdThreads) token_logprob_bwd_kernel(
     float x[VEC];
     unpack16<T>(load16(row + w0 + v * VEC), x);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = grad(x[i]);
+    for (int i = 0; i < VEC; i += 2) {  // grad(), for two
+      float2 d = add2(add2(make_float2(x[i], x[i + 1]), make_float2(-m, -m)), make_float2(-ls, -ls));
+      d = make_float2(fmaxf(d.x, -200.f), fmaxf(d.y, -200.f));
+      const float2 y = mul2(d, make_float2(1.4426950408889634f, 1.4426950408889634f));
+      const float2 g2 = mul2(make_float2(sm100::ex2_approx(y.x), sm100::ex2_approx(y.y)),
+                             fma2(make_float2(c1, c1), d, make_float2(c0, c0)));
+      x[i] = g2.x;
+      x[i + 1] = g2.y;
+    }
     store16(out + w0 + v * VEC, x);
   }
   for (int j = j0 + threadIdx.x; j < w0; j += kBwdThreads) out[j] = from_f<T>(grad(to_f(row[j])));
@@ -380,10 +431,10 @@ template <typename T, bool TOP>
 static cudaError_t token_logprob_launch(const void* logits, long long ld, long long rows, int V, const long long* tgt,
                                         int k, float* m, float* ls, float* lp, float* ent, float* top_lp,
                                         long long* top_ids, int sms, int* status, cudaStream_t s) {
-  // Slices: as long as the CTAs fit on the GPU at a time and a slice keeps half a round of logits (a single row of 128256 in
-  // bf16 takes 8 of them; with more rows than SMs a row stays whole).
+  // Slices: as long as the CTAs fit on the GPU at a time and a slice keeps a round of logits (a single row of 128256 in
+  // bf16 takes 8 of them; from 2 rows per SM on a row stays whole).
   int slices = 1;
-  while (slices < 8 && rows * slices * 2 <= 2LL * sms && V / (slices * 2) >= kRound / 2) slices *= 2;
+  while (slices < 8 && rows * slices * 2 <= (long long)kCtas * sms && V / (slices * 2) >= kRound) slices *= 2;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = slices;
