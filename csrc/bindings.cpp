@@ -47,8 +47,8 @@ inline void check_contig(const at::Tensor& t, const char* name) {
 // Every tensor a kernel dereferences must live on the device of the tensor that picks the launch device; a
 // host tensor handed to a kernel is an illegal address on the GPU.
 inline void check_dev(const at::Tensor& t, const at::Tensor& ref, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == ref.device(), name, " must be a CUDA tensor on ", ref.device(),
-              ", got ", t.device());
+  TORCH_CHECK(t.is_cuda() && t.device() == ref.device(), name, " must be a CUDA tensor on ", ref.device().str(),
+              ", got ", t.device().str());  // (text: see check_ints)
 }
 inline void check_dev(const c10::optional<at::Tensor>& t, const at::Tensor& ref, const char* name) {
   if (t.has_value()) check_dev(*t, ref, name);
@@ -864,6 +864,7 @@ at::Tensor q4_decode(const at::Tensor& q, const at::Tensor& k_pool, const at::Te
   const int64_t Hkv = k_pool.size(1);
   TORCH_CHECK(Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16, "q: a multiple of the KV heads, at most 16 per KV head");
   TORCH_CHECK(B < 65536, "at most 65535 sequences in a call");
+  TORCH_CHECK(window < (1LL << 31), "window: fewer than 2^31 tokens");
   TORCH_CHECK(tables.dim() == 2 && tables.size(1) < (1LL << 27), "block_tables: [B, max_blocks]");
   check_ints(tables, k_pool, {B, tables.size(1)}, "block_tables");
   check_ints(lens, k_pool, {B}, "ctx_lens");
@@ -903,7 +904,7 @@ std::vector<at::Tensor> q4_evict(at::Tensor& k_pool, at::Tensor& v_pool, const a
   check_ints(lens, k_pool, {B}, "ctx_lens");
   check_ints(new_tables, k_pool, {B, new_tables.size(1)}, "new_tables");
   check_weights(weights, weight_rows, k_pool, B);
-  TORCH_CHECK(keep >= 1 && recent >= 0 && sink >= 0 && recent + sink <= keep,
+  TORCH_CHECK(keep >= 1 && keep < (1LL << 31) && recent >= 0 && sink >= 0 && recent <= keep && recent + sink <= keep,
                     "keep at least one token, and no fewer than sink + recent");
   TORCH_CHECK(new_tables.size(1) < (1LL << 27) && new_tables.size(1) * 16 >= keep,
                     "new_tables: blocks for `keep` tokens");
@@ -929,7 +930,7 @@ static int logit_type(const at::Tensor& x) {
 std::vector<at::Tensor> token_logprob(const at::Tensor& logits, const at::Tensor& targets, int64_t k, bool stats,
                                       const c10::optional<at::Tensor>& status) {
   check_cuda(logits, "logits");
-  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) < (1LL << 31) && logits.stride(1) == 1 &&
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) < (1LL << 30) && logits.stride(1) == 1 &&
                   logits.size(0) < (1LL << 31), "logits: [N, V] with unit inner stride");
   TORCH_CHECK(logit_type(logits) >= 0, "logits: fp32, bf16 or fp16");
   check_dev(targets, logits, "targets");

@@ -84,6 +84,27 @@ RLB_DEVICE bf16x8 pack8(const float* f) {
 RLB_DEVICE bf16x8 ldg8(const __nv_bfloat16* p) { return *reinterpret_cast<const bf16x8*>(p); }
 RLB_DEVICE void stg8(__nv_bfloat16* p, const bf16x8& v) { *reinterpret_cast<bf16x8*>(p) = v; }
 
+// Pairs of fp32 numbers in one instruction.
+RLB_DEVICE float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+RLB_DEVICE float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+RLB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return r;
+}
+
 RLB_DEVICE float silu(float x) { return x / (1.f + __expf(-x)); }
 
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }

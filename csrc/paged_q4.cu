@@ -81,11 +81,14 @@ RLB_DEVICE uint32_t q4_codes(const bf16x8& x, float lo, float s) {
       word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(f[e] - lo, s)), 0.f), 15.f) << (4 * e);  // NaN becomes 0
     return word;
   }
-  const float inv = __frcp_rn(s);
+  const float inv = __fdividef(1.f, s);  // (the remainder makes up for its last bit)
+  const float2 inv2 = make_float2(inv, inv), minus_s = make_float2(-s, -s), minus_lo = make_float2(-lo, -lo);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float d = f[e] - lo, q = d * inv, y = fmaf(fmaf(-q, s, d), inv, q) + 12582912.f;
-    word += __float_as_uint(y) << (4 * e);
+  for (int e = 0; e < 8; e += 2) {
+    const float2 d = add2(make_float2(f[e], f[e + 1]), minus_lo), q = mul2(d, inv2);
+    const float2 y = add2(fma2(fma2(q, minus_s, d), inv2, q), make_float2(12582912.f, 12582912.f));
+    word += __float_as_uint(y.x) << (4 * e);
+    word += __float_as_uint(y.y) << (4 * e + 4);
   }
   // y's bits are 0x4b400000 + code; no code is above 15, s being within 2^-9 of a 15th of the spread
   return word - 0x4b400000u * 0x11111111u;
@@ -119,15 +122,14 @@ __global__ void __launch_bounds__(256) q4_write_kernel(
     uint8_t* pool = i ? v_pool : k_pool;
     __nv_bfloat162 mn = __hmin2_nan(__hmin2_nan(x.h[0], x.h[1]), __hmin2_nan(x.h[2], x.h[3]));
     __nv_bfloat162 mx = __hmax2_nan(__hmax2_nan(x.h[0], x.h[1]), __hmax2_nan(x.h[2], x.h[3]));
+    // minimum and negated maximum side by side: one shuffle and one minimum a step
+    __nv_bfloat162 ends = __halves2bfloat162(__hmin_nan(mn.x, mn.y), __hneg(__hmax_nan(mx.x, mx.y)));
 #pragma unroll
-    for (int o = 1; o < L::kLanes; o <<= 1) {
-      mn = __hmin2_nan(mn, __shfl_xor_sync(mask, mn, o));
-      mx = __hmax2_nan(mx, __shfl_xor_sync(mask, mx, o));
-    }
-    const __nv_bfloat16 lo = __hmin_nan(mn.x, mn.y);
+    for (int o = 1; o < L::kLanes; o <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(mask, ends, o));
+    const __nv_bfloat16 lo = ends.x;
     const float lof = __bfloat162float(lo);
     // the range over 15, correctly rounded (a quotient and its remainder's)
-    const float range = __bfloat162float(__hmax_nan(mx.x, mx.y)) - lof, q0 = range * (1.f / 15.f);
+    const float range = -__bfloat162float(ends.y) - lof, q0 = range * (1.f / 15.f);
     const __nv_bfloat16 scale = __float2bfloat16(fmaf(fmaf(-15.f, q0, range), 1.f / 15.f, q0));
     *reinterpret_cast<uint32_t*>(pool + at) = q4_codes(x, lof, __bfloat162float(scale));
     if (lane == 0)
@@ -837,20 +839,21 @@ RLB_DEVICE float2 q4_add_parts(const float* part, const float* stats, int G, int
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
                                                         const float* __restrict__ ml, const int2* __restrict__ plan,
-                                                        __nv_bfloat16* __restrict__ out,
+                                                        int slots, __nv_bfloat16* __restrict__ out,
                                                         const float* __restrict__ scores, int Gs,
                                                         float* __restrict__ weights,
                                                         const int* __restrict__ weight_rows, long long w_rows,
                                                         int w_len, int* status) {
   constexpr int E = D / 32;
   __shared__ float2 stat[16];
-  __shared__ float sums[WIDE ? 8 : 1][D];
   cudaGridDependencySynchronize();  // (every CTA: what follows this kernel must not overtake the one before)
   const int h = blockIdx.x, b = blockIdx.y, z = blockIdx.z, G = c.G, joins = WIDE ? G : (G + 7) / 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = (long long)b * c.Hkv + h;
   const int len = q4_len(c, b, nullptr);
   const int2 at = len > 0 ? plan[row] : make_int2(0, 0);  // first slot, parts
+  // (a decode kernel that gave up on a copy, and reported it, has left rows without a plan)
+  if (at.x < 0 || at.y < (len > 0) || at.x >= slots || at.y > slots - at.x) return;
   const float* stats = ml + (long long)at.x * G * 2;
   if (z < joins) {
     const int head = WIDE ? z : z * 8 + warp;
@@ -859,29 +862,30 @@ __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* 
     float acc[E] = {};
     const float* from = part + ((long long)at.x * G + head) * D;
     float2 s = q4_add_parts<D>(from, stats + 2 * head, G, WIDE ? warp : 0, WIDE ? 8 : 1, at.y, acc);
-    if (!WIDE) {
+    if constexpr (!WIDE) {
       const float inv = s.y != 0.f ? 1.f / s.y : 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) dst[lane + 32 * e] = __float2bfloat16(acc[e] * inv);
-      return;
-    }
+    } else {
+      __shared__ float sums[8][D];
 #pragma unroll
-    for (int e = 0; e < E; ++e) sums[warp][lane + 32 * e] = acc[e];
-    if (lane == 0) stat[warp] = s;
-    __syncthreads();
-    float most = -INFINITY, total = 0.f, f[8];
+      for (int e = 0; e < E; ++e) sums[warp][lane + 32 * e] = acc[e];
+      if (lane == 0) stat[warp] = s;
+      __syncthreads();
+      float most = -INFINITY, total = 0.f, f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = fmaxf(most, stat[i].x);
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, stat[i].x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = stat[i].x == -INFINITY ? 1.f : sm100::ex2_approx(stat[i].x - most);
-      total += stat[i].y * f[i];
-    }
-    for (int d = threadIdx.x; d < D; d += 256) {
-      float a = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        f[i] = stat[i].x == -INFINITY ? 1.f : sm100::ex2_approx(stat[i].x - most);
+        total += stat[i].y * f[i];
+      }
+      for (int d = threadIdx.x; d < D; d += 256) {
+        float a = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a += sums[i][d] * f[i];
-      dst[d] = __float2bfloat16(total != 0.f ? a / total : 0.f);
+        for (int i = 0; i < 8; ++i) a += sums[i][d] * f[i];
+        dst[d] = __float2bfloat16(total != 0.f ? a / total : 0.f);
+      }
     }
     return;
   }
@@ -1250,7 +1254,8 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
   if (B == 0) return cudaSuccess;
   // the kernel counts turns and blocks of all heads in 32 bits
   if ((long long)B * Hkv * ((max_blocks + q4_turn_of(D) - 1) / q4_turn_of(D)) >= (1LL << 31) - (1 << 20) ||
-      (long long)num_blocks * Hkv >= 1LL << 31)
+      (long long)num_blocks * Hkv >= 1LL << 31 ||
+      (long long)ctas * kDecodeWarps + (long long)B * Hkv >= 1LL << 31)
     return cudaErrorInvalidValue;
   const Q4Cache c{(const uint8_t*)k_pool, (const uint8_t*)v_pool, tables, lens, Hkv, G, max_blocks, num_blocks,
                   window, q4_turn_of(D), scale, softcap};
@@ -1284,7 +1289,7 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  RLB_Q4_D(e = cudaLaunchKernelEx(&cfg, wide ? q4_finish_kernel<DD, true> : q4_finish_kernel<DD, false>, c, (const float*)part, (const float*)ml, (const int2*)plan,
+  RLB_Q4_D(e = cudaLaunchKernelEx(&cfg, wide ? q4_finish_kernel<DD, true> : q4_finish_kernel<DD, false>, c, (const float*)part, (const float*)ml, (const int2*)plan, (int)slots,
                                   (__nv_bfloat16*)out, (const float*)scores, Gs, weights, weight_rows, w_rows, w_len,
                                   status));
   return e;

@@ -65,27 +65,6 @@ RLB_DEVICE RowStats warp_stats(RowStats a) {
   return RowStats{m, warp_sum(a.s), warp_sum(a.t)};
 }
 
-// Pairs of fp32 numbers in one instruction.
-RLB_DEVICE float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-  return r;
-}
-RLB_DEVICE float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-  return r;
-}
-RLB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(r))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
-        "l"(reinterpret_cast<unsigned long long&>(c)));
-  return r;
-}
-
 // VEC logits into the statistics; vm: their maximum, NaN if one is.
 template <int VEC>
 RLB_DEVICE void add_logits(RowStats& a, const float (&x)[VEC], float vm) {

@@ -46,6 +46,11 @@ class _HFSpec:
                 "hidden_size": getattr(c, "hidden_size", None), "num_hidden_layers": getattr(c, "num_hidden_layers", None)}
 
 
+def _scorable(logits: torch.Tensor) -> torch.Tensor:
+    """Logits in a type that ``token_logprobs`` takes (double ones in fp32)."""
+    return logits.float() if logits.dtype == torch.float64 else logits
+
+
 class HFPolicy(nn.Module):
     backend = "huggingface"
 
@@ -148,7 +153,7 @@ class HFPolicy(nn.Module):
 
     def token_logprobs(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         """Per-position ``log p(targets | input_ids)`` ``[B, T]``; 0 where ``targets == -1``."""
-        logits = self.token_logits(input_ids)
+        logits = _scorable(self.token_logits(input_ids))
         return token_logprobs(logits, targets.to(logits.device)).logprobs
 
     def token_ce(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
@@ -160,7 +165,7 @@ class HFPolicy(nn.Module):
     def logprobs_with_entropy(self, prompt_ids, response_ids):
         """Response-token log-probs and the policy's entropy at each response position."""
         full, out = self._forward(prompt_ids, response_ids)
-        r = token_logprobs(out.logits[:, prompt_ids.shape[1] - 1:-1], full[:, prompt_ids.shape[1]:])
+        r = token_logprobs(_scorable(out.logits[:, prompt_ids.shape[1] - 1:-1]), full[:, prompt_ids.shape[1]:])
         return r.logprobs, r.entropy
 
     def with_frozen_reference(self) -> "HFPolicy":

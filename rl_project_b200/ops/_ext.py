@@ -24,7 +24,7 @@ except BaseException as exc:  # noqa: BLE001
 
 
 # kernels launched by each binding (launch accounting for benchmarks)
-_LAUNCHES = {"rmsnorm_bwd": 2, "q4_evict": 2, "grad_norm": 2, "adam_chunk_size": 0, "adam_tensor_desc_bytes": 0, "bounds_status": 0}
+_LAUNCHES = {"rmsnorm_bwd": 2, "q4_evict": 2, "q4_decode": 2, "grad_norm": 2, "adam_chunk_size": 0, "adam_tensor_desc_bytes": 0, "bounds_status": 0}
 
 
 class _Counted:

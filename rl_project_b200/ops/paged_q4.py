@@ -126,6 +126,8 @@ def paged_decode_q4(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         p = s.softmax(-1)
         out[b] = torch.einsum("hgt,htd->hgd", p, v).reshape(Hq, D)
         if weights is not None and int(weight_rows[b]) >= 0:
+            _inside(int(weight_rows[b]), weights.shape[0], "weight_rows")
+            _inside(n - 1, weights.shape[2], "a context's last token")
             weights[int(weight_rows[b]), :, :n] += p.sum(1)
     return out.to(q.dtype)
 
@@ -140,7 +142,7 @@ def paged_evict_q4(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: tor
     accumulated ``weights`` (``paged_decode_q4``), the earliest among equals (NaN ranks lowest).  Kept tokens stay in
     order: their rows are copied to the blocks of ``new_tables [B, blocks]``, which must not be among the sequences'
     own blocks (those stay as they are, so they may be shared with other sequences), and their weights move to the
-    front of their row, the rest of the old length becoming zero.  A sequence of at most ``keep`` tokens is copied
+    front of their row (one to a sequence), the rest of the old length becoming zero.  A sequence of at most ``keep`` tokens is copied
     whole.  Returns ``(kept [B, Hkv, keep], new_lens [B])``, int32: the old positions (-1 behind the last) and lengths.
     """
     if k_pool.is_cuda:

@@ -98,7 +98,8 @@ def packed_response_logprobs(policy, trajectories, width: int, with_entropy: boo
     else:  # other backends: from full logits
         from rl_project_b200.ops.logprob import token_logprobs
 
-        lp, ent = token_logprobs(policy.token_logits(inputs), targets)[:2]
+        logits = policy.token_logits(inputs)
+        lp, ent = token_logprobs(logits.float() if logits.dtype == torch.float64 else logits, targets)[:2]
     starts = torch.tensor([len(p) - 1 for p, _ in pairs], device=dev)
     cols = (starts[:, None] + torch.arange(width, device=dev)[None, :]).clamp(max=lp.shape[1] - 1)
     return lp.float().gather(1, cols), (ent.float().gather(1, cols) if ent is not None else None)

@@ -288,6 +288,9 @@ def test_decode_bad_index(dev):
             o, _, a = attention(q[0], ks[0][left], vs[0][left], 0.125, 0.0, 0)
             check_decode(out[0], o, a)
     index_error(dev, lambda: paged_decode_q4(q, *pools, tables, n + 30, 0.125))
+    short = torch.zeros(2, 1, 39, device=dev)  # (tokens that have a place are accumulated all the same)
+    index_error(dev, lambda: paged_decode_q4(q, *pools, tables, n, 0.125, 0.0, 0, short,
+                                             torch.tensor([0, 1], dtype=torch.int32, device=dev)))
     w = torch.zeros(2, 1, 48, device=dev)
     index_error(dev, lambda: paged_decode_q4(q, *pools, tables, n, 0.125, 0.0, 0, w,
                                              torch.tensor([0, 2], dtype=torch.int32, device=dev)))
@@ -362,6 +365,24 @@ def test_evict(dev, lens, Hkv, D, keep, sink, recent, kind):
         assert torch.equal(p[rest], q.cpu()[rest])
 
 
+def test_empty_calls(dev):
+    """No rows, no sequences, tables without blocks, and a batch of nothing but padding."""
+    D = 64
+    pools = [torch.zeros(2, 2, q4_block_bytes(D), dtype=torch.uint8, device=dev) for _ in range(2)]
+    i0, t0 = (torch.zeros(*s, dtype=torch.int32, device=dev) for s in ((0,), (0, 3)))
+    assert paged_decode_q4(torch.zeros(0, 4, D, dtype=BF, device=dev), *pools, t0, i0, 1.0).shape == (0, 4, D)
+    kept, lens = paged_evict_q4(*pools, t0, i0, t0, torch.zeros(1, 2, 48, device=dev), i0, 8, D)
+    assert kept.shape == (0, 2, 8) and lens.shape == (0,)
+    assert paged_gather_q4(*pools, t0, i0, D, 5)[0].shape == (0, 5, 2, D)
+    n, none = torch.zeros(3, dtype=torch.int32, device=dev), torch.zeros(3, 0, dtype=torch.int32, device=dev)
+    out = paged_decode_q4(torch.ones(3, 4, D, dtype=BF, device=dev), *pools, none, n, 1.0)
+    assert not out.any()
+    assert paged_gather_q4(*pools, none, n, D, 0)[0].shape == (3, 0, 2, D)
+    w = torch.ones(3, 2, 16, device=dev)
+    kept, lens = paged_evict_q4(*pools, none, n, torch.zeros(3, 1, dtype=torch.int32, device=dev), w, n - 1, 4, D)
+    assert (kept == -1).all() and not lens.any() and (w == 1).all()
+
+
 def test_evict_shared_source(dev):
     """Two sequences over the same blocks (a shared prompt) are cut by their own weights."""
     ks, vs, pools, tables, n, ids = cache([80], 1, 64, dev, extra=4)
@@ -416,6 +437,19 @@ def test_refusals(dev):
         lambda: paged_evict_q4(*pools, t, n, t[:2], w, i3, 16, D),
     ):
         with pytest.raises(ValueError if dev == "cpu" else (ValueError, RuntimeError)):
+            call()
+
+
+@pytest.mark.gpu
+def test_refuses_other_devices():
+    D = 64
+    pools = [torch.zeros(4, 2, q4_block_bytes(D), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    t, n = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(3, 4, D, dtype=BF, device="cuda")
+    for call in (lambda: paged_decode_q4(q, *pools, t, n.cpu(), 1.0), lambda: paged_decode_q4(q.cpu(), *pools, t, n, 1.0),
+                 lambda: paged_decode_q4(q, pools[0], pools[1].cpu(), t, n, 1.0),
+                 lambda: paged_decode_q4(q, *pools, t, n, 1.0, window=1 << 32)):
+        with pytest.raises(RuntimeError):
             call()
 
 
