@@ -23,7 +23,8 @@ struct Q4 {
   static constexpr int kRow = kGroup / 2;                     // code bytes of one token in one group
   static constexpr int kCodes = kTok * D / 2;                 // code bytes of a block
   static constexpr int kBytes = kCodes + kTok * kGroups * 4;  // bytes of a block
-  static constexpr int kLanes = kGroup / 8;                   // threads that share a group, 8 elements each
+  static constexpr int kLanes = kGroup / 16;                  // threads that share a group, 16 elements each
+  static constexpr int kRows = 4096 / D;                      // rows of 256 threads with 16 elements each
 };
 
 RLB_DEVICE float bf16_lo_f(uint32_t v) { return __uint_as_float(v << 16); }
@@ -66,8 +67,8 @@ RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
 }
 
 // ---------------------------------------------------------------- storing rows
-// A group's threads reduce its minimum and maximum by shuffles (NaN-propagating), then each quantises its 8
-// elements to one 32-bit word.  Bound by memory: 2 bytes read and about 0.56 written per element.
+// A group's four threads (two at D 32) reduce its minimum and maximum by shuffles (NaN-propagating), then each
+// quantises its 16 elements to two 32-bit words.  STORE_NOTE
 //
 // code = clamp(rint((x - lo) / s)) without a division per element: q = (x - lo) (1 / s) and its remainder's share
 // q + (x - lo - q s) (1 / s) is the correctly rounded quotient, and adding 1.5 2^23 rounds that to a whole number.
@@ -94,110 +95,122 @@ RLB_DEVICE uint32_t q4_codes(const bf16x8& x, float lo, float s) {
   return word - 0x4b400000u * 0x11111111u;
 }
 
-// A block of threads takes one KV head of 2048 / D rows, keys and values alike; blocks of a row's heads are neighbours.
+RLB_DEVICE __nv_bfloat162 min8(const bf16x8& a, const bf16x8& b) {
+  return __hmin2_nan(__hmin2_nan(__hmin2_nan(a.h[0], a.h[1]), __hmin2_nan(a.h[2], a.h[3])),
+                     __hmin2_nan(__hmin2_nan(b.h[0], b.h[1]), __hmin2_nan(b.h[2], b.h[3])));
+}
+RLB_DEVICE __nv_bfloat162 max8(const bf16x8& a, const bf16x8& b) {
+  return __hmax2_nan(__hmax2_nan(__hmax2_nan(a.h[0], a.h[1]), __hmax2_nan(a.h[2], a.h[3])),
+                     __hmax2_nan(__hmax2_nan(b.h[0], b.h[1]), __hmax2_nan(b.h[2], b.h[3])));
+}
+
+// Blocks of threads take 4096 / D rows of one KV head, keys and values alike; the heads (x) of the same rows (y) are
+// neighbours in the grid, as they are in memory.
 template <int D>
 __global__ void __launch_bounds__(256) q4_write_kernel(
     const __nv_bfloat16* __restrict__ k_new, const __nv_bfloat16* __restrict__ v_new, long long k_sn, long long k_sh,
     long long v_sn, long long v_sh, uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool,
-    const int* __restrict__ slot_block, const int* __restrict__ slot_off, long long N, int Hkv, int num_blocks,
-    int* status) {
+    const int* __restrict__ slot_block, const int* __restrict__ slot_off, long long N, int num_blocks, int* status) {
   using L = Q4<D>;
-  const int h = blockIdx.x % Hkv;
-  const long long n = (long long)(blockIdx.x / Hkv) * (2048 / D) + threadIdx.x / (D / 8);
-  const int grp = threadIdx.x % (D / 8) / L::kLanes, lane = threadIdx.x % L::kLanes;
-  if (n >= N) return;  // whole groups leave together: kLanes divides the block
-  const bf16x8 k = ldg8(k_new + n * k_sn + h * k_sh + threadIdx.x % (D / 8) * 8);
-  const bf16x8 v = ldg8(v_new + n * v_sn + h * v_sh + threadIdx.x % (D / 8) * 8);
-  const int blk = slot_block[n], off = slot_off[n];
-  if (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok) {
-    if (lane == 0) report(status, kBadIndex);
-    return;
-  }
+  const int h = blockIdx.x, Hkv = gridDim.x, part = threadIdx.x % (D / 16);
+  const int grp = part / L::kLanes, lane = part % L::kLanes;
   const unsigned mask = ((1u << L::kLanes) - 1) << (threadIdx.x & 31 & ~(L::kLanes - 1));
-  const long long at = ((long long)blk * Hkv + h) * L::kBytes + (grp * kTok + off) * L::kRow + lane * 4;
-  const long long meta = ((long long)blk * Hkv + h) * L::kBytes + L::kCodes + (grp * kTok + off) * 4;
+  for (long long n = (long long)blockIdx.y * L::kRows + threadIdx.x / (D / 16); n < N; n += (long long)gridDim.y * L::kRows) {
+    const __nv_bfloat16* kp = k_new + n * k_sn + h * k_sh + part * 16;
+    const __nv_bfloat16* vp = v_new + n * v_sn + h * v_sh + part * 16;
+    const bf16x8 x[2][2] = {{ldg8(kp), ldg8(kp + 8)}, {ldg8(vp), ldg8(vp + 8)}};
+    const int blk = slot_block[n], off = slot_off[n];
+    if (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok) {  // (whole groups: they share a row)
+      if (lane == 0) report(status, kBadIndex);
+      continue;
+    }
+    const long long at = ((long long)blk * Hkv + h) * L::kBytes;
+    const int code = (grp * kTok + off) * L::kRow + lane * 8, meta = L::kCodes + (grp * kTok + off) * 4;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const bf16x8& x = i ? v : k;
-    uint8_t* pool = i ? v_pool : k_pool;
-    __nv_bfloat162 mn = __hmin2_nan(__hmin2_nan(x.h[0], x.h[1]), __hmin2_nan(x.h[2], x.h[3]));
-    __nv_bfloat162 mx = __hmax2_nan(__hmax2_nan(x.h[0], x.h[1]), __hmax2_nan(x.h[2], x.h[3]));
-    // minimum and negated maximum side by side: one shuffle and one minimum a step
-    __nv_bfloat162 ends = __halves2bfloat162(__hmin_nan(mn.x, mn.y), __hneg(__hmax_nan(mx.x, mx.y)));
+    for (int i = 0; i < 2; ++i) {
+      uint8_t* pool = (i ? v_pool : k_pool) + at;
+      const __nv_bfloat162 mn = min8(x[i][0], x[i][1]), mx = max8(x[i][0], x[i][1]);
+      // minimum and negated maximum side by side: one shuffle and one minimum a step
+      __nv_bfloat162 ends = __halves2bfloat162(__hmin_nan(mn.x, mn.y), __hneg(__hmax_nan(mx.x, mx.y)));
 #pragma unroll
-    for (int o = 1; o < L::kLanes; o <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(mask, ends, o));
-    const __nv_bfloat16 lo = ends.x;
-    const float lof = __bfloat162float(lo);
-    // the range over 15, correctly rounded (a quotient and its remainder's)
-    const float range = -__bfloat162float(ends.y) - lof, q0 = range * (1.f / 15.f);
-    const __nv_bfloat16 scale = __float2bfloat16(fmaf(fmaf(-15.f, q0, range), 1.f / 15.f, q0));
-    *reinterpret_cast<uint32_t*>(pool + at) = q4_codes(x, lof, __bfloat162float(scale));
-    if (lane == 0)
-      *reinterpret_cast<uint32_t*>(pool + meta) =
-          (uint32_t)__bfloat16_as_ushort(scale) | ((uint32_t)__bfloat16_as_ushort(lo) << 16);
+      for (int o = 1; o < L::kLanes; o <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(mask, ends, o));
+      const __nv_bfloat16 lo = ends.x;
+      const float lof = __bfloat162float(lo);
+      // the range over 15, correctly rounded (a quotient and its remainder's)
+      const float range = -__bfloat162float(ends.y) - lof, q0 = range * (1.f / 15.f);
+      const __nv_bfloat16 scale = __float2bfloat16(fmaf(fmaf(-15.f, q0, range), 1.f / 15.f, q0));
+      const float sf = __bfloat162float(scale);
+      *reinterpret_cast<uint2*>(pool + code) = make_uint2(q4_codes(x[i][0], lof, sf), q4_codes(x[i][1], lof, sf));
+      if (lane == 0)
+        *reinterpret_cast<uint32_t*>(pool + meta) =
+            (uint32_t)__bfloat16_as_ushort(scale) | ((uint32_t)__bfloat16_as_ushort(lo) << 16);
+    }
   }
 }
 
 // ---------------------------------------------------------------- reading rows
-RLB_DEVICE bf16x8 q4_elements(uint32_t word, uint32_t meta) {
-  const float s = bf16_lo_f(meta), lo = bf16_hi_f(meta);
+// The 8 elements of a word: codes become fp16 numbers by their bits.
+RLB_DEVICE bf16x8 q4_elements(uint32_t word, float s, float lo) {
   uint32_t two[4];
   codes_f16<true, 0>(word, two, 0x64006400u);
   float f[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&two[j]));
-    f[j] = fmaf(n.x, s, lo);
-    f[j + 4] = fmaf(n.y, s, lo);
+  for (int j = 0; j < 4; ++j) {  // elements j and j + 4
+    const float2 n = fma2(__half22float2(*reinterpret_cast<const __half2*>(&two[j])), make_float2(s, s), make_float2(lo, lo));
+    f[j] = n.x;
+    f[j + 4] = n.y;
   }
   return pack8(f);
 }
 
-// One thread per 8 elements of a key and of a value, blocks as above.  Row n is slot (slot_block[n], slot_off[n]), or,
-// with a block table, position n % max_len of sequence n / max_len.  Rows without a place in the pool read as zeros.
+// One thread per 8 elements of a key and of a value (16 of each would write every sector in two halves: 119 us where
+// this takes 39 for 32768 rows of 8 x 128).  Row n is slot (slot_block[n], slot_off[n]), or, with a block table, position
+// n % max_len of sequence n / max_len.  Rows without a place in the pool read as zeros.  Bound by the write of the rows.
 template <int D>
 __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict__ k_pool,
                                                       const uint8_t* __restrict__ v_pool,
                                                       const int* __restrict__ slot_block,
                                                       const int* __restrict__ slot_off, const int* __restrict__ tables,
                                                       const int* __restrict__ lens, int max_blocks, int max_len,
-                                                      long long N, int Hkv, int num_blocks,
+                                                      long long N, int num_blocks,
                                                       __nv_bfloat16* __restrict__ k_out,
                                                       __nv_bfloat16* __restrict__ v_out, int* status) {
   using L = Q4<D>;
-  const int h = blockIdx.x % Hkv, d8 = threadIdx.x % (D / 8);
-  const long long n = (long long)(blockIdx.x / Hkv) * (2048 / D) + threadIdx.x / (D / 8);
-  if (n >= N) return;
-  int blk = -1, off = 0;
-  bool absent = false;
-  if (tables == nullptr) {
-    blk = slot_block[n];
-    off = slot_off[n];
-  } else {
-    const long long b = n >> 31 == 0 ? (long long)((unsigned)n / (unsigned)max_len) : n / max_len;
-    const int pos = (int)(n - b * max_len);
-    off = pos % kTok;
-    absent = pos >= lens[b];
-    if (!absent && pos / kTok < max_blocks) blk = tables[b * max_blocks + pos / kTok];
-  }
-  bf16x8 k, v;
-  *reinterpret_cast<uint4*>(&k) = *reinterpret_cast<uint4*>(&v) = make_uint4(0, 0, 0, 0);
-  if (!absent) {
-    if (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok) {
-      if (d8 == 0 && h == 0) report(status, kBadIndex);
+  constexpr int ROWS = L::kRows / 2;
+  const int h = blockIdx.x, Hkv = gridDim.x, part = threadIdx.x % (D / 8);
+  const int grp = part * 8 / L::kGroup, lane = part % (L::kGroup / 8);
+  for (long long n = (long long)blockIdx.y * ROWS + threadIdx.x / (D / 8); n < N; n += (long long)gridDim.y * ROWS) {
+    int blk = -1, off = 0;
+    bool absent = false;
+    if (tables == nullptr) {
+      blk = slot_block[n];
+      off = slot_off[n];
     } else {
-      const int grp = d8 / L::kLanes, lane = d8 % L::kLanes;
-      const long long at = ((long long)blk * Hkv + h) * L::kBytes, code = at + (grp * kTok + off) * L::kRow + lane * 4;
-      const long long meta = at + L::kCodes + (grp * kTok + off) * 4;
-      const uint32_t kw = *reinterpret_cast<const uint32_t*>(k_pool + code), km = *reinterpret_cast<const uint32_t*>(k_pool + meta);
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(v_pool + code), vm = *reinterpret_cast<const uint32_t*>(v_pool + meta);
-      k = q4_elements(kw, km);
-      v = q4_elements(vw, vm);
+      const long long b = n >> 31 == 0 ? (long long)((unsigned)n / (unsigned)max_len) : n / max_len;
+      const int pos = (int)(n - b * max_len);
+      off = pos % kTok;
+      absent = pos >= lens[b];
+      if (!absent && pos / kTok < max_blocks) blk = tables[b * max_blocks + pos / kTok];
     }
+    bf16x8 k, v;
+    if (!absent && (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok)) {
+      if (part == 0 && h == 0) report(status, kBadIndex);
+      absent = true;
+    }
+    if (absent) {
+      *reinterpret_cast<uint4*>(&k) = *reinterpret_cast<uint4*>(&v) = make_uint4(0, 0, 0, 0);
+    } else {
+      const long long at = ((long long)blk * Hkv + h) * L::kBytes;
+      const int code = (grp * kTok + off) * L::kRow + lane * 4, meta = L::kCodes + (grp * kTok + off) * 4;
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(k_pool + at + code), km = *reinterpret_cast<const uint32_t*>(k_pool + at + meta);
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(v_pool + at + code), vm = *reinterpret_cast<const uint32_t*>(v_pool + at + meta);
+      k = q4_elements(kw, bf16_lo_f(km), bf16_hi_f(km));
+      v = q4_elements(vw, bf16_lo_f(vm), bf16_hi_f(vm));
+    }
+    const long long to = (n * Hkv + h) * D + part * 8;
+    stg8(k_out + to, k);
+    stg8(v_out + to, v);
   }
-  const long long to = (n * Hkv + h) * D + d8 * 8;
-  stg8(k_out + to, k);
-  stg8(v_out + to, v);
 }
 
 // ---------------------------------------------------------------- decode attention
@@ -1207,11 +1220,11 @@ cudaError_t rlb_q4_write(const void* k_new, const void* v_new, long long k_sn, l
                          long long v_sh, void* k_pool, void* v_pool, const int* slot_block, const int* slot_off,
                          long long N, int Hkv, int D, int num_blocks, int* status, cudaStream_t s) {
   if (N == 0) return cudaSuccess;
-  const long long grid = (N + 2048 / D - 1) / (2048 / D) * Hkv;
-  if (grid > (1LL << 31) - 1) return cudaErrorInvalidValue;
-  RLB_Q4_D((q4_write_kernel<DD><<<(unsigned)grid, 256, 0, s>>>(
+  const long long chunks = (N + 4096 / D - 1) / (4096 / D);
+  const dim3 grid(Hkv, (unsigned)(chunks < 65535 ? chunks : 65535));
+  RLB_Q4_D((q4_write_kernel<DD><<<grid, 256, 0, s>>>(
       (const __nv_bfloat16*)k_new, (const __nv_bfloat16*)v_new, k_sn, k_sh, v_sn, v_sh, (uint8_t*)k_pool,
-      (uint8_t*)v_pool, slot_block, slot_off, N, Hkv, num_blocks, status)));
+      (uint8_t*)v_pool, slot_block, slot_off, N, num_blocks, status)));
   return cudaGetLastError();
 }
 
@@ -1219,10 +1232,10 @@ cudaError_t rlb_q4_read(const void* k_pool, const void* v_pool, const int* slot_
                         const int* tables, const int* lens, int max_blocks, int max_len, long long N, int Hkv, int D,
                         int num_blocks, void* k_out, void* v_out, int* status, cudaStream_t s) {
   if (N == 0) return cudaSuccess;
-  const long long grid = (N + 2048 / D - 1) / (2048 / D) * Hkv;
-  if (grid > (1LL << 31) - 1) return cudaErrorInvalidValue;
-  RLB_Q4_D((q4_read_kernel<DD><<<(unsigned)grid, 256, 0, s>>>((const uint8_t*)k_pool, (const uint8_t*)v_pool, slot_block,
-                                                    slot_off, tables, lens, max_blocks, max_len, N, Hkv, num_blocks,
+  const long long chunks = (N + 2048 / D - 1) / (2048 / D);
+  const dim3 grid(Hkv, (unsigned)(chunks < 65535 ? chunks : 65535));
+  RLB_Q4_D((q4_read_kernel<DD><<<grid, 256, 0, s>>>((const uint8_t*)k_pool, (const uint8_t*)v_pool, slot_block,
+                                                    slot_off, tables, lens, max_blocks, max_len, N, num_blocks,
                                                     (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, status)));
   return cudaGetLastError();
 }
