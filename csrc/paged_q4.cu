@@ -7,6 +7,7 @@
 //   minimum = min x,  scale = bf16((max x - min x) / 15),  code = clamp(rint((x - minimum) / scale), 0, 15)
 // over the group: the inputs are bf16, so the minimum is exact, and the codes are chosen against the rounded scale.
 // Group-major codes keep the 16 tokens x 64 dimensions that a matrix instruction works on contiguous (512 bytes).
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -68,7 +69,9 @@ RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
 
 // ---------------------------------------------------------------- storing rows
 // A group's four threads (two at D 32) reduce its minimum and maximum by shuffles (NaN-propagating), then each
-// quantises its 16 elements to two 32-bit words.  STORE_NOTE
+// quantises its 16 elements to two 32-bit words.  Bound by memory latency and pattern (rows of 256 bytes in, 32-byte
+// pieces of a block out): 32768 rows of 8 heads x 128 in 48 us, 3.6 TB/s; 8 elements a thread took 4 us more, and 40
+// registers for half as many warps again 59.
 //
 // code = clamp(rint((x - lo) / s)) without a division per element: q = (x - lo) (1 / s) and its remainder's share
 // q + (x - lo - q s) (1 / s) is the correctly rounded quotient, and adding 1.5 2^23 rounds that to a whole number.
@@ -931,8 +934,8 @@ RLB_DEVICE uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Choosing what stays has two forms.  This one, a CTA per (KV head, sequence), takes sequences whose weights do not fit
-// into a CTA's registers.  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
+// Choosing what stays has three forms.  This one, a CTA per (KV head, sequence), takes sequences whose weights do not fit
+// into the registers of a cluster.  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
 // a histogram in shared memory, whose bins a scan then walks from the top).  Each warp then takes a stretch of the
 // tokens: it counts the tokens above that weight and those equal to it, a scan over the warps gives it its place, and
 // it writes its kept positions in order.  The weights move to the front last, tile by tile: a token never moves to a
@@ -1058,11 +1061,11 @@ __global__ void __launch_bounds__(kSelect) q4_select_kernel(const int* __restric
   for (int t = keep + tid; t < n; t += kSelect) w[t] = 0.f;
 }
 
-// The same with K keys a thread in registers: the weights are read once.  A bar that exactly
-// `keep` keys reach is searched by halving the interval of keys and counting: 10 to 20 times K compares and a barrier
-// (32 where many weights are equal), where histograms pay for colliding atomics, weights crowding in few exponents.  Warp w holds tokens [32 K w, 32 K (w + 1)), 32 neighbours at a
-// time.  (A cluster of 8 CTAs a row, exchanging its counts over distributed shared memory, took 35 us for 8 rows of 40000
-// tokens where one CTA takes 40: the barriers of the cluster eat what the additional SMs bring.)
+// The same with K keys a thread in registers: the weights are read once.  A bar that exactly `keep` keys reach is
+// searched by halving the interval of keys and counting: 10 to 20 times K compares and a barrier (32 where many weights
+// are equal), where histograms pay for colliding atomics, weights crowding in few exponents.  Warp w holds tokens
+// [32 K w, 32 K (w + 1)), 32 neighbours at a time.  Bound by the chain of barriers (K 4: 128 rows of 4096 tokens in
+// 10 us) and by the compares (K 40: 8 rows of 40000 in 41 us, up to 148 such rows in no more).
 template <int K>
 __global__ void __launch_bounds__(kSelect) q4_select_regs_kernel(const int* __restrict__ lens, float* __restrict__ weights,
                                                                  const int* __restrict__ weight_rows,
@@ -1149,7 +1152,7 @@ __global__ void __launch_bounds__(kSelect) q4_select_regs_kernel(const int* __re
   unsigned in[(K + 31) / 32] = {};
 #pragma unroll
   for (int i = 0; i < K; ++i) {
-    if (key[i] >= bar) in[i / 32] |= 1u << (i % 32);
+    in[i / 32] |= (unsigned)(key[i] >= bar) << (i % 32);
     x[i] = key[i] >= bar ? w[t0 + 32 * i] : 0.f;
   }
   __syncthreads();  // every weight has been read
@@ -1166,6 +1169,143 @@ __global__ void __launch_bounds__(kSelect) q4_select_regs_kernel(const int* __re
     done += __popc(all);
   }
   for (int t = keep + tid; t < n; t += kSelect) w[t] = 0.f;
+}
+
+// For few long sequences a cluster of 8 CTAs per (KV head, sequence), 16 keys a thread: there one CTA's loads and
+// compares leave most SMs idle.  A barrier of the cluster costs above 1 us, so the bar is found in three turns (two where
+// the second leaves no bin in part): each CTA counts its keys' digits (11, 11 and 10 bits) in a histogram of its own, and
+// every CTA adds the eight up over distributed shared memory.  8 rows of 40000 tokens take 18 us (41 by one CTA each,
+// 35 by clusters that halve the interval), 13 us more for each further 18 rows, as one cluster fills 8 SMs.
+constexpr int kCtas = 8;
+__global__ void __launch_bounds__(kSelect) q4_select_cluster_kernel(const int* __restrict__ lens,
+                                                                    float* __restrict__ weights,
+                                                                    const int* __restrict__ weight_rows,
+                                                                    int* __restrict__ kept, int* __restrict__ new_lens,
+                                                                    int Hkv, long long w_rows, int w_len, int keep,
+                                                                    int recent, int sink, int* status) {
+  constexpr int K = 16, threads = kCtas * kSelect;
+  __shared__ __align__(8) int hist[3][2048];
+  __shared__ int part[32], place[32], pick[2], sums[2];
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int h = blockIdx.x / kCtas, rank = blockIdx.x % kCtas, b = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = rank * kSelect + tid;
+  int n = lens[b];
+  const int r = weight_rows[b];
+  if (n > min(w_len, K * threads) || (n > 0 && (r < 0 || r >= w_rows))) {
+    if (me == 0) report(status, kBadIndex);
+    n = 0;
+  }
+  n = max(n, 0);
+  int* out = kept + ((long long)b * Hkv + h) * keep;
+  if (h == 0 && me == 0) new_lens[b] = min(n, keep);
+  if (n <= keep) {
+    for (int j = me; j < keep; j += threads) out[j] = j < n ? j : -1;
+    return;  // (the whole cluster)
+  }
+  float* w = weights + ((long long)r * Hkv + h) * w_len;
+  const int used = (n + threads - 1) / threads;  // keys that a thread holds
+  const int t0 = (rank * 32 + warp) * 32 * used + lane;
+  float x[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) x[i] = i < used && t0 + 32 * i < n ? w[t0 + 32 * i] : 0.f;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) (&hist[0][0])[tid + i * kSelect] = 0;
+  auto key_of = [&](int i) {  // above all for protected tokens, 0 for absent ones (a NaN's is 1)
+    const int t = t0 + 32 * i;
+    return i >= used || t >= n ? 0u : t < sink || t >= n - recent ? 0xffffffffu : max(weight_key(x[i]), 1u);
+  };
+  __syncthreads();
+  // Of the keys that agree with `bar` in the bits `known` (none at first), `need` are kept, and all above them.
+  uint32_t bar = 0, known = 0;
+  int need = keep;
+  bool whole = false;
+  for (int step = 0; step < 3 && !whole; ++step) {
+    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bins = step == 2 ? 1024 : 2048;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      if (i >= used) break;
+      const uint32_t key = key_of(i);
+      if (key != 0 && (key & known) == bar) atomicAdd(&hist[step][(key >> shift) & (bins - 1)], 1);
+    }
+    cluster.sync();
+    // this thread's two bins, counted from the top; how many lie in higher bins
+    const int d = bins - 1 - 2 * tid;
+    int c0 = 0, c1 = 0;
+    if (d > 0)
+#pragma unroll
+      for (int i = 0; i < kCtas; ++i) {
+        const int2 two = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[step][d - 1], i));
+        c1 += two.x;
+        c0 += two.y;
+      }
+    int incl = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    const int above = incl - c0 - c1 + __reduce_add_sync(0xffffffffu, lane < warp ? part[lane] : 0);
+    if (above < need && need <= above + c0) {
+      pick[0] = d;
+      pick[1] = need - above;
+      sums[0] = c0;
+    } else if (above + c0 < need && need <= above + c0 + c1) {
+      pick[0] = d - 1;
+      pick[1] = need - above - c0;
+      sums[0] = c1;
+    }
+    __syncthreads();
+    bar |= (uint32_t)pick[0] << shift;
+    known |= (uint32_t)(bins - 1) << shift;
+    need = pick[1];
+    whole = need == sums[0];
+  }
+  const unsigned below = (1u << lane) - 1;
+  // Sums over the warps before this one: in the cluster for the tied keys (only if some of them go), then for the kept.
+  auto before_me = [&](int mine, int& slot) {
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) place[warp] = mine;
+    __syncthreads();
+    const int all = __reduce_add_sync(0xffffffffu, place[lane]);
+    int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? place[lane] : 0);
+    if (tid == 0) slot = all;
+    cluster.sync();
+    return ahead + __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(&slot, lane) : 0);
+  };
+  unsigned in = 0;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) in |= (unsigned)(key_of(i) >= bar) << i;
+  } else {
+    int ties = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) ties += key_of(i) == bar;
+    int before = before_me(ties, sums[1]);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      if (i >= used) break;
+      const uint32_t key = key_of(i);
+      const unsigned tied = __ballot_sync(0xffffffffu, key == bar);
+      in |= (unsigned)(key > bar || (key == bar && before + __popc(tied & below) < need)) << i;
+      before += __popc(tied);
+    }
+  }
+  int done = before_me(__popc(in), pick[0]);  // every weight has been read by then
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    if (i >= used) break;
+    const unsigned all = __ballot_sync(0xffffffffu, in >> i & 1);
+    const int to = done + __popc(all & below);
+    if (in >> i & 1) {
+      out[to] = t0 + 32 * i;
+      w[to] = x[i];
+    }
+    done += __popc(all);
+  }
+  for (int t = keep + me; t < n; t += threads) w[t] = 0.f;
+  cluster.sync();  // the others' shared memory is still read until here
 }
 
 // Moves the kept tokens' stored rows (codes and scales) to the new blocks: 16 bytes of a key and of a value a thread.
@@ -1319,12 +1459,30 @@ cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const in
                          int recent, int sink, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
   const long long most = (long long)max_blocks * kTok < w_len ? (long long)max_blocks * kTok : w_len;  // tokens
-  auto select = most <= 4 * kSelect    ? q4_select_regs_kernel<4>
-                : most <= 16 * kSelect ? q4_select_regs_kernel<16>
-                : most <= 40 * kSelect ? q4_select_regs_kernel<40>  // (64 registers a thread hold no more)
-                                       : q4_select_kernel;
-  select<<<dim3(Hkv, B), kSelect, 0, s>>>(lens, weights, weight_rows, kept, new_lens, Hkv, w_rows, w_len, keep, recent,
-                                          sink, status);
+  // Clusters while their rows take less than one CTA each does (rows x 0.9 us and up, against 41).
+  const bool few = (long long)B * Hkv <= 32 || most > 40 * kSelect;
+  if (few && most > 16 * kSelect && most <= 16 * kSelect * kCtas) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kCtas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(Hkv * kCtas, B);
+    cfg.blockDim = dim3(kSelect);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_select_cluster_kernel, lens, weights, weight_rows, kept, new_lens,
+                                             Hkv, w_rows, w_len, keep, recent, sink, status);
+    if (e != cudaSuccess) return e;
+  } else {
+    auto select = most <= 4 * kSelect    ? q4_select_regs_kernel<4>
+                  : most <= 16 * kSelect ? q4_select_regs_kernel<16>
+                  : most <= 40 * kSelect ? q4_select_regs_kernel<40>  // (64 registers a thread hold no more)
+                                         : q4_select_kernel;
+    select<<<dim3(Hkv, B), kSelect, 0, s>>>(lens, weights, weight_rows, kept, new_lens, Hkv, w_rows, w_len, keep,
+                                            recent, sink, status);
+  }
   const int rows = (keep + kTok - 1) / kTok * kTok;  // the new blocks that can hold a token
   RLB_Q4_D((q4_move_kernel<DD><<<dim3((unsigned)(((long long)rows * Q4<DD>::kGroups * (Q4<DD>::kRow / 16) + 255) / 256), Hkv, B),
                                  256, 0, s>>>((uint8_t*)k_pool, (uint8_t*)v_pool, tables, new_tables, kept, new_lens,

@@ -322,6 +322,12 @@ def chosen(w, n, keep, sink, recent):
     ([16384], 1, 32, 16000, 0, 0, "ties"),
     ([132000, 131073], 1, 32, 3000, 2, 9, "random"),
     ([132000], 1, 32, 131000, 2, 9, "odd"),
+    ([20000, 17, 9000, 5001], 2, 64, 5000, 4, 30, "ties"),
+    ([40000, 16385], 2, 32, 3000, 0, 2900, "odd"),
+    ([131072, 70000], 1, 32, 100, 0, 0, "zeros"),
+    ([131072], 1, 32, 77, 70, 7, "random"),
+    ([17000, 30, 400], 12, 32, 300, 3, 50, "ties"),
+    ([40960, 16500, 90], 11, 32, 16500, 1, 0, "odd"),
     ([90, 33], 2, 64, 30, 1, 1, "odd"),
     ([70], 2, 64, 90, 1, 1, "random"),
 ])
