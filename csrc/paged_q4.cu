@@ -45,12 +45,11 @@ RLB_DEVICE uint32_t half2_add(uint32_t x, uint32_t both) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
-// Nibbles j and j + 4 of a word as two fp16 numbers: code - MINUS for j = 0 and 2, for j = 1 and 3 the same (ALL) or
+// Nibbles j and j + 4 of a word as two fp16 numbers: code - 8 for j = 0 and 2, for j = 1 and 3 the same (ALL) or
 // 1024 + 16 code.
-template <bool ALL, int MINUS = 8>
+template <bool ALL>
 RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
-  static_assert(MINUS == 0 || MINUS == 8, "-1024 and -64, or -1032 and -72");
-  constexpr uint32_t off = MINUS == 8 ? 0xe408e408u : 0xe400e400u;
+  constexpr uint32_t off = 0xe408e408u;  // -1032
   const uint32_t x = w >> 8;
   r[0] = half2_add(nibbles<0x000f000fu>(w, magic), off);
   r[1] = nibbles<0x00f000f0u>(w, magic);
@@ -58,7 +57,7 @@ RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
   r[3] = nibbles<0x00f000f0u>(x, magic);
   if (ALL) {
     const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
-    const __half2 off16 = __half2half2(__ushort_as_half(MINUS == 8 ? 0xd480 : 0xd400));
+    const __half2 off16 = __half2half2(__ushort_as_half(0xd480));
 #pragma unroll
     for (int j = 1; j < 4; j += 2) {
       const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&r[j]), sixteenth, off16);
@@ -71,7 +70,7 @@ RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
 // A group's four threads (two at D 32) reduce its minimum and maximum by shuffles (NaN-propagating), then each
 // quantises its 16 elements to two 32-bit words.  Bound by memory latency and pattern (rows of 256 bytes in, 32-byte
 // pieces of a block out): 32768 rows of 8 heads x 128 in 48 us, 3.6 TB/s; 8 elements a thread took 4 us more, and 40
-// registers for half as many warps again 59.
+// registers for half as many warps again 59, a grid of one wave that fetches the next row ahead 56.
 //
 // code = clamp(rint((x - lo) / s)) without a division per element: q = (x - lo) (1 / s) and its remainder's share
 // q + (x - lo - q s) (1 / s) is the correctly rounded quotient, and adding 1.5 2^23 rounds that to a whole number.
@@ -152,18 +151,20 @@ __global__ void __launch_bounds__(256) q4_write_kernel(
 }
 
 // ---------------------------------------------------------------- reading rows
-// The 8 elements of a word: codes become fp16 numbers by their bits.
-RLB_DEVICE bf16x8 q4_elements(uint32_t word, float s, float lo) {
-  uint32_t two[4];
-  codes_f16<true, 0>(word, two, 0x64006400u);
-  float f[8];
+// The 8 elements of a word: codes become bf16 numbers by their bits (128 + code), and minimum + scale code is rounded once.
+RLB_DEVICE uint4 q4_elements(uint32_t word, uint32_t scale_min) {
+  const uint32_t ss = __byte_perm(scale_min, 0, 0x1010), ll = __byte_perm(scale_min, 0, 0x3232);
+  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&ss), lo = *reinterpret_cast<const __nv_bfloat162*>(&ll);
+  uint32_t x[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {  // elements j and j + 4
-    const float2 n = fma2(__half22float2(*reinterpret_cast<const __half2*>(&two[j])), make_float2(s, s), make_float2(lo, lo));
-    f[j] = n.x;
-    f[j + 4] = n.y;
+    const uint32_t m = nibbles<0x000f000fu>(word >> (4 * j), 0x43004300u);
+    const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), __float2bfloat162_rn(128.f));
+    const __nv_bfloat162 y = __hfma2(n, s, lo);
+    x[j] = *reinterpret_cast<const uint32_t*>(&y);
   }
-  return pack8(f);
+  return make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632),
+                    __byte_perm(x[2], x[3], 0x7632));
 }
 
 // One thread per 8 elements of a key and of a value (16 of each would write every sector in two halves: 119 us where
@@ -195,24 +196,22 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
       absent = pos >= lens[b];
       if (!absent && pos / kTok < max_blocks) blk = tables[b * max_blocks + pos / kTok];
     }
-    bf16x8 k, v;
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
     if (!absent && (blk < 0 || blk >= num_blocks || off < 0 || off >= kTok)) {
       if (part == 0 && h == 0) report(status, kBadIndex);
       absent = true;
     }
-    if (absent) {
-      *reinterpret_cast<uint4*>(&k) = *reinterpret_cast<uint4*>(&v) = make_uint4(0, 0, 0, 0);
-    } else {
+    if (!absent) {
       const long long at = ((long long)blk * Hkv + h) * L::kBytes;
       const int code = (grp * kTok + off) * L::kRow + lane * 4, meta = L::kCodes + (grp * kTok + off) * 4;
       const uint32_t kw = *reinterpret_cast<const uint32_t*>(k_pool + at + code), km = *reinterpret_cast<const uint32_t*>(k_pool + at + meta);
       const uint32_t vw = *reinterpret_cast<const uint32_t*>(v_pool + at + code), vm = *reinterpret_cast<const uint32_t*>(v_pool + at + meta);
-      k = q4_elements(kw, bf16_lo_f(km), bf16_hi_f(km));
-      v = q4_elements(vw, bf16_lo_f(vm), bf16_hi_f(vm));
+      k = q4_elements(kw, km);
+      v = q4_elements(vw, vm);
     }
     const long long to = (n * Hkv + h) * D + part * 8;
-    stg8(k_out + to, k);
-    stg8(v_out + to, v);
+    *reinterpret_cast<uint4*>(k_out + to) = k;
+    *reinterpret_cast<uint4*>(v_out + to) = v;
   }
 }
 
