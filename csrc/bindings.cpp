@@ -864,7 +864,7 @@ at::Tensor q4_decode(const at::Tensor& q, const at::Tensor& k_pool, const at::Te
   const int64_t Hkv = k_pool.size(1);
   TORCH_CHECK(Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16, "q: a multiple of the KV heads, at most 16 per KV head");
   TORCH_CHECK(B < 65536, "at most 65535 sequences in a call");
-  TORCH_CHECK(window < (1LL << 31), "window: fewer than 2^31 tokens");
+  TORCH_CHECK(window > -(1LL << 31) && window < (1LL << 31), "window: fewer than 2^31 tokens");
   TORCH_CHECK(tables.dim() == 2 && tables.size(1) < (1LL << 27), "block_tables: [B, max_blocks]");
   check_ints(tables, k_pool, {B, tables.size(1)}, "block_tables");
   check_ints(lens, k_pool, {B}, "ctx_lens");

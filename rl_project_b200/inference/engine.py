@@ -99,9 +99,10 @@ class InferenceEngine:
         self.allocator = PagedBlockAllocator(block_size=block_size, max_blocks=max_blocks)
         self.scheduler = Scheduler(self.allocator, max_batch=max_batch, max_seq_len=self.max_seq_len)
         self.kv: Optional[PagedKVCache] = None
+        if kv_recent is None:
+            kv_recent = 0 if kv_budget is None else max(0, min(kv_budget // 4, kv_budget - kv_sink))
         self._check_kv(kv_cache, kv_budget, kv_sink, kv_recent)
-        self.kv_budget, self.kv_sink = kv_budget, kv_sink
-        self.kv_recent = 0 if kv_budget is None else kv_budget // 4 if kv_recent is None else kv_recent
+        self.kv_budget, self.kv_sink, self.kv_recent = kv_budget, kv_sink, kv_recent
         self.evictions = 0
         self._free_rows: List[int] = list(range(max_batch)) if kv_budget is not None else []
         if self.paged:
@@ -143,7 +144,7 @@ class InferenceEngine:
         if self.decode_graphs:
             self._pad_block = self.allocator.allocate("__graph_padding__", 1)[0]
 
-    def _check_kv(self, kv_cache: str, budget: Optional[int], sink: int, recent: Optional[int]) -> None:
+    def _check_kv(self, kv_cache: str, budget: Optional[int], sink: int, recent: int) -> None:
         if kv_cache not in ("bf16", "q4"):
             raise ServingError(f"kv_cache must be 'bf16' or 'q4', got {kv_cache!r}")
         if kv_cache == "q4":
@@ -160,7 +161,7 @@ class InferenceEngine:
             raise ServingError("kv_budget needs kv_cache='q4'")
         if any(blk.attn.window_size for blk in self.model.transformer.h):
             raise ServingError("kv_budget does not go with sliding windows, which count cached tokens")
-        if sink < 0 or (recent is not None and recent < 0) or sink + (recent or 0) > budget or budget < KERNEL_BLOCK:
+        if sink < 0 or recent < 0 or sink + recent > budget or budget < KERNEL_BLOCK:
             raise ServingError(f"kv_budget must hold kv_sink + kv_recent tokens and at least {KERNEL_BLOCK}")
 
     # ------------------------------------------------------------ submission

@@ -173,21 +173,23 @@ class PagedKVCache:
 
     def write_prefix(self, layer: int, k: torch.Tensor, v: torch.Tensor, table: List[int]) -> None:
         """Store a prompt's keys/values ``[Hkv, T, D]`` (positions 0..T-1) into its blocks."""
-        from rl_project_b200.ops.paged_attention import paged_write
-
         T = k.shape[1]
         pos = torch.arange(T)
         blocks = torch.as_tensor(table, dtype=torch.int32)[pos // self.block_size]
         offs = (pos % self.block_size).to(torch.int32)
         dev = self.k.device
-        kl, vl = self.layer(layer)
-        paged_write(k.transpose(0, 1), v.transpose(0, 1), kl, vl, blocks.to(dev, non_blocking=True),
-                    offs.to(dev, non_blocking=True))
+        self._write_rows(layer, k.transpose(0, 1), v.transpose(0, 1), blocks.to(dev, non_blocking=True),
+                        offs.to(dev, non_blocking=True))
+
+    def _write_rows(self, layer: int, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, offs: torch.Tensor) -> None:
+        """Store rows ``[N, Hkv, D]`` in the slots ``(blocks[i], offs[i])`` (int32, on the cache's device)."""
+        from rl_project_b200.ops.paged_attention import paged_write
+
+        paged_write(k, v, *self.layer(layer), blocks, offs)
 
 
-class PagedQ4KVCache:
-    """K/V pools in 4 bits, uint8 ``[n_layer, num_blocks, Hkv, block bytes]`` (layout: ops/paged_q4.py), with the
-    interface of ``PagedKVCache``.
+class PagedQ4KVCache(PagedKVCache):
+    """K/V pools in 4 bits, uint8 ``[n_layer, num_blocks, Hkv, block bytes]`` (layout: ops/paged_q4.py).
 
     With ``weight_rows`` sequences of up to ``weight_tokens`` cached tokens each have an accumulator row of
     attention weights per layer and KV head (fp32 ``[n_layer, rows, Hkv, tokens]``).
@@ -218,9 +220,10 @@ class PagedQ4KVCache:
     def nbytes(self) -> int:
         return 2 * self.k.numel() + (0 if self.weights is None else 4 * self.weights.numel())
 
-    def copy_block(self, src: int, dst: int) -> None:
-        self.k[:, dst].copy_(self.k[:, src])
-        self.v[:, dst].copy_(self.v[:, src])
+    def _write_rows(self, layer: int, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, offs: torch.Tensor) -> None:
+        from rl_project_b200.ops.paged_q4 import paged_write_q4
+
+        paged_write_q4(k, v, *self.layer(layer)[:2], blocks, offs)
 
     def evict(self, tables: torch.Tensor, lens: torch.Tensor, new_tables: torch.Tensor, rows: torch.Tensor, keep: int,
               recent: int, sink: int) -> None:

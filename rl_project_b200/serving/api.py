@@ -14,6 +14,7 @@ import json
 import threading
 import time
 from collections import deque
+from dataclasses import replace
 from typing import Any, Callable, Dict, Iterator, Optional, Tuple, Union
 
 from rl_project_b200.core.errors import BackendUnavailableError, ServingError
@@ -111,7 +112,7 @@ class Router:
             self.requests_total += 1
         t0 = time.perf_counter()
         if req.stream:
-            pieces = backend.stream(prompt, req.sampling(), rid, stop=req.stop)
+            pieces = backend.stream(prompt, replace(req.sampling(), logprobs=None), rid, stop=req.stop)
             return 200, self._sse(pieces, lambda t, fr: chunk(rid, name, t, fr), t0, name)
         res = backend.complete(prompt, req.sampling(), rid, stop=req.stop)
         self._record(t0, res.completion_tokens, name)

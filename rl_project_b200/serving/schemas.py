@@ -32,7 +32,7 @@ def _stop_list(value: Any) -> List[str]:
 
 def _logprobs(d: Dict[str, Any]) -> Optional[int]:
     """Alternatives per token to report, None for no log-probs: ``logprobs: n`` (completions), or ``logprobs: true``
-    with ``top_logprobs: n`` (chat)."""
+    with ``top_logprobs: n`` (chat).  Streamed answers carry none."""
     want, top = d.get("logprobs"), d.get("top_logprobs")
     if want is None or want is False:
         if top:
@@ -51,6 +51,9 @@ def _common(d: Dict[str, Any]) -> Dict[str, Any]:
         raise ServingError(f"invalid numeric field: {exc}") from exc
 
 
+_LEAST = -9999.0  # stands for the log-prob of a token that cannot occur
+
+
 @dataclass
 class TokenLogprob:
     """One generated token: its text, where it begins in the completion, its log-prob and alternatives (text, log-prob)."""
@@ -59,6 +62,10 @@ class TokenLogprob:
     offset: int
     logprob: float
     top: List[Tuple[str, float]]
+
+    def __post_init__(self) -> None:  # -inf has no place in JSON
+        self.logprob = max(self.logprob, _LEAST)
+        self.top = [(text, max(lp, _LEAST)) for text, lp in self.top]
 
 
 @dataclass

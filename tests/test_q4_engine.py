@@ -188,8 +188,47 @@ def test_served_logprobs():
     assert "".join(said["tokens"]) == out["choices"][0]["text"] and said["top_logprobs"] == [{}] * len(said["tokens"])
     status, out = router.handle("POST", "/v1/completions", {"prompt": "abc", "max_tokens": 3})
     assert out["choices"][0]["logprobs"] is None
+    status, lines = router.handle("POST", "/v1/completions", {"prompt": "abc", "max_tokens": 3, "logprobs": 2, "stream": True})
+    assert status == 200 and "[DONE]" in "".join(lines)
     for bad in ({"logprobs": 21}, {"logprobs": -1}, {"logprobs": "x"}, {"top_logprobs": 3}):
         assert router.handle("POST", "/v1/completions", {"prompt": "abc", **bad})[0] == 400
+
+
+def test_impossible_tokens_stay_within_json():
+    import json
+
+    from rl_project_b200.serving.schemas import TokenLogprob, chat_response, completion_response
+
+    said = [TokenLogprob("a", 0, -0.5, [("b", -math.inf)]), TokenLogprob("c", 1, -math.inf, [])]
+    for make in (chat_response, completion_response):
+        json.dumps(make("r", "m", "ac", 1, 2, "length", logprobs=said), allow_nan=False)
+    assert said[0].top == [("b", -9999.0)] and said[1].logprob == -9999.0 and said[0].logprob == -0.5
+
+
+def test_sink_fills_the_budget():
+    """What the first tokens leave of the budget bounds the default share of the last ones."""
+    m = model("cpu")
+    eng = InferenceEngine(m, max_batch=2, kv_cache="q4", kv_budget=16, kv_sink=15)
+    req, = eng.generate_batch([list(range(1, 41))], SamplingParams(max_tokens=30, **GREEDY))
+    assert eng.kv_recent == 1 and eng.evictions > 0 and len(req.generated_tokens) == 30
+    with pytest.raises(ServingError):
+        InferenceEngine(m, kv_cache="q4", kv_budget=16, kv_sink=17)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_prompts_written_by_table(dev):
+    from rl_project_b200.inference import PagedQ4KVCache
+    from rl_project_b200.ops.paged_q4 import paged_gather_q4
+
+    kv = PagedQ4KVCache(2, 2, 32, 4, torch.device(dev))
+    k, v = (torch.randint(0, 16, (2, 20, 32), device=dev).bfloat16() for _ in range(2))
+    k[..., 0], k[..., 1], v[..., 0], v[..., 1] = 0, 15, 0, 15  # codes are the values
+    kv.write_prefix(1, k, v, [3, 1])
+    kv.copy_block(3, 0)
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=dev)
+    got = paged_gather_q4(*kv.layer(1), table, torch.tensor([20], dtype=torch.int32, device=dev), 32, 20)
+    assert torch.equal(got[0][0].transpose(0, 1), k) and torch.equal(got[1][0].transpose(0, 1), v)
+    assert not kv.k[0].any() and not kv.k[1, 2].any()
 
 
 def test_refusals():
