@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // words and takes nibbles j and j + 4 of a word as one operand register.
 // O^T = V^T P^T.  The token's scale goes into the weight and its minimum into a separate fp32 sum of p (m + 8 s).
 // The weights p s are rounded to fp16 (2^-11 of each, an eighth of what the output's own rounding to bf16 may
-// add); to stay in range, p is kept times a power of two that takes the largest scale so far below 2^4: p s <= 2^12.
+// add); to stay in range, p is kept times a power of two that takes the largest scale so far below 2^4: p s <= 2^12.  (Where that
+// is so large that small p would leave fp32's range, from 2^64, V's scales and minima are scaled down instead.)
 // The tokens' order is free too: row g of S^T (of each half of the block) is token g / 2 for even g and
 // 4 + (g / 2 ^ 2) for odd g.  After the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's, lane
 // t of a quad has the tokens t and 4 + (t ^ 2) of both halves; neither its four V words nor the K words that a half
@@ -255,6 +256,7 @@ struct Q4Cache {
 };
 
 constexpr int kDecodeWarps = 4;
+constexpr int kMostVe = 190;  // weights are scaled down for scales of V up to 2^64; beyond, V's scales and minima are
 constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
 
 RLB_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2,
@@ -360,8 +362,8 @@ struct Q4Warp {
   float m[NT][2], lim[NT][2];                    // maximum when it was last raised, the s that lies 8 above it
   float mref[NT][2], l[NT][2];                   // what exponents are taken against, sum of p
   float z[NT][NG][2], o[NT][NG][MT][4];          // sums of p (m + 8 s) and of p s (code - 8)
-  int ve;                                        // exponent field of the largest scale of V so far: p is kept times
-                                                 // 2^(130 - ve), and so are the sums
+  int ve;                                        // exponent field of the largest scale of V so far: p and l are kept
+                                                 // times 2^(130 - ve) (from kMostVe on no less), z and o times that
   uint32_t magic;                                // 0x64006400
 
   RLB_DEVICE void load_q(const __nv_bfloat16* q, int G, float scale) {
@@ -539,8 +541,8 @@ struct Q4Warp {
       int e_all = e_here;
 #pragma unroll
       for (int k = 1; k < 32; k <<= 1) e_all = max(e_all, __shfl_xor_sync(0xffffffffu, e_all, k));
-      e_all = min(max(e_all, ve), 252);
-      const float fv = pow2(max(ve - e_all, -126));
+      e_all = max(e_all, ve);
+      const float fl = pow2(min(ve, kMostVe) - min(e_all, kMostVe)), fv = pow2(max(ve - e_all, -126));
       ve = e_all;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -551,11 +553,11 @@ struct Q4Warp {
           for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
           const float was = m[n][e];
           x = fmaxf(ceilf(x), was);
-          const float f = (was == -INFINITY ? 0.f : sm100::ex2_approx(was - x)) * fv;
+          const float up = was == -INFINITY ? 0.f : sm100::ex2_approx(was - x), f = up * fv;
           m[n][e] = x;
           lim[n][e] = (x + 8.f) / qf[n][e];
-          mref[n][e] = (x == -INFINITY ? 0.f : x) - (float)(130 - ve);
-          l[n][e] *= f;
+          mref[n][e] = (x == -INFINITY ? 0.f : x) - (float)(130 - min(ve, kMostVe));
+          l[n][e] *= up * fl;
 #pragma unroll
           for (int r = 0; r < NG; ++r) {
             z[n][r][e] *= f;
@@ -566,6 +568,18 @@ struct Q4Warp {
             }
           }
         }
+    }
+    if (ve > kMostVe) {  // (a whole warp; exact, but for what is far below the largest scale)
+      const __nv_bfloat162 down = __float2bfloat162_rn(pow2(kMostVe - ve));
+#pragma unroll
+      for (int k = 0; k < BT; ++k)
+#pragma unroll
+        for (int r = 0; r < NG; ++r)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&vm[k][r][i]), down);
+            vm[k][r][i] = *reinterpret_cast<const uint32_t*>(&x);
+          }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -736,13 +750,13 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
     // the part's sums: over the quads for l and z, the outputs are whole in each lane (8 or 4 dimensions of two heads)
     const long long slot = me + row;
     const bool whole = p0 == 0 && p1 == n;
-    const float back = pow2(w.ve - 130);
+    const float back = pow2(w.ve - 130), back_l = pow2(min(w.ve, kMostVe) - 130);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int head = nt * 8 + 2 * t + e;
-        float l = w.l[nt][e] * back;
+        float l = w.l[nt][e] * back_l;
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
         const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -916,12 +930,25 @@ __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* 
   __syncthreads();
   float* w = weights + ((long long)r * c.Hkv + h) * w_len;
   const float* sc = scores + row * c.max_blocks * kTok * Gs;
-  const int step = (gridDim.z - joins) * 256;
-  for (int t = q4_first(c, len) + (z - joins) * 256 + threadIdx.x; t < min(len, w_len); t += step) {
-    float p = 0.f;
-    for (int head = 0; head < G; ++head)
-      p += sm100::ex2_approx(sc[(long long)t * Gs + head] - stat[head].x) * stat[head].y;
-    if (p > 0.f) atomicAdd(w + t, p);
+  const int end = min(len, w_len);
+  constexpr int U = 4;  // tokens a thread takes at a time
+  for (long long t0 = q4_first(c, len) + (z - joins) * 256LL * U + threadIdx.x; t0 < end; t0 += (gridDim.z - joins) * 256LL * U) {
+    float p[U] = {};
+    for (int head = 0; head < G; head += 2) {
+      float2 x[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        x[i] = t0 + 256 * i < end ? *reinterpret_cast<const float2*>(sc + (t0 + 256 * i) * Gs + head) : make_float2(0.f, 0.f);
+      const float2 s0 = stat[head], s1 = stat[head + 1];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        p[i] += sm100::ex2_approx(x[i].x - s0.x) * s0.y;
+        if (head + 1 < G) p[i] += sm100::ex2_approx(x[i].y - s1.x) * s1.y;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (t0 + 256 * i < end && p[i] != 0.f) atomicAdd(w + t0 + 256 * i, p[i]);
   }
 }
 
@@ -1422,9 +1449,12 @@ cudaError_t rlb_q4_decode(const void* q, const void* k_pool, const void* v_pool,
   RLB_Q4_D(e = G <= 8 ? (q4_decode_launch<DD, 1>(q, c, out, B, ctas, part, ml, plan, scores, Gs, status, s))
                       : (q4_decode_launch<DD, 2>(q, c, out, B, ctas, part, ml, plan, scores, Gs, status, s)));
   if (e != cudaSuccess) return e;
-  int chunks = 0;  // CTAs per row that add weights: four waves of the GPU, 256 tokens each at least
+  // CTAs per row that add weights: one wave of the GPU, 1024 tokens each at least (192 rows of 5000 tokens and 4 heads:
+  // 11 us with the join; four waves of 256 tokens at a time, each reading the statistics again, took 19)
+  int chunks = 0;
   if (weighted) {
-    const long long rows = (long long)B * Hkv, want = (32LL * sms + rows - 1) / rows, most = ((long long)max_blocks * kTok + 255) / 256;
+    const long long rows = (long long)B * Hkv, want = (8LL * sms + rows - 1) / rows;
+    const long long most = ((long long)max_blocks * kTok + 1023) / 1024;
     chunks = (int)(want < most ? want : most);
     if (chunks < 1) chunks = 1;
   }

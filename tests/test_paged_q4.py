@@ -272,6 +272,57 @@ def test_decode_offset_channels(dev):
     check_decode(out[0], o, a)
 
 
+@pytest.mark.parametrize("size", [1e-12, 1e-4, 1e15, 1e19, 1e22, 1e30])
+def test_decode_value_sizes(dev, size):
+    """Values of any size, alone and behind ordinary ones; the weights do not depend on them."""
+    lens, D = [300, 2000], 64
+    ks, vs, pools, tables, n, _ = cache(lens, 1, D, dev)
+    k, v = (torch.cat(x) for x in (ks, vs))
+    big = v * size
+    big[300:1700] = v[300:1700]  # the second sequence's last values only
+    pos = torch.cat([torch.arange(m) for m in lens])
+    seq = torch.arange(2).repeat_interleave(torch.tensor(lens))
+    big = big.to(BF)
+    paged_write_q4(k.to(BF).to(dev), big.to(dev), *pools, tables[seq.to(dev), (pos // 16).to(dev)].contiguous(),
+                   (pos % 16).int().to(dev))
+    ks, vs = (stored(x.to(BF))[3].split(lens) for x in (k, big))
+    q = torch.randn(2, 4, D).to(BF).to(dev)
+    w = torch.zeros(2, 1, tables.shape[1] * 16, device=dev)
+    out = paged_decode_q4(q, *pools, tables, n, 0.125, weights=w, weight_rows=torch.tensor([0, 1], dtype=torch.int32, device=dev))
+    for b in range(2):
+        o, p, a = attention(q[b], ks[b], vs[b], 0.125, 0.0, 0)
+        check_decode(out[b], o, a)
+        assert ((w[b, 0, :lens[b]].cpu().to(F64) - p.sum(0).flatten()).abs() <= 2 ** -15 * p.sum(0).flatten()).all()
+
+
+def test_decode_not_a_number(dev):
+    """A key or a value that holds NaN: its head's output is NaN (with a NaN key its weights too), others are as ever."""
+    lens, D = [50, 700], 64
+    ks, vs, pools, tables, n, _ = cache(lens, 2, D, dev)
+    # a row's weights sum up to its 2 query heads, off by 700 roundings and exponents of 2^-24 to 2^-22 each
+    bad = torch.full((1, 2, D), math.nan, dtype=BF, device=dev)
+    for b, h, pos, pool in ((0, 1, 3, 0), (1, 0, 650, 0), (1, 1, 699, 1)):
+        both = [p.clone() for p in pools]
+        i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=dev)
+        paged_write_q4(bad, bad, *both, i32(int(tables[b, pos // 16])), i32(pos % 16))
+        blk, other = int(tables[b, pos // 16]), 1 - h
+        pools_b = [p.clone() for p in pools]
+        pools_b[pool][blk, h] = both[pool][blk, h]
+        q = torch.randn(2, 4, D).to(BF).to(dev)
+        w = torch.zeros(2, 2, tables.shape[1] * 16, device=dev)
+        rows_ = torch.tensor([1, 0], dtype=torch.int32, device=dev)
+        out = paged_decode_q4(q, *pools_b, tables, n, 0.125, weights=w, weight_rows=rows_).view(2, 2, 2, D)
+        assert out[b, h].isnan().all()
+        if pool == 0:
+            assert w[rows_[b], h, :lens[b]].isnan().all()
+        else:
+            assert abs(float(w[rows_[b], h].sum()) - 2) < 1e-4
+        for s, head in ((b, other), (1 - b, 0), (1 - b, 1)):
+            o, p, a = attention(q[s].view(2, 2, D)[head], ks[s][:, head:head + 1], vs[s][:, head:head + 1], 0.125, 0.0, 0)
+            check_decode(out[s, head], o, a)
+            assert abs(float(w[rows_[s], head].sum()) - 2) < 1e-4 and not w[rows_[s], head, lens[s]:].any()
+
+
 def test_decode_bad_index(dev):
     """A block outside the pool, a context longer than its table, an accumulator row that is not there."""
     lens, D = [40, 40], 64
