@@ -169,7 +169,8 @@ RLB_DEVICE uint4 q4_elements(uint32_t word, uint32_t scale_min) {
 
 // One thread per 8 elements of a key and of a value (16 of each would write every sector in two halves: 119 us where
 // this takes 39 for 32768 rows of 8 x 128).  Row n is slot (slot_block[n], slot_off[n]), or, with a block table, position
-// n % max_len of sequence n / max_len.  Rows without a place in the pool read as zeros.  Bound by the write of the rows.
+// n % max_len of sequence n / max_len.  Rows without a place in the pool read as zeros.  Bound by the write of the rows:
+// 32768 rows of 8 x 128 in 37 us (4.7 TB/s, reads and writes); 16 sequences of 1024 by table in 18.
 template <int D>
 __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict__ k_pool,
                                                       const uint8_t* __restrict__ v_pool,
@@ -224,7 +225,10 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // (mma.sync m16n8k16, fp16 x fp16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
 // query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
 // them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
-// memory) would need the unpacked values written back to shared memory first.
+// memory) would need the unpacked values written back to shared memory first.  32 ragged sequences of up to 8192 tokens
+// (8 KV heads x 128, 4 queries each, 189 MB): 54 us, 3.5 TB/s; one of 100001: 35 us, 3.3 TB/s; 64 of up to 4096 with
+// heads of 64 (90 MB): 35 us.  The copies alone would run at 5.2 TB/s; what holds it there is issue, 365 instructions
+// per block of 16 tokens and 128 dimensions at 2.3 a cycle and SM, with no single pipe above 51 %.
 //
 // Codes become fp16 numbers exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are 1024 + 16 code, so
 // half of the nibbles need no shift, and a packed add or fma makes code - 8 of them.
@@ -864,7 +868,8 @@ RLB_DEVICE float2 q4_add_parts(const float* part, const float* stats, int G, int
 // Joins the parts of the rows that several warps of q4_decode_kernel shared, and writes zeros for empty sequences.
 // WIDE: CTA z of a row does query head z, its eight warps taking the parts in turn (few rows, long contexts);
 // otherwise a warp does a query head.  With `weights` the CTAs behind add a stretch each of the tokens' attention
-// weights, summed over the heads, to their accumulators.
+// weights, summed over the heads, to their accumulators.  Bound by latency (plan, statistics, parts, output: 4 to 8 us
+// alone, 2 to 5 behind the decode kernel's end).
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) q4_finish_kernel(Q4Cache c, const float* __restrict__ part,
                                                         const float* __restrict__ ml, const int2* __restrict__ plan,
@@ -1334,7 +1339,9 @@ __global__ void __launch_bounds__(kSelect) q4_select_cluster_kernel(const int* _
   cluster.sync();  // the others' shared memory is still read until here
 }
 
-// Moves the kept tokens' stored rows (codes and scales) to the new blocks: 16 bytes of a key and of a value a thread.
+// Moves the kept tokens' stored rows (codes and scales) to the new blocks: 16 bytes of a key and of a value a thread, and
+// nothing shared, so that all reads are in flight at once.  Kept rows lie 32 bytes here and there: 16 x 1024 rows of
+// 8 x 128 in 12 us (38 MB read and written, 3.2 TB/s), of which about 4 are the chain of tables, positions and rows.
 template <int D>
 __global__ void __launch_bounds__(256) q4_move_kernel(uint8_t* k_pool, uint8_t* v_pool, const int* __restrict__ tables,
                                                       const int* __restrict__ new_tables, const int* __restrict__ kept,

