@@ -414,10 +414,12 @@ template <typename T, bool TOP>
 static cudaError_t token_logprob_launch(const void* logits, long long ld, long long rows, int V, const long long* tgt,
                                         int k, float* m, float* ls, float* lp, float* ent, float* top_lp,
                                         long long* top_ids, int sms, int* status, cudaStream_t s) {
-  // Slices: as long as the CTAs fit on the GPU at a time and a slice keeps a round of logits (a single row of 128256 in
-  // bf16 takes 8 of them; from 2 rows per SM on a row stays whole).
+  // Slices: two as long as the CTAs fit on the GPU at a time, four and eight while three CTAs an SM hold them, and a slice
+  // keeps a round of logits.  (Rows of 128256 in bf16 with 5 alternatives, in us, by 1, 2, 4 and 8 slices: 1 row
+  // 33, 25, 18, 16; 48 rows 35, 27, 23, 21; 74 rows 37, 27, 25, 29; 148 rows 37, 29, 37, 39; 296 rows 41, 37, 53, 64;
+  // 400 rows 45, 53, 62, 82.)
   int slices = 1;
-  while (slices < 8 && rows * slices * 2 <= (long long)kCtas * sms && V / (slices * 2) >= kRound) slices *= 2;
+  while (slices < 8 && rows * slices * 2 <= (slices == 1 ? kCtas : 3LL) * sms && V / (slices * 2) >= kRound) slices *= 2;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = slices;
