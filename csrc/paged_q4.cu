@@ -45,9 +45,7 @@ RLB_DEVICE uint32_t half2_add(uint32_t x, uint32_t both) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
-// Nibbles j and j + 4 of a word as two fp16 numbers: code - 8 for j = 0 and 2, for j = 1 and 3 the same (ALL) or
-// 1024 + 16 code.
-template <bool ALL>
+// Nibbles j and j + 4 of a word as two fp16 numbers: code - 8 for j = 0 and 2, 1024 + 16 code for j = 1 and 3.
 RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
   constexpr uint32_t off = 0xe408e408u;  // -1032
   const uint32_t x = w >> 8;
@@ -55,14 +53,16 @@ RLB_DEVICE void codes_f16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
   r[1] = nibbles<0x00f000f0u>(w, magic);
   r[2] = half2_add(nibbles<0x000f000fu>(x, magic), off);
   r[3] = nibbles<0x00f000f0u>(x, magic);
-  if (ALL) {
-    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
-    const __half2 off16 = __half2half2(__ushort_as_half(0xd480));
+}
+
+// The same nibbles as two bf16 numbers, code - 8 (bits 0x4300 | code are 128 + code; bf16 has too few bits for the
+// second nibble's 16 code).
+RLB_DEVICE void codes_bf16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
 #pragma unroll
-    for (int j = 1; j < 4; j += 2) {
-      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&r[j]), sixteenth, off16);
-      r[j] = *reinterpret_cast<const uint32_t*>(&y);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x = nibbles<0x000f000fu>(w >> (4 * j), magic);
+    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(136.f));
+    r[j] = *reinterpret_cast<const uint32_t*>(&y);
   }
 }
 
@@ -222,26 +222,28 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // whole rows or of fixed parts leaves SMs idle at the end.  A warp works alone, with no barrier: it brings blocks (codes,
 // scales and minima of K and V, one contiguous piece each) into its own ring of shared memory with bulk copies, which
 // run ahead across the rows' borders, and computes on matrix instructions
-// (mma.sync m16n8k16, fp16 x fp16 -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
+// (mma.sync m16n8k16, two fp16 or two bf16 operands -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
 // query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
 // them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
 // memory) would need the unpacked values written back to shared memory first.  32 ragged sequences of up to 8192 tokens
-// (8 KV heads x 128, 4 queries each, 189 MB): 54 us, 3.5 TB/s; one of 100001: 35 us, 3.3 TB/s; 64 of up to 4096 with
-// heads of 64 (90 MB): 35 us.  The copies alone would run at 5.2 TB/s; what holds it there is issue, 365 instructions
-// per block of 16 tokens and 128 dimensions at 2.3 a cycle and SM, with no single pipe above 51 %.
+// (8 KV heads x 128, 4 queries each, 189 MB): 66 us with the join, 2.9 TB/s; one of 100001: 45 us, 2.6 TB/s; 64 of up to
+// 4096 with heads of 64 (90 MB): 39 us.  (With one fp16 weight 59, 41 and 37 us.)
 //
-// Codes become fp16 numbers exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are 1024 + 16 code, so
-// half of the nibbles need no shift, and a packed add or fma makes code - 8 of them.
+// K's codes become fp16 numbers exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are 1024 + 16 code, so
+// half of the nibbles need no shift, and a packed add makes code - 8 of the others.
 // S^T = K Q^T.  With a token's scale s and minimum m:  k . q = s (code . q) + m sum(q), per group of dimensions.  Q
 // is fp16 after division by a power of two per head (its largest element then lies in [2^13, 2^14)): bf16's 8 bits
 // fit, and what falls below 2^-24 is 2^-38 of the largest.  K's odd nibbles stay 1024 + 16 code: their q are divided by 16,
 // and the sums start at 8 sum(q even) - 64 sum(q odd) instead of zero, which leaves code . q.  The order of the
 // dimensions inside the product is free as long as Q's registers use the same: a lane reads 16 consecutive dimensions of a token as two
 // words and takes nibbles j and j + 4 of a word as one operand register.
-// O^T = V^T P^T.  The token's scale goes into the weight and its minimum into a separate fp32 sum of p (m + 8 s).
-// The weights p s are rounded to fp16 (2^-11 of each, an eighth of what the output's own rounding to bf16 may
-// add); to stay in range, p is kept times a power of two that takes the largest scale so far below 2^4: p s <= 2^12.  (Where that
-// is so large that small p would leave fp32's range, from 2^64, V's scales and minima are scaled down instead.)
+// O^T = V^T P^T in bf16.  The token's scale goes into the weight and its minimum into a separate fp32 sum of
+// p (m + 8 s).  A weight p s is held in two bf16 parts, its upper 8 bits and what is left of it rounded to 8 bits
+// (2^-16 of each weight, below a hundredth of the output's own rounding to bf16), and both go through the matrix
+// instruction.  bf16 has fp32's exponents, so that values of any size keep these bits beside each other: p is kept times
+// 2^-32, with which 2^20 tokens of the type's largest values stay in range and values from 2^-58 on keep all their bits.
+// (One fp16 weight, 2^-11 of each, needed the weights scaled by V's largest scale, from which values below 2^-17 of it
+// lost bits even where that token's weight was nothing.)
 // The tokens' order is free too: row g of S^T (of each half of the block) is token g / 2 for even g and
 // 4 + (g / 2 ^ 2) for odd g.  After the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's, lane
 // t of a quad has the tokens t and 4 + (t ^ 2) of both halves; neither its four V words nor the K words that a half
@@ -260,7 +262,7 @@ struct Q4Cache {
 };
 
 constexpr int kDecodeWarps = 4;
-constexpr int kMostVe = 190;  // weights are scaled down for scales of V up to 2^64; beyond, V's scales and minima are
+constexpr float kDown = 32.f;  // weights, their sums and the outputs are kept times 2^-kDown
 constexpr uint32_t kWaitLimit = 1u << 22;  // polls; a copy takes microseconds
 
 RLB_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2,
@@ -268,6 +270,12 @@ RLB_DEVICE void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+RLB_DEVICE void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 RLB_DEVICE uint32_t transpose8x8(uint32_t x) {
@@ -280,6 +288,14 @@ RLB_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+
+// Two fp32 numbers as two bf16 parts of each: the upper bits, and what they leave, rounded.
+RLB_DEVICE void split_bf16(float x, float y, uint32_t& upper, uint32_t& rest) {
+  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  upper = __byte_perm(a, b, 0x7632);
+  const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(a & 0xffff0000u), y - __uint_as_float(b & 0xffff0000u));
+  rest = *reinterpret_cast<const uint32_t*>(&r);
 }
 
 RLB_DEVICE uint32_t pack_f16(float lo, float hi) {
@@ -366,9 +382,7 @@ struct Q4Warp {
   float m[NT][2], lim[NT][2];                    // maximum when it was last raised, the s that lies 8 above it
   float mref[NT][2], l[NT][2];                   // what exponents are taken against, sum of p
   float z[NT][NG][2], o[NT][NG][MT][4];          // sums of p (m + 8 s) and of p s (code - 8)
-  int ve;                                        // exponent field of the largest scale of V so far: p and l are kept
-                                                 // times 2^(130 - ve) (from kMostVe on no less), z and o times that
-  uint32_t magic;                                // 0x64006400
+  uint32_t magic, magic_bf16;                    // 0x64006400, 0x43004300
 
   RLB_DEVICE void load_q(const __nv_bfloat16* q, int G, float scale) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -422,8 +436,8 @@ struct Q4Warp {
   }
 
   RLB_DEVICE void reset() {
-    ve = 70;  // (p is then at most 2^8 2^60)
-    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));  // kept in a register
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));  // kept in registers
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(magic_bf16));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -470,8 +484,8 @@ struct Q4Warp {
 #pragma unroll
         for (int w = 0; w < WPL; ++w) {
           uint32_t c0[4], c1[4];
-          codes_f16<false>(u0[w], c0, magic);
-          codes_f16<false>(u1[w], c1, magic);
+          codes_f16(u0[w], c0, magic);
+          codes_f16(u1[w], c1, magic);
 #pragma unroll
           for (int j = 0; j < 4; j += 2) {
             const uint32_t a[4] = {c0[j], c1[j], c0[j + 1], c1[j + 1]};
@@ -509,7 +523,6 @@ struct Q4Warp {
           }
     }
     bool raise = false;
-    uint32_t vm[BT][NG][2], vmax = 0;  // V's (scale, minimum) of this lane's tokens
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -529,25 +542,7 @@ struct Q4Warp {
                   make_float2(s[n][k][2 * i] * qf[n][0], s[n][k][2 * i + 1] * qf[n][1]);
       }
     }
-#pragma unroll
-    for (int k = 0; k < BT; ++k)
-#pragma unroll
-      for (int r = 0; r < NG; ++r)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          vm[k][r][i] = *reinterpret_cast<const uint32_t*>(ks + (2 * k + 1) * L::kBytes + L::kCodes + (r * kTok + tok + 8 * i) * 4);
-          if (MASKED && !((seen >> (2 * k + i)) & 1)) vm[k][r][i] = 0;  // unseen slots may hold anything, NaN too
-          vmax = __vmaxu2(vmax, vm[k][r][i]);
-        }
-    const int e_here = (vmax >> 7) & 0xff;  // the exponent field of the largest scale (scales are not negative)
-    raise |= e_here > ve;
     if (__any_sync(0xffffffffu, raise)) {
-      int e_all = e_here;
-#pragma unroll
-      for (int k = 1; k < 32; k <<= 1) e_all = max(e_all, __shfl_xor_sync(0xffffffffu, e_all, k));
-      e_all = max(e_all, ve);
-      const float fl = pow2(min(ve, kMostVe) - min(e_all, kMostVe)), fv = pow2(max(ve - e_all, -126));
-      ve = e_all;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -557,33 +552,21 @@ struct Q4Warp {
           for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
           const float was = m[n][e];
           x = fmaxf(ceilf(x), was);
-          const float up = was == -INFINITY ? 0.f : sm100::ex2_approx(was - x), f = up * fv;
+          const float up = was == -INFINITY ? 0.f : sm100::ex2_approx(was - x);
           m[n][e] = x;
           lim[n][e] = (x + 8.f) / qf[n][e];
-          mref[n][e] = (x == -INFINITY ? 0.f : x) - (float)(130 - min(ve, kMostVe));
-          l[n][e] *= up * fl;
+          mref[n][e] = (x == -INFINITY ? 0.f : x) + kDown;
+          l[n][e] *= up;
 #pragma unroll
           for (int r = 0; r < NG; ++r) {
-            z[n][r][e] *= f;
+            z[n][r][e] *= up;
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
-              o[n][r][k][e] *= f;
-              o[n][r][k][e + 2] *= f;
+              o[n][r][k][e] *= up;
+              o[n][r][k][e + 2] *= up;
             }
           }
         }
-    }
-    if (ve > kMostVe) {  // (a whole warp; exact, but for what is far below the largest scale)
-      const __nv_bfloat162 down = __float2bfloat162_rn(pow2(kMostVe - ve));
-#pragma unroll
-      for (int k = 0; k < BT; ++k)
-#pragma unroll
-        for (int r = 0; r < NG; ++r)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&vm[k][r][i]), down);
-            vm[k][r][i] = *reinterpret_cast<const uint32_t*>(&x);
-          }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -599,13 +582,23 @@ struct Q4Warp {
 #pragma unroll
       for (int r = 0; r < NG; ++r) {
         const uint8_t* blk = ks + (2 * k + 1) * L::kBytes;
-        const float s0 = bf16_lo_f(vm[k][r][0]), s1 = bf16_lo_f(vm[k][r][1]);
-        const float z0 = fmaf(8.f, s0, bf16_hi_f(vm[k][r][0])), z1 = fmaf(8.f, s1, bf16_hi_f(vm[k][r][1]));
-        uint32_t b[NT][2];
+        uint32_t vm[2];  // (scale, minimum) of this lane's tokens
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          vm[i] = *reinterpret_cast<const uint32_t*>(blk + L::kCodes + (r * kTok + tok + 8 * i) * 4);
+          if (MASKED && !((seen >> (2 * k + i)) & 1)) vm[i] = 0;  // unseen slots may hold anything, NaN too
+        }
+        const float s0 = bf16_lo_f(vm[0]), s1 = bf16_lo_f(vm[1]);
+        const float z0 = fmaf(8.f, s0, bf16_hi_f(vm[0])), z1 = fmaf(8.f, s1, bf16_hi_f(vm[1]));
+        uint32_t b[NT][2][2];  // [upper part, rest]
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          b[n][0] = transpose8x8(pack_f16(s[n][k][0] * s0, s[n][k][1] * s0));
-          b[n][1] = transpose8x8(pack_f16(s[n][k][2] * s1, s[n][k][3] * s1));
+          split_bf16(s[n][k][0] * s0, s[n][k][1] * s0, b[n][0][0], b[n][1][0]);
+          split_bf16(s[n][k][2] * s1, s[n][k][3] * s1, b[n][0][1], b[n][1][1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) b[n][i][e] = transpose8x8(b[n][i][e]);
           z[n][r][0] = fmaf(s[n][k][0], z0, fmaf(s[n][k][2], z1, z[n][r][0]));
           z[n][r][1] = fmaf(s[n][k][1], z0, fmaf(s[n][k][3], z1, z[n][r][1]));
         }
@@ -618,12 +611,12 @@ struct Q4Warp {
           if constexpr (WPL == 2) {
             const uint32_t x = *reinterpret_cast<const uint32_t*>(row + t * L::kRow);
             const uint32_t y = *reinterpret_cast<const uint32_t*>(row + u * L::kRow);
-            codes_f16<true>(__byte_perm(x, y, 0x5410), c[i][0], magic);
-            codes_f16<true>(__byte_perm(x, y, 0x7632), c[i][1], magic);
+            codes_bf16(__byte_perm(x, y, 0x5410), c[i][0], magic_bf16);
+            codes_bf16(__byte_perm(x, y, 0x7632), c[i][1], magic_bf16);
           } else {
-            codes_f16<true>(*reinterpret_cast<const uint16_t*>(row + t * L::kRow) |
-                                ((uint32_t)*reinterpret_cast<const uint16_t*>(row + u * L::kRow) << 16),
-                            c[i][0], magic);
+            codes_bf16(*reinterpret_cast<const uint16_t*>(row + t * L::kRow) |
+                           ((uint32_t)*reinterpret_cast<const uint16_t*>(row + u * L::kRow) << 16),
+                       c[i][0], magic_bf16);
           }
         }
 #pragma unroll
@@ -631,8 +624,10 @@ struct Q4Warp {
           const int w = i >> 1, j = 2 * (i & 1);
           const uint32_t a[4] = {c[0][w][j], c[0][w][j + 1], c[1][w][j], c[1][w][j + 1]};
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            mma_f16(o[n][r][i], a, b[n][0], b[n][1], o[n][r][i][0], o[n][r][i][1], o[n][r][i][2], o[n][r][i][3]);
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16(o[n][r][i], a, b[n][1][0], b[n][1][1]);
+            mma_bf16(o[n][r][i], a, b[n][0][0], b[n][0][1]);
+          }
         }
       }
   }
@@ -754,19 +749,18 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
     // the part's sums: over the quads for l and z, the outputs are whole in each lane (8 or 4 dimensions of two heads)
     const long long slot = me + row;
     const bool whole = p0 == 0 && p1 == n;
-    const float back = pow2(w.ve - 130), back_l = pow2(min(w.ve, kMostVe) - 130);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int head = nt * 8 + 2 * t + e;
-        float l = w.l[nt][e] * back_l;
+        float l = w.l[nt][e];
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
         const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int r = 0; r < W::NG; ++r) {
-          float z = w.z[nt][r][e] * back;
+          float z = w.z[nt][r][e];
 #pragma unroll
           for (int k = 4; k < 32; k <<= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
           if (head >= G) continue;
@@ -774,8 +768,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
           float x[W::MT * 2];
 #pragma unroll
           for (int k = 0; k < W::MT; ++k) {
-            x[2 * k] = fmaf(w.o[nt][r][k][e], back, z);
-            x[2 * k + 1] = fmaf(w.o[nt][r][k][e + 2], back, z);
+            x[2 * k] = w.o[nt][r][k][e] + z;
+            x[2 * k + 1] = w.o[nt][r][k][e + 2] + z;
           }
           if (whole) {
             __nv_bfloat16* dst = out + (row * G + head) * D + d;
@@ -790,7 +784,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
           }
         }
         if (g == 0 && head < G && (!whole || scores != nullptr))
-          *reinterpret_cast<float2*>(ml + (slot * G + head) * 2) = make_float2(w.m[nt][e], l);
+          *reinterpret_cast<float2*>(ml + (slot * G + head) * 2) = make_float2(w.m[nt][e] + kDown, l);
       }
     if (p0 == 0 && lane == 0) {  // the row's first slot and its parts, for q4_finish_kernel
       const int last = base + h * n + n - 1;

@@ -295,6 +295,63 @@ def test_decode_value_sizes(dev, size):
         assert ((w[b, 0, :lens[b]].cpu().to(F64) - p.sum(0).flatten()).abs() <= 2 ** -15 * p.sum(0).flatten()).all()
 
 
+@pytest.mark.parametrize("D,G", [(32, 3), (64, 4), (128, 1), (128, 11)])
+@pytest.mark.parametrize("lens", [[1, 5], [40, 700]])
+def test_decode_weights_keep_their_bits(dev, D, G, lens):
+    """Dimensions that are zero in every value, while their groups' scales are not, come out as zero: the minimum's part
+    and the codes' part cancel up to the weights' own rounding."""
+    ks, vs, pools, tables, n, _ = cache(lens, 1, D, dev)
+    q = torch.randn(len(lens), G, D).to(BF).to(dev)
+    for b, m in enumerate(lens):
+        v = torch.rand(m, 1, D).to(BF) + 1
+        v[..., ::5] = 0
+        pos = torch.arange(m)
+        paged_write_q4(ks[b].to(BF).to(dev), v.to(dev), *pools, tables[b][(pos // 16).to(dev)].contiguous(),
+                       (pos % 16).int().to(dev))
+        vs[b] = v
+    out = paged_decode_q4(q, *pools, tables, n, 1 / math.sqrt(D)).cpu().to(F64)
+    # a weight is held in two bf16 parts, 2^-16 of it; it multiplies 8 scales, a scale being 2 / 15 at most
+    # (bf16's rounding included: 0.14); the fp32 sums add 700 * 2^-24 of the same
+    assert out[..., ::5].abs().max() <= (2 ** -16 + 2 ** -14) * 8 * 0.14
+    assert (out[..., 1::5] > 0.9).all()
+
+
+@pytest.mark.parametrize("D,G", [(32, 2), (64, 4), (128, 9)])
+@pytest.mark.parametrize("ratio", [10, 20, 28, 60])
+def test_decode_values_far_apart(dev, ratio, D, G):
+    """Tokens whose values are 2^ratio times the others', but whose weight makes them count for nothing, take no bits
+    from the others."""
+    lens = [2000, 37]
+    ks, vs, pools, tables, n, _ = cache(lens, 1, D, dev)
+    q = torch.randn(2, G, D).to(BF)
+    q[..., 0] = 8
+    gap = (ratio + 12) * math.log(2) + 12  # in scores; the others lie within 4 of 0 or so
+    for b, m in enumerate(lens):
+        k, v = torch.randn(m, 1, D) * 0.3, torch.randn(m, 1, D)
+        far = torch.arange(m) % 29 == 20
+        k[far] *= 0.1
+        k[far, :, 0] = -gap
+        v[far] *= 2.0 ** ratio
+        pos = torch.arange(m)
+        paged_write_q4(k.to(BF).to(dev), v.to(BF).to(dev), *pools, tables[b][(pos // 16).to(dev)].contiguous(),
+                       (pos % 16).int().to(dev))
+        ks[b], vs[b] = stored(k.to(BF))[3], stored(v.to(BF))[3]
+    out = paged_decode_q4(q.to(dev), *pools, tables, n, 0.125).cpu().to(F64)
+    for b in range(2):
+        o, _, a = attention(q[b], ks[b], vs[b], 0.125, 0.0, 0)
+        near = torch.arange(lens[b]) % 29 != 20
+        # without the far tokens: theirs is 2^-12 of a value or less, which `a` holds
+        _, _, rest = attention(q[b], ks[b][near], vs[b][near], 0.125, 0.0, 0)
+        assert (a <= 2 * rest).all()
+        # check_decode's bound, on a measure without the 8 times 8 scales of a single fp16 weight
+        p = torch.softmax(torch.einsum("hd,td->ht", q[b].to(F64), ks[b][:, 0]) * 0.125, -1)
+        groups = vs[b][:, 0].unflatten(-1, (-1, min(D, 64)))
+        eight = ((groups.amax(-1) - groups.amin(-1)) * 8 / 15)[..., None].expand_as(groups).flatten(-2)
+        bound = torch.einsum("ht,td->hd", p, vs[b][:, 0].abs() + eight)
+        err = (out[b] - o).abs() - 2 ** -8 * o.abs()
+        assert (err <= 2 ** -14 * bound).all(), (err / bound).max()
+
+
 def test_decode_not_a_number(dev):
     """A key or a value that holds NaN: its head's output is NaN (with a NaN key its weights too), others are as ever."""
     lens, D = [50, 700], 64
