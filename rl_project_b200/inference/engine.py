@@ -332,8 +332,10 @@ class InferenceEngine:
 
     # ------------------------------------------------------------ decode
     def _evict(self, seqs: List[_Seq]) -> None:
-        """Cut the caches that have outgrown the budget (see the module's notes)."""
-        due = [s for s in seqs if s.cached >= self.kv_budget + max(KERNEL_BLOCK, self.kv_budget // 8)]
+        """Cut the caches that have outgrown the budget (see the module's notes).  A prompt's cache is left whole
+        until its first decode step has weighed the tokens: prefill accumulates nothing to rank them by."""
+        due = [s for s in seqs if s.cached >= self.kv_budget + max(KERNEL_BLOCK, self.kv_budget // 8)
+               and s.position > len(s.req.prompt_tokens)]
         plan = []
         for s in due:
             try:  # the token that the coming step adds has its place in the new blocks too

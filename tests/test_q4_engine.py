@@ -81,6 +81,38 @@ def test_evictions(dev):
     assert sorted(eng._free_rows) == [0, 1, 2, 3]
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_cuts_by_weights_that_exist(monkeypatch, dev):
+    """Every cut, a long prompt's first one too, follows the attention weights of the decode steps before it."""
+    from rl_project_b200.ops import paged_q4
+
+    cuts, evict = [], paged_q4.paged_evict_q4
+
+    def spy(k_pool, v_pool, tables, lens, new, weights, rows, keep, head_dim, recent=0, sink=0, status=None):
+        before = weights.clone()
+        kept, left = evict(k_pool, v_pool, tables, lens, new, weights, rows, keep, head_dim, recent, sink, status)
+        cuts.extend((before[int(r)].cpu(), int(n), kept[b].cpu()) for b, (r, n) in enumerate(zip(rows, lens)))
+        return kept, left
+
+    monkeypatch.setattr(paged_q4, "paged_evict_q4", spy)
+    m = model(dev)
+    eng = InferenceEngine(m, max_batch=2, kv_cache="q4", kv_budget=32, kv_sink=2, kv_recent=8)
+    reqs = [eng.submit(p, SamplingParams(max_tokens=40, **GREEDY)) for p in (list(range(3, 73)) * 2, PROMPTS[2])]
+    eng.step()
+    assert not cuts and eng.evictions == 0  # prefilled and decoded once
+    eng.step()
+    assert len(cuts) == 2 and cuts[0][1] == 141  # (two layers; the short prompt has not grown enough yet)
+    # one step of two query heads per KV head has weighed the prompt's tokens and its own
+    assert ((cuts[0][0].sum(-1) - 2).abs() < 1e-2).all() and (cuts[0][0][:, 140] > 0).all()
+    eng.run_until_idle()
+    assert all(len(r.generated_tokens) == 40 for r in reqs) and len(cuts) > 8
+    for row, n, kept in cuts:
+        assert (row.sum(-1) > 1).all()
+        for h in range(2):
+            free = sorted(range(2, n - 8), key=lambda t: (-float(row[h, t]), t))[:22]
+            assert kept[h].tolist() == sorted([0, 1] + free + list(range(n - 8, n)))
+
+
 def test_budget_never_reached_changes_nothing():
     m = model("cpu")
     params = SamplingParams(max_tokens=24, **GREEDY)
