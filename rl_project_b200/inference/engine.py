@@ -350,8 +350,16 @@ class InferenceEngine:
         lens, rows = (torch.tensor(x, dtype=torch.int32) for x in ([s.cached for s, _, _ in plan],
                                                                     [s.row for s, _, _ in plan]))
         dev = self.device
-        self.kv.evict(table.to(dev), lens.to(dev), new.to(dev), rows.to(dev), self.kv_budget, self.kv_recent,
-                      self.kv_sink)
+        try:
+            self.kv.evict(table.to(dev), lens.to(dev), new.to(dev), rows.to(dev), self.kv_budget, self.kv_recent,
+                          self.kv_sink)
+        except Exception as exc:  # noqa: BLE001 - some layers may be cut, others not: these sequences are lost
+            if dev.type == "cuda":
+                torch.cuda.current_stream(dev).synchronize()
+            for s, old, _ in plan:
+                self.allocator.release(old)
+                self._fail(s, exc)
+            return
         for s, old, _ in plan:
             self.allocator.release(old)  # (their next user's writes come behind the copies, on the same stream)
             s.evicted += s.cached - self.kv_budget
@@ -361,6 +369,9 @@ class InferenceEngine:
     def _decode(self, seqs: List[_Seq]) -> int:
         if self.kv_budget is not None:
             self._evict(seqs)
+            seqs = [s for s in seqs if s.req.id in self.states]
+            if not seqs:
+                return 0
         if self.decode_graphs and not self.profile:
             try:
                 done = self._decode_graph(seqs)

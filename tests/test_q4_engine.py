@@ -113,6 +113,26 @@ def test_cuts_by_weights_that_exist(monkeypatch, dev):
             assert kept[h].tolist() == sorted([0, 1] + free + list(range(n - 8, n)))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_failed_eviction(monkeypatch, dev):
+    """An eviction that raises fails the sequences that it was cutting, nobody else, and leaves no block behind."""
+    eng = InferenceEngine(model(dev), max_batch=4, kv_cache="q4", kv_budget=32, kv_sink=2, kv_recent=8)
+    evict = eng.kv.evict
+
+    def fails_once(*args):
+        monkeypatch.setattr(eng.kv, "evict", evict)
+        raise RuntimeError("no eviction today")
+
+    monkeypatch.setattr(eng.kv, "evict", fails_once)
+    long, short = (eng.submit(p, SamplingParams(max_tokens=60, **GREEDY)) for p in (PROMPTS[1], PROMPTS[0]))
+    eng.run_until_idle()
+    assert long.finish_reason == "error" and "no eviction today" in long.error and len(long.generated_tokens) == 2
+    assert len(short.generated_tokens) == 60 and short.finish_reason == "length" and eng.evictions > 0
+    assert eng.allocator.used_blocks == (1 if eng.decode_graphs else 0) and sorted(eng._free_rows) == [0, 1, 2, 3]
+    again = eng.generate(PROMPTS[1], SamplingParams(max_tokens=60, **GREEDY))
+    assert again.finish_reason == "length" and len(again.generated_tokens) == 60
+
+
 def test_budget_never_reached_changes_nothing():
     m = model("cpu")
     params = SamplingParams(max_tokens=24, **GREEDY)
