@@ -34,7 +34,9 @@ the dense 1B model, batch 64: 26.9k generated tokens/s against 13.5k eager, iden
 less to read per step.  ``kv_budget`` bounds it further: each decode step accumulates every cached token's attention
 weight, and a sequence whose cache has grown an eighth (at least a block) beyond the budget is cut back to it, per layer
 and KV head, keeping its first ``kv_sink`` and last ``kv_recent`` tokens and those with the most weight.  Prompts
-longer than the budget are read whole and cut after their first decode step.
+longer than the budget are read whole and cut after their first decode step.  A cut copies to fresh blocks: as many as one
+sequence of the budget takes are kept free for it (on top of the default ``max_blocks``, within a given one), and a
+sequence beyond its budget that finds no block for its next token is cut at once.
 
 ``SamplingParams.logprobs`` records each generated token's log-prob and its most likely alternatives.
 """
@@ -92,11 +94,13 @@ class InferenceEngine:
         self.model = model.eval()
         self.device = device or next(model.parameters()).device
         self.max_seq_len = min(max_seq_len or model.spec.block_size, model.spec.block_size)
-        max_blocks = max_blocks or max_batch * ((self.max_seq_len + block_size - 1) // block_size + 1)
+        # what a cut copies to (none is made of a budget that no sequence can outgrow)
+        reserve = 0 if kv_budget is None else -(-(min(kv_budget, self.max_seq_len) + 1) // block_size)
+        max_blocks = max_blocks or max_batch * ((self.max_seq_len + block_size - 1) // block_size + 1) + reserve
         self.paged = bool(getattr(model, "supports_paged_decode", lambda: False)())
         if self.paged and block_size != KERNEL_BLOCK:
             raise ServingError(f"paged decoding uses {KERNEL_BLOCK}-token blocks (got block_size={block_size})")
-        self.allocator = PagedBlockAllocator(block_size=block_size, max_blocks=max_blocks)
+        self.allocator = PagedBlockAllocator(block_size=block_size, max_blocks=max_blocks, reserve=reserve)
         self.scheduler = Scheduler(self.allocator, max_batch=max_batch, max_seq_len=self.max_seq_len)
         self.kv: Optional[PagedKVCache] = None
         if kv_recent is None:
@@ -331,19 +335,38 @@ class InferenceEngine:
         p["steps"] = p.get("steps", 0.0) + 1
 
     # ------------------------------------------------------------ decode
+    def _can_cut(self, s: _Seq) -> bool:
+        """A prompt's cache is left whole until its first decode step has weighed the tokens: prefill accumulates
+        nothing to rank them by."""
+        return self.kv_budget is not None and s.cached > self.kv_budget and s.position > len(s.req.prompt_tokens)
+
+    def _has_slot(self, s: _Seq) -> bool:
+        return self.allocator.lengths[s.req.id] > s.cached
+
     def _evict(self, seqs: List[_Seq]) -> None:
-        """Cut the caches that have outgrown the budget (see the module's notes).  A prompt's cache is left whole
-        until its first decode step has weighed the tokens: prefill accumulates nothing to rank them by."""
-        due = [s for s in seqs if s.cached >= self.kv_budget + max(KERNEL_BLOCK, self.kv_budget // 8)
-               and s.position > len(s.req.prompt_tokens)]
-        plan = []
-        for s in due:
-            try:  # the token that the coming step adds has its place in the new blocks too
-                plan.append((s, *self.allocator.replace(s.req.id, self.kv_budget + 1)))
-            except OutOfBlocksError:  # no room to copy to now: the cache keeps growing until there is
-                continue
-        if not plan:
-            return
+        """Cut the caches that have outgrown the budget (see the module's notes), as many at a time as there are blocks
+        to copy to; each group's old blocks are free for the next one."""
+        most = self.kv_budget + max(KERNEL_BLOCK, self.kv_budget // 8)
+        due = [s for s in seqs if self._can_cut(s) and (s.cached >= most or not self._has_slot(s))]
+        due.sort(key=self._has_slot)  # first who cannot go on without
+        while due:
+            plan = []
+            for s in due:
+                try:  # the token that the coming step adds has its place in the new blocks too
+                    plan.append((s, *self.allocator.replace(s.req.id, self.kv_budget + 1)))
+                except OutOfBlocksError:
+                    break
+            if plan:
+                due = due[len(plan):]
+                self._cut(plan)
+            elif self._has_slot(due[0]):  # (what earlier cuts left is shared with others) the caches grow on
+                return
+            else:
+                s = due.pop(0)
+                self._fail(s, OutOfBlocksError(f"sequence {s.req.id}: no blocks to cut its cache into"))
+
+    def _cut(self, plan: List[Tuple[_Seq, List[int], List[int]]]) -> None:
+        """Move what the budget keeps of each sequence from its old blocks to its new ones."""
         width, new_width = max(len(old) for _, old, _ in plan), max(len(new) for _, _, new in plan)
         table = torch.tensor([old + [0] * (width - len(old)) for _, old, _ in plan], dtype=torch.int32)
         new = torch.tensor([new + [0] * (new_width - len(new)) for _, _, new in plan], dtype=torch.int32)
@@ -684,7 +707,8 @@ class InferenceEngine:
                 if cow is not None and self.kv is not None:
                     self.kv.copy_block(*cow)
             except OutOfBlocksError as exc:
-                self._fail(st, exc)
+                if not self._can_cut(st):  # (a cut before the next step gives this one its slot)
+                    self._fail(st, exc)
         return 1
 
     # ------------------------------------------------------------ retirement

@@ -15,7 +15,8 @@ optionally with accumulators of the cached tokens' attention weights, by which t
 reference counts: ``share_prefix`` lets a new sequence reuse the blocks of a
 running one that has the same prompt (the G samples of one GRPO prompt are
 prefilled once), and ``append_token`` copies a shared, partly filled last
-block before the sequence writes into it (copy-on-write).
+block before the sequence writes into it (copy-on-write).  ``reserve`` blocks are
+kept for ``replace`` alone, so that a cache can be cut when the pool is full.
 """
 
 from __future__ import annotations
@@ -34,10 +35,13 @@ class OutOfBlocksError(ServingError):
 
 
 class PagedBlockAllocator:
-    def __init__(self, block_size: int = 16, max_blocks: int = 1024):
+    def __init__(self, block_size: int = 16, max_blocks: int = 1024, reserve: int = 0):
         if block_size < 1 or max_blocks < 1:
             raise ServingError("block_size and max_blocks must be >= 1")
+        if not 0 <= reserve < max_blocks:
+            raise ServingError("reserve must leave blocks to allocate")
         self.block_size = block_size
+        self.reserve = reserve
         self.max_blocks = max_blocks
         self.free_blocks: List[int] = list(range(max_blocks - 1, -1, -1))  # pop() hands out 0, 1, 2, ...
         self.tables: Dict[str, List[int]] = {}
@@ -49,9 +53,14 @@ class PagedBlockAllocator:
     def blocks_needed(self, n_tokens: int) -> int:
         return (n_tokens + self.block_size - 1) // self.block_size
 
+    @property
+    def available(self) -> int:
+        """Free blocks that are not kept for ``replace``."""
+        return max(0, len(self.free_blocks) - self.reserve)
+
     def can_allocate(self, seq_id: str, n_tokens: int) -> bool:
         have = len(self.tables.get(seq_id, []))
-        return self.blocks_needed(n_tokens) - have <= len(self.free_blocks)
+        return self.blocks_needed(n_tokens) - have <= self.available
 
     def _take(self) -> int:
         b = self.free_blocks.pop()
@@ -67,8 +76,8 @@ class PagedBlockAllocator:
         """Ensure ``seq_id`` owns enough blocks for ``n_tokens``; returns its block table."""
         table = self.tables.setdefault(seq_id, [])
         need = self.blocks_needed(n_tokens) - len(table)
-        if need > len(self.free_blocks):
-            raise OutOfBlocksError(f"sequence {seq_id} needs {need} more blocks, {len(self.free_blocks)} free")
+        if need > 0 and need > self.available:
+            raise OutOfBlocksError(f"sequence {seq_id} needs {need} more blocks, {self.available} free")
         for _ in range(max(need, 0)):
             table.append(self._take())
         self.lengths[seq_id] = n_tokens
@@ -83,7 +92,7 @@ class PagedBlockAllocator:
         n = self.lengths.get(seq_id, 0)
         table = self.tables.setdefault(seq_id, [])
         if n % self.block_size != 0 and table and self.refs[table[-1]] > 1:
-            if not self.free_blocks:
+            if not self.available:
                 raise OutOfBlocksError(f"sequence {seq_id} needs a copy-on-write block, none free")
             src = table[-1]
             dst = self._take()
@@ -113,8 +122,8 @@ class PagedBlockAllocator:
         return self.tables[child_id]
 
     def replace(self, seq_id: str, n_tokens: int) -> Tuple[List[int], List[int]]:
-        """Give ``seq_id`` fresh blocks for ``n_tokens`` and return ``(old, new)`` tables.  The old blocks stay
-        referenced until the caller, done copying from them, passes them to ``release``."""
+        """Give ``seq_id`` fresh blocks for ``n_tokens``, reserved ones too, and return ``(old, new)`` tables.  The old
+        blocks stay referenced until the caller, done copying from them, passes them to ``release``."""
         need = self.blocks_needed(n_tokens)
         if need > len(self.free_blocks):
             raise OutOfBlocksError(f"sequence {seq_id} needs {need} fresh blocks, {len(self.free_blocks)} free")

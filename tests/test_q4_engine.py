@@ -133,6 +133,45 @@ def test_failed_eviction(monkeypatch, dev):
     assert again.finish_reason == "length" and len(again.generated_tokens) == 60
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("blocks", [15, 16, 19])
+@pytest.mark.parametrize("same", [False, True])
+def test_cuts_in_a_full_pool(dev, blocks, same):
+    """Four sequences due in one step, in pools that hold them at their budget and one cut's copy, and little or nothing
+    more: nobody fails for want of a block."""
+    eng = InferenceEngine(model(dev), max_batch=4, kv_cache="q4", kv_budget=32, kv_sink=2, kv_recent=8,
+                          max_blocks=blocks + (dev == "cuda"))  # (and the padding block)
+    assert eng.allocator.reserve == 3 and eng.kv.num_blocks == blocks + (dev == "cuda")
+    prompts = [[3 + i * (not same), 4, 5, 6] for i in range(4)]
+    reqs = eng.generate_batch(prompts, SamplingParams(max_tokens=120, **GREEDY))
+    assert [r.finish_reason for r in reqs] == ["length"] * 4 and all(len(r.generated_tokens) == 120 for r in reqs)
+    assert eng.evictions >= 4 * 4 and eng.allocator.used_blocks == (1 if eng.decode_graphs else 0)
+
+
+def test_blocks_kept_for_cuts():
+    from rl_project_b200.inference import OutOfBlocksError, PagedBlockAllocator
+
+    a = PagedBlockAllocator(block_size=4, max_blocks=6, reserve=2)
+    a.allocate("a", 8)
+    assert a.available == 2 and a.can_allocate("b", 8) and not a.can_allocate("b", 9)
+    a.allocate("b", 8)
+    with pytest.raises(OutOfBlocksError):
+        a.append_token("a")
+    assert a.lengths["a"] == 8
+    old, new = a.replace("a", 5)
+    assert not set(old) & set(new) and a.available == 0 and len(a.free_blocks) == 0
+    a.release(old)
+    assert a.available == 0 and len(a.free_blocks) == 2
+    a.append_token("a")  # (its block has room)
+    a.free("b")
+    assert a.available == 2
+    for bad in (6, -1):
+        with pytest.raises(ServingError):
+            PagedBlockAllocator(block_size=4, max_blocks=6, reserve=bad)
+    with pytest.raises(ServingError):  # no block but the reserved ones
+        InferenceEngine(model("cpu"), max_batch=1, kv_cache="q4", kv_budget=32, max_blocks=3)
+
+
 def test_budget_never_reached_changes_nothing():
     m = model("cpu")
     params = SamplingParams(max_tokens=24, **GREEDY)
