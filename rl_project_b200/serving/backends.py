@@ -127,18 +127,20 @@ class EngineBackend(_Toggle):
             text, finish = text[:cut], "stop"
         return CompletionResult(text=text, prompt_tokens=len(req.prompt_tokens), completion_tokens=len(tokens),
                                 finish_reason=finish or req.finish_reason or "length", backend=self.name,
-                                request_id=req.id, logprobs=self._token_logprobs(req, tokens, len(text)))
+                                request_id=req.id, logprobs=self._token_logprobs(req, tokens, text, cut is not None))
 
-    def _token_logprobs(self, req: GenerationRequest, tokens: List[int], end: int) -> Optional[List[TokenLogprob]]:
-        """The recorded log-probs of the tokens that begin within the first ``end`` characters of the text."""
+    def _token_logprobs(self, req: GenerationRequest, tokens: List[int], text: str,
+                        cut: bool) -> Optional[List[TokenLogprob]]:
+        """The recorded log-probs: one entry for every token, also where it adds no character of its own (a part of
+        one, an end mark); of a text that was ``cut`` at a stop string, for the tokens that begin within it."""
         if req.params.logprobs is None:
             return None
         decode, out = self.tokenizer.decode, []
         for i, lp in enumerate(req.token_logprobs[:len(tokens)]):
             offset = len(decode(tokens[:i]))
-            if offset >= end:
+            if cut and offset >= len(text):
                 break
-            out.append(TokenLogprob(decode([tokens[i]]), offset, lp,
+            out.append(TokenLogprob(decode([tokens[i]]), min(offset, len(text)), lp,
                                     [(decode([t]), x) for t, x in req.top_logprobs[i]]))
         return out
 

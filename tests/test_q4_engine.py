@@ -285,6 +285,56 @@ def test_served_logprobs():
         assert router.handle("POST", "/v1/completions", {"prompt": "abc", **bad})[0] == 400
 
 
+class Scripted:
+    """An engine that answers every prompt with given tokens (all as likely as each other) and counts nothing else."""
+
+    eos_token_id = None
+
+    def __init__(self, tokens):
+        self.tokens = tokens
+
+    def submit(self, ids, params, **kw):
+        from rl_project_b200.inference import GenerationRequest
+
+        self.req = GenerationRequest(prompt_tokens=list(ids), params=params, **kw)
+        self.req.start()
+        for t in self.tokens:
+            self.req.push_token(t, -1.0, [(t, -1.0)])
+        self.req.finish("stop")
+        return self.req
+
+    def cancel(self, request_id):
+        return True
+
+
+def said_by(tokens, tokenizer, stop=()):
+    from rl_project_b200.serving import EngineBackend
+
+    return EngineBackend("m", Scripted(tokens), tokenizer, background=False).complete("x", SamplingParams(logprobs=1),
+                                                                                     stop=stop)
+
+
+def test_served_logprobs_of_every_token():
+    """Bytes of one character and end marks that print nothing have their entries too."""
+    from rl_project_b200.data.tokenizers import ByteTokenizer
+
+    class WithEnd(ByteTokenizer):
+        def decode(self, ids):
+            return super().decode([i for i in ids if i != 0])
+
+    for text in ("ab\U0001f600", "a\u00e9", "\u00e9b\U0001f600\U0001f600c"):
+        for end in ([], [0], [0, 0]):
+            ids = list(text.encode()) + end
+            res = said_by(ids, WithEnd())
+            assert res.text == text and res.completion_tokens == len(res.logprobs) == len(ids)
+            offsets = [t.offset for t in res.logprobs]
+            assert offsets == sorted(offsets) and all(0 <= o <= len(text) for o in offsets)
+    assert len(said_by([0], WithEnd()).logprobs) == 1 and said_by([0], WithEnd()).text == ""
+    res = said_by(list(b"abXcd"), WithEnd(), stop=("X",))  # cut at a stop string: what was cut off says nothing
+    assert res.text == "ab" and [t.text for t in res.logprobs] == ["a", "b"]
+    assert said_by(list(b"Xcd"), WithEnd(), stop=("X",)).logprobs == []
+
+
 def test_impossible_tokens_stay_within_json():
     import json
 
