@@ -11,7 +11,7 @@ test double (prompt reversed, cut to ``max_tokens`` characters), as in
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Any, Dict, Iterator, List, Optional, Protocol, Sequence
+from typing import Any, Callable, Dict, Iterator, List, Optional, Protocol, Sequence
 
 from rl_project_b200.core.errors import BackendUnavailableError, ServingError
 from rl_project_b200.inference.requests import GenerationRequest, SamplingParams
@@ -72,6 +72,25 @@ def _stop_prefix_len(text: str, stop: Sequence[str]) -> int:
                 best = k
                 break
     return best
+
+
+def _token_offsets(decode: Callable[[Sequence[int]], str], tokens: Sequence[int]) -> List[int]:
+    """Where each token's text begins in the decoded text (the parts of a character: where it begins), in time linear in
+    the tokens: each chunk of whole characters is decoded behind the chunk before it, as tokenizers treat a text's first
+    token in a way of its own."""
+    offsets, at, start, done = [], 0, 0, 0  # tokens [start, done) are the chunk before, [done, i] the open one
+    before = ""
+    for i in range(len(tokens)):
+        offsets.append(at)
+        text = decode(tokens[start:i + 1])
+        if text.endswith("\ufffd") and i + 1 - done < 4:  # (no character has more than four parts)
+            continue
+        at += max(0, len(text) - len(before))
+        if len(text) > len(before) or i + 1 - start >= 16:  # (what prints nothing joins the chunk before)
+            start = done
+        done = i + 1
+        before = decode(tokens[start:done])
+    return offsets
 
 
 class EngineBackend(_Toggle):
@@ -136,8 +155,8 @@ class EngineBackend(_Toggle):
         if req.params.logprobs is None:
             return None
         decode, out = self.tokenizer.decode, []
-        for i, lp in enumerate(req.token_logprobs[:len(tokens)]):
-            offset = len(decode(tokens[:i]))
+        said = zip(_token_offsets(decode, tokens), req.token_logprobs)
+        for i, (offset, lp) in enumerate(said):
             if cut and offset >= len(text):
                 break
             out.append(TokenLogprob(decode([tokens[i]]), min(offset, len(text)), lp,

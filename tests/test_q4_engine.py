@@ -335,6 +335,39 @@ def test_served_logprobs_of_every_token():
     assert said_by(list(b"Xcd"), WithEnd(), stop=("X",)).logprobs == []
 
 
+def test_offsets_in_linear_time():
+    """A long answer's offsets, as its whole prefixes give them, from a number of decoded tokens in proportion to it."""
+    from rl_project_b200.data.tokenizers import ByteTokenizer
+
+    class Words:
+        """Words with a leading space that the text's first word loses, as of some subword tokenizers; id 0 prints
+        nothing."""
+
+        seen = 0
+
+        def encode(self, text):
+            return [1]
+
+        def decode(self, ids):
+            Words.seen += len(ids)
+            return "".join("" if i == 0 else " " + "w" * (int(i) % 5 + 1) for i in ids).removeprefix(" ")
+
+    for end in (0, 30):
+        ids = [(7 * i * i + i) % 23 for i in range(2000)] + [0] * end
+        Words.seen = 0
+        res = said_by(ids, Words())
+        assert Words.seen <= 40 * len(ids)
+        w = Words()
+        assert [t.offset for t in res.logprobs] == [len(w.decode(ids[:i])) for i in range(len(ids))]
+    text = "na\u00efve \U0001f600\u20ac " * 40
+    res = said_by(list(text.encode()), ByteTokenizer())
+    starts = [n for n, c in enumerate(text) for _ in c.encode()]
+    assert [t.offset for t in res.logprobs] == starts and res.text == text
+    broken = [0xff, 0x61, 0xf0, 0x9f, 0x98, 0x62] + [0xf0] * 9  # bytes that are no character: some offset, in order
+    offsets = [t.offset for t in said_by(broken, ByteTokenizer()).logprobs]
+    assert len(offsets) == len(broken) and offsets == sorted(offsets)
+
+
 def test_impossible_tokens_stay_within_json():
     import json
 
