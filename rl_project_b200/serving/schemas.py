@@ -144,12 +144,20 @@ def _usage(prompt_tokens: int, completion_tokens: int) -> Dict[str, int]:
             "total_tokens": prompt_tokens + completion_tokens}
 
 
+def _by_text(top: List[Tuple[str, float]]) -> Dict[str, float]:
+    """Alternatives, in falling order, by their text: of those that print alike, the likeliest."""
+    out: Dict[str, float] = {}
+    for text, lp in top:
+        out.setdefault(text, lp)
+    return out
+
+
 def completion_response(request_id: str, model: str, text: str, prompt_tokens: int, completion_tokens: int,
                         finish_reason: str, backend: Optional[str] = None,
                         logprobs: Optional[List[TokenLogprob]] = None) -> Dict[str, Any]:
     said = None if logprobs is None else {
         "tokens": [t.text for t in logprobs], "token_logprobs": [t.logprob for t in logprobs],
-        "top_logprobs": [dict(t.top) for t in logprobs], "text_offset": [t.offset for t in logprobs]}
+        "top_logprobs": [_by_text(t.top) for t in logprobs], "text_offset": [t.offset for t in logprobs]}
     out: Dict[str, Any] = {"id": f"cmpl-{request_id}", "object": "text_completion", "created": int(time.time()),
                            "model": model,
                            "choices": [{"text": text, "index": 0, "finish_reason": finish_reason, "logprobs": said}],

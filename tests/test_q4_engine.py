@@ -368,6 +368,18 @@ def test_offsets_in_linear_time():
     assert len(offsets) == len(broken) and offsets == sorted(offsets)
 
 
+def test_alternatives_that_print_alike():
+    """The completions answer names alternatives by their text: the likeliest of equal texts stays."""
+    from rl_project_b200.serving.schemas import TokenLogprob, chat_response, completion_response
+
+    top = [("\ufffd", -0.1), ("\ufffd", -3.0), ("b", -4.0)]
+    said = [TokenLogprob("a", 0, -0.5, top)]
+    out = completion_response("r", "m", "a", 1, 1, "length", logprobs=said)["choices"][0]["logprobs"]
+    assert [list(t.items()) for t in out["top_logprobs"]] == [[("\ufffd", -0.1), ("b", -4.0)]]
+    out = chat_response("r", "m", "a", 1, 1, "length", logprobs=said)["choices"][0]["logprobs"]["content"][0]
+    assert [(e["token"], e["logprob"]) for e in out["top_logprobs"]] == top
+
+
 def test_impossible_tokens_stay_within_json():
     import json
 
