@@ -9,6 +9,7 @@ validation errors raise ``ServingError`` (HTTP 400 at the router).
 
 from __future__ import annotations
 
+import math
 import time
 import uuid
 from dataclasses import dataclass, field
@@ -51,7 +52,12 @@ def _common(d: Dict[str, Any]) -> Dict[str, Any]:
         raise ServingError(f"invalid numeric field: {exc}") from exc
 
 
-_LEAST = -9999.0  # stands for the log-prob of a token that cannot occur
+_LEAST = -9999.0  # stands for the log-prob of a token that cannot occur, and for one that is not a number
+
+
+def _said(lp: float) -> float:
+    """A log-prob as JSON can hold it."""
+    return max(lp, _LEAST) if lp < math.inf else _LEAST
 
 
 @dataclass
@@ -63,9 +69,9 @@ class TokenLogprob:
     logprob: float
     top: List[Tuple[str, float]]
 
-    def __post_init__(self) -> None:  # -inf has no place in JSON
-        self.logprob = max(self.logprob, _LEAST)
-        self.top = [(text, max(lp, _LEAST)) for text, lp in self.top]
+    def __post_init__(self) -> None:
+        self.logprob = _said(self.logprob)
+        self.top = [(text, _said(lp)) for text, lp in self.top]
 
 
 @dataclass

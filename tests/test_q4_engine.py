@@ -391,6 +391,17 @@ def test_impossible_tokens_stay_within_json():
     assert said[0].top == [("b", -9999.0)] and said[1].logprob == -9999.0 and said[0].logprob == -0.5
 
 
+def test_no_number_stays_within_json():
+    import json
+
+    from rl_project_b200.serving.schemas import TokenLogprob, chat_response, completion_response
+
+    said = [TokenLogprob("a", 0, math.nan, [("b", math.nan), ("c", math.inf), ("d", -math.inf), ("e", -0.25)])]
+    for make in (chat_response, completion_response):
+        json.dumps(make("r", "m", "a", 1, 1, "length", logprobs=said), allow_nan=False)
+    assert said[0].logprob == -9999.0 and [x for _, x in said[0].top] == [-9999.0] * 3 + [-0.25]
+
+
 def test_sink_fills_the_budget():
     """What the first tokens leave of the budget bounds the default share of the last ones."""
     m = model("cpu")
