@@ -71,6 +71,9 @@ class RolloutEngine:
         if self._engine is None:
             model = self._paged_model()
             if model is None:
+                if self.cfg.engine_kv_cache != "bf16":
+                    raise RolloutError(f"engine_kv_cache={self.cfg.engine_kv_cache!r} needs the paged engine "
+                                       "(engine='paged', or 'auto' with a model on CUDA)")
                 return None
             from rl_project_b200.inference.engine import InferenceEngine
 

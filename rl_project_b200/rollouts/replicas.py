@@ -32,7 +32,8 @@ from rl_project_b200.core.errors import DistributedConfigError
 
 class RolloutReplicas:
     def __init__(self, spec: ModelSpec, tp_size: int, device: torch.device, dtype: torch.dtype = torch.bfloat16, *,
-                 max_batch: int = 256, max_blocks: Optional[int] = None, timeout_s: Optional[float] = None):
+                 max_batch: int = 256, max_blocks: Optional[int] = None, timeout_s: Optional[float] = None,
+                 kv_cache: str = "bf16"):
         from rl_project_b200.inference.engine import InferenceEngine
         from rl_project_b200.models.transformer.model import TransformerLM
         from rl_project_b200.parallel.tensor_parallel import apply_tensor_parallel
@@ -64,7 +65,7 @@ class RolloutReplicas:
         self._params = dict(model.named_parameters())
         per_seq = (spec.block_size + 15) // 16 + 1
         self.engine = InferenceEngine(model, max_batch=max_batch, max_blocks=max_blocks or max_batch * per_seq,
-                                      decode_graphs=False)
+                                      decode_graphs=False, kv_cache=kv_cache)
 
     # ------------------------------------------------------------ weights
     @torch.no_grad()

@@ -162,7 +162,8 @@ class GRPOAlgorithm(PostTrainingAlgorithm):
             dt = next(self.policy.model.parameters()).dtype
             self._replica_set = RolloutReplicas(self.policy.spec, rc.replica_tp, self.policy.device,
                                                 dt if dt in (torch.bfloat16, torch.float16) else torch.float32,
-                                                max_batch=rc.engine_max_batch, max_blocks=rc.engine_kv_blocks)
+                                                max_batch=rc.engine_max_batch, max_blocks=rc.engine_kv_blocks,
+                                                kv_cache=rc.engine_kv_cache)
         rep = self._replica_set
         if self._strategy is not None and getattr(self._strategy, "units", None):
             rep.sync_from_fsdp(self._strategy)

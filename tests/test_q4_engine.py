@@ -443,6 +443,47 @@ def test_refusals():
         SamplingParams(logprobs=21).validate()
 
 
+def test_rollouts_hold_their_cache_as_configured(monkeypatch):
+    """engine_kv_cache reaches the engine of every rollout path, or is refused."""
+    from types import SimpleNamespace
+
+    import torch.distributed as dist
+
+    from rl_project_b200.core.errors import RolloutError
+    from rl_project_b200.parallel.runtime import free_port
+    from rl_project_b200.rollouts import replicas
+    from rl_project_b200.rollouts.engine import RolloutConfig, RolloutEngine
+    from rl_project_b200.training.grpo import GRPOAlgorithm
+
+    m = model("cpu")
+    policy = SimpleNamespace(model=m, spec=m.spec, device=torch.device("cpu"))
+    cfg = RolloutConfig(engine="paged", engine_kv_cache="q4", engine_max_batch=4, replica_tp=1)
+    assert isinstance(RolloutEngine(policy, cfg).inference_engine().kv, PagedQ4KVCache)
+    for name in ("generate", "auto"):  # no paged engine: on the CPU "auto" takes generate()
+        other = RolloutConfig(engine=name, engine_kv_cache="q4")
+        with pytest.raises(RolloutError):
+            RolloutEngine(policy, other).inference_engine()
+        assert RolloutEngine(policy, RolloutConfig(engine=name)).inference_engine() is None
+
+    built = []
+
+    class Replicas(replicas.RolloutReplicas):
+        def __init__(self, *args, **kw):
+            super().__init__(*args, **kw)
+            built.append(self.engine.kv)
+            raise StopIteration
+
+    monkeypatch.setattr(replicas, "RolloutReplicas", Replicas)
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{free_port()}", rank=0, world_size=1)
+    try:
+        with pytest.raises(StopIteration):
+            GRPOAlgorithm._collect_replicated(SimpleNamespace(rollouts=RolloutEngine(policy, cfg), policy=policy,
+                                                     _replica_set=None), 0)
+    finally:
+        dist.destroy_process_group()
+    assert isinstance(built[0], PagedQ4KVCache)
+
+
 def test_packed_scoring_through_logits():
     """The scoring path of policies that have logits only: values and gradients as from a plain log-softmax."""
     from types import SimpleNamespace
