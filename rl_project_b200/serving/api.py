@@ -14,14 +14,13 @@ import json
 import threading
 import time
 from collections import deque
-from dataclasses import replace
 from typing import Any, Callable, Dict, Iterator, Optional, Tuple, Union
 
 from rl_project_b200.core.errors import BackendUnavailableError, ServingError
 from rl_project_b200.observability.events import Event
 from rl_project_b200.observability.logging import get_logger
 from rl_project_b200.observability.metrics import MetricsSink, NoOpMetricsSink
-from rl_project_b200.serving.backends import Backend
+from rl_project_b200.serving.backends import Backend, StreamPiece
 from rl_project_b200.serving.schemas import (ChatCompletionRequest, CompletionRequest, chat_chunk, chat_response,
                                              completion_chunk, completion_response, error_response, new_request_id)
 
@@ -111,10 +110,13 @@ class Router:
         with self._lock:
             self.requests_total += 1
         t0 = time.perf_counter()
+        params = req.sampling()
         if req.stream:
-            pieces = backend.stream(prompt, replace(req.sampling(), logprobs=None), rid, stop=req.stop)
-            return 200, self._sse(pieces, lambda t, fr: chunk(rid, name, t, fr), t0, name)
-        res = backend.complete(prompt, req.sampling(), rid, stop=req.stop)
+            if params.logprobs is not None:
+                params.validate()  # (a stream begins before the engine looks)
+            pieces = backend.stream(prompt, params, rid, stop=req.stop)
+            return 200, self._sse(pieces, lambda t, fr, **kw: chunk(rid, name, t, fr, **kw), t0, name)
+        res = backend.complete(prompt, params, rid, stop=req.stop)
         self._record(t0, res.completion_tokens, name)
         return 200, respond(rid, name, res.text, res.prompt_tokens, res.completion_tokens, res.finish_reason, name,
                             logprobs=getattr(res, "logprobs", None))
@@ -127,11 +129,12 @@ class Router:
         req = ChatCompletionRequest.from_dict(body)
         return self._serve(req, req.to_prompt(), chat_response, chat_chunk)
 
-    def _sse(self, pieces: Iterator[str], make, t0: float, backend: str) -> Iterator[str]:
+    def _sse(self, pieces: Iterator[Union[str, StreamPiece]], make, t0: float, backend: str) -> Iterator[str]:
         n = 0
-        for text in pieces:
+        for piece in pieces:
             n += 1
-            yield f"data: {json.dumps(make(text, None))}\n\n"
+            out = make(piece, None) if isinstance(piece, str) else make(piece.text, None, logprobs=piece.logprobs)
+            yield f"data: {json.dumps(out)}\n\n"
         yield f"data: {json.dumps(make('', 'stop'))}\n\n"
         yield "data: [DONE]\n\n"
         self._record(t0, n, backend)

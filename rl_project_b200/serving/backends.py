@@ -10,8 +10,9 @@ test double (prompt reversed, cut to ``max_tokens`` characters), as in
 
 from __future__ import annotations
 
+from collections import deque
 from dataclasses import dataclass
-from typing import Any, Callable, Dict, Iterator, List, Optional, Protocol, Sequence
+from typing import Any, Callable, Dict, Iterator, List, Optional, Protocol, Sequence, Union
 
 from rl_project_b200.core.errors import BackendUnavailableError, ServingError
 from rl_project_b200.inference.requests import GenerationRequest, SamplingParams
@@ -29,6 +30,14 @@ class CompletionResult:
     logprobs: Optional[List[TokenLogprob]] = None  # with SamplingParams.logprobs
 
 
+@dataclass
+class StreamPiece:
+    """A piece of a streamed answer with SamplingParams.logprobs: its text and the tokens that begin in it."""
+
+    text: str
+    logprobs: List[TokenLogprob]
+
+
 class Backend(Protocol):
     name: str
 
@@ -36,7 +45,7 @@ class Backend(Protocol):
                  stop: Sequence[str] = ()) -> CompletionResult: ...
 
     def stream(self, prompt: str, params: SamplingParams, request_id: Optional[str] = None,
-               stop: Sequence[str] = ()) -> Iterator[str]: ...
+               stop: Sequence[str] = ()) -> Iterator[Union[str, StreamPiece]]: ...
 
     def healthy(self) -> bool: ...
 
@@ -159,16 +168,31 @@ class EngineBackend(_Toggle):
         for i, (offset, lp) in enumerate(said):
             if cut and offset >= len(text):
                 break
-            out.append(TokenLogprob(decode([tokens[i]]), min(offset, len(text)), lp,
-                                    [(decode([t]), x) for t, x in req.top_logprobs[i]]))
+            out.append(self._said(req, i, tokens[i], min(offset, len(text)), lp))
         return out
 
+    def _said(self, req: GenerationRequest, i: int, token: int, offset: int, lp: float) -> TokenLogprob:
+        decode = self.tokenizer.decode
+        return TokenLogprob(decode([token]), offset, lp, [(decode([t]), x) for t, x in req.top_logprobs[i]])
+
     def stream(self, prompt: str, params: SamplingParams, request_id: Optional[str] = None,
-               stop: Sequence[str] = ()) -> Iterator[str]:
+               stop: Sequence[str] = ()) -> Iterator[Union[str, StreamPiece]]:
         req = self._submit(prompt, params, request_id)
         pending: List[int] = []
         buf = ""  # decoded text not yet yielded (may hold the start of a stop string)
-        for tok in self._tokens(req):
+        sent = 0  # characters yielded
+        said: deque[TokenLogprob] = deque()  # tokens whose place in the text has not been yielded
+
+        def piece(text: str, whole: bool = False) -> Union[str, StreamPiece]:
+            nonlocal sent
+            sent += len(text)
+            if params.logprobs is None:
+                return text
+            return StreamPiece(text, [said.popleft() for t in list(said) if whole or t.offset < sent])
+
+        for i, tok in enumerate(self._tokens(req)):
+            if params.logprobs is not None:
+                said.append(self._said(req, i, tok, sent + len(buf), req.token_logprobs[i]))
             pending.append(tok)
             text = self.tokenizer.decode(pending)
             if not text or "\ufffd" in text:  # wait until the bytes decode to whole characters
@@ -179,18 +203,18 @@ class EngineBackend(_Toggle):
                 cut = _cut_at_stop(buf, stop)
                 if cut is not None:
                     if cut:
-                        yield buf[:cut]
+                        yield piece(buf[:cut])
                     self.engine.cancel(req.id)
                     return
                 hold = _stop_prefix_len(buf, stop)
                 out, buf = buf[: len(buf) - hold], buf[len(buf) - hold:]
                 if out:
-                    yield out
+                    yield piece(out)
             else:
-                yield buf
+                yield piece(buf)
                 buf = ""
-        if buf:
-            yield buf
+        if buf or said:
+            yield piece(buf, whole=True)
         if req.error:
             raise ServingError(f"generation failed: {req.error}")
 

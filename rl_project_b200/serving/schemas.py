@@ -33,7 +33,7 @@ def _stop_list(value: Any) -> List[str]:
 
 def _logprobs(d: Dict[str, Any]) -> Optional[int]:
     """Alternatives per token to report, None for no log-probs: ``logprobs: n`` (completions), or ``logprobs: true``
-    with ``top_logprobs: n`` (chat).  Streamed answers carry none."""
+    with ``top_logprobs: n`` (chat)."""
     want, top = d.get("logprobs"), d.get("top_logprobs")
     if want is None or want is False:
         if top:
@@ -158,12 +158,22 @@ def _by_text(top: List[Tuple[str, float]]) -> Dict[str, float]:
     return out
 
 
+def _completion_logprobs(said: List[TokenLogprob]) -> Dict[str, Any]:
+    return {"tokens": [t.text for t in said], "token_logprobs": [t.logprob for t in said],
+            "top_logprobs": [_by_text(t.top) for t in said], "text_offset": [t.offset for t in said]}
+
+
+def _chat_logprobs(said: List[TokenLogprob]) -> Dict[str, Any]:
+    def entry(text: str, lp: float) -> Dict[str, Any]:
+        return {"token": text, "logprob": lp, "bytes": list(text.encode())}
+
+    return {"content": [{**entry(t.text, t.logprob), "top_logprobs": [entry(*x) for x in t.top]} for t in said]}
+
+
 def completion_response(request_id: str, model: str, text: str, prompt_tokens: int, completion_tokens: int,
                         finish_reason: str, backend: Optional[str] = None,
                         logprobs: Optional[List[TokenLogprob]] = None) -> Dict[str, Any]:
-    said = None if logprobs is None else {
-        "tokens": [t.text for t in logprobs], "token_logprobs": [t.logprob for t in logprobs],
-        "top_logprobs": [_by_text(t.top) for t in logprobs], "text_offset": [t.offset for t in logprobs]}
+    said = None if logprobs is None else _completion_logprobs(logprobs)
     out: Dict[str, Any] = {"id": f"cmpl-{request_id}", "object": "text_completion", "created": int(time.time()),
                            "model": model,
                            "choices": [{"text": text, "index": 0, "finish_reason": finish_reason, "logprobs": said}],
@@ -182,24 +192,24 @@ def chat_response(request_id: str, model: str, text: str, prompt_tokens: int, co
                                         "finish_reason": finish_reason}],
                            "usage": _usage(prompt_tokens, completion_tokens)}
     if logprobs is not None:
-        def entry(text: str, lp: float) -> Dict[str, Any]:
-            return {"token": text, "logprob": lp, "bytes": list(text.encode())}
-
-        out["choices"][0]["logprobs"] = {"content": [
-            {**entry(t.text, t.logprob), "top_logprobs": [entry(*x) for x in t.top]} for t in logprobs]}
+        out["choices"][0]["logprobs"] = _chat_logprobs(logprobs)
     if backend:
         out["forgeline"] = {"backend": backend}
     return out
 
 
-def completion_chunk(request_id: str, model: str, text: str, finish_reason: Optional[str] = None) -> Dict[str, Any]:
+def completion_chunk(request_id: str, model: str, text: str, finish_reason: Optional[str] = None,
+                     logprobs: Optional[List[TokenLogprob]] = None) -> Dict[str, Any]:
+    said = {} if logprobs is None else {"logprobs": _completion_logprobs(logprobs)}
     return {"id": f"cmpl-{request_id}", "object": "text_completion", "created": int(time.time()), "model": model,
-            "choices": [{"text": text, "index": 0, "finish_reason": finish_reason}]}
+            "choices": [{"text": text, "index": 0, "finish_reason": finish_reason, **said}]}
 
 
-def chat_chunk(request_id: str, model: str, text: str, finish_reason: Optional[str] = None) -> Dict[str, Any]:
+def chat_chunk(request_id: str, model: str, text: str, finish_reason: Optional[str] = None,
+               logprobs: Optional[List[TokenLogprob]] = None) -> Dict[str, Any]:
+    said = {} if logprobs is None else {"logprobs": _chat_logprobs(logprobs)}
     return {"id": f"chatcmpl-{request_id}", "object": "chat.completion.chunk", "created": int(time.time()),
-            "model": model, "choices": [{"index": 0, "delta": {"content": text}, "finish_reason": finish_reason}]}
+            "model": model, "choices": [{"index": 0, "delta": {"content": text}, "finish_reason": finish_reason, **said}]}
 
 
 def error_response(message: str, kind: str = "invalid_request_error", code: int = 400) -> Dict[str, Any]:

@@ -335,6 +335,41 @@ def test_served_logprobs_of_every_token():
     assert said_by(list(b"Xcd"), WithEnd(), stop=("X",)).logprobs == []
 
 
+@pytest.mark.parametrize("stop", [(), ("\u00e9X",), ("never",)])
+@pytest.mark.parametrize("path", ["/v1/completions", "/v1/chat/completions"])
+def test_streamed_logprobs(path, stop):
+    """A streamed answer's chunks carry, together, what the whole answer does."""
+    import json
+
+    from rl_project_b200.data.tokenizers import ByteTokenizer
+    from rl_project_b200.serving import EngineBackend, Router
+
+    class WithEnd(ByteTokenizer):
+        def decode(self, ids):
+            return super().decode([i for i in ids if i != 0])
+
+    ids = list("n\U0001f600 a\u00e9\u00e9Xb\u00e9".encode()) + [0]
+    router = Router({"m": EngineBackend("m", Scripted(ids), WithEnd(), background=False)}, "m")
+    chat = "chat" in path
+    body = {"prompt": "x", "messages": [{"role": "user", "content": "x"}], "stop": list(stop),
+            **({"logprobs": True, "top_logprobs": 1} if chat else {"logprobs": 1})}
+    whole = router.handle("POST", path, body)[1]["choices"][0]
+    lines = list(router.handle("POST", path, {**body, "stream": True})[1])
+    assert lines[-1] == "data: [DONE]\n\n"
+    chunks = [json.loads(x[6:])["choices"][0] for x in lines[:-1]]
+    text = whole["message"]["content"] if chat else whole["text"]
+    assert "".join(c["delta"]["content"] if chat else c["text"] for c in chunks) == text
+    assert len(chunks) > 4 and all("logprobs" in c for c in chunks[:-1]) and "logprobs" not in chunks[-1]
+    for key, want in whole["logprobs"].items():
+        assert [x for c in chunks[:-1] for x in c["logprobs"][key]] == want
+    assert len(whole["logprobs"]["content" if chat else "tokens"]) == (
+        len(text.encode()) + (stop != ("\u00e9X",)))  # (and the end mark, where the text was not cut)
+    plain = [json.loads(x[6:])["choices"][0] for x in router.handle("POST", path, {
+        "prompt": "x", "messages": body["messages"], "stream": True, "stop": list(stop)})[1] if "DONE" not in x]
+    assert all("logprobs" not in c for c in plain)
+    assert router.handle("POST", path, {**body, "stream": True, "logprobs": 21})[0] == 400
+
+
 def test_offsets_in_linear_time():
     """A long answer's offsets, as its whole prefixes give them, from a number of decoded tokens in proportion to it."""
     from rl_project_b200.data.tokenizers import ByteTokenizer
