@@ -282,7 +282,8 @@ def cmd_serve(args: argparse.Namespace) -> int:
 
     policy = _load_policy(args)
     engine = InferenceEngine(policy.model, max_batch=args.max_batch, max_seq_len=args.max_seq_len,
-                             kv_cache=args.kv_cache, kv_budget=args.kv_budget)
+                             kv_cache=args.kv_cache, kv_budget=args.kv_budget, kv_sink=args.kv_sink,
+                             kv_recent=args.kv_recent)
     backend = EngineBackend(args.model_name, engine, policy.tokenizer)
     route_fn = None
     if args.routing:
@@ -550,6 +551,9 @@ _SERVE = _POLICY_SOURCE + [
     A("--kv-cache", default="bf16", choices=["bf16", "q4"], help="how keys and values are held (q4: 4 bits)"),
     A("--kv-budget", type=int, default=None,
       help="tokens a sequence keeps cached, by accumulated attention weight (needs --kv-cache q4)"),
+    A("--kv-sink", type=int, default=4, help="first tokens that --kv-budget always keeps"),
+    A("--kv-recent", type=int, default=None,
+      help="last tokens that --kv-budget always keeps (default: a quarter of it)"),
     A("--routing", default=None, help="routing policy JSON"), A("--metrics", default="none"),
     A("--output-dir", default="runs/serve")]
 

@@ -478,6 +478,29 @@ def test_refusals():
         SamplingParams(logprobs=21).validate()
 
 
+def test_serve_sets_every_option_of_the_cache(monkeypatch):
+    import importlib
+    from types import SimpleNamespace
+
+    from rl_project_b200.inference import engine as eng_mod
+
+    cli, built = importlib.import_module("rl_project_b200.cli.main"), []
+
+    class Engine(InferenceEngine):
+        def __init__(self, *args, **kw):
+            super().__init__(*args, **kw)
+            built.append(self)
+            raise StopIteration
+
+    monkeypatch.setattr(eng_mod, "InferenceEngine", Engine)
+    monkeypatch.setattr(cli, "_load_policy", lambda args: SimpleNamespace(model=model("cpu"), tokenizer=None))
+    for flags, want in (([], (64, 4, 16)), (["--kv-sink", "0", "--kv-recent", "30"], (64, 0, 30))):
+        args = cli.build_parser().parse_args(["serve", "--kv-cache", "q4", "--kv-budget", "64", *flags])
+        with pytest.raises(StopIteration):
+            cli.cmd_serve(args)
+        assert (built[-1].kv_budget, built[-1].kv_sink, built[-1].kv_recent) == want
+
+
 def test_rollouts_hold_their_cache_as_configured(monkeypatch):
     """engine_kv_cache reaches the engine of every rollout path, or is refused."""
     from types import SimpleNamespace
