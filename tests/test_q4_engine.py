@@ -495,7 +495,7 @@ def test_serve_sets_every_option_of_the_cache(monkeypatch):
     monkeypatch.setattr(eng_mod, "InferenceEngine", Engine)
     monkeypatch.setattr(cli, "_load_policy", lambda args: SimpleNamespace(model=model("cpu"), tokenizer=None))
     for flags, want in (([], (64, 4, 16)), (["--kv-sink", "0", "--kv-recent", "30"], (64, 0, 30))):
-        args = cli.build_parser().parse_args(["serve", "--kv-cache", "q4", "--kv-budget", "64", *flags])
+        args = cli.build_parser().parse_args(["serve", "--checkpoint", "x", "--kv-cache", "q4", "--kv-budget", "64", *flags])
         with pytest.raises(StopIteration):
             cli.cmd_serve(args)
         assert (built[-1].kv_budget, built[-1].kv_sink, built[-1].kv_recent) == want
