@@ -24,6 +24,7 @@ import os
 from typing import List, NamedTuple, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn.functional as F
 
 from rl_project_b200.ops._ext import native
@@ -167,16 +168,32 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, targets, top, status):
         lp, ent, top_lp, top_ids, m, ls = native().token_logprob(x, targets, top, True, status)
+        ctx.top = top
         ctx.save_for_backward(x, targets, m, ls, ent, top_ids)
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
         return lp, ent, top_lp, top_ids
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_lp, g_ent, g_top, _):
         grads = [g.float().contiguous() if g is not None else None for g in (g_lp, g_ent, g_top)]
-        return native().token_logprob_bwd(*ctx.saved_tensors, *grads), None, None, None
+        if not torch.is_grad_enabled():
+            return native().token_logprob_bwd(*ctx.saved_tensors, *grads), None, None, None
+        # a gradient that is itself to be differentiated (create_graph): the plain form's
+        x, targets = ctx.saved_tensors[:2]
+        outs = _token_logprobs_reference(x, _within(targets, x.shape[-1]), ctx.top)[:3]
+        used = [(o, g) for o, g in zip(outs, grads) if g is not None]
+        return torch.autograd.grad(*zip(*used), create_graph=True)[0], None, None, None
+
+
+def _within(targets: torch.Tensor, V: int) -> torch.Tensor:
+    """Targets without those outside the vocabulary."""
+    return targets.masked_fill(targets >= V, -1)
+
+
+def _plainly(x: torch.Tensor) -> bool:
+    """Whether the call is under a transform that kernels do not go through: torch.func's, or forward-mode AD."""
+    return torch._C._are_functorch_transforms_active() or forward_ad.unpack_dual(x).tangent is not None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
@@ -186,7 +203,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     One pass over the logits; gradients flow to them from the log-probs, the entropy and the alternatives' log-probs.
     Entries of -inf are tokens that cannot occur; a row of nothing else has log-probs -inf, entropy 0 and no
     gradient, a row with NaN or +inf gives NaN.  ``top`` is at most 64.  A target outside the vocabulary has log-prob
-    0 and is reported in ``status`` or the device's index-error word (on CPU: ``IndexError``).
+    0 and is reported in ``status`` or the device's index-error word (on CPU: ``IndexError``).  Second derivatives
+    (``create_graph``), forward-mode AD and ``torch.func`` transforms go through the plain form, in several passes and
+    without that report.
     """
     V = logits.shape[-1]
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
@@ -198,7 +217,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     x = logits.reshape(-1, V)
     t = targets.reshape(-1).to(torch.long).contiguous()
     shape = targets.shape
-    if x.is_cuda:
+    if _plainly(x):
+        lp, ent, top_lp, ids = _token_logprobs_reference(x, _within(t, V), int(top))
+    elif x.is_cuda:
         x = x if x.stride(1) == 1 else x.contiguous()
         if x.requires_grad and torch.is_grad_enabled():
             lp, ent, top_lp, ids = _TokenLogprobs.apply(x, t, int(top), status)
@@ -223,7 +244,7 @@ def _token_logprobs_reference(x: torch.Tensor, t: torch.Tensor, top: int):
     if top:
         ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top]
     else:
-        ids = torch.empty(x.shape[0], 0, dtype=torch.long)
+        ids = torch.empty(x.shape[0], 0, dtype=torch.long, device=x.device)
     inf, zero = torch.full_like(lp, float("-inf")), torch.zeros_like(lp)
     lp = torch.where(t >= 0, torch.where(dead[:, 0], inf, lp), zero)
     return lp, torch.where(dead[:, 0], zero, ent), logp.gather(-1, ids).masked_fill(dead, float("-inf")), ids

@@ -225,6 +225,42 @@ def test_bad_target(dev):
     assert status.item() != 0
 
 
+def test_derivatives_of_derivatives(dev):
+    """Second derivatives, forward-mode AD and torch.func transforms, as through the definition in 64 bits."""
+    torch.manual_seed(11)
+    N, V, k = 5, 37, 3
+    x0, v = torch.randn(N, V) * 2, torch.randn(N, V)
+    x0[1, ::4] = -math.inf
+    v[1, ::4] = 0
+    t = torch.tensor([4, 1, -1, 7, 36])
+    c = [torch.randn(N), torch.randn(N), torch.randn(N, k)]
+    td = t.to(dev)
+
+    def f(x, targets, c, by=lambda x, t: token_logprobs(x, t, top=k)):
+        lp, ent, top = by(x, targets)[:3]
+        return (lp * c[0]).sum() + (ent ** 2 * c[1]).sum() + (top * c[2]).sum()
+
+    xd, vd, cd = x0.to(dev).requires_grad_(), v.to(dev), [y.to(dev) for y in c]
+    xo, co = x0.to(F64).requires_grad_(), [y.to(F64) for y in c]
+    want, = torch.autograd.grad(f(xo, t, co, lambda x, t: oracle(x, t, k)), xo, create_graph=True)
+    curve, = torch.autograd.grad((want * v).sum(), xo)
+    got, = torch.autograd.grad(f(xd, td, cd), xd, create_graph=True)
+    # values up to 2^5 and their products in fp32, sums of 37: 2^5 * 2^-24 * 37 * 4, below 2^-11
+    assert ((got.detach().cpu().to(F64) - want.detach()).abs() <= 2 ** -11).all()
+    twice, = torch.autograd.grad((got * vd).sum(), xd)
+    assert twice.abs().max() > 0.1 and ((twice.cpu().to(F64) - curve).abs() <= 2 ** -11).all()
+    slope = (want.detach() * v).sum()
+    with torch.autograd.forward_ad.dual_level():
+        out = f(torch.autograd.forward_ad.make_dual(xd.detach(), vd), td, cd)
+        assert abs(float(torch.autograd.forward_ad.unpack_dual(out).tangent) - float(slope)) <= 2 ** -9
+    _, tangent = torch.func.jvp(lambda x: f(x, td, cd), (xd.detach(),), (vd,))
+    assert abs(float(tangent) - float(slope)) <= 2 ** -9
+    grad = torch.func.grad(lambda x: f(x, td, cd))(xd.detach())
+    assert ((grad.cpu().to(F64) - want.detach()).abs() <= 2 ** -11).all()
+    lp = torch.func.vmap(lambda x, t: token_logprobs(x[None], t[None]).logprobs[0])(xd.detach(), td)
+    assert ((lp.cpu().to(F64) - oracle(x0, t, 0)[0]).abs() <= LP_TOL).all()
+
+
 def test_refusals(dev):
     x, t = torch.randn(3, 10).to(dev), torch.zeros(3, dtype=torch.long).to(dev)
     for call in (lambda: token_logprobs(x.double(), t), lambda: token_logprobs(x, t[:2]),
