@@ -182,8 +182,8 @@ class _TokenLogprobs(torch.autograd.Function):
         # a gradient that is itself to be differentiated (create_graph): the plain form's
         x, targets = ctx.saved_tensors[:2]
         outs = _token_logprobs_reference(x, _within(targets, x.shape[-1]), ctx.top)[:3]
-        used = [(o, g) for o, g in zip(outs, grads) if g is not None]
-        return torch.autograd.grad(*zip(*used), create_graph=True)[0], None, None, None
+        outs, grads = zip(*((o, g) for o, g in zip(outs, grads) if g is not None))
+        return torch.autograd.grad(outs, x, grads, create_graph=True)[0], None, None, None
 
 
 def _within(targets: torch.Tensor, V: int) -> torch.Tensor:
