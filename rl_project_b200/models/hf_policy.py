@@ -152,8 +152,13 @@ class HFPolicy(nn.Module):
         return lp * response_mask.to(lp.device, lp.dtype) if response_mask is not None else lp
 
     def token_logprobs(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-        """Per-position ``log p(targets | input_ids)`` ``[B, T]``; 0 where ``targets == -1``."""
+        """Per-position ``log p(targets | input_ids)`` ``[B, T]``; 0 where ``targets == -1``.  A target beyond the
+        vocabulary raises ``IndexError`` where the model or ``targets`` is on the CPU; among targets on the GPU it scores 0
+        and is reported in the device's index-error word (``ops._ext.check_bounds``; the trainer reads it at its
+        log steps and fails the run)."""
         logits = _scorable(self.token_logits(input_ids))
+        if targets.device.type == "cpu" and targets.numel() and int(targets.max()) >= logits.shape[-1]:
+            raise IndexError("a target lies outside the vocabulary")
         return token_logprobs(logits, targets.to(logits.device)).logprobs
 
     def token_ce(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:

@@ -225,6 +225,28 @@ def test_bad_target(dev):
     assert status.item() != 0
 
 
+def test_policy_targets_outside_the_vocabulary(dev):
+    """Hugging Face scoring: raised where the host can see it, reported in the index-error word where it cannot."""
+    from types import SimpleNamespace
+
+    from rl_project_b200.models.hf_policy import HFPolicy
+
+    x = torch.randn(1, 3, 20).to(dev)
+    policy = SimpleNamespace(token_logits=lambda ids: x)
+    good, bad = torch.tensor([[1, -1, 19]]), torch.tensor([[1, 20, 3]])
+    assert HFPolicy.token_logprobs(policy, good, good)[0, 1] == 0
+    with pytest.raises(IndexError):
+        HFPolicy.token_logprobs(policy, bad, bad)
+    if dev == "cuda":
+        from rl_project_b200.core.errors import KernelError
+        from rl_project_b200.ops._ext import check_bounds
+
+        lp = HFPolicy.token_logprobs(policy, bad, bad.cuda())
+        with pytest.raises(KernelError):
+            check_bounds(torch.device("cuda", 0))
+        assert lp[0, 1] == 0 and lp[0, 0] < 0
+
+
 def test_derivatives_of_derivatives(dev):
     """Second derivatives, forward-mode AD and torch.func transforms, as through the definition in 64 bits."""
     torch.manual_seed(11)
