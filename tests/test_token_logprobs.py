@@ -225,6 +225,25 @@ def test_bad_target(dev):
     assert status.item() != 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [4099, 50257])
+def test_one_logit_dominates(dev, dtype, V):
+    """No log-prob above 0 and no entropy below it, wherever the largest logit lies and however far above the others:
+    the reference that the sums are taken against is one of the row's own logits."""
+    N = 48
+    for rest in (-6e4, -60.0, -12.0, -math.inf):
+        x = torch.full((N, V), rest) + torch.rand(N, V) * 2
+        x[:, 3] = 0.0  # early, and what comes behind lies up to 9 above it
+        x.scatter_(1, torch.randint(V // 2, V, (N, 1)), torch.rand(N, 1) * 9)
+        x = x.to(dtype)
+        r = token_logprobs(x.to(dev), x.argmax(-1).to(dev), top=1)
+        lp, ent, _, _ = oracle(x, x.argmax(-1), 1)
+        assert (r.logprobs <= 0).all() and (r.top_logprobs <= 0).all() and (r.entropy >= 0).all()
+        # one or two large terms, logs below 2^4: a few roundings of 2^-20
+        assert ((r.logprobs.cpu().to(F64) - lp).abs() <= 2 ** -17).all()
+        assert ((r.entropy.cpu().to(F64) - ent).abs() <= 2 ** -13).all()
+
+
 def test_policy_targets_outside_the_vocabulary(dev):
     """Hugging Face scoring: raised where the host can see it, reported in the index-error word where it cannot."""
     from types import SimpleNamespace
