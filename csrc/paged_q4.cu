@@ -804,7 +804,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, q4_ctas(D, NT)) q4_decode_k
   }
 }
 
-// Maximum and 1 / sum of one query head over a row's parts; a whole warp calls it.
+// Maximum and 1 / sum of one query head over a row's parts; a whole warp calls it.  Where no block of the row was there
+// to be read, its scores are all -inf: the maximum then is 0, and the weights 0.
 RLB_DEVICE float2 q4_join(const float* ml, int G, int parts) {
   const int lane = threadIdx.x & 31;
   float M = -INFINITY, sum = 0.f;
@@ -817,7 +818,7 @@ RLB_DEVICE float2 q4_join(const float* ml, int G, int parts) {
     sum += ms == -INFINITY ? ls : ls * sm100::ex2_approx(ms - M);
   }
   sum = warp_sum(sum);
-  return make_float2(M, sum != 0.f ? 1.f / sum : 0.f);
+  return make_float2(M == -INFINITY ? 0.f : M, sum != 0.f ? 1.f / sum : 0.f);
 }
 
 // Unnormalised output (dimensions lane + 32 e) and statistics of parts first, first + step, ... of one query head, by a

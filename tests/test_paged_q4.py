@@ -404,6 +404,24 @@ def test_decode_bad_index(dev):
                                              torch.tensor([0, 2], dtype=torch.int32, device=dev)))
 
 
+def test_decode_without_any_block(dev):
+    """A sequence none of whose blocks exist: reported, its output zero, its weights as they were, the others' right."""
+    lens, D = [40, 700], 64
+    ks, vs, pools, tables, n, _ = cache(lens, 2, D, dev)
+    q = torch.randn(2, 4, D).to(BF).to(dev)
+    for b in range(2):
+        t = tables.clone()
+        t[b] = -1
+        w = torch.ones(2, 2, tables.shape[1] * 16, device=dev)
+        out = index_error(dev, lambda: paged_decode_q4(q, *pools, t, n, 0.125, 0.0, 0, w,
+                                                       torch.tensor([0, 1], dtype=torch.int32, device=dev)))
+        if out is not None:
+            o, p, a = attention(q[1 - b], ks[1 - b], vs[1 - b], 0.125, 0.0, 0)
+            check_decode(out[1 - b], o, a)
+            assert not out[b].any() and (w[b] == 1).all()
+            assert ((w[1 - b, :, :lens[1 - b]].cpu() - 1 - p).abs() <= 2 ** -15 * p + 2 ** -23 * (1 + p)).all()
+
+
 # ---------------------------------------------------------------- eviction
 def chosen(w, n, keep, sink, recent):
     """Positions kept of one head's weights (a list of floats), by definition."""
