@@ -18,6 +18,7 @@ import time
 import uuid
 from dataclasses import dataclass, field
 from enum import Enum
+from numbers import Integral
 from typing import Iterator, List, Optional, Tuple
 
 from rl_project_b200.core.errors import ServingError
@@ -68,8 +69,9 @@ class SamplingParams:
             problems.append("top_p must be in (0, 1]")
         if self.min_p is not None and not _in_range(self.min_p, 0.0, 1.0):
             problems.append("min_p must be in [0, 1]")
-        if self.logprobs is not None and not _in_range(self.logprobs, 0, MAX_LOGPROBS):
-            problems.append(f"logprobs must be between 0 and {MAX_LOGPROBS}")
+        if self.logprobs is not None and (not isinstance(self.logprobs, Integral) or isinstance(self.logprobs, bool)
+                                          or not _in_range(self.logprobs, 0, MAX_LOGPROBS)):
+            problems.append(f"logprobs must be a whole number between 0 and {MAX_LOGPROBS}")
         if self.repetition_penalty <= 0:
             problems.append("repetition_penalty must be > 0")
         if problems:

@@ -478,6 +478,19 @@ def test_refusals():
         SamplingParams(logprobs=21).validate()
 
 
+def test_numbers_of_alternatives_are_whole():
+    """A request that asks for 2.5 alternatives is refused alone; accepted, it would end the step of all the others."""
+    import numpy as np
+
+    eng = InferenceEngine(model("cpu"), max_batch=2)
+    for bad in (2.5, float("nan"), True, "3", -1, 21):
+        with pytest.raises(Exception) as err:
+            eng.submit([1, 2], SamplingParams(max_tokens=2, logprobs=bad))
+        assert isinstance(err.value, ServingError)
+    req = eng.generate([1, 2], SamplingParams(max_tokens=2, logprobs=np.int64(2), **GREEDY))
+    assert req.finish_reason == "length" and [len(t) for t in req.top_logprobs] == [2, 2]
+
+
 def test_serve_sets_every_option_of_the_cache(monkeypatch):
     import importlib
     from types import SimpleNamespace
