@@ -930,7 +930,8 @@ static int logit_type(const at::Tensor& x) {
 std::vector<at::Tensor> token_logprob(const at::Tensor& logits, const at::Tensor& targets, int64_t k, bool stats,
                                       const c10::optional<at::Tensor>& status) {
   check_cuda(logits, "logits");
-  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) < (1LL << 30) && logits.stride(1) == 1 &&
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) < (1LL << 30) &&
+                  (logits.stride(1) == 1 || logits.size(1) == 1) &&
                   logits.size(0) < (1LL << 31), "logits: [N, V] with unit inner stride");
   TORCH_CHECK(logit_type(logits) >= 0, "logits: fp32, bf16 or fp16");
   check_dev(targets, logits, "targets");

@@ -225,6 +225,18 @@ def test_bad_target(dev):
     assert status.item() != 0
 
 
+def test_vocabulary_of_one(dev):
+    """One column, whatever its stride says: transposed rows, columns of wider ones, expanded rows."""
+    t = torch.tensor([0, -1, 0], device=dev)
+    wide = torch.randn(3, 5, device=dev)
+    for x in (torch.randn(1, 3, device=dev).t(), wide[:, 2:3], wide[:1, :1].expand(3, 1)):
+        x = x.detach().requires_grad_()
+        r = token_logprobs(x, t, top=1)
+        assert not r.logprobs.any() and not r.entropy.any() and not r.top_logprobs.any() and not r.top_ids.any()
+        grad, = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), x)
+        assert grad.shape == (3, 1) and not grad.any()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [4099, 50257])
 def test_one_logit_dominates(dev, dtype, V):
