@@ -961,7 +961,7 @@ RLB_DEVICE uint32_t weight_key(float w) {
 }
 
 // Choosing what stays has three forms.  This one, a CTA per (KV head, sequence), takes sequences whose weights do not fit
-// into the registers of a cluster.  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
+// into a CTA's registers, where they do not fit into a cluster's either or are too many rows for clusters.  The weight of the last kept token is found by a radix selection (11, 11 and 10 bits:
 // a histogram in shared memory, whose bins a scan then walks from the top).  Each warp then takes a stretch of the
 // tokens: it counts the tokens above that weight and those equal to it, a scan over the warps gives it its place, and
 // it writes its kept positions in order.  The weights move to the front last, tile by tile: a token never moves to a
@@ -1490,8 +1490,11 @@ cudaError_t rlb_q4_evict(void* k_pool, void* v_pool, const int* tables, const in
                          int recent, int sink, int* status, cudaStream_t s) {
   if (B == 0) return cudaSuccess;
   const long long most = (long long)max_blocks * kTok < w_len ? (long long)max_blocks * kTok : w_len;  // tokens
-  // Clusters while their rows take less than one CTA each does (rows x 0.9 us and up, against 41).
-  const bool few = (long long)B * Hkv <= 32 || most > 40 * kSelect;
+  // Clusters while their rows take less than one CTA each does: up to 40960 tokens, keys in registers, rows x 0.9 us and
+  // up against 41; beyond, in us of the whole call by clusters and by one CTA a row: 8 rows of 60000 tokens 35 and 80, 64
+  // rows 94 and 85, 256 rows 297 and 145, 64 rows of 100000 110 and 122.  (Above 131072 tokens one CTA a row is all there
+  // is: 8 or 64 rows of 140000 take 160, 8 rows of 400000 405.)
+  const bool few = (long long)B * Hkv <= (most > 40 * kSelect ? 64 : 32);
   if (few && most > 16 * kSelect && most <= 16 * kSelect * kCtas) {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;

@@ -497,6 +497,11 @@ def test_evict(dev, lens, Hkv, D, keep, sink, recent, kind):
         assert torch.equal(p[rest], q.cpu()[rest])
 
 
+def test_evict_many_long_rows(dev):
+    """More long rows than clusters take: one CTA a row."""
+    test_evict(dev, [41000, 40970, 500], 22, 32, 700, 3, 60, "ties")
+
+
 def test_empty_calls(dev):
     """No rows, no sequences, tables without blocks, and a batch of nothing but padding."""
     D = 64
