@@ -73,7 +73,8 @@ RLB_DEVICE void codes_bf16(uint32_t w, uint32_t (&r)[4], uint32_t magic) {
 // registers for half as many warps again 59, a grid of one wave that fetches the next row ahead 56.
 //
 // code = clamp(rint((x - lo) / s)) without a division per element: q = (x - lo) (1 / s) and its remainder's share
-// q + (x - lo - q s) (1 / s) is the correctly rounded quotient, and adding 1.5 2^23 rounds that to a whole number.
+// q + (x - lo - q s) (1 / s) is the correctly rounded quotient (a quotient corrected by its remainder, after P. Markstein,
+// 1990), and adding 1.5 2^23 rounds that to a whole number.
 RLB_DEVICE uint32_t q4_codes(const bf16x8& x, float lo, float s) {
   float f[8];
   unpack8(x, f);
@@ -223,14 +224,17 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // scales and minima of K and V, one contiguous piece each) into its own ring of shared memory with bulk copies, which
 // run ahead across the rows' borders, and computes on matrix instructions
 // (mma.sync m16n8k16, two fp16 or two bf16 operands -> fp32) with the 16 tokens, then the dimensions, as the 16 rows and up to 8
-// query heads of the KV head as the 8 columns.  The kernel is bound by bytes and by the instructions that unpack
-// them, not by tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least, operands in shared
-// memory) would need the unpacked values written back to shared memory first.  32 ragged sequences of up to 8192 tokens
-// (8 KV heads x 128, 4 queries each, 189 MB): 66 us with the join, 2.9 TB/s; one of 100001: 45 us, 2.6 TB/s; 64 of up to
-// 4096 with heads of 64 (90 MB): 39 us.  (With one fp16 weight 59, 41 and 37 us.)
+// query heads of the KV head as the 8 columns.  The kernel is bound by the latency of the dependent instructions that
+// unpack the codes, not by bytes or tensor throughput: at 1/8 of the rows a tcgen05 tile (64 or 128 rows at least,
+// operands in shared memory) would need the unpacked values written back to shared memory first.  32 ragged sequences of
+// up to 8192 tokens (8 KV heads x 128, 4 queries each, 189 MB): 66 us with the join (kernel 61, 3.1 TB/s); one of 100001:
+// 45 us, 2.6 TB/s; 64 of up to 4096 with heads of 64 (90 MB): 39 us.  (With one fp16 weight 59, 41 and 37 us.)  406
+// instructions per block of 16 tokens and 128 dimensions, issued at 2.2 of the 4 a cycle that an SM has slots for: 2.8
+// warps a scheduler (167 registers a thread) do not cover the fixed latencies, no pipe is above 51 %, and memory is
+// waited for least.
 //
-// K's codes become fp16 numbers exactly: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4 are 1024 + 16 code, so
-// half of the nibbles need no shift, and a packed add makes code - 8 of the others.
+// K's codes become fp16 numbers exactly, by the format alone: bits 0x6400 | code are 1024 + code and 0x6400 | code << 4
+// are 1024 + 16 code, so half of the nibbles need no shift, and a packed add makes code - 8 of the others.
 // S^T = K Q^T.  With a token's scale s and minimum m:  k . q = s (code . q) + m sum(q), per group of dimensions.  Q
 // is fp16 after division by a power of two per head (its largest element then lies in [2^13, 2^14)): bf16's 8 bits
 // fit, and what falls below 2^-24 is 2^-38 of the largest.  K's odd nibbles stay 1024 + 16 code: their q are divided by 16,
