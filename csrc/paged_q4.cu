@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const uint8_t* __restrict_
 // (2^-16 of each weight, below a hundredth of the output's own rounding to bf16), and both go through the matrix
 // instruction.  bf16 has fp32's exponents, so that values of any size keep these bits beside each other: p is kept times
 // 2^-32, with which 2^20 tokens of the type's largest values stay in range and values from 2^-58 on keep all their bits.
-// (One fp16 weight, 2^-11 of each, needed the weights scaled by V's largest scale, from which values below 2^-17 of it
+// (One fp16 weight, 2^-11 of each, needed the weights scaled by V's largest scale, from which values far below it
 // lost bits even where that token's weight was nothing.)
 // The tokens' order is free too: row g of S^T (of each half of the block) is token g / 2 for even g and
 // 4 + (g / 2 ^ 2) for odd g.  After the 8 x 8 transposition (movmatrix) that turns S^T's registers into P^T's, lane
