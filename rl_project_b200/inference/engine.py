@@ -208,7 +208,10 @@ class InferenceEngine:
         vocab = int(self.model.spec.vocab_size)
         for req in reqs:
             st = _Seq(req)
+            before = self.states.get(req.id)
             self.states[req.id] = st
+            if before is not None and before.row >= 0:  # a request under the id of one that still ran takes its place
+                self._free_rows.append(before.row)
             if self.kv_budget is not None:
                 st.row = self._free_rows.pop()
                 self.kv.weights[:, st.row].zero_()

@@ -148,6 +148,19 @@ def test_cuts_in_a_full_pool(dev, blocks, same):
     assert eng.evictions >= 4 * 4 and eng.allocator.used_blocks == (1 if eng.decode_graphs else 0)
 
 
+def test_request_ids_used_again():
+    """A request under the id of one that still runs takes its place, as without a budget, and its accumulators' row."""
+    for kw in ({}, {"kv_cache": "q4", "kv_budget": 32}):
+        eng = InferenceEngine(model("cpu"), max_batch=2, **kw)
+        for _ in range(5):
+            last = eng.submit([1, 2, 3], SamplingParams(max_tokens=60, **GREEDY), id="same")
+            eng.step()
+        other = eng.submit([4, 5], SamplingParams(max_tokens=4, **GREEDY))
+        eng.run_until_idle()
+        assert len(last.generated_tokens) == 60 and len(other.generated_tokens) == 4
+        assert sorted(eng._free_rows) == ([0, 1] if kw else [])
+
+
 def test_blocks_kept_for_cuts():
     from rl_project_b200.inference import OutOfBlocksError, PagedBlockAllocator
 
